@@ -140,6 +140,20 @@ PTO_HIP_API int pto_hip_sync(void* stream);
  *      tensors: x[T,H], gamma[1,H] fp32, w_gate8[I,H] e4m3, w_gate_scale[I] fp32, w_up8[I,H], w_up_scale[I],
  *               w_down8[H,I], w_down_scale[H], out[T,H] (fp32 or dtype of x);  codes are one row per OUTPUT
  *               channel with k contiguous;  scalars: eps (f32 bits)
+ *  "rms_norm_fp8_block"   RMSNorm with an e4m3 output of one scale per 128 columns (no counterpart in the reference)
+ *      tensors: x[T,H], gamma[1,H] fp32, [normed_out[T,H],] codes[T,H] e4m3, scale[T,ceil(H/128)] fp32, or with the residual's
+ *               addition x, residual[T,H], gamma, sum_out[T,H], [normed_out,] codes, scale;  scalars: eps (f32 bits)
+ *  "quantize_fp8_block"   the same output without the norm
+ *      tensors: x[T,H], codes[T,H] e4m3, scale[T,ceil(H/128)] fp32
+ *  "projection_fp8_block"  product of such operands (no counterpart in the reference)
+ *      tensors: a8[M,K] e4m3, a_scale[M,K/128] fp32, w8[N,K] e4m3 (one row per OUTPUT channel), w_scale[ceil(N/128),K/128] fp32,
+ *               out[M,N] (fp32, bf16 or fp16)
+ *  "route_experts"     a router's choice of experts (no counterpart in the reference)
+ *      tensors: logits[T,E] (fp32, bf16 or fp16), [bias[E] fp32,] expert_ids[T,top_k] i32, expert_weights[T,top_k] fp32
+ *      scalars: n_groups, topk_groups, score function (0 softmax, 1 sigmoid), renormalize (0, 1), scale (f32 bits)
+ *  "experts_ffn_fp8_block"  the chosen experts' FFN (no counterpart in the reference)
+ *      tensors: x8[T,H] e4m3, x_scale[T,H/128] fp32, expert_ids[T,top_k] i32, expert_weights[T,top_k] fp32, w_gate8[E,I,H],
+ *               w_gate_scale[E,I/128,H/128], w_up8, w_up_scale, w_down8[E,H,I], w_down_scale[E,H/128,I/128], out[T,H]
  *  "llama_mini"        examples/models/08_llama_mini.py:384-483
  *      tensors: hidden[S,D], causal_mask[S,S], cos_emb[S,D/2], sin_emb[S,D/2], wq, wk, wv, w_dense, w_gate, w_up,
  *               w_down [D,D], w_lm[D,V], logits[S,V], all fp32
@@ -346,6 +360,53 @@ PTO_HIP_API int pto_hip_projection_fp8(const void* a8, const float* a_scale, con
  * multiple of 8, at most 16384.  No counterpart in the reference. */
 PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* scale, int64_t rows, int64_t cols,
                                           int x_dtype, void* stream);
+
+/* ---- e4m3 operands with a scale for each block of 128 (none has a counterpart in the reference) ----
+ * Activations: codes [rows, cols] with one fp32 scale per 128 columns of a row, [rows, ceil(cols / 128)].  Weights: codes one row per
+ * OUTPUT channel with k contiguous, [n, k], with one fp32 scale per block of 128 x 128, [ceil(n / 128), k / 128].  A value is its
+ * code times its scale; scales may be any fp32 values. */
+
+/* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
+ * codes = e4m3(n / scale), round to nearest even; sum_out = x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every
+ * output is rounded once.  residual, gamma, sum_out and normed_out may each be NULL; sum_out may be x or residual itself.  NaN
+ * elements are left out of amax and give NaN codes.  cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the
+ * last group may be shorter).  quantize_fp8_block: codes and scales of x itself. */
+PTO_HIP_API int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out,
+                                           void* codes, float* scale, int64_t rows, int64_t cols, float eps, int x_dtype,
+                                           void* stream);
+PTO_HIP_API int pto_hip_quantize_fp8_block(const void* x, void* codes, float* scale, int64_t rows, int64_t cols, int x_dtype,
+                                           void* stream);
+
+/* out[m, n] = sum_kb a_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} a8[m, k] * w8[n, k], fp32 accumulation, any M
+ * and N; K a multiple of 128 and at most 65536 (PTO_HIP_ERR_UNSUPPORTED otherwise).  out FP32, BF16 or FP16. */
+PTO_HIP_API int pto_hip_projection_fp8_block(const void* a8, const float* a_scale, const void* w8, const float* w_scale, void* out,
+                                             int64_t m, int64_t k, int64_t n, int out_dtype, void* stream);
+
+/* A router's choice.  score = softmax over the experts, or sigmoid, of the logits; key = score + bias, or the logits themselves
+ * where bias is NULL.  The experts are n_groups groups of consecutive ones; a group's key is the sum of its two best keys with a
+ * bias and its best key without, and the topk_groups best groups stay.  expert_ids[t, :] are the top_k experts of those by
+ * key, best first, expert_weights[t, :] their scores - divided by their sum if renormalize (0 where that is 0) - times scale.
+ * Ties go to the lowest index, of groups and of experts.  Keys with a bias are compared in 64 bits.  A NaN logit counts as -inf, a
+ * NaN key as the smallest; infinite logits that are equal share a softmax evenly.  At most 1024 experts, 64 groups and top_k 64
+ * (PTO_HIP_ERR_UNSUPPORTED otherwise). */
+#define PTO_HIP_SCORE_SOFTMAX 0
+#define PTO_HIP_SCORE_SIGMOID 1
+PTO_HIP_API int pto_hip_route_experts(const void* logits, const float* bias, int32_t* expert_ids, float* expert_weights, int64_t tokens,
+                                      int64_t experts, int64_t top_k, int64_t n_groups, int64_t topk_groups, int score_fn,
+                                      int renormalize, float scale, int logits_dtype, void* stream);
+
+/* out[t] = sum_j expert_weights[t, j] * (SiLU(x Wg_e) * (x Wu_e)) Wd_e with e = expert_ids[t, j] and x the token's values: the
+ * experts' half of a mixture layer behind pto_hip_rms_norm_fp8_block and pto_hip_route_experts.  Products as
+ * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 as pto_hip_quantize_fp8_block does, the sum over a token's
+ * experts is fp32.  A negative id leaves its slot out (a token without any gives zeros); an id of an expert that there is
+ * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  H and I multiples of 128 and at
+ * most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the
+ * other: w_gate8, w_up8 [E, I, H], w_down8 [E, H, I].  out FP32, BF16 or FP16. */
+PTO_HIP_API int pto_hip_experts_ffn_fp8_block(const void* x8, const float* x_scale, const int32_t* expert_ids,
+                                              const float* expert_weights, const void* w_gate8, const float* w_gate_scale,
+                                              const void* w_up8, const float* w_up_scale, const void* w_down8,
+                                              const float* w_down_scale, void* out, int64_t tokens, int64_t hidden,
+                                              int64_t intermediate, int64_t experts, int64_t top_k, int out_dtype, void* stream);
 
 /* out[M, N] = x[M, K] @ w[K, N] (+ residual[M, N]), 16-bit x and w of the same type, fp32
  * accumulation, out FP32 or that type: the reference's projection kernels

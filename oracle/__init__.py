@@ -61,6 +61,8 @@ Pinning status (what fixes each function independently of its own formula):
                                  only (rounding bound, row maximum on +-448,
                                  idempotence, exact small-integer case, distance
                                  to the 16-bit block; tests/test_oracle_ffn.py).
+* fp8_block.py                   block-scaled e4m3 operands, router and experts (not in the reference:
+                                 PARITY UNPINNED against it; tests/test_oracle_fp8_block.py)
 """
 
 from .attention import (  # noqa: F401
@@ -74,7 +76,7 @@ from .attention import (  # noqa: F401
     paged_gather,
     quantize_kv_fp8,
 )
-from . import stages, tile_ops  # noqa: F401
+from . import fp8_block, stages, tile_ops  # noqa: F401
 from .ffn import (ffn_block, ffn_block_fp8, ffn_gelu, ffn_relu, ffn_swiglu, projection, quantize_rows_fp8, rms_norm,  # noqa: F401
                   swiglu)
 from .layer import (  # noqa: F401

@@ -33,6 +33,8 @@ EXPORTS = (
     "pto_hip_hbm_read_probe",
     "pto_hip_ffn_swiglu_fp8", "pto_hip_quantize_rows_fp8", "pto_hip_rms_norm_quantize_fp8",
     "pto_hip_gate_up_swiglu_fp8", "pto_hip_projection_fp8", "pto_hip_llama_mini",
+    "pto_hip_rms_norm_fp8_block", "pto_hip_quantize_fp8_block", "pto_hip_projection_fp8_block", "pto_hip_route_experts",
+    "pto_hip_experts_ffn_fp8_block",
     "pto_hip_write_manifest", "pto_hip_backend_info", "pto_hip_backend_op_name", "pto_hip_backend_op_info",
     "pto_hip_backend_codegen", "pto_hip_backend_check_ops", "pto_hip_backend_program_ops",
     "pto_hip_backend_mem_path", "pto_hip_backend_handler_query",
@@ -135,6 +137,11 @@ def load() -> C.CDLL:
         "pto_hip_rms_norm_quantize_fp8": [vp, vp, vp, vp, i64, i64, C.c_float, C.c_int, vp],
         "pto_hip_gate_up_swiglu_fp8": [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, vp],
         "pto_hip_projection_fp8": [vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, vp],
+        "pto_hip_rms_norm_fp8_block": [vp] * 7 + [i64, i64, C.c_float, C.c_int, vp],
+        "pto_hip_quantize_fp8_block": [vp, vp, vp, i64, i64, C.c_int, vp],
+        "pto_hip_projection_fp8_block": [vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, vp],
+        "pto_hip_route_experts": [vp, vp, vp, vp, i64, i64, i64, i64, i64, C.c_int, C.c_int, C.c_float, C.c_int, vp],
+        "pto_hip_experts_ffn_fp8_block": [vp] * 11 + [i64] * 5 + [C.c_int, vp],
         "pto_hip_llama_mini": [vp] * 13 + [i64, i64, i64, C.c_float, vp],
         "pto_hip_w8a16_matmul": [vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, C.c_int, C.c_int, vp],
         "pto_hip_w8a16_swiglu": [vp, vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, C.c_int, vp],

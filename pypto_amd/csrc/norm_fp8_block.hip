@@ -1,0 +1,168 @@
+// RMSNorm with the residual's addition in front and an e4m3 output with a scale per 128 columns behind, one pass:
+//
+//   s = x + residual      n = s * rsqrt(mean s^2 + eps) * gamma      scale = amax_group |n| / 448      codes = e4m3(n / scale)
+//
+// and, where asked for, s (the next residual) and n in the 16-bit type of x.  s and n stay in 32 bits from the loads to the
+// outputs, so that each output is rounded once: the codes are those of n itself, not of its 16-bit copy.
+// Without the norm the same kernel is the quantiser of activations that come from elsewhere.
+//
+// Bound by memory: 2 bytes an element for x and for each of residual, sum and normed, 1 for the codes.  One workgroup holds a row in
+// registers; a group of 128 columns is 16 lanes of 8 columns, its maximum four lane exchanges.
+#include <hip/hip_runtime.h>
+
+#include "block_fp8.h"
+#include "common.h"
+
+namespace {
+
+using pto_hip::block8::codes4;
+using pto_hip::block8::group_scale;
+using pto_hip::block8::GroupQuotient;
+using pto_hip::block8::kBlock;
+
+constexpr int kThreads = 256;
+constexpr int kVecs = 8;  // most groups of eight columns a thread holds
+
+// sum_out and normed_out may be x or residual themselves: a thread writes the columns that it alone has read.
+template <typename T, bool NORM, int VECS>
+__global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, const T* residual, const float* __restrict__ gamma,
+                                                                  T* sum_out, T* normed_out, uint8_t* __restrict__ codes,
+                                                                  float* __restrict__ scale, int cols, float eps) {
+  typedef __attribute__((__vector_size__(8 * sizeof(T)))) T vec8;
+  __shared__ float red[kThreads / 64];
+  const int64_t row = blockIdx.x;
+  const int nvec = cols / 8, groups = (cols + kBlock - 1) / kBlock;
+  const vec8* xr = reinterpret_cast<const vec8*>(x + row * cols);
+  const vec8* rr = residual ? reinterpret_cast<const vec8*>(residual + row * cols) : nullptr;
+  vec8 in[VECS], res[VECS];
+#pragma unroll
+  for (int u = 0; u < VECS; ++u) {
+    const int i = threadIdx.x + u * kThreads;
+    if (i < nvec) {
+      in[u] = xr[i];
+      if (rr) res[u] = rr[i];
+    }
+  }
+  float s[VECS][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int u = 0; u < VECS; ++u) {
+    const bool live = (int)threadIdx.x + u * kThreads < nvec;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[u][e] = !live ? 0.f : rr ? (float)in[u][e] + (float)res[u][e] : (float)in[u][e];
+      ss += s[u][e] * s[u][e];
+    }
+  }
+  if (sum_out) {
+    vec8* out = reinterpret_cast<vec8*>(sum_out + row * cols);
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      vec8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)s[u][e];
+      if (i < nvec) out[i] = v;
+    }
+  }
+  if constexpr (NORM) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    float tot = red[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) tot += red[w];
+    const float inv = rsqrtf(tot / (float)cols + eps);
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+      if (i < nvec) {
+        float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (gamma) {
+          *reinterpret_cast<float4*>(&g[0]) = reinterpret_cast<const float4*>(gamma)[2 * i];
+          *reinterpret_cast<float4*>(&g[4]) = reinterpret_cast<const float4*>(gamma)[2 * i + 1];
+        }
+        vec8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s[u][e] = s[u][e] * inv * g[e];
+          v[e] = (T)s[u][e];
+        }
+        if (normed_out) reinterpret_cast<vec8*>(normed_out + row * cols)[i] = v;
+      }
+    }
+  }
+  uint2* crow = reinterpret_cast<uint2*>(codes + row * cols);
+  float* srow = scale + row * groups;
+#pragma unroll
+  for (int u = 0; u < VECS; ++u) {
+    const int i = threadIdx.x + u * kThreads;
+    float amax = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(s[u][e]));
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+    const float sc = group_scale(amax);
+    const GroupQuotient q(sc);
+    if (i < nvec) {
+      crow[i] = uint2{codes4(q(s[u][0]), q(s[u][1]), q(s[u][2]), q(s[u][3])), codes4(q(s[u][4]), q(s[u][5]), q(s[u][6]), q(s[u][7]))};
+      if (i % 16 == 0) srow[i / 16] = sc;
+    }
+  }
+}
+
+template <typename T, bool NORM>
+int launch(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out, void* codes, float* scale,
+           int64_t rows, int64_t cols, float eps, hipStream_t st) {
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(kThreads), 0, st, reinterpret_cast<const T*>(x),
+                       reinterpret_cast<const T*>(residual), gamma, reinterpret_cast<T*>(sum_out), reinterpret_cast<T*>(normed_out),
+                       reinterpret_cast<uint8_t*>(codes), scale, (int)cols, eps);
+  };
+  const int64_t vecs = (cols / 8 + kThreads - 1) / kThreads;
+  if (vecs <= 1) go(norm_fp8_block_kernel<T, NORM, 1>);
+  else if (vecs <= 2) go(norm_fp8_block_kernel<T, NORM, 2>);
+  else if (vecs <= 4) go(norm_fp8_block_kernel<T, NORM, 4>);
+  else go(norm_fp8_block_kernel<T, NORM, kVecs>);
+  PTO_CHECK_HIP(hipGetLastError());
+  return PTO_HIP_OK;
+}
+
+int run(const char* what, bool norm, const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out, void* codes,
+        float* scale, int64_t rows, int64_t cols, float eps, int x_dtype, hipStream_t st) {
+  using namespace pto_hip;
+  PTO_CHECK_ARG(rows >= 0 && cols > 0 && rows < (1ll << 31), "%s: bad shape [%lld, %lld]", what, (long long)rows, (long long)cols);
+  PTO_CHECK_ARG(x_dtype == PTO_HIP_BF16 || x_dtype == PTO_HIP_FP16, "%s: dtype %s not in {BF16, FP16}", what, dtype_name(x_dtype));
+  if (cols % 8 != 0 || cols > 8 * kThreads * kVecs)
+    return fail(PTO_HIP_ERR_UNSUPPORTED, "%s: %lld columns; rows must be a multiple of 8 and at most %d long", what, (long long)cols,
+                8 * kThreads * kVecs);
+  if (!ctx().initialized) return fail(PTO_HIP_ERR_NOT_INITIALIZED, "pto_hip_init has not been called");
+  if (rows == 0) return PTO_HIP_OK;
+  PTO_CHECK_ARG(x && codes && scale, "%s: null tensor pointer", what);
+  PTO_CHECK_ARG(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)gamma | (uintptr_t)sum_out | (uintptr_t)normed_out) % 16 == 0 &&
+                    (uintptr_t)codes % 8 == 0 && (uintptr_t)scale % 4 == 0,
+                "%s: misaligned operand", what);
+  PTO_CHECK_ARG(!sum_out || sum_out != normed_out, "%s: sum_out and normed_out are the same tensor", what);
+  if (x_dtype == PTO_HIP_BF16)
+    return norm ? launch<__bf16, true>(x, residual, gamma, sum_out, normed_out, codes, scale, rows, cols, eps, st)
+                : launch<__bf16, false>(x, residual, gamma, sum_out, normed_out, codes, scale, rows, cols, eps, st);
+  return norm ? launch<_Float16, true>(x, residual, gamma, sum_out, normed_out, codes, scale, rows, cols, eps, st)
+              : launch<_Float16, false>(x, residual, gamma, sum_out, normed_out, codes, scale, rows, cols, eps, st);
+}
+
+}  // namespace
+
+extern "C" int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out,
+                                          void* codes, float* scale, int64_t rows, int64_t cols, float eps, int x_dtype, void* stream) {
+  PTO_DISPATCH_LOCK();
+  return run("rms_norm_fp8_block", true, x, residual, gamma, sum_out, normed_out, codes, scale, rows, cols, eps, x_dtype,
+             (hipStream_t)stream);
+}
+
+extern "C" int pto_hip_quantize_fp8_block(const void* x, void* codes, float* scale, int64_t rows, int64_t cols, int x_dtype,
+                                          void* stream) {
+  PTO_DISPATCH_LOCK();
+  return run("quantize_fp8_block", false, x, nullptr, nullptr, nullptr, nullptr, codes, scale, rows, cols, 0.f, x_dtype,
+             (hipStream_t)stream);
+}

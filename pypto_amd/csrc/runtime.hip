@@ -115,6 +115,11 @@ enum ProgramKind {
   kPagedAttentionSpmd,
   kFfnGelu,
   kFfnRelu,
+  kRmsNormFp8Block,
+  kQuantizeFp8Block,
+  kProjectionFp8Block,
+  kRouteExperts,
+  kExpertsFfnFp8Block,
   kNumPrograms
 };
 
@@ -122,7 +127,8 @@ const char* const kProgramNames[kNumPrograms] = {
     "paged_attention", "paged_gather",  "rms_norm",           "ffn_swiglu",          "ffn_block",
     "w8a16_matmul",    "w8a16_swiglu",  "rope_kv_cache_update", "rope_kv_cache_update_fp8",
     "decoder_layer_decode", "projection", "gate_up_swiglu", "ffn_block_fp8", "llama_mini",
-    "paged_attention_batch", "paged_attention_dynamic", "paged_attention_spmd", "ffn_gelu", "ffn_relu"};
+    "paged_attention_batch", "paged_attention_dynamic", "paged_attention_spmd", "ffn_gelu", "ffn_relu",
+    "rms_norm_fp8_block", "quantize_fp8_block", "projection_fp8_block", "route_experts", "experts_ffn_fp8_block"};
 
 std::mutex g_mu;
 std::vector<int> g_callables;  // callable id -> ProgramKind, -1 once unregistered
@@ -483,6 +489,150 @@ int run_ffn_fp8(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hi
                                 scalar_f32(s[0]), (int)x.dtype, (int)out.dtype, stream);
 }
 
+// ---- e4m3 operands with a scale for each block of 128 ----
+// Codes [rows, cols] and one FP32 scale per 128 columns of a row.
+int check_codes(const char* prog, const char* name, const PtoHipChipTensor& codes, const PtoHipChipTensor& scale, int64_t rows, int64_t cols) {
+  PTO_CHECK_ARG(codes.dtype == PTO_HIP_FP8E4M3FN && codes.ndims == 2 && codes.shapes[0] == rows && codes.shapes[1] == cols,
+                "%s: %s must be FP8E4M3FN [%lld, %lld]", prog, name, (long long)rows, (long long)cols);
+  const int64_t groups = (cols + 127) / 128;
+  PTO_CHECK_ARG(scale.dtype == PTO_HIP_FP32 && scale.ndims == 2 && scale.shapes[0] == rows && scale.shapes[1] == groups,
+                "%s: the scales of %s must be FP32 [%lld, %lld], one per 128 columns of a row", prog, name, (long long)rows, (long long)groups);
+  return PTO_HIP_OK;
+}
+
+int check_each(const char* prog, const char* const* names, const PtoHipChipTensor* t, int nt) {
+  for (int i = 0; i < nt; ++i) {
+    // scales and small tensors are read element by element
+    const int rc = check_tensor(prog, names[i], t[i], 1, 3, t[i].dtype == PTO_HIP_FP32 ? 4 : 0);
+    if (rc) return rc;
+  }
+  return PTO_HIP_OK;
+}
+
+// x, [residual,] gamma, [sum_out,] [normed_out,] codes, scale + eps
+int run_rms_norm_fp8_block(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hipStream_t stream) {
+  const char* prog = "rms_norm_fp8_block";
+  PTO_CHECK_ARG(nt >= 4 && nt <= 7 && ns == 1,
+                "%s: expected x, gamma, [normed_out,] codes, scale or x, residual, gamma, sum_out, [normed_out,] codes, scale + 1 scalar (eps), "
+                "got %d + %d", prog, nt, ns);
+  const bool add = nt >= 6, normed = nt == 5 || nt == 7;
+  static const char* const plain[5] = {"x", "gamma", "normed_out", "codes", "scale"};
+  static const char* const added[7] = {"x", "residual", "gamma", "sum_out", "normed_out", "codes", "scale"};
+  const char* names[7];
+  for (int i = 0, from = 0; i < nt; ++i, ++from) {
+    if (!normed && from == (add ? 4 : 2)) ++from;
+    names[i] = add ? added[from] : plain[from];
+  }
+  const int rc = check_each(prog, names, t, nt);
+  if (rc) return rc;
+  const PtoHipChipTensor &x = t[0], &gamma = t[add ? 2 : 1], &codes = t[nt - 2], &scale = t[nt - 1];
+  PTO_CHECK_ARG(x.ndims == 2, "%s: x must be 2-D", prog);
+  const int64_t rows = x.shapes[0], cols = x.shapes[1];
+  PTO_CHECK_ARG(gamma.dtype == PTO_HIP_FP32 && numel(gamma) == cols, "%s: gamma must be FP32 with %lld elements", prog, (long long)cols);
+  for (int i = 0; i < nt - 2; ++i) {
+    if (&t[i] == &gamma) continue;
+    PTO_CHECK_ARG(t[i].dtype == x.dtype && t[i].ndims == 2 && t[i].shapes[0] == rows && t[i].shapes[1] == cols,
+                  "%s: %s must be %s [%lld, %lld] like x", prog, names[i], dtype_name(x.dtype), (long long)rows, (long long)cols);
+  }
+  const int rc2 = check_codes(prog, "codes", codes, scale, rows, cols);
+  if (rc2) return rc2;
+  return pto_hip_rms_norm_fp8_block(tptr(x), add ? tptr(t[1]) : nullptr, reinterpret_cast<const float*>(tptr(gamma)),
+                                    add ? tptr_mut(t[3]) : nullptr, normed ? tptr_mut(t[nt - 3]) : nullptr, tptr_mut(codes),
+                                    reinterpret_cast<float*>(tptr_mut(scale)), rows, cols, scalar_f32(s[0]), (int)x.dtype, stream);
+}
+
+int run_quantize_fp8_block(const PtoHipChipTensor* t, int nt, const uint64_t*, int ns, hipStream_t stream) {
+  const char* prog = "quantize_fp8_block";
+  PTO_CHECK_ARG(nt == 3 && ns == 0, "%s: expected x, codes, scale and no scalars, got %d + %d", prog, nt, ns);
+  static const char* const names[3] = {"x", "codes", "scale"};
+  int rc = check_each(prog, names, t, nt);
+  if (rc) return rc;
+  PTO_CHECK_ARG(t[0].ndims == 2, "%s: x must be 2-D", prog);
+  rc = check_codes(prog, "codes", t[1], t[2], t[0].shapes[0], t[0].shapes[1]);
+  if (rc) return rc;
+  return pto_hip_quantize_fp8_block(tptr(t[0]), tptr_mut(t[1]), reinterpret_cast<float*>(tptr_mut(t[2])), t[0].shapes[0], t[0].shapes[1],
+                                    (int)t[0].dtype, stream);
+}
+
+// a8, a_scale, w8, w_scale, out
+int run_projection_fp8_block(const PtoHipChipTensor* t, int nt, const uint64_t*, int ns, hipStream_t stream) {
+  const char* prog = "projection_fp8_block";
+  PTO_CHECK_ARG(nt == 5 && ns == 0, "%s: expected a8, a_scale, w8, w_scale, out and no scalars, got %d + %d", prog, nt, ns);
+  static const char* const names[5] = {"a8", "a_scale", "w8", "w_scale", "out"};
+  int rc = check_each(prog, names, t, nt);
+  if (rc) return rc;
+  PTO_CHECK_ARG(t[0].ndims == 2 && t[2].ndims == 2 && t[3].ndims == 2 && t[4].ndims == 2, "%s: codes, weight scales and out must be 2-D", prog);
+  const int64_t m = t[0].shapes[0], k = t[0].shapes[1], n = t[2].shapes[0];
+  rc = check_codes(prog, "a8", t[0], t[1], m, k);
+  if (rc) return rc;
+  PTO_CHECK_ARG(t[2].dtype == PTO_HIP_FP8E4M3FN && t[2].shapes[1] == k, "%s: w8 must be FP8E4M3FN [N, K=%lld]", prog, (long long)k);
+  PTO_CHECK_ARG(t[3].dtype == PTO_HIP_FP32 && t[3].shapes[0] == (n + 127) / 128 && t[3].shapes[1] == (k + 127) / 128,
+                "%s: w_scale must be FP32 [%lld, %lld], one per block of 128 x 128", prog, (long long)((n + 127) / 128),
+                (long long)((k + 127) / 128));
+  PTO_CHECK_ARG(t[4].shapes[0] == m && t[4].shapes[1] == n, "%s: out must be [M, N]", prog);
+  return pto_hip_projection_fp8_block(tptr(t[0]), reinterpret_cast<const float*>(tptr(t[1])), tptr(t[2]),
+                                      reinterpret_cast<const float*>(tptr(t[3])), tptr_mut(t[4]), m, k, n, (int)t[4].dtype, stream);
+}
+
+// logits, [bias,] expert_ids, expert_weights + n_groups, topk_groups, score function, renormalize, scale
+int run_route_experts(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hipStream_t stream) {
+  const char* prog = "route_experts";
+  PTO_CHECK_ARG((nt == 3 || nt == 4) && ns == 5,
+                "%s: expected logits, [bias,] expert_ids, expert_weights + 5 scalars (n_groups, topk_groups, score_fn, renormalize, scale), "
+                "got %d + %d", prog, nt, ns);
+  const bool biased = nt == 4;
+  static const char* const names[4] = {"logits", "bias", "expert_ids", "expert_weights"};
+  for (int i = 0; i < nt; ++i) {
+    const int rc = check_tensor(prog, names[biased || i == 0 ? i : i + 1], t[i], 1, 2, dtype_bytes(t[i].dtype) ? dtype_bytes(t[i].dtype) : 1);
+    if (rc) return rc;
+  }
+  const PtoHipChipTensor &logits = t[0], &ids = t[nt - 2], &weights = t[nt - 1];
+  PTO_CHECK_ARG(logits.ndims == 2 && ids.ndims == 2 && weights.ndims == 2, "%s: logits, expert_ids and expert_weights must be 2-D", prog);
+  const int64_t tokens = logits.shapes[0], experts = logits.shapes[1], top_k = ids.shapes[1];
+  PTO_CHECK_ARG(ids.dtype == PTO_HIP_INT32 && ids.shapes[0] == tokens, "%s: expert_ids must be INT32 [T=%lld, top_k]", prog, (long long)tokens);
+  PTO_CHECK_ARG(weights.dtype == PTO_HIP_FP32 && weights.shapes[0] == tokens && weights.shapes[1] == top_k,
+                "%s: expert_weights must be FP32 [T, top_k] like expert_ids", prog);
+  if (biased)
+    PTO_CHECK_ARG(t[1].dtype == PTO_HIP_FP32 && numel(t[1]) == experts, "%s: bias must be FP32 with %lld elements", prog, (long long)experts);
+  auto as_int = [](uint64_t v) { return v > 1u << 30 ? -1 : (int)v; };
+  return pto_hip_route_experts(tptr(logits), biased ? reinterpret_cast<const float*>(tptr(t[1])) : nullptr,
+                               reinterpret_cast<int32_t*>(tptr_mut(ids)), reinterpret_cast<float*>(tptr_mut(weights)), tokens, experts, top_k,
+                               (int64_t)s[0], (int64_t)s[1], as_int(s[2]), as_int(s[3]), scalar_f32(s[4]), (int)logits.dtype, stream);
+}
+
+// x8, x_scale, expert_ids, expert_weights, w_gate8, w_gate_scale, w_up8, w_up_scale, w_down8, w_down_scale, out
+int run_experts_ffn_fp8_block(const PtoHipChipTensor* t, int nt, const uint64_t*, int ns, hipStream_t stream) {
+  const char* prog = "experts_ffn_fp8_block";
+  PTO_CHECK_ARG(nt == 11 && ns == 0, "%s: expected 11 tensors and no scalars, got %d + %d", prog, nt, ns);
+  static const char* const names[11] = {"x8", "x_scale", "expert_ids", "expert_weights", "w_gate8", "w_gate_scale",
+                                        "w_up8", "w_up_scale", "w_down8", "w_down_scale", "out"};
+  int rc = check_each(prog, names, t, nt - 1);
+  if (!rc) rc = check_tensor(prog, names[10], t[10], 2, 2);
+  if (rc) return rc;
+  PTO_CHECK_ARG(t[0].ndims == 2 && t[2].ndims == 2 && t[3].ndims == 2 && t[4].ndims == 3 && t[10].ndims == 2,
+                "%s: x8, expert_ids, expert_weights and out must be 2-D, the weights 3-D", prog);
+  const int64_t tokens = t[0].shapes[0], hidden = t[0].shapes[1], top_k = t[2].shapes[1], experts = t[4].shapes[0], inter = t[4].shapes[1];
+  rc = check_codes(prog, "x8", t[0], t[1], tokens, hidden);
+  if (rc) return rc;
+  PTO_CHECK_ARG(t[2].dtype == PTO_HIP_INT32 && t[2].shapes[0] == tokens, "%s: expert_ids must be INT32 [T=%lld, top_k]", prog, (long long)tokens);
+  PTO_CHECK_ARG(t[3].dtype == PTO_HIP_FP32 && t[3].shapes[0] == tokens && t[3].shapes[1] == top_k,
+                "%s: expert_weights must be FP32 [T, top_k] like expert_ids", prog);
+  for (int i = 4; i < 10; i += 2) {
+    const int64_t n = i == 8 ? hidden : inter, k = i == 8 ? inter : hidden;
+    PTO_CHECK_ARG(t[i].dtype == PTO_HIP_FP8E4M3FN && t[i].ndims == 3 && t[i].shapes[0] == experts && t[i].shapes[1] == n && t[i].shapes[2] == k,
+                  "%s: %s must be FP8E4M3FN [E=%lld, %lld, %lld]", prog, names[i], (long long)experts, (long long)n, (long long)k);
+    PTO_CHECK_ARG(t[i + 1].dtype == PTO_HIP_FP32 && t[i + 1].ndims == 3 && t[i + 1].shapes[0] == experts &&
+                      t[i + 1].shapes[1] == (n + 127) / 128 && t[i + 1].shapes[2] == (k + 127) / 128,
+                  "%s: %s must be FP32 [E, %lld, %lld], one per block of 128 x 128", prog, names[i + 1], (long long)((n + 127) / 128),
+                  (long long)((k + 127) / 128));
+  }
+  PTO_CHECK_ARG(t[10].shapes[0] == tokens && t[10].shapes[1] == hidden, "%s: out must be [T, H]", prog);
+  auto f32 = [&](int i) { return reinterpret_cast<const float*>(tptr(t[i])); };
+  return pto_hip_experts_ffn_fp8_block(tptr(t[0]), f32(1), reinterpret_cast<const int32_t*>(tptr(t[2])), f32(3), tptr(t[4]), f32(5), tptr(t[6]),
+                                       f32(7), tptr(t[8]), f32(9), tptr_mut(t[10]), tokens, hidden, inter, experts, top_k,
+                                       (int)t[10].dtype, stream);
+}
+
 // hidden, causal_mask, cos_emb, sin_emb, wq, wk, wv, w_dense, w_gate, w_up, w_down, w_lm, logits
 // (the orchestration signature of examples/models/08_llama_mini.py:385-407), all fp32
 int run_llama_mini(const PtoHipChipTensor* t, int nt, const uint64_t*, int ns, hipStream_t stream) {
@@ -786,6 +936,11 @@ int dispatch(int kind, const PtoHipChipTensor* t, int nt, const uint64_t* s, int
     case kFfnBlockFp8: return run_ffn_fp8(t, nt, s, ns, stream);
     case kFfnGelu: return run_ffn_activation(t, nt, s, ns, stream, PTO_HIP_ACT_GELU);
     case kFfnRelu: return run_ffn_activation(t, nt, s, ns, stream, PTO_HIP_ACT_RELU);
+    case kRmsNormFp8Block: return run_rms_norm_fp8_block(t, nt, s, ns, stream);
+    case kQuantizeFp8Block: return run_quantize_fp8_block(t, nt, s, ns, stream);
+    case kProjectionFp8Block: return run_projection_fp8_block(t, nt, s, ns, stream);
+    case kRouteExperts: return run_route_experts(t, nt, s, ns, stream);
+    case kExpertsFfnFp8Block: return run_experts_ffn_fp8_block(t, nt, s, ns, stream);
     case kLlamaMini: return run_llama_mini(t, nt, s, ns, stream);
     case kW8a16Matmul: return run_w8a16_matmul(t, nt, s, ns, stream);
     case kProjection: return run_projection(t, nt, s, ns, stream);
@@ -955,9 +1110,9 @@ int pto_hip_sync(void* stream) {
   PTO_DISPATCH_LOCK();
   if (!ctx().initialized) return fail(PTO_HIP_ERR_NOT_INITIALIZED, "the library was closed during the wait");
   // Device-side argument errors of launches that do not block are reported here.
-  int flags[3] = {0, 0, 0};
+  int flags[4] = {0, 0, 0, 0};
   PTO_CHECK_HIP(hipMemcpy(flags, ctx().flags, sizeof(flags), hipMemcpyDeviceToHost));
-  if (flags[0] || flags[1] || flags[2]) {
+  if (flags[0] || flags[1] || flags[2] || flags[3]) {
     PTO_CHECK_HIP(hipMemset(ctx().flags, 0, sizeof(flags)));
     if (flags[0])
       return fail(PTO_HIP_ERR_INVALID_VALUE,
@@ -965,6 +1120,7 @@ int pto_hip_sync(void* stream) {
     if (flags[1])
       return fail(PTO_HIP_ERR_INVALID_VALUE,
                   "rope_kv_cache_update: a decode position lies outside the rope table, the block table or the cache");
+    if (flags[3]) return fail(PTO_HIP_ERR_INVALID_VALUE, "experts_ffn_fp8_block: an expert id names an expert that there is not");
     return fail(PTO_HIP_ERR_INVALID_VALUE,
                 "paged_attention: a block_table entry a sequence uses addresses a block outside the cache");
   }

@@ -83,6 +83,21 @@ ffn_block = HipProgram("ffn_block", (IN, IN, IN, IN, IN, OUT), scalars=("eps",))
 # the block on e4m3 operands: x, gamma, then (codes [out, in], scale [out]) for gate, up and down
 ffn_block_fp8 = HipProgram("ffn_block_fp8", (IN,) * 8 + (OUT,), scalars=("eps",))
 
+# e4m3 operands with a scale for each block of 128.  RMSNorm: x, gamma, [normed_out,] codes, scale ...
+rms_norm_fp8_block = HipProgram("rms_norm_fp8_block", (IN, IN, OUT, OUT), scalars=("eps",))
+rms_norm_fp8_block_normed = HipProgram("rms_norm_fp8_block", (IN, IN, OUT, OUT, OUT), scalars=("eps",))
+# ... and behind the residual's addition: x, residual, gamma, sum_out, [normed_out,] codes, scale
+add_rms_norm_fp8_block = HipProgram("rms_norm_fp8_block", (IN, IN, IN, OUT, OUT, OUT), scalars=("eps",))
+add_rms_norm_fp8_block_normed = HipProgram("rms_norm_fp8_block", (IN, IN, IN, OUT, OUT, OUT, OUT), scalars=("eps",))
+quantize_fp8_block = HipProgram("quantize_fp8_block", (IN, OUT, OUT))
+projection_fp8_block = HipProgram("projection_fp8_block", (IN, IN, IN, IN, OUT))
+# logits, [bias,] expert_ids, expert_weights
+route_experts = HipProgram("route_experts", (IN, OUT, OUT), scalars=("n_groups", "topk_groups", "score_fn", "renormalize", "scale"))
+route_experts_biased = HipProgram("route_experts", (IN, IN, OUT, OUT),
+                                  scalars=("n_groups", "topk_groups", "score_fn", "renormalize", "scale"))
+# x8, x_scale, expert_ids, expert_weights, then (codes [E, out, in], scales [E, out/128, in/128]) for gate, up and down
+experts_ffn_fp8_block = HipProgram("experts_ffn_fp8_block", (IN,) * 10 + (OUT,))
+
 # the reference's minimal single-head LLaMA forward: hidden, causal_mask, cos, sin, 7 x [D,D], w_lm, logits
 llama_mini = HipProgram("llama_mini", (IN,) * 12 + (OUT,))
 
@@ -116,7 +131,9 @@ decoder_layer_decode_w16_fp8kv = HipProgram(
     scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "eps"))
 
 PROGRAMS = {p.name: p for p in (paged_attention, paged_attention_batch, paged_attention_dynamic, paged_attention_spmd,
-                                paged_gather, rms_norm, ffn_swiglu, ffn_gelu, ffn_relu, ffn_block, ffn_block_fp8, llama_mini,
+                                paged_gather, rms_norm, ffn_swiglu, ffn_gelu, ffn_relu, ffn_block, ffn_block_fp8,
+                                rms_norm_fp8_block, quantize_fp8_block, projection_fp8_block, route_experts,
+                                experts_ffn_fp8_block, llama_mini,
                                 projection, gate_up_swiglu,
                                 w8a16_matmul,
                                 w8a16_swiglu, rope_kv_cache_update, rope_kv_cache_update_fp8,

@@ -1,0 +1,517 @@
+"""Block-scaled e4m3 operators on the GPU - norm and quantiser, product, router, experts - against the 64-bit oracle."""
+
+import pytest
+import torch
+
+from oracle import fp8_block as ob
+from pypto_amd import _lib, runtime
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}  # relative, of a rounding to the type
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}    # half a step among the smallest values
+GUARD = 256
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape):
+    return torch.randn(shape, device="cuda", generator=g)
+
+
+class _Fenced:
+    """A tensor with a fence of known bytes on either side of it, checked by intact()."""
+
+    def __init__(self, shape, dtype, fill=0x5B, inside=None):
+        n = torch.Size(shape).numel() * torch.empty(0, dtype=dtype).element_size()
+        self.buf = torch.full((2 * GUARD + (n + 15) // 16 * 16,), fill, dtype=torch.uint8, device="cuda")
+        self.n, self.fill = n, fill
+        self.t = self.buf[GUARD:GUARD + n].view(dtype).view(shape)
+        if inside is not None:
+            self.t.copy_(inside)
+
+    def intact(self):
+        return bool((self.buf[:GUARD] == self.fill).all() and (self.buf[GUARD + self.n:] == self.fill).all())
+
+
+def _codes_of(values):
+    """Codes between fences of NaN codes."""
+    return _Fenced(values.shape, F8, fill=0x7F, inside=values.to(F8)).t
+
+
+# ---- norm and quantiser --------------------------------------------------------------------------------
+
+NORM_SHAPES = [(1, 8), (3, 120), (2, 128), (5, 136), (7, 1000), (4, 2048), (3, 2056), (2, 4104), (33, 5120), (3, 8200), (2, 16384)]
+
+
+def _check_codes(codes, scale, n, slack):
+    """Codes and scales against the exact rows n: every value within half a step of its group's scale, `slack` relative aside."""
+    cols = n.shape[-1]
+    wide = scale.double().repeat_interleave(128, -1)[:, :cols]
+    _, want = ob.quantize_rows(n)
+    assert ((scale.double() - want).abs() <= want * (slack + 2.0 ** -23)).all()
+    got = codes.double() * wide
+    half = torch.maximum(n.abs() * 2.0 ** -4, wide * 2.0 ** -10)
+    assert ((got - n).abs() <= half * (1 + 2.0 ** -20) + slack * n.abs()).all()
+
+
+@pytest.mark.parametrize("rows,cols", NORM_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("normed", [False, True])
+def test_norm(worker, rows, cols, dtype, residual, normed):
+    """The sum's rounding is exact; the norm's fp32 evaluation is off by at most 2^-17: 64 squares in a row and 8 + log2(256) joins are 80
+    half-ulps of 2^-24, halved by the root, and half a dozen roundings behind it."""
+    g = _gen(rows * cols)
+    x, r = (_randn(g, rows, cols) * 3).to(dtype), (_randn(g, rows, cols) * torch.where(torch.rand(cols, device="cuda", generator=g) < 0.05, 30.0, 1.0)).to(dtype)
+    if rows > 1:
+        x[1], r[1] = 0, 0  # a row of zeros: every group's scale is 1
+    gamma = 1 + 0.2 * _randn(g, cols)
+    codes, scale = _Fenced((rows, cols), F8), _Fenced((rows, -(-cols // 128)), torch.float32)
+    sums, out = _Fenced((rows, cols), dtype), _Fenced((rows, cols), dtype)
+    program = {(0, 0): runtime.rms_norm_fp8_block, (0, 1): runtime.rms_norm_fp8_block_normed, (1, 0): runtime.add_rms_norm_fp8_block,
+               (1, 1): runtime.add_rms_norm_fp8_block_normed}[residual, normed]
+    worker.run(program, x, *((r,) if residual else ()), gamma, *((sums.t,) if residual else ()), *((out.t,) if normed else ()), codes.t, scale.t, 1e-6)
+    worker.sync()
+    s, n = ob.rms_norm(x, r if residual else None, gamma, 1e-6)
+    slack = 2.0 ** -17
+    _check_codes(codes.t, scale.t, n, slack)
+    if rows > 1:
+        assert (scale.t[1] == 1).all() and (codes.t[1].float() == 0).all()
+    if residual:
+        assert torch.equal(sums.t, (x.float() + r.float()).to(dtype))
+    if normed:
+        assert ((out.t.double() - n).abs() <= n.abs() * (HALF_STEP[dtype] + slack) + TINY[dtype]).all()
+    assert all(f.intact() for f in (codes, scale, sums, out))
+
+
+def test_norm_in_place_and_without_a_weight(worker):
+    """sum_out may be x or residual, normed_out x: the calls have the bits of the one with buffers of their own."""
+    lib, g = _lib.load(), _gen(5)
+    x, r = _randn(g, 9, 4104).bfloat16(), _randn(g, 9, 4104).bfloat16()
+
+    def call(x, r, s, n):
+        codes, scale = torch.zeros((9, 4104), dtype=torch.uint8, device="cuda"), torch.zeros((9, 33), device="cuda")
+        _lib.check(lib.pto_hip_rms_norm_fp8_block(x.data_ptr(), r.data_ptr(), None, s.data_ptr(), n.data_ptr(), codes.data_ptr(), scale.data_ptr(),
+                                                  9, 4104, 1e-5, 0x40, None))
+        worker.sync()
+        return s.clone(), n.clone(), codes, scale
+
+    want = call(x, r, torch.empty_like(x), torch.empty_like(x))
+    _check_codes(want[2].view(F8), want[3], ob.rms_norm(x, r, None, 1e-5)[1], 2.0 ** -17)
+    for which in ("x", "r"):
+        a, b = x.clone(), r.clone()
+        got = call(a, b, a if which == "x" else b, b if which == "x" else a)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert lib.pto_hip_rms_norm_fp8_block(x.data_ptr(), r.data_ptr(), None, x.data_ptr(), x.data_ptr(), want[2].data_ptr(), want[3].data_ptr(), 9,
+                                          4104, 1e-5, 0x40, None) == _lib.ERR_INVALID_VALUE
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,cols", [(1, 8), (5, 200), (3, 4096), (2, 16384)])
+def test_quantiser_is_exact(worker, dtype, rows, cols):
+    """Without a norm nothing is computed but the scale's division and the quotients: the codes are the oracle's to the bit."""
+    g = _gen(cols)
+    x = (_randn(g, rows, cols) * torch.exp2(torch.randint(-14, 8, (rows, 1), device="cuda", generator=g).float())).to(dtype)
+    x[0, :8] = 0
+    codes, scale = _Fenced((rows, cols), F8), _Fenced((rows, -(-cols // 128)), torch.float32)
+    worker.run(runtime.quantize_fp8_block, x, codes.t, scale.t)
+    worker.sync()
+    # on the CPU: torch multiplies by 1 / 448 on the GPU, which is not the division
+    x = x.cpu().float()
+    amax = torch.nn.functional.pad(x, (0, -cols % 128)).unflatten(-1, (-1, 128)).abs().amax(-1)
+    want = torch.where(amax > 0, (amax / 448).clamp(min=2.0 ** -126), 1.0)
+    assert torch.equal(scale.t.cpu(), want)
+    wide = want.repeat_interleave(128, -1)[:, :cols]
+    assert torch.equal(codes.t.cpu().view(torch.uint8), (x / wide).to(F8).view(torch.uint8))
+    assert codes.intact() and scale.intact()
+
+
+def test_quantiser_on_infinities_nan_and_the_smallest_values(worker):
+    x = torch.zeros((6, 256), dtype=torch.bfloat16, device="cuda")
+    x[0, 3], x[0, 200] = float("inf"), 5.0
+    x[1, 7], x[1, 8] = float("nan"), 2.0
+    x[2, 0], x[2, 1] = 2.0 ** -133, -2.0 ** -130  # subnormal: the scale stays a normal number
+    x[3, 0] = -0.0
+    x[4, 5], x[4, 6] = 3e38, 1e30
+    x[5, 100] = -float("inf")
+    codes, scale = torch.zeros((6, 256), dtype=F8, device="cuda"), torch.zeros((6, 2), device="cuda")
+    worker.run(runtime.quantize_fp8_block, x, codes, scale)
+    worker.sync()
+    c, s = codes.float().cpu(), scale.cpu()
+    assert s[0, 0] == float("inf") and c[0, 3].isnan() and (c[0, 4:128] == 0).all() and c[0, 200] == 448
+    assert c[1, 7].isnan() and c[1, 8] == 448 and s[1, 0] == torch.tensor(2.0) / 448
+    assert s[2, 0] == 2.0 ** -126 and c[2, 0] == 2.0 ** -7 and c[2, 1] == -2.0 ** -4
+    assert codes.view(torch.uint8)[3, 0].item() == 0x80 and s[3, 0] == 1
+    assert c[4, 5] == 448 and c[4, 6] == 0
+    assert c[5, 100].isnan() and s[5, 1] == 1
+
+
+# ---- product -------------------------------------------------------------------------------------------
+
+# rows and channels at, below and above every tile's; one block of k to many, with and without an odd one behind
+PRODUCT_SHAPES = [(1, 128, 1), (1, 4096, 130), (3, 256, 5), (15, 384, 100), (16, 512, 128), (17, 640, 129), (33, 1024, 257), (64, 1152, 384), (65, 2816, 100),
+                  (127, 896, 511), (128, 128, 256), (130, 4224, 48), (255, 1664, 260), (257, 512, 1003), (300, 2048, 640), (513, 768, 321)]
+
+
+def _product(worker, a, sa, w, sw, dtype):
+    out = _Fenced((a.shape[0], w.shape[0]), dtype)
+    worker.run(runtime.projection_fp8_block, a, sa, w, sw, out.t)
+    worker.sync()
+    assert out.intact()
+    return out.t
+
+
+@pytest.mark.parametrize("m,k,n", PRODUCT_SHAPES)
+def test_product_is_exact_on_whole_numbers_and_stays_inside(worker, m, k, n):
+    """Whole numbers up to 8 and scales of 2^-8 and 2^-7: every sum is a multiple of 2^-16 below 64 * 4224 * 2^-14, which
+    fp32 holds exactly in any order.  Past the operands' ends lie NaN codes."""
+    g = torch.Generator().manual_seed(m + k + n)
+    num = lambda rows: torch.randint(-8, 9, (rows, k), generator=g).float()
+    scale = lambda rows: torch.exp2(-7.0 - torch.randint(0, 2, (rows, k // 128), generator=g).float())
+    a, w, sa, sw = num(m), num(n), scale(m), scale(-(-n // 128))
+    want = ob.projection(a.cuda(), sa.cuda(), w.cuda(), sw.cuda())
+    fenced = lambda t: _Fenced(t.shape, torch.float32, fill=0xFF, inside=t).t  # all ones: a NaN
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = _product(worker, _codes_of(a), fenced(sa), _codes_of(w), fenced(sw), dtype)
+        assert torch.equal(got, want.float().to(dtype)), dtype
+
+
+def _operands(g, m, k, n):
+    a, sa = ob.quantize_rows(_randn(g, m, k))
+    w, sw = ob.quantize_matrix(_randn(g, n, k) * k ** -0.5)
+    return a.to(F8), sa.float(), w, sw
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 515), (24, 2816, 96), (130, 4096, 256), (300, 11008, 300), (600, 1024, 900)])
+def test_product_on_quantised_values(worker, m, k, n, dtype):
+    """fp32 sums of k products in any order: at most (128 + k / 128 + 4) roundings in a row, each of the sum of magnitudes."""
+    a, sa, w, sw = _operands(_gen(k + n), m, k, n)
+    got = _product(worker, a, sa, w, sw, dtype).double()
+    want = ob.projection(a, sa, w, sw)
+    sizes = ob.dequantize_rows(a, sa).abs() @ ob.dequantize_matrix(w, sw).abs().t()
+    bound = sizes * (132 + k // 128) * 2.0 ** -24
+    assert ((got - want).abs() <= bound + (want.abs() + bound) * HALF_STEP[dtype] + TINY[dtype]).all()
+
+
+def test_product_rows_do_not_depend_on_their_batch(worker):
+    """A row's scales and codes are its own: NaN in one row stays in that row."""
+    a, sa, w, sw = _operands(_gen(9), 70, 1024, 260)
+    want = _product(worker, a, sa, w, sw, torch.float32)
+    bad = a.clone()
+    bad.view(torch.uint8)[33, 5] = 0x7F
+    got = _product(worker, bad, sa, w, sw, torch.float32)
+    assert got[33].isnan().all()
+    keep = torch.arange(70, device="cuda") != 33
+    assert torch.equal(got[keep], want[keep])
+
+
+def test_product_refusals(worker):
+    a, sa, w, sw = _operands(_gen(1), 4, 256, 200)
+    out = torch.zeros((4, 200), dtype=torch.bfloat16, device="cuda")
+    run = lambda *args: worker.run(runtime.projection_fp8_block, *args)
+    with pytest.raises(ValueError, match="a8 must be FP8E4M3FN"):
+        run(a.float(), sa, w, sw, out)
+    with pytest.raises(ValueError, match=r"scales of a8 must be FP32 \[4, 2\]"):
+        run(a, sa[:, :1].contiguous(), w, sw, out)
+    with pytest.raises(ValueError, match="w8 must be"):
+        run(a, sa, w[:, :128].contiguous(), sw, out)
+    with pytest.raises(ValueError, match=r"w_scale must be FP32 \[2, 2\]"):
+        run(a, sa, w, sw[:1].contiguous(), out)
+    with pytest.raises(ValueError, match=r"out must be \[M, N\]"):
+        run(a, sa, w, sw, out[:, :100].contiguous())
+    with pytest.raises(ValueError, match="contiguous"):
+        run(a, sa, w, sw, out.t())
+    with pytest.raises(ValueError, match="multiple of 16"):
+        run(torch.zeros(4 * 256 + 8, dtype=torch.uint8, device="cuda")[8:].view(F8).view(4, 256), sa, w, sw, out)
+    run(a[:0], sa[:0], w, sw, out[:0])  # no rows: nothing happens
+    worker.sync()
+
+
+# ---- router --------------------------------------------------------------------------------------------
+
+
+def _route(worker, logits, bias, top_k, n_groups=1, topk_groups=1, sigmoid=False, renormalize=True, scale=1.0):
+    t = logits.shape[0]
+    ids, weights = _Fenced((t, top_k), torch.int32), _Fenced((t, top_k), torch.float32)
+    worker.run(runtime.route_experts if bias is None else runtime.route_experts_biased, logits, *(() if bias is None else (bias,)), ids.t,
+               weights.t, n_groups, topk_groups, int(sigmoid), int(renormalize), scale)
+    worker.sync()
+    assert ids.intact() and weights.intact()
+    return ids.t, weights.t
+
+
+def _check_route(worker, logits, bias, *args, **kw):
+    ids, weights = _route(worker, logits, bias, *args, **kw)
+    want, w = ob.route(logits.cpu(), None if bias is None else bias.cpu(), *args, **kw)
+    assert torch.equal(ids.cpu(), want)
+    # one rounding at the end and, in 32 bits, a few of an exponential and a sum of up to 1024
+    assert ((weights.cpu().double() - w).abs() <= w.abs() * 2.0 ** -20 + 2.0 ** -140).all()
+
+
+@pytest.mark.parametrize("experts,top_k,groups,kept", [(1, 1, 1, 1), (8, 2, 1, 1), (60, 4, 1, 1), (64, 6, 8, 3), (65, 65 - 1, 1, 1), (128, 8, 4, 4), (160, 6, 8, 3),
+                                                       (256, 8, 8, 4), (320, 10, 64, 7), (512, 8, 16, 2), (1000, 3, 50, 20), (1024, 64, 64, 64)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+def test_router(worker, experts, top_k, groups, kept, sigmoid, biased):
+    g = _gen(experts + top_k)
+    bias = 0.1 * _randn(g, experts) if biased else None
+    for tokens, dtype in ((1, torch.float32), (37, torch.float32), (30, torch.bfloat16), (9, torch.float16)):
+        logits = (_randn(g, tokens, experts) * 2).to(dtype)
+        _check_route(worker, logits, bias, top_k, groups, kept, sigmoid=sigmoid, renormalize=tokens != 9, scale=2.5)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+def test_router_ties_go_to_the_lowest_index(worker, sigmoid, biased):
+    """Few distinct logits, so that most choices are ties; with a bias of zeros as well as without."""
+    g = _gen(3)
+    for experts, groups, kept in ((64, 1, 1), (256, 8, 3), (130, 5, 2)):
+        logits = torch.randint(-2, 3, (25, experts), device="cuda", generator=g).float()
+        _check_route(worker, logits, torch.zeros(experts, device="cuda") if biased else None, 7, groups, kept, sigmoid=sigmoid)
+        _check_route(worker, torch.zeros_like(logits), torch.zeros(experts, device="cuda") if biased else None, 7, groups, kept, sigmoid=sigmoid)
+
+
+def test_router_keys_that_differ_past_32_bits(worker):
+    """Two experts whose keys differ by less than an ulp of 32 bits, either way round."""
+    logits = torch.full((2, 96), -4.0, device="cuda")
+    logits[:, 10], logits[:, 70] = 0.0, 0.0
+    bias = torch.zeros(96, device="cuda")
+    bias[10], bias[70] = 1.0, 1.0
+    logits[0, 70], logits[1, 10] = 1e-9, 1e-9
+    ids, _ = _route(worker, logits, bias, 2, sigmoid=True)
+    assert ids.tolist() == [[70, 10], [10, 70]]
+    _check_route(worker, logits, bias, 2, sigmoid=True)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (4, 2)])
+def test_router_on_rows_that_leave_little(worker, sigmoid, biased, groups, kept):
+    inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
+    logits = _randn(_gen(4), 9, 72)
+    logits[0] = -inf
+    logits[1] = low
+    logits[2, 3:] = -inf
+    logits[3, ::2] = nan
+    logits[4] = nan
+    logits[5, 5] = inf
+    logits[6, 5], logits[6, 60], logits[6, 61] = inf, inf, nan
+    logits[7] = inf
+    logits[8, :70] = low
+    bias = None
+    if biased:
+        bias = 0.1 * _randn(_gen(5), 72)
+        bias[2], bias[40] = -inf, nan
+    _check_route(worker, logits, bias, 5, groups, kept, sigmoid=sigmoid)
+
+
+def test_router_refusals(worker):
+    logits = torch.zeros((4, 64), device="cuda")
+    ids, w = torch.zeros((4, 6), dtype=torch.int32, device="cuda"), torch.zeros((4, 6), device="cuda")
+    run = lambda *a: worker.run(runtime.route_experts, *a)
+    with pytest.raises(ValueError, match="logits dtype INT32"):
+        run(logits.int(), ids, w, 1, 1, 0, 1, 1.0)
+    with pytest.raises(ValueError, match="expert_ids must be INT32"):
+        run(logits, ids.long(), w, 1, 1, 0, 1, 1.0)
+    with pytest.raises(ValueError, match="expert_weights must be FP32"):
+        run(logits, ids, w[:, :5].contiguous(), 1, 1, 0, 1, 1.0)
+    with pytest.raises(ValueError, match="bias must be FP32 with 64"):
+        worker.run(runtime.route_experts_biased, logits, torch.zeros(63, device="cuda"), ids, w, 1, 1, 0, 1, 1.0)
+    with pytest.raises(ValueError, match="neither softmax"):
+        run(logits, ids, w, 1, 1, -1, 1, 1.0)
+    with pytest.raises(ValueError, match="do not divide"):
+        run(logits, ids, w, 5, 1, 0, 1, 1.0)
+    run(logits[:0], ids[:0], w[:0], 1, 1, 0, 1, 1.0)
+    worker.sync()
+
+
+# ---- experts -------------------------------------------------------------------------------------------
+
+
+def _experts_case(seed, tokens, hidden, inter, experts, top_k):
+    g = _gen(seed)
+    x, xs = ob.quantize_rows(_randn(g, tokens, hidden))
+    ids = torch.rand((tokens, experts), device="cuda", generator=g).argsort(-1)[:, :top_k]
+    if ids.shape[1] < top_k:
+        ids = torch.randint(0, experts, (tokens, top_k), device="cuda", generator=g)
+    w = torch.rand((tokens, top_k), device="cuda", generator=g) + 0.1
+    mats = []
+    for n, k in ((inter, hidden), (inter, hidden), (hidden, inter)):
+        mats += list(ob.quantize_matrix(_randn(g, experts, n, k) * (2.0 * k ** -0.5)))
+    return [x.to(F8), xs.float(), ids.int().contiguous(), w] + mats
+
+
+def _check_experts(worker, args, dtype):
+    out = _Fenced(args[0].shape, dtype)
+    worker.run(runtime.experts_ffn_fp8_block, *args, out.t)
+    worker.sync()
+    want, slack = ob.experts_ffn(*args)
+    # slack: codes of h next to a border, and fp32 sums on both sides of the codes
+    bad = ((out.t.double() - want).abs() > slack * (1 + HALF_STEP[dtype]) + want.abs() * HALF_STEP[dtype] + TINY[dtype]).sum().item()
+    assert bad == 0 and out.intact(), bad
+    return out.t
+
+
+EXPERT_SHAPES = [(1, 256, 128, 4, 2), (1, 1024, 1408, 16, 8), (2, 128, 256, 8, 1), (3, 512, 384, 8, 8), (7, 640, 256, 60, 4), (16, 256, 128, 1, 1), (40, 512, 512, 60, 4),
+                 (33, 384, 128, 2, 2), (100, 1024, 256, 16, 2), (130, 256, 640, 8, 3), (300, 512, 256, 8, 2), (515, 1152, 384, 4, 2), (700, 256, 256, 64, 8)]
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", EXPERT_SHAPES)
+def test_experts(worker, tokens, hidden, inter, experts, top_k):
+    args = _experts_case(tokens + hidden, tokens, hidden, inter, experts, top_k)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        _check_experts(worker, args, dtype)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 90, 600])
+def test_experts_on_uneven_routes(worker, tokens):
+    """Slots without an expert, tokens without any, one expert for all, the same expert twice in a row."""
+    args = _experts_case(tokens, tokens, 384, 256, 12, 4)
+    ids = args[2]
+    ids[::3, 1] = -1
+    ids[::2, 3] = -(2 ** 31)
+    ids[-1] = -1
+    out = _check_experts(worker, args, torch.bfloat16)
+    assert (out[-1] == 0).all()
+    ids[:] = 7
+    _check_experts(worker, args, torch.bfloat16)
+    ids[:] = -1
+    assert (_check_experts(worker, args, torch.float32) == 0).all()
+
+
+def test_an_expert_that_there_is_not_is_left_out_and_reported(worker):
+    args = _experts_case(2, 6, 256, 128, 4, 2)
+    args[2][3, 0] = 4
+    args[2][5, 1] = 2 ** 31 - 1
+    out = torch.empty((6, 256), dtype=torch.float32, device="cuda")
+    worker.run(runtime.experts_ffn_fp8_block, *args, out)
+    with pytest.raises(ValueError, match="an expert that there is not"):
+        worker.sync()
+    worker.sync()  # reported once
+    want, slack = ob.experts_ffn(*args)
+    assert ((out.double() - want).abs() <= slack + want.abs() * 2.0 ** -24).all()
+
+
+def test_a_token_s_result_does_not_depend_on_its_batch(worker):
+    """NaN and infinities of one token, and weights that nobody asked for, reach no other token."""
+    args = _experts_case(8, 50, 512, 256, 16, 3)
+    args[2].clamp_(max=14)
+    want = _check_experts(worker, args, torch.float32)
+    for i in (4, 6, 8):
+        args[i].view(torch.uint8)[15] = 0x7F
+    x = args[0].clone()
+    x.view(torch.uint8)[20] = 0x7F
+    args[1][20] = float("inf")
+    out = torch.empty_like(want)
+    worker.run(runtime.experts_ffn_fp8_block, x, *args[1:], out)
+    worker.sync()
+    keep = torch.arange(50, device="cuda") != 20
+    assert out[20].isnan().all() and torch.equal(out[keep], want[keep])
+
+
+def test_experts_refusals(worker):
+    args = _experts_case(3, 4, 256, 128, 4, 2)
+    out = torch.zeros((4, 256), dtype=torch.bfloat16, device="cuda")
+
+    def run(i, t, out=out):
+        worker.run(runtime.experts_ffn_fp8_block, *args[:i], t, *args[i + 1:], out)
+
+    with pytest.raises(ValueError, match="x8 must be FP8E4M3FN"):
+        run(0, args[0].float())
+    with pytest.raises(ValueError, match="scales of x8"):
+        run(1, args[1][:, :1].contiguous())
+    with pytest.raises(ValueError, match="expert_ids must be INT32"):
+        run(2, args[2].long())
+    with pytest.raises(ValueError, match="expert_weights must be FP32"):
+        run(3, args[3].bfloat16())
+    with pytest.raises(ValueError, match="w_up8 must be"):
+        run(6, args[6][:3].contiguous())
+    with pytest.raises(ValueError, match="w_down_scale must be FP32"):
+        run(9, args[9][:, :1].contiguous())
+    with pytest.raises(ValueError, match=r"out must be \[T, H\]"):
+        run(0, args[0], out[:2])
+    worker.run(runtime.experts_ffn_fp8_block, args[0][:0], args[1][:0], args[2][:0], args[3][:0], *args[4:], out[:0])
+    worker.sync()
+
+
+# ---- together ------------------------------------------------------------------------------------------
+
+
+class _Layer:
+    """The feed-forward half of a mixture layer as a serving loop calls it, on buffers of its own."""
+
+    def __init__(self, worker, tokens, hidden, inter, experts, top_k, seed):
+        g = _gen(seed)
+        self.w = worker
+        self.h = {p: worker.register(getattr(runtime, p)) for p in ("add_rms_norm_fp8_block_normed", "projection", "route_experts_biased", "experts_ffn_fp8_block")}
+        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device="cuda")
+        self.x, self.res = _randn(g, tokens, hidden).bfloat16(), (2 * _randn(g, tokens, hidden)).bfloat16()
+        self.gamma, self.router = 1 + 0.1 * _randn(g, hidden), (_randn(g, hidden, experts) * hidden ** -0.5).bfloat16()
+        self.bias = 0.1 * _randn(g, experts)
+        self.mats = _experts_case(seed, 1, hidden, inter, experts, 1)[4:]
+        self.sum, self.normed, self.out = new((tokens, hidden), torch.bfloat16), new((tokens, hidden), torch.bfloat16), new((tokens, hidden), torch.bfloat16)
+        self.codes, self.scale = new((tokens, hidden), F8), new((tokens, hidden // 128), torch.float32)
+        self.logits, self.ids, self.weights = new((tokens, experts), torch.float32), new((tokens, top_k), torch.int32), new((tokens, top_k), torch.float32)
+        self.top_k = top_k
+
+    def step(self, stream=0):
+        call = lambda p, *a: self.h[p](*a, stream=stream)
+        call("add_rms_norm_fp8_block_normed", self.x, self.res, self.gamma, self.sum, self.normed, self.codes, self.scale, 1e-6)
+        call("projection", self.normed, self.router, self.logits)
+        call("route_experts_biased", self.logits, self.bias, self.ids, self.weights, 4, 2, 1, 1, 2.0)
+        call("experts_ffn_fp8_block", self.codes, self.scale, self.ids, self.weights, *self.mats, self.out)
+
+    def check(self):
+        s, n = ob.rms_norm(self.x, self.res, self.gamma, 1e-6)
+        _check_codes(self.codes, self.scale, n, 2.0 ** -17)
+        want, w = ob.route(self.logits.cpu(), self.bias.cpu(), self.top_k, 4, 2, sigmoid=True, scale=2.0)
+        assert torch.equal(self.ids.cpu(), want) and torch.allclose(self.weights.cpu().double(), w, rtol=2.0 ** -20, atol=0)
+        logits = self.normed.double() @ self.router.double()
+        sizes = self.normed.double().abs() @ self.router.double().abs()
+        assert ((self.logits.double() - logits).abs() <= sizes * self.x.shape[1] * 2.0 ** -24).all()
+        out, slack = ob.experts_ffn(self.codes, self.scale, self.ids, self.weights, *self.mats)
+        assert ((self.out.double() - out).abs() <= slack * (1 + 2.0 ** -8) + out.abs() * 2.0 ** -8 + 2.0 ** -134).all()
+
+    def results(self):
+        return [t.clone() for t in (self.sum, self.normed, self.codes.view(torch.uint8), self.scale, self.logits, self.ids, self.weights, self.out)]
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 50, 400])
+def test_the_operators_of_a_layer_together(worker, tokens):
+    layer = _Layer(worker, tokens, 512, 256, 16, 4, seed=tokens)
+    layer.step()
+    worker.sync()
+    layer.check()
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 50, 400])
+def test_a_captured_layer_on_another_stream(worker, tokens):
+    """Recorded once, replayed with other inputs and with eager calls of another size between the replays; every replay has the
+    bits of an eager call on its inputs."""
+    layer, other = _Layer(worker, tokens, 512, 256, 16, 4, seed=tokens), _Layer(worker, 7, 512, 256, 16, 4, seed=99)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        layer.step(stream.cuda_stream)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        layer.step(torch.cuda.current_stream().cuda_stream)
+    for i in range(4):
+        layer.x.copy_(_randn(_gen(i), *layer.x.shape))
+        torch.cuda.synchronize()
+        layer.step()
+        worker.sync()
+        want = layer.results()
+        for t in (layer.sum, layer.normed, layer.scale, layer.logits, layer.weights, layer.out):
+            t.fill_(float("nan"))
+        layer.ids.fill_(-1)
+        other.step()
+        worker.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(layer.results(), want)), i
+    worker.sync()
