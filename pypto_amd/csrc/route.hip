@@ -4,12 +4,14 @@
 //   group key = the sum of its two best keys with a bias, its best key without; the topk_groups best groups stay
 //   ids = the top_k experts of those groups by key    weight = score [/ the chosen ones' sum] * scale
 //
-// Ties go to the lowest index.  Keys with a bias are compared in 64 bits: two experts' scores differ by less than an ulp of 32 bits
-// often enough to matter among thousands of tokens times hundreds of experts.  Without one the order of the scores is the order of
-// the logits, which are compared as they are.  NaN counts as -inf; equal infinities share a softmax's mass evenly.
+// Ties go to the lowest index.  Without a bias the order of the scores is the order of the logits, which are compared as they are.
+// With one, the order is that of the 64-bit keys: two experts' scores differ by less than an ulp of 32 bits often enough to matter
+// among thousands of tokens times hundreds of experts.  The choice is made on 32-bit keys all the same, and made again on 64-bit
+// ones where two keys next to each other in it, or the last group or expert chosen and the first that is not, are nearer than the
+// 32-bit keys' error: about one token in a hundred.  NaN counts as -inf; equal infinities share a softmax's mass evenly.
 //
 // One wavefront per token, expert e in lane e % 64.  Keys are mapped to unsigned integers of the same order, so that the
-// best of a wavefront is a maximum of their upper halves by six lane exchanges, and of the lower halves only among equals.
+// best of a wavefront is an integer maximum.  Bound by the chain of top_k maxima (six lane exchanges each), not by memory.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -25,11 +27,12 @@ struct Params {
   int32_t* ids;
   float* weights;
   int tokens, experts, top_k, groups, kept, group_size;
+  int group_lanes;  // lanes that look through a group together: the largest power of two that lets all groups be looked through at once
   bool sigmoid, renormalize;
   float scale;
 };
 
-// Unsigned integers in the order of the values.
+// Unsigned integers in the order of the values, and back.  No value maps to 0: a key that is taken, left out, or not there.
 __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v == 0.f ? 0.f : v);  // -0 and 0 are equal
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -38,125 +41,277 @@ __device__ __forceinline__ uint64_t ordered(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v == 0.0 ? 0.0 : v);
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-// ... and what no value maps to, below all of them: taken, left out, or not there
-constexpr uint64_t kNone = 0;
+__device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_with(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xf, false));
+}
+// The largest of a wavefront's values (wave-uniform): along rows of 16 lanes, then from row to row; lane 63 has seen all.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off));
-  return v;
+  v = max_with<0x111, 0xf>(v);
+  v = max_with<0x112, 0xf>(v);
+  v = max_with<0x114, 0xf>(v);
+  v = max_with<0x118, 0xf>(v);
+  v = max_with<0x142, 0xa>(v);
+  v = max_with<0x143, 0xc>(v);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
-  return v;
+// The sum of a wavefront's values (wave-uniform), over the same lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_from(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_from(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, true);
+  return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float of_lane(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+__device__ __forceinline__ double of_lane(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <typename V>
+__device__ __forceinline__ V wave_sum(V v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  v = add_from<0x143, 0xc>(v);
+  return of_lane(v, 63);
 }
 
-template <typename T, int J, bool BIAS>
-__global__ __launch_bounds__(kWaves * 64) void route_kernel(Params p) {
-  __shared__ double keys[kWaves][J * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int token = blockIdx.x * kWaves + wave;
-  const bool live = token < p.tokens;  // every wavefront reaches the barriers
-  const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)(live ? token : 0) * p.experts;
-  float logit[J];
-  float top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int e = lane + 64 * j;
-    const float v = e < p.experts ? (float)row[e] : -INFINITY;
-    logit[j] = v == v ? v : -INFINITY;
-    top = fmaxf(top, logit[j]);
+// The lane with the best key of a wavefront, ties to the lowest expert; `top` is that key.
+__device__ __forceinline__ int best_lane(uint32_t key, int expert, uint32_t* top) {
+  *top = wave_max(key);
+  uint64_t equal = __ballot(key == *top);
+  if (__builtin_expect((equal & (equal - 1)) != 0, 0)) {
+    const uint32_t lowest = wave_max(key == *top ? ~(uint32_t)expert : 0u);  // all lanes take part
+    equal = __ballot(~(uint32_t)expert == lowest);
   }
-  double score[J];
-  if (p.sigmoid) {
+  return __builtin_ctzll(equal);
+}
+__device__ __forceinline__ int best_lane(uint64_t key, int expert, uint64_t* top) {
+  const uint32_t hi = wave_max((uint32_t)(key >> 32));
+  const bool first = (uint32_t)(key >> 32) == hi;
+  const uint32_t lo = wave_max(first ? (uint32_t)key : 0u);
+  const bool equal = first && (uint32_t)key == lo;
+  *top = (uint64_t)hi << 32 | lo;
+  uint64_t lanes = __ballot(equal);
+  if (__builtin_expect((lanes & (lanes - 1)) != 0, 0)) {
+    const uint32_t lowest = wave_max(equal ? ~(uint32_t)expert : 0u);
+    lanes = __ballot(~(uint32_t)expert == lowest);
+  }
+  return __builtin_ctzll(lanes);
+}
+
+// How far apart two 32-bit keys have to be for their order to be the 64-bit keys'.  A sigmoid's exponential is off by (|v| + 2) 2^-24 of itself,
+// which moves the score by at most 2^-23, as do sum and quotient: 2^-21 together with room.  A softmax's sum of up to 16 + 6 steps is off by
+// 2^-19 of itself.  The sum with the bias adds 2^-24 of its size.  Both keys are off; a group's key is the sum of two.
+__device__ __forceinline__ float margin(float key, bool sigmoid) { return (sigmoid ? 0x1p-20f : 0x1p-17f) + 0x1p-21f * fabsf(key); }
+
+template <typename V>
+struct KeyOf {
+  typedef uint32_t type;
+};
+template <>
+struct KeyOf<double> {
+  typedef uint64_t type;
+};
+
+__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+__device__ __forceinline__ float over(float a, float b) { return a * __builtin_amdgcn_rcpf(b); }  // b in [1, 1024] or so
+__device__ __forceinline__ double over(double a, double b) { return a / b; }
+
+// The keys' exponential: off by (|v| + 2) 2^-24 of itself in 32 bits, where exp_of is off by an ulp.
+__device__ __forceinline__ float key_exp(float v) { return __expf(v); }
+__device__ __forceinline__ double key_exp(double v) { return exp(v); }
+
+template <typename V>
+__device__ __forceinline__ V sigmoid_key(V v) {
+  const V e = key_exp(v >= V(0) ? -v : v);
+  return over(v >= V(0) ? V(1) : e, V(1) + e);
+}
+template <typename V>
+__device__ __forceinline__ V sigmoid_of(V v) {
+  const V e = exp_of(v >= V(0) ? -v : v);
+  return over(v >= V(0) ? V(1) : e, V(1) + e);
+}
+
+// The choice on keys of type V: lane i < top_k gets the i-th expert.  False: made on 32-bit keys that are too near to each other.
+// top: the largest logit (softmax).  values: a row of LDS for the wavefront.
+template <typename V, int J, bool BIAS>
+__device__ __forceinline__ bool choose(const Params& p, const float (&logit)[J], const float (&bias)[J], float top, int lane, V* values, int* mine) {
+  typedef typename KeyOf<V>::type Key;
+  constexpr bool kNear = BIAS && sizeof(V) == 4;
+  V value[J];
+  if constexpr (BIAS) {
+    if (p.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) score[j] = 1.0 / (1.0 + exp(-(double)logit[j]));
-  } else {
-    top = wave_max(top);
-    double sum = 0.0;
+      for (int j = 0; j < J; ++j) value[j] = sigmoid_key((V)logit[j]);
+    } else {
+      V sum = 0;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        value[j] = lane + 64 * j >= p.experts ? V(0) : logit[j] == top ? V(1) : key_exp((V)logit[j] - (V)top);
+        sum += value[j];
+      }
+      sum = wave_sum(sum);
+#pragma unroll
+      for (int j = 0; j < J; ++j) value[j] = over(value[j], sum);
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      score[j] = lane + 64 * j >= p.experts ? 0.0 : logit[j] == top ? 1.0 : exp((double)logit[j] - (double)top);
-      sum += score[j];
+      value[j] += (V)bias[j];
+      if (!(value[j] == value[j])) value[j] = -INFINITY;
     }
-    sum = wave_sum(sum);
+  } else {
 #pragma unroll
-    for (int j = 0; j < J; ++j) score[j] /= sum;
+    for (int j = 0; j < J; ++j) value[j] = (V)logit[j];
   }
-  uint64_t key[J];
+  Key key[J];
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int e = lane + 64 * j;
-    double k = (double)logit[j];
-    if (BIAS && e < p.experts) k = score[j] + (double)p.bias[e];
-    if (!(k == k)) k = -INFINITY;
-    if (p.groups > 1) keys[wave][e] = k;
-    key[j] = e < p.experts ? ordered(k) : kNone;
-  }
+  for (int j = 0; j < J; ++j) key[j] = lane + 64 * j < p.experts ? ordered(value[j]) : Key(0);
+  bool near = false;
   if (p.groups > 1) {
-    __syncthreads();
-    // lane g: the key of group g
-    double best = -INFINITY, second = -INFINITY;
-    const int g = lane < p.groups ? lane : 0;
-    for (int i = 0; i < p.group_size; ++i) {
-      const double k = keys[wave][g * p.group_size + i];
-      second = fmax(second, fmin(best, k));
-      best = fmax(best, k);
+#pragma unroll
+    for (int j = 0; j < J; ++j) values[lane + 64 * j] = value[j];
+    __builtin_amdgcn_wave_barrier();
+    // group_lanes lanes look through group g together; its key ends up in all of them
+    const int g = lane / p.group_lanes, part = lane % p.group_lanes;
+    V best = -INFINITY, second = -INFINITY;
+    if (g < p.groups)
+      for (int i = part; i < p.group_size; i += p.group_lanes) {
+        const V v = values[g * p.group_size + i];
+        second = fmax(second, fmin(best, v));
+        best = fmax(best, v);
+      }
+    for (int off = 1; off < p.group_lanes; off <<= 1) {
+      const V ob = __shfl_xor(best, off), os = __shfl_xor(second, off);
+      second = fmax(fmax(second, os), fmin(best, ob));
+      best = fmax(best, ob);
     }
-    const double worth = BIAS && p.group_size > 1 ? best + second : best;
-    const uint64_t mine = lane < p.groups ? ordered(worth == worth ? worth : -INFINITY) : kNone;
+    V worth = BIAS && p.group_size > 1 ? best + second : best;
+    if (!(worth == worth)) worth = -INFINITY;
+    const Key own = g < p.groups ? ordered(worth) : Key(0);
     int ahead = 0;
+    bool close = false;
     for (int o = 0; o < p.groups; ++o) {
-      const uint64_t other = (uint64_t)__shfl((long long)mine, o);
-      ahead += other > mine || (other == mine && o < lane);
+      const V other = of_lane(worth, o * p.group_lanes);
+      const Key k = ordered(other);
+      ahead += k > own || (k == own && o < g);
+      if (kNear && o != g && !(fabsf((float)(other - worth)) > 2.f * margin((float)worth, p.sigmoid))) close = true;  // (equal infinities give NaN)
     }
-    const uint64_t stay = __ballot(lane < p.groups && ahead < p.kept);
+    const bool stays = g < p.groups && ahead < p.kept;
+    const uint64_t stay = __ballot(stays);
+    // only a group next to the line between those that stay and those that do not can change sides: the last that stays, the first that does not
+    if (kNear && p.kept < p.groups && __ballot(g < p.groups && close && (ahead == p.kept - 1 || ahead == p.kept))) near = true;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int e = lane + 64 * j;
-      if (e < p.experts && !((stay >> (e / p.group_size)) & 1)) key[j] = kNone;
+      if (e < p.experts) {
+        // e / group_size: (e + 1/2) / size lies at least 1 / (2 size) from a whole number, far more than this product's error
+        const int group = (int)(((float)e + 0.5f) * (1.f / (float)p.group_size));
+        if (!((stay >> (group * p.group_lanes)) & 1)) key[j] = Key(0);
+      }
     }
+    __builtin_amdgcn_wave_barrier();
   }
-  int my_id = 0;
-  double my_score = 0.0, total = 0.0;
-  for (int i = 0; i < p.top_k; ++i) {
-    uint64_t best = key[0];
-    int at = 0;
+  Key best = 0;
+  int at = 0;
+  auto look = [&] {  // this lane's best
+    best = key[0];
+    at = 0;
 #pragma unroll
     for (int j = 1; j < J; ++j)
       if (key[j] > best) {
         best = key[j];
         at = j;
       }
-    const uint32_t hi = (uint32_t)(best >> 32), top_hi = wave_max(hi);
-    const uint32_t lo = hi == top_hi ? (uint32_t)best : 0u, top_lo = wave_max(lo);
-    const bool candidate = hi == top_hi && lo == top_lo;
-    const int e = (int)~wave_max(candidate ? ~(uint32_t)(lane + 64 * at) : 0u);  // the lowest index among equals
-    double s = 0.0;
+  };
+  look();
+  Key last = 0;
+  const int picks = kNear ? p.top_k + 1 : p.top_k;  // one more to know how far the first left out is
+  for (int i = 0; i < picks; ++i) {
+    Key first;
+    const int winner = best_lane(best, lane + 64 * at, &first);
+    if constexpr (kNear) {
+      if (first == 0) break;  // nothing is left out
+      const float a = value_of(last), b = value_of(first);
+      if (i > 0 && !(a - b > margin(a, p.sigmoid))) near = true;
+      if (near) break;
+      last = first;
+      if (i == p.top_k) break;
+    }
+    const int e = __builtin_amdgcn_readlane(lane + 64 * at, winner);
+    if (lane == i) *mine = e;
+    if (lane == winner) {
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (lane + 64 * j == e) {
-        s = score[j];
-        key[j] = kNone;
-      }
-    s = __shfl(s, e & 63);
-    total += s;
-    if (lane == i) {
-      my_id = e;
-      my_score = s;
+      for (int j = 0; j < J; ++j)
+        if (j == at) key[j] = 0;
+      look();
     }
   }
-  if (live && lane < p.top_k) {
+  return !near;
+}
+
+template <typename T, int J, bool BIAS>
+__global__ __launch_bounds__(kWaves * 64) void route_kernel(Params p) {
+  __shared__ double rows[kWaves][BIAS ? J * 64 : J * 32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int token = blockIdx.x * kWaves + wave;
+  if (token >= p.tokens) return;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (int64_t)token * p.experts;
+  float logit[J], bias[J];
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int e = lane + 64 * j;
+    const float v = e < p.experts ? (float)row[e] : -INFINITY;
+    logit[j] = v == v ? v : -INFINITY;
+    bias[j] = BIAS && e < p.experts ? p.bias[e] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) top = fmaxf(top, logit[j]);
+  top = value_of(wave_max(ordered(top)));
+  int mine = 0;
+  if (!choose<float, J, BIAS>(p, logit, bias, top, lane, reinterpret_cast<float*>(rows[wave]), &mine)) {
+    if constexpr (BIAS) choose<double, J, BIAS>(p, logit, bias, top, lane, rows[wave], &mine);
+  }
+  // The chosen ones' scores, in 64 bits where a score is below what 32 bits hold well (a renormalised weight may be large all the same).
+  const float chosen = (float)row[mine], l = chosen == chosen ? chosen : -INFINITY;
+  const bool small = __ballot(lane < p.top_k && (p.sigmoid ? l < -60.f : l < top && !(l - top > -60.f))) != 0;
+  float sum = 1.f;
+  if (!p.sigmoid) {
+    sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) sum += lane + 64 * j >= p.experts ? 0.f : logit[j] == top ? 1.f : expf(logit[j] - top);
+    sum = wave_sum(sum);
+  }
+  float weight;
+  auto weigh = [&](auto zero) {
+    typedef decltype(zero) V;
+    V s = p.sigmoid ? sigmoid_of((V)l) : over(l == top ? V(1) : exp_of((V)l - (V)top), (V)sum);
+    if (p.renormalize) {
+      const V total = wave_sum(lane < p.top_k ? s : V(0));
+      s = total > V(0) ? s / total : V(0);  // (not over(): a total may be tiny)
+    }
+    weight = (float)(s * (V)p.scale);
+  };
+  if (small) weigh(0.0);
+  else weigh(0.f);
+  if (lane < p.top_k) {
     const int64_t at = (int64_t)token * p.top_k + lane;
-    p.ids[at] = my_id;
-    const double w = p.renormalize ? (total > 0.0 ? my_score / total : 0.0) : my_score;
-    p.weights[at] = (float)(w * (double)p.scale);
+    p.ids[at] = mine;
+    p.weights[at] = weight;
   }
 }
 
@@ -199,8 +354,10 @@ extern "C" int pto_hip_route_experts(const void* logits, const float* bias, int3
   PTO_CHECK_ARG(((uintptr_t)bias | (uintptr_t)expert_ids | (uintptr_t)expert_weights) % 4 == 0 &&
                     (uintptr_t)logits % (size_t)dtype_bytes(logits_dtype) == 0,
                 "route_experts: misaligned operand");
+  int group_lanes = 64;
+  while (group_lanes * n_groups > 64) group_lanes /= 2;
   const Params p{logits, bias, expert_ids, expert_weights, (int)tokens, (int)experts, (int)top_k, (int)n_groups, (int)topk_groups,
-                 (int)(experts / n_groups), score_fn == PTO_HIP_SCORE_SIGMOID, renormalize != 0, scale};
+                 (int)(experts / n_groups), group_lanes, score_fn == PTO_HIP_SCORE_SIGMOID, renormalize != 0, scale};
   hipStream_t st = (hipStream_t)stream;
   if (logits_dtype == PTO_HIP_FP32) bias ? launch<float, true>(p, st) : launch<float, false>(p, st);
   else if (logits_dtype == PTO_HIP_BF16) bias ? launch<__bf16, true>(p, st) : launch<__bf16, false>(p, st);
