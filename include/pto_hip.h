@@ -377,8 +377,10 @@ PTO_HIP_API int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, 
 PTO_HIP_API int pto_hip_quantize_fp8_block(const void* x, void* codes, float* scale, int64_t rows, int64_t cols, int x_dtype,
                                            void* stream);
 
-/* out[m, n] = sum_kb a_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} a8[m, k] * w8[n, k], fp32 accumulation, any M
- * and N; K a multiple of 128 and at most 65536 (PTO_HIP_ERR_UNSUPPORTED otherwise).  out FP32, BF16 or FP16. */
+/* out[m, n] = sum_kb a_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} a8[m, k] * w8[n, k], any M and N; K a multiple
+ * of 128 and at most 65536 (PTO_HIP_ERR_UNSUPPORTED otherwise).  out FP32, BF16 or FP16.  Blocks are added in fp32.  Inside a block the
+ * 8-bit matrix instructions drop what lies 2^-13 below the largest of eight products, 1.4e-5 of the result in norm; with FP32
+ * results, and up to 16 rows, the codes are widened and nothing is dropped. */
 PTO_HIP_API int pto_hip_projection_fp8_block(const void* a8, const float* a_scale, const void* w8, const float* w_scale, void* out,
                                              int64_t m, int64_t k, int64_t n, int out_dtype, void* stream);
 
@@ -399,8 +401,9 @@ PTO_HIP_API int pto_hip_route_experts(const void* logits, const float* bias, int
  * experts' half of a mixture layer behind pto_hip_rms_norm_fp8_block and pto_hip_route_experts.  Products as
  * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 as pto_hip_quantize_fp8_block does, the sum over a token's
  * experts is fp32.  A negative id leaves its slot out (a token without any gives zeros); an id of an expert that there is
- * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  H and I multiples of 128 and at
- * most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the
+ * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  Where out is BF16 both products are as
+ * pto_hip_projection_fp8_block's of 16-bit results, where it is FP16 the second one is; the widened form has the rest.  With
+ * BF16 results the experts' rows are added from fp16 with a power of two per 128 channels.  H and I multiples of 128 and at most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the
  * other: w_gate8, w_up8 [E, I, H], w_down8 [E, H, I].  out FP32, BF16 or FP16. */
 PTO_HIP_API int pto_hip_experts_ffn_fp8_block(const void* x8, const float* x_scale, const int32_t* expert_ids,
                                               const float* expert_weights, const void* w_gate8, const float* w_gate_scale,
@@ -664,6 +667,12 @@ PTO_HIP_API int pto_hip_backend_handler_query(const char* hook, int32_t arg, cha
  *                               input RMSNorm, 2 = SwiGLU of the pair in front, 4 = the merge of the attention
  *                               partials (a sum of these; default 7, 0 = never)
  *  "skinny_fused"               read only: which of these the last decoder layer or FFN block (pto_hip_ffn_swiglu) took
+ *  "block_gemm_rows"            tile height of the products of block-scaled e4m3 operands (pto_hip_projection_fp8_block and both
+ *                               products of pto_hip_experts_ffn_fp8_block): 0 = by estimate (default); 16 = operands straight to
+ *                               registers (experts: every slot for itself, up to 1024 of them); 64, 128, 256 = tiles through LDS
+ *                               (256 only where the codes are multiplied as they are, 128 otherwise).  "gemm_splits" gives
+ *                               the ranges of k of the projection's tiles
+ *  "block_gemm_cols"            channels of the projection's tiles of 64 rows: 0 = by estimate (default), 64, 128, 256
  *  "w8a16_gemm_rows"            rows from which the int8 projections run as one tiled GEMM (codes
  *                               widened inside the kernel, weights read once) instead of 32-row
  *                               passes (default 33; 0 = never)

@@ -46,9 +46,12 @@ FLAGS = [
 
 
 # Per-file additions.  The attention kernels keep their MFMA accumulators in architectural VGPRs
-# (they are rescaled by VALU code every chunk); the GEMM keeps the default AGPR form.
+# (they are rescaled by VALU code every chunk), and so do the block-scaled products (added with a scale every block of k);
+# the GEMM keeps the default AGPR form.
 EXTRA_FLAGS = {
     "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "block_gemm8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "experts.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

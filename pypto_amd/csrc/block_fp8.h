@@ -18,9 +18,19 @@ constexpr int kMaxK = 65536;  // longest rows of the products: byte offsets insi
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
 typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 
+template <int N>
+struct IntConst {
+  static constexpr int value = N;
+};
+
 // Scale of a group whose largest magnitude is amax: 1 for a group of zeros, and never below the smallest normal number (whose
 // reciprocal is one too).
 __device__ __forceinline__ float group_scale(float amax) { return amax > 0.f ? fmaxf(amax / 448.f, 0x1p-126f) : 1.f; }
+
+// The size of a finite value, 0 of others.
+__device__ __forceinline__ float finite_size(float v) { return fabsf(v) <= 3.4028234664e38f ? fabsf(v) : 0.f; }
+// The power of two that, divided out, puts a largest size of amax into [2^14, 2^15); 0 for none, and within what fp32 holds.
+__device__ __forceinline__ int half_exponent(float amax) { return amax > 0.f ? max(ilogbf(amax) - 14, -126) : 0; }
 
 // v / scale, correctly rounded, as often as a group has elements: the reciprocal is refined once to half an ulp, the quotient
 // twice by its exact remainder (as in ffn_fp8.hip's row quantiser).  No quotient of a finite group leaves +-448 (1 + 2^-23), which rounds to a code

@@ -27,8 +27,10 @@ struct Params {
   const uint8_t* b1;  // gate/up pass: the up weights
   const float* sb1;
   void* c;       // [rows, n]
-  float* c_scale;  // gate/up pass: [rows, n / 128], c being codes
+  float* c_scale;  // [rows, n / 128] where c is codes (gate/up pass) or scaled fp16 (down pass)
   int m, n, k, kb;
+  // Tiled form: the blocks of k cut into ranges of this many, each a workgroup's own, whose sums go to slabs [range][m, n] in c (0: whole)
+  int per_split;
   // Experts: the rows of a tile belong to one expert and are listed by the plan (experts.hip).
   const int4* tiles;       // {expert, first place, rows, 0}
   const int* n_tiles;
@@ -101,44 +103,34 @@ __device__ __forceinline__ f32x4 block_product(const i32x4 (&w)[2], const i32x4 
   return part;
 }
 
-// Few rows: a tile of 16 MT rows x 16 CT channels, both operands straight from memory to registers; the workgroup's KW wavefronts take
-// the steps of 128 codes in turn, NS of them in flight, and sum through LDS in wavefront order.
-template <int MAP, int CT, int MT, int KW, int NS, typename OutT>
+// Up to 16 rows a tile: 16 rows x 16 CT channels, both operands straight from memory to registers; the workgroup's KW wavefronts take
+// the steps of 128 codes in turn, NS of them in flight, and sum through LDS in wavefront order.  Bound by the stream of the weights.
+template <int CT, int KW, int NS, typename OutT>
 __global__ __launch_bounds__(KW * 64) void narrow_kernel(Params p, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) f32x4 red[KW][CT][MT][64];
+  __shared__ __attribute__((aligned(16))) f32x4 red[KW][CT][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, kg = lane >> 4;
   const int tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-  if (MAP != kPlain && tm >= *p.n_tiles) return;
-  const Tile<MAP> tile(p, tm, 16 * MT);
+  const int m0 = tm * 16, rows = min(16, p.m - m0);
   const int n0 = tn * 16 * CT;
   const int mine = (p.kb - wave + KW - 1) / KW;  // steps of this wavefront
 
-  const uint8_t* xp[MT];
-  const float* sp[MT];
-#pragma unroll
-  for (int h = 0; h < MT; ++h) {
-    const size_t row = tile.a_row(min(16 * h + c, tile.rows - 1));
-    xp[h] = p.a + row * p.k + wave * kBlock + kg * 16;
-    sp[h] = p.sa + row * p.kb + wave;
-  }
-  const size_t matrix = (size_t)tile.expert * p.n * p.k;
+  const size_t a_row = m0 + min(c, rows - 1);
+  const uint8_t* xp = p.a + a_row * p.k + wave * kBlock + kg * 16;
+  const float* sp = p.sa + a_row * p.kb + wave;
   const uint8_t* wp[CT];
 #pragma unroll
-  for (int i = 0; i < CT; ++i) wp[i] = p.b0 + matrix + (size_t)min(n0 + 16 * i + c, p.n - 1) * p.k + wave * kBlock + kg * 16;
-  const int blocks_n = (p.n + kBlock - 1) / kBlock;
-  const float* wsp = p.sb0 + ((size_t)tile.expert * blocks_n + n0 / kBlock) * p.kb + wave;  // 16 CT divides 128: one block
+  for (int i = 0; i < CT; ++i) wp[i] = p.b0 + (size_t)min(n0 + 16 * i + c, p.n - 1) * p.k + wave * kBlock + kg * 16;
+  const float* wsp = p.sb0 + (size_t)(n0 / kBlock) * p.kb + wave;  // 16 CT divides 128: one block
 
   struct Held {
-    i32x4 w[CT][2], x[MT][2];
-    float sx[MT], sw;
+    i32x4 w[CT][2], x[2];
+    float sx, sw;
   };
-  f32x4 acc[CT][MT];
+  f32x4 acc[CT];
 #pragma unroll
-  for (int i = 0; i < CT; ++i)
-#pragma unroll
-    for (int h = 0; h < MT; ++h) acc[i][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < CT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   // Past its last step a wavefront asks for its first again (the requests in flight stay known at compile time).
   auto load = [&](Held& s, int round) {
     const size_t step = round < mine ? (size_t)round * KW : 0, at = step * kBlock;
@@ -148,22 +140,16 @@ __global__ __launch_bounds__(KW * 64) void narrow_kernel(Params p, int tiles_n) 
       for (int q = 0; q < 2; ++q) s.w[i][q] = *reinterpret_cast<const i32x4*>(wp[i] + at + q * 64);
     s.sw = wsp[step];
 #pragma unroll
-    for (int h = 0; h < MT; ++h) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) s.x[h][q] = *reinterpret_cast<const i32x4*>(xp[h] + at + q * 64);
-      s.sx[h] = sp[h][step];
-    }
+    for (int q = 0; q < 2; ++q) s.x[q] = *reinterpret_cast<const i32x4*>(xp + at + q * 64);
+    s.sx = sp[step];
   };
   auto compute = [&](const Held& s) {
+    const float scale = s.sx * s.sw;
 #pragma unroll
-    for (int h = 0; h < MT; ++h) {
-      const float scale = s.sx[h] * s.sw;
+    for (int i = 0; i < CT; ++i) {  // weights first: a lane then holds four consecutive channels of a row
+      const f32x4 part = block_product(s.w[i], s.x);
 #pragma unroll
-      for (int i = 0; i < CT; ++i) {  // weights first: a lane then holds four consecutive channels of a row
-        const f32x4 part = block_product(s.w[i], s.x[h]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][h][e] = fmaf(part[e], scale, acc[i][h][e]);
-      }
+      for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(part[e], scale, acc[i][e]);
     }
   };
   Held st[NS];
@@ -183,149 +169,16 @@ __global__ __launch_bounds__(KW * 64) void narrow_kernel(Params p, int tiles_n) 
       if (r + i < mine) compute(st[i]);
   }
 #pragma unroll
-  for (int i = 0; i < CT; ++i)
-#pragma unroll
-    for (int h = 0; h < MT; ++h) red[wave][i][h][lane] = acc[i][h];
+  for (int i = 0; i < CT; ++i) red[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int u = tid; u < CT * MT * 64; u += KW * 64) {
-    const int l = u & 63, h = (u >> 6) % MT, i = (u >> 6) / MT;
-    const int row = 16 * h + (l & 15), col = n0 + 16 * i + 4 * (l >> 4);
-    if (row >= tile.rows || col >= p.n) continue;
-    f32x4 sum = red[0][i][h][l];
+  for (int u = tid; u < CT * 64; u += KW * 64) {
+    const int l = u & 63, i = u >> 6;
+    const int row = l & 15, col = n0 + 16 * i + 4 * (l >> 4);
+    if (row >= rows || col >= p.n) continue;
+    f32x4 sum = red[0][i][l];
 #pragma unroll
-    for (int w = 1; w < KW; ++w) sum += red[w][i][h][l];
-    store_upto4(reinterpret_cast<OutT*>(p.c) + (size_t)tile.c_row(row) * p.n + col, sum, p.n - col);
-  }
-}
-
-// The first product of an FFN on few rows: SiLU(gate) * up of 16 MT rows x 128 channels as codes and their scales.  Each of eight wavefronts
-// streams the 16 gate and 16 up channels of its own over the whole of k; the eight together hold a group of 128 channels, whose
-// maximum they find through LDS, so that h leaves the registers as codes.  KS of these sets share k.
-template <int MT, int KS, int NS>
-__global__ __launch_bounds__(KS * 512) void narrow_gate_up_kernel(Params p, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) f32x4 red[KS > 1 ? KS - 1 : 1][KS > 1 ? 8 : 1][2][MT][64];
-  __shared__ float top[8][MT][16];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int share = wave & 7, part_k = wave >> 3;
-  const int c = lane & 15, kg = lane >> 4;
-  const int tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
-  if (tm >= *p.n_tiles) return;
-  const Tile<kGateUp> tile(p, tm, 16 * MT);
-  const int n0 = tn * kBlock;
-  const int mine = (p.kb - part_k + KS - 1) / KS;
-
-  const uint8_t* xp[MT];
-  const float* sp[MT];
-#pragma unroll
-  for (int h = 0; h < MT; ++h) {
-    const size_t row = tile.a_row(min(16 * h + c, tile.rows - 1));
-    xp[h] = p.a + row * p.k + part_k * kBlock + kg * 16;
-    sp[h] = p.sa + row * p.kb + part_k;
-  }
-  const size_t at0 = (size_t)tile.expert * p.n * p.k + (size_t)(n0 + 16 * share + c) * p.k + part_k * kBlock + kg * 16;
-  const uint8_t* wp[2] = {p.b0 + at0, p.b1 + at0};
-  const size_t sat = ((size_t)tile.expert * (p.n / kBlock) + tn) * p.kb + part_k;
-  const float* wsp[2] = {p.sb0 + sat, p.sb1 + sat};
-
-  struct Held {
-    i32x4 w[2][2], x[MT][2];
-    float sx[MT], sw[2];
-  };
-  f32x4 acc[2][MT];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int h = 0; h < MT; ++h) acc[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto load = [&](Held& s, int round) {
-    const size_t step = round < mine ? (size_t)round * KS : 0, at = step * kBlock;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) s.w[t][q] = *reinterpret_cast<const i32x4*>(wp[t] + at + q * 64);
-      s.sw[t] = wsp[t][step];
-    }
-#pragma unroll
-    for (int h = 0; h < MT; ++h) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) s.x[h][q] = *reinterpret_cast<const i32x4*>(xp[h] + at + q * 64);
-      s.sx[h] = sp[h][step];
-    }
-  };
-  auto compute = [&](const Held& s) {
-#pragma unroll
-    for (int h = 0; h < MT; ++h)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const f32x4 part = block_product(s.w[t], s.x[h]);
-        const float scale = s.sx[h] * s.sw[t];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][h][e] = fmaf(part[e], scale, acc[t][h][e]);
-      }
-  };
-  Held st[NS];
-  if (mine > 0) {
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) load(st[i], i);
-    int r = 0;
-    for (; r + NS <= mine; r += NS) {
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        load(st[(i + NS - 1) % NS], r + i + NS - 1);
-        compute(st[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i)
-      if (r + i < mine) compute(st[i]);
-  }
-  if constexpr (KS > 1) {
-    if (part_k > 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int h = 0; h < MT; ++h) red[part_k - 1][share][t][h][lane] = acc[t][h];
-    }
-    __syncthreads();
-    if (part_k == 0) {
-#pragma unroll
-      for (int w = 0; w < KS - 1; ++w)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int h = 0; h < MT; ++h) acc[t][h] += red[w][share][t][h][lane];
-    }
-  }
-  f32x4 y[MT];
-  if (part_k == 0) {
-#pragma unroll
-    for (int h = 0; h < MT; ++h) {
-      float amax = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[h][e] = silu(acc[0][h][e]) * acc[1][h][e];
-        amax = fmaxf(amax, fabsf(y[h][e]));
-      }
-      amax = fmaxf(amax, __shfl_xor(amax, 16));
-      amax = fmaxf(amax, __shfl_xor(amax, 32));
-      if (kg == 0) top[share][h][c] = amax;
-    }
-  }
-  __syncthreads();
-  if (part_k > 0) return;
-  uint8_t* codes = reinterpret_cast<uint8_t*>(p.c);
-#pragma unroll
-  for (int h = 0; h < MT; ++h) {
-    float amax = top[0][h][c];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) amax = fmaxf(amax, top[w][h][c]);
-    const int row = 16 * h + c;
-    if (row >= tile.rows) continue;
-    const float s = group_scale(amax);
-    const GroupQuotient q(s);
-    const size_t out_row = tile.c_row(row);
-    *reinterpret_cast<uint32_t*>(codes + out_row * p.n + n0 + 16 * share + 4 * kg) = codes4(q(y[h][0]), q(y[h][1]), q(y[h][2]), q(y[h][3]));
-    if (share == 0 && kg == 0) p.c_scale[out_row * (p.n / kBlock) + tn] = s;
+    for (int w = 1; w < KW; ++w) sum += red[w][i][l];
+    store_upto4(reinterpret_cast<OutT*>(p.c) + (size_t)(m0 + row) * p.n + col, sum, p.n - col);
   }
 }
 

@@ -2,23 +2,72 @@
 #include <hip/hip_runtime.h>
 
 #include "block_gemm8.h"
+#include "block_tiled8.h"
 #include "common.h"
+#include "launch_choice.h"
 
 namespace pto_hip {
 namespace block8 {
 
+// out = the sum of the k ranges' slabs, in their order
 template <typename OutT>
-int launch_projection(const Params& p, hipStream_t st) {
-  constexpr int CT = 2;
-  const int tiles_n = (p.n + 16 * CT - 1) / (16 * CT);
-  auto go = [&](auto kern, int height, int waves) {
-    const int64_t tiles = (int64_t)tiles_n * ((p.m + height - 1) / height);
-    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(waves * 64), 0, st, p, tiles_n);
-  };
-  if (p.m <= 16) go(narrow_kernel<kPlain, CT, 1, 4, 3, OutT>, 16, 4);
-  else go(narrow_kernel<kPlain, CT, 2, 4, 3, OutT>, 32, 4);
+__global__ __launch_bounds__(256) void sum_ranges_kernel(const float* __restrict__ slabs, int ranges, int64_t count, OutT* __restrict__ out) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= count) return;
+  const int here = (int)(count - at < 4 ? count - at : 4);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < ranges; ++r) {
+    const float* src = slabs + r * count + at;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < here) sum[e] += src[e];
+  }
+  store_upto4(out + at, sum, here);
+}
+
+template <int BM, int BN, bool EXACT, typename OutT>
+int launch_tiles(Params p, int per_split, hipStream_t st) {
+  const int tiles_m = (p.m + BM - 1) / BM;
+  if (per_split <= 0 || per_split >= p.kb) return launch_tiled<kPlain, BM, BN, EXACT, OutT>(p, tiles_m, st);
+  const int ranges = (p.kb + per_split - 1) / per_split;
+  const int64_t count = (int64_t)p.m * p.n;
+  void* slabs = nullptr;
+  int rc = gemm_slabs((size_t)ranges * count * sizeof(float), st, &slabs);
+  if (rc) return rc;
+  if (!slabs) return launch_tiled<kPlain, BM, BN, EXACT, OutT>(p, tiles_m, st);
+  OutT* const out = reinterpret_cast<OutT*>(p.c);
+  p.c = slabs;
+  p.per_split = per_split;
+  rc = launch_tiled<kPlain, BM, BN, EXACT, float>(p, tiles_m, st);
+  if (rc) return rc;
+  hipLaunchKernelGGL(sum_ranges_kernel<OutT>, dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, st, reinterpret_cast<const float*>(slabs),
+                     ranges, count, out);
   PTO_CHECK_HIP(hipGetLastError());
   return PTO_HIP_OK;
+}
+
+template <typename OutT>
+int launch_projection(const Params& p, hipStream_t st) {
+  constexpr bool kExact = std::is_same<OutT, float>::value;
+  const BlockTile t = choose_block_tile(p.m, p.n, p.kb, kExact, ctx().num_cu, (int)ctx().block_gemm_rows, (int)ctx().block_gemm_cols,
+                                        (int)ctx().gemm_splits);
+  if (t.rows == 16) {
+    const int tiles_n = (p.n + t.cols - 1) / t.cols;
+    const int64_t wgs = (int64_t)tiles_n * ((p.m + 15) / 16);
+    if (wgs >= (1 << 23)) return fail(PTO_HIP_ERR_UNSUPPORTED, "a product of %lld tiles is more than one launch holds", (long long)wgs);
+    const dim3 grid((unsigned)wgs);
+    if (t.cols == 16) hipLaunchKernelGGL((narrow_kernel<1, 8, 4, OutT>), grid, dim3(512), 0, st, p, tiles_n);
+    else hipLaunchKernelGGL((narrow_kernel<2, 4, 3, OutT>), grid, dim3(256), 0, st, p, tiles_n);
+    PTO_CHECK_HIP(hipGetLastError());
+    return PTO_HIP_OK;
+  }
+  if (t.rows == 64 && t.cols == 64) return launch_tiles<64, 64, kExact, OutT>(p, t.per_split, st);
+  if (t.rows == 64 && t.cols == 128) return launch_tiles<64, 128, kExact, OutT>(p, t.per_split, st);
+  if (t.rows == 64) return launch_tiles<64, 256, kExact, OutT>(p, t.per_split, st);
+  if constexpr (!kExact) {
+    if (t.rows == 256) return launch_tiles<256, 256, false, OutT>(p, t.per_split, st);
+  }
+  return launch_tiles<128, 256, kExact, OutT>(p, t.per_split, st);
 }
 
 }  // namespace block8

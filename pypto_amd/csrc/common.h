@@ -78,6 +78,8 @@ struct Context {
   int64_t w8a16_min_steps = 2;   // fewest 32-row steps per wavefront before k is split further
   int64_t gemm_stream = 1;         // projections of 33 to 96 rows that stream their weights: 0 never, 1 where measured ahead, 2 whenever shapes allow
   int64_t attn_order = -1;         // sequences by length: -1 where measured faster, 0 never, 1 always (partition grid and workgroup form)
+  int64_t block_gemm_rows = 0;   // tile height of the block-scaled e4m3 products: 0 by estimate, 16 straight to registers
+  int64_t block_gemm_cols = 0;   // ... channels of their tiles of 64 rows: 0 by estimate
   int64_t w8a16_gemm_rows = 33;  // rows from which int8 projections run as a tiled GEMM (0 = never)
 };
 

@@ -8,34 +8,57 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "block_gemm8.h"
+#include "block_tiled8.h"
 #include "common.h"
+#include "launch_choice.h"
 
 namespace pto_hip {
 namespace block8 {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kPlanThreads = 1024;
+// Tokens are worked through in passes of so many slots, so that the scratch stays below a gigabyte or two and every index inside 32 bits.
+constexpr int64_t kPassSlots = 32768;
+constexpr int64_t kMostDirectSlots = 1024;
 
 // The plan: slots by expert, and tiles of `height` rows of one expert each.  One workgroup; a slot with a negative expert is in no
-// tile, one with an expert that there is not is reported.  Places inside an expert are taken in the order of atomics: which row of
-// which tile a slot becomes changes no bit of its result.
+// tile, one with an expert that there is not is reported.  Each wavefront counts for itself ([wavefronts][experts] in LDS), so that the
+// counters of a busy expert are shared by 64 lanes and not by all, and a slot's rank in its wavefront's count is its place: with
+// one set of counters and a second round of atomics for the places 16384 slots of 64 experts took 19 us.  The order of the ranks is
+// that of the atomics: which row of which tile a slot becomes changes no bit of its result.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __restrict__ ids, int slots, int experts, int height,
                                                             int32_t* __restrict__ order, int4* __restrict__ tiles, int* __restrict__ n_tiles,
                                                             int* __restrict__ flag) {
-  __shared__ int count[kMaxExperts], first[kMaxExperts], waves[2][kPlanThreads / 64];
+  constexpr int kWaves = kPlanThreads / 64, kEach = kPassSlots / kPlanThreads;  // slots of a thread
+  extern __shared__ int count[];  // [kWaves][experts]
+  __shared__ int sums[2][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int e = tid; e < experts; e += kPlanThreads) count[e] = 0;
-  __syncthreads();
-  for (int s = tid; s < slots; s += kPlanThreads) {
-    const int e = ids[s];
-    if (e >= experts) *flag = 1;
-    else if (e >= 0) atomicAdd(&count[e], 1);
+  for (int i = tid; i < kWaves * experts; i += kPlanThreads) count[i] = 0;
+  int e[kEach], rank[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int s = i * kPlanThreads + tid;
+    e[i] = s < slots ? ids[s] : -1;
   }
   __syncthreads();
-  // thread e: exclusive sums over the experts in front, of rows and of tiles
-  const int rows = tid < experts ? count[tid] : 0, mine = (rows + height - 1) / height;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (e[i] >= experts) {
+      *flag = 1;
+      e[i] = -1;
+    }
+    rank[i] = e[i] >= 0 ? atomicAdd(&count[wave * experts + e[i]], 1) : 0;
+  }
+  __syncthreads();
+  // thread t: expert t's rows and tiles, exclusive sums over the experts in front, then over its wavefronts
+  int rows = 0;
+  if (tid < experts)
+    for (int w = 0; w < kWaves; ++w) rows += count[w * experts + tid];
+  const int mine = (rows + height - 1) / height;
   int sum[2] = {rows, mine};
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
@@ -44,45 +67,54 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
       const int o = __shfl_up(sum[q], off);
       if (lane >= off) sum[q] += o;
     }
-    if (lane == 63) waves[q][wave] = sum[q];
+    if (lane == 63) sums[q][wave] = sum[q];
   }
   __syncthreads();
   int before[2] = {sum[0] - rows, sum[1] - mine};
   for (int w = 0; w < wave; ++w) {
-    before[0] += waves[0][w];
-    before[1] += waves[1][w];
+    before[0] += sums[0][w];
+    before[1] += sums[1][w];
   }
   if (tid < experts) {
-    first[tid] = before[0];
     for (int i = 0; i < mine; ++i) tiles[before[1] + i] = int4{tid, before[0] + i * height, min(height, rows - i * height), 0};
+    int at = before[0];
+    for (int w = 0; w < kWaves; ++w) {
+      const int here = count[w * experts + tid];
+      count[w * experts + tid] = at;
+      at += here;
+    }
   }
   if (tid == kPlanThreads - 1) *n_tiles = before[1] + mine;
   __syncthreads();
-  for (int s = tid; s < slots; s += kPlanThreads) {
-    const int e = ids[s];
-    if (e >= 0 && e < experts) order[atomicAdd(&first[e], 1)] = s;
-  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (e[i] >= 0) order[count[wave * experts + e[i]] + rank[i]] = i * kPlanThreads + tid;
 }
 
-// out[t] = sum over j of weights[t, j] * y[t * top_k + j], the slots without an expert left out.
-template <typename OutT>
-__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids,
+// out[t] = sum over j of weights[t, j] * y[t * top_k + j], the slots without an expert left out.  Y _Float16: times the row's power
+// of two of each 128 channels.  One workgroup per token and 2048 channels, eight a thread.
+template <typename Y, typename OutT>
+__global__ __launch_bounds__(256) void combine_kernel(const Y* __restrict__ y, const float* __restrict__ y_scale, const int32_t* __restrict__ ids,
                                                       const float* __restrict__ weights, OutT* __restrict__ out, int hidden, int experts,
                                                       int top_k) {
-  const int col = (blockIdx.x * 256 + threadIdx.x) * 4;
+  typedef __attribute__((__vector_size__(8 * sizeof(Y)))) Y vec8;
+  const int col = (blockIdx.x * 256 + threadIdx.x) * 8;
   if (col >= hidden) return;
   const int64_t token = blockIdx.y;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int j = 0; j < top_k; ++j) {
     const int64_t slot = token * top_k + j;
     const int e = ids[slot];
     if (e < 0 || e >= experts) continue;
-    const float w = weights[slot];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(y + slot * hidden + col);
+    float w = weights[slot];
+    if constexpr (sizeof(Y) == 2) w *= y_scale[slot * (hidden / kBlock) + col / kBlock];
+    const vec8 v = *reinterpret_cast<const vec8*>(y + slot * hidden + col);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+    for (int i = 0; i < 8; ++i) sum[i] = fmaf(w, (float)v[i], sum[i]);
   }
-  store_upto4(out + token * hidden + col, sum, 4);
+  store_upto4(out + token * hidden + col, f32x4{sum[0], sum[1], sum[2], sum[3]}, 4);
+  store_upto4(out + token * hidden + col + 4, f32x4{sum[4], sum[5], sum[6], sum[7]}, 4);
 }
 
 struct Experts {
@@ -96,11 +128,225 @@ struct Experts {
   int hidden, inter, experts, top_k;
 };
 
-// Scratch of a pass over `tokens` tokens.
+// ---- a few tokens: every slot reads its expert's matrices for itself, without a plan ----------------------------------------
+// Bound by the stream of those matrices; the matrix unit's 16 rows are one and the same.  A workgroup has 16 channels (of gate and up),
+// its wavefronts share k.
+constexpr int kDirectUp = 4, kDirectDown = 8;  // wavefronts
+
+// h[slot, n] = SiLU(g) * u in 32 bits, 16 outputs of one slot a workgroup.
+template <int NS>
+__global__ __launch_bounds__(kDirectUp * 64) void direct_gate_up_kernel(Experts x, float* __restrict__ h, int* __restrict__ flag) {
+  __shared__ __attribute__((aligned(16))) f32x4 red[kDirectUp][2][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, kg = lane >> 4;
+  const int tiles_n = x.inter / 16;
+  const int slot = blockIdx.x / tiles_n, n0 = (blockIdx.x - slot * tiles_n) * 16;
+  const int expert = __builtin_amdgcn_readfirstlane(x.ids[slot]);
+  if (expert < 0 || expert >= x.experts) {
+    if (expert >= 0 && tid == 0) *flag = 1;
+    return;
+  }
+  const int kb = x.hidden / kBlock, mine = (kb - wave + kDirectUp - 1) / kDirectUp;
+  const size_t token = slot / x.top_k;
+  const uint8_t* xp = x.x + token * x.hidden + wave * kBlock + kg * 16;
+  const float* sp = x.x_scale + token * kb + wave;
+  const size_t at0 = ((size_t)expert * x.inter + n0 + c) * x.hidden + wave * kBlock + kg * 16;
+  const uint8_t* wp[2] = {x.gate + at0, x.up + at0};
+  const size_t sat = ((size_t)expert * (x.inter / kBlock) + n0 / kBlock) * kb + wave;
+  const float* wsp[2] = {x.gate_scale + sat, x.up_scale + sat};
+  struct Held {
+    i32x4 w[2][2], a[2];
+    float sa, sw[2];
+  };
+  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  auto load = [&](Held& s, int round) {  // past the last step: the first again
+    const size_t step = round < mine ? (size_t)round * kDirectUp : 0, at = step * kBlock;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) s.w[t][q] = *reinterpret_cast<const i32x4*>(wp[t] + at + q * 64);
+      s.sw[t] = wsp[t][step];
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) s.a[q] = *reinterpret_cast<const i32x4*>(xp + at + q * 64);
+    s.sa = sp[step];
+  };
+  auto compute = [&](const Held& s) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f32x4 part = block_product(s.w[t], s.a);
+      const float scale = s.sa * s.sw[t];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(part[e], scale, acc[t][e]);
+    }
+  };
+  Held st[NS];
+  if (mine > 0) {
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load(st[i], i);
+    int r = 0;
+    for (; r + NS <= mine; r += NS) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        load(st[(i + NS - 1) % NS], r + i + NS - 1);
+        compute(st[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+      if (r + i < mine) compute(st[i]);
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) red[wave][t][lane] = acc[t];
+  __syncthreads();
+  if (wave > 0) return;
+  f32x4 sum[2] = {red[0][0][lane], red[0][1][lane]};
+#pragma unroll
+  for (int w = 1; w < kDirectUp; ++w)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sum[t] += red[w][t][lane];
+  if (c > 0) return;
+  f32x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = silu(sum[0][e]) * sum[1][e];
+  *reinterpret_cast<f32x4*>(h + (size_t)slot * x.inter + n0 + 4 * kg) = y;
+}
+
+// out[t, n] of 16 channels a workgroup: the token's rows of h are quantised into LDS, their scales times the slots' weights, and all
+// its experts' products are one sum over (slot, block of k), shared by the wavefronts in turn.
+template <int NS, typename OutT>
+__global__ __launch_bounds__(kDirectDown * 64) void direct_down_kernel(Experts x, const float* __restrict__ h) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t codes[];  // [top_k][inter], then scales [top_k][inter / 128]
+  __shared__ __attribute__((aligned(16))) f32x4 red[kDirectDown][64];
+  __shared__ int experts[64], slots[64], count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, kg = lane >> 4;
+  const int tiles_n = x.hidden / 16;
+  const int token = blockIdx.x / tiles_n, n0 = (blockIdx.x - token * tiles_n) * 16;
+  const int kb = x.inter / kBlock;
+  float* const scales = reinterpret_cast<float*>(codes + x.top_k * x.inter);
+  if (wave == 0) {  // the slots that have an expert
+    const int e = lane < x.top_k ? x.ids[(size_t)token * x.top_k + lane] : -1;
+    const bool used = e >= 0 && e < x.experts;
+    const uint64_t all = __ballot(used);
+    if (used) {
+      const int at = __popcll(all & ((1ull << lane) - 1));
+      experts[at] = e;
+      slots[at] = lane;
+    }
+    if (lane == 0) count = __popcll(all);
+  }
+  __syncthreads();
+  const int units = count * kb, mine = (units - wave + kDirectDown - 1) / kDirectDown;  // (slot, block) pairs of this wavefront
+  struct Held {
+    i32x4 w[2];
+    float sw;
+  };
+  auto load = [&](Held& s, int round) {  // past the last unit: the first again
+    const int u = (round < mine ? round * kDirectDown : 0) + wave, j = u / kb, b = u - j * kb;
+    const size_t expert = experts[j];
+    const uint8_t* src = x.down + (expert * x.hidden + n0 + c) * x.inter + b * kBlock + kg * 16;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) s.w[q] = *reinterpret_cast<const i32x4*>(src + q * 64);
+    s.sw = x.down_scale[(expert * (x.hidden / kBlock) + n0 / kBlock) * kb + b];
+  };
+  // Half a wavefront quantises a group of 128 at a time, four values a lane; a round is kGroups of them, asked for at once.  The first
+  // round's values are asked for ahead of the weights: loads come back in order, and the weights are then on their way meanwhile.
+  constexpr int kGroups = 6;
+  const int half = wave * 2 + (lane >> 5), lane32 = lane & 31;
+  float4 v[kGroups];
+  float weight[kGroups];
+  auto ask = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int u = min(first + i * 2 * kDirectDown + half, units - 1), j = u / kb, b = u - j * kb;
+      const size_t slot = (size_t)token * x.top_k + slots[j];
+      v[i] = *reinterpret_cast<const float4*>(h + slot * x.inter + b * kBlock + 4 * lane32);
+      weight[i] = x.weights[slot];
+    }
+  };
+  if (units > 0) ask(0);
+  Held st[NS];
+  if (mine > 0) {
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load(st[i], i);
+  }
+  for (int first = 0; first < units; first += kGroups * 2 * kDirectDown) {
+    if (first > 0) ask(first);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const int u = first + i * 2 * kDirectDown + half;
+      float amax = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+      const float s = group_scale(amax);
+      const GroupQuotient q(s);
+      if (u < units) {  // rows and groups lie one behind the other in units' order
+        *reinterpret_cast<uint32_t*>(codes + u * kBlock + 4 * lane32) = codes4(q(v[i].x), q(v[i].y), q(v[i].z), q(v[i].w));
+        if (lane32 == 0) scales[u] = s * weight[i];
+      }
+    }
+  }
+  __syncthreads();
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto compute = [&](const Held& s, int round) {
+    const int u = round * kDirectDown + wave;
+    i32x4 a[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) a[q] = *reinterpret_cast<const i32x4*>(codes + u * kBlock + kg * 16 + q * 64);
+    const f32x4 part = block_product(s.w, a);
+    const float scale = scales[u] * s.sw;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(part[e], scale, acc[e]);
+  };
+  if (mine > 0) {
+    int r = 0;
+    for (; r + NS <= mine; r += NS) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        load(st[(i + NS - 1) % NS], r + i + NS - 1);
+        compute(st[i], r + i);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+      if (r + i < mine) compute(st[i], r + i);
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave > 0 || c > 0) return;
+  f32x4 sum = red[0][lane];
+#pragma unroll
+  for (int w = 1; w < kDirectDown; ++w) sum += red[w][lane];
+  store_upto4(reinterpret_cast<OutT*>(x.out) + (size_t)token * x.hidden + n0 + 4 * kg, sum, 4);
+}
+
+size_t direct_smem(const Experts& x) { return (size_t)x.top_k * x.inter + (size_t)x.top_k * (x.inter / kBlock) * sizeof(float); }
+constexpr size_t kDirectSmem = 48 * 1024;  // a token's rows of h as codes
+
+template <typename OutT>
+int run_direct(const Experts& x, int64_t tokens, hipStream_t st) {
+  const int64_t slots = tokens * x.top_k;
+  void* ws = nullptr;
+  const int rc = workspace((size_t)slots * x.inter * sizeof(float), &ws);
+  if (rc) return rc;
+  float* const h = reinterpret_cast<float*>(ws);
+  hipLaunchKernelGGL(direct_gate_up_kernel<3>, dim3((unsigned)(slots * (x.inter / 16))), dim3(kDirectUp * 64), 0, st, x, h, ctx().flags + 3);
+  hipLaunchKernelGGL((direct_down_kernel<3, OutT>), dim3((unsigned)(tokens * (x.hidden / 16))), dim3(kDirectDown * 64), direct_smem(x), st, x,
+                     reinterpret_cast<const float*>(h));
+  PTO_CHECK_HIP(hipGetLastError());
+  return PTO_HIP_OK;
+}
+
+// ---- more tokens: the plan, two tiled products, the sum -------------------------------------------------------------------
+
+// Scratch of a pass over `tokens` tokens; y_bytes: of an element of the second product's rows.
 struct Scratch {
-  size_t order, tiles, n_tiles, h, h_scale, y, bytes;
+  size_t order, tiles, n_tiles, h, h_scale, y, y_scale, bytes;
   int max_tiles;
-  Scratch(int64_t tokens, const Experts& x, int height) {
+  Scratch(int64_t tokens, const Experts& x, int height, size_t y_bytes) {
     const int64_t slots = tokens * x.top_k;
     max_tiles = (int)(std::min<int64_t>(slots, x.experts) + slots / height);
     size_t at = 0;
@@ -114,19 +360,26 @@ struct Scratch {
     n_tiles = take(sizeof(int));
     h = take((size_t)slots * x.inter);
     h_scale = take((size_t)slots * (x.inter / kBlock) * 4);
-    y = take((size_t)slots * x.hidden * 4);
+    y = take((size_t)slots * x.hidden * y_bytes);
+    y_scale = take((size_t)slots * (x.hidden / kBlock) * 4);
     bytes = at;
   }
 };
 
 template <typename OutT>
 int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, char* ws, hipStream_t st) {
-  const int slots = (int)(tokens * x.top_k);
+  // The first product's sums decide codes of h: on the 8-bit matrix instructions, 1.4e-5 off, one in 3000 is another one, which costs a
+  // bf16 result a fifth more error (2.0e-3 against 1.7e-3) and an fp16 result five times its own rounding (1.3e-3 against 2.1e-4).
+  // The second product's only add theirs.  Its rows go through fp16 to a bf16 result, half the bytes, which adds an eighth of that result's
+  // own rounding; to an fp16 result it would add as much as that.
+  constexpr bool kExactUp = !std::is_same<OutT, __bf16>::value, kExactDown = std::is_same<OutT, float>::value;
+  typedef typename std::conditional<kExactUp, float, _Float16>::type Y;
   int32_t* order = reinterpret_cast<int32_t*>(ws + s.order);
   int4* tiles = reinterpret_cast<int4*>(ws + s.tiles);
   int* n_tiles = reinterpret_cast<int*>(ws + s.n_tiles);
-  float* y = reinterpret_cast<float*>(ws + s.y);
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, x.ids, slots, x.experts, height, order, tiles, n_tiles, ctx().flags + 3);
+  const size_t counters = (size_t)(kPlanThreads / 64) * x.experts * sizeof(int);
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), counters, st, x.ids, (int)(tokens * x.top_k), x.experts, height, order, tiles,
+                     n_tiles, ctx().flags + 3);
   Params p{};
   p.tiles = tiles;
   p.n_tiles = n_tiles;
@@ -143,35 +396,49 @@ int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, cha
   p.n = x.inter;
   p.k = x.hidden;
   p.kb = x.hidden / kBlock;
-  const int groups = x.inter / kBlock;
-  if (height == 16) hipLaunchKernelGGL((narrow_gate_up_kernel<1, 1, 4>), dim3((unsigned)(s.max_tiles * groups)), dim3(512), 0, st, p, groups);
-  else hipLaunchKernelGGL((narrow_gate_up_kernel<2, 1, 3>), dim3((unsigned)(s.max_tiles * groups)), dim3(512), 0, st, p, groups);
+  int rc;
+  if (height == 64) rc = launch_tiled<kGateUp, 64, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
+  else if (height == 128 || kExactUp) rc = launch_tiled<kGateUp, 128, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
+  else rc = launch_tiled<kGateUp, kExactUp ? 128 : 256, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
+  if (rc) return rc;
   Params d = p;
   d.a = reinterpret_cast<const uint8_t*>(ws + s.h);
   d.sa = reinterpret_cast<const float*>(ws + s.h_scale);
   d.b0 = x.down;
   d.sb0 = x.down_scale;
-  d.c = y;
+  d.c = ws + s.y;
+  d.c_scale = reinterpret_cast<float*>(ws + s.y_scale);
   d.n = x.hidden;
   d.k = x.inter;
   d.kb = x.inter / kBlock;
-  const int tiles_n = x.hidden / 32;
-  if (height == 16) hipLaunchKernelGGL((narrow_kernel<kDown, 2, 1, 4, 3, float>), dim3((unsigned)(s.max_tiles * tiles_n)), dim3(256), 0, st, d, tiles_n);
-  else hipLaunchKernelGGL((narrow_kernel<kDown, 2, 2, 4, 3, float>), dim3((unsigned)(s.max_tiles * tiles_n)), dim3(256), 0, st, d, tiles_n);
-  hipLaunchKernelGGL(combine_kernel<OutT>, dim3((unsigned)((x.hidden + 1023) / 1024), (unsigned)tokens), dim3(256), 0, st, y, x.ids, x.weights,
+  if (height == 64) rc = launch_tiled<kDown, 64, 256, kExactDown, Y>(d, s.max_tiles, st);
+  else if (height == 128 || kExactUp) rc = launch_tiled<kDown, 128, 256, kExactDown, Y>(d, s.max_tiles, st);
+  else rc = launch_tiled<kDown, kExactUp ? 128 : 256, 256, kExactDown, Y>(d, s.max_tiles, st);
+  if (rc) return rc;
+  hipLaunchKernelGGL((combine_kernel<Y, OutT>), dim3((unsigned)((x.hidden + 2047) / 2048), (unsigned)tokens), dim3(256), 0, st,
+                     reinterpret_cast<const Y*>(ws + s.y), reinterpret_cast<const float*>(ws + s.y_scale), x.ids, x.weights,
                      reinterpret_cast<OutT*>(x.out), x.hidden, x.experts, x.top_k);
   PTO_CHECK_HIP(hipGetLastError());
   return PTO_HIP_OK;
 }
 
-// Tokens are worked through in passes, so that the scratch stays below a gigabyte or two and every index inside 32 bits.
-constexpr int64_t kPassSlots = 32768;
-
 template <typename OutT>
 int run_experts(Experts x, int64_t tokens, hipStream_t st) {
+  static std::atomic<bool> attr_set{false};  // callers hold the dispatch lock
+  if (!attr_set.load(std::memory_order_acquire)) {
+    PTO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      kPlanThreads / 64 * kMaxExperts * (int)sizeof(int)));
+    attr_set.store(true, std::memory_order_release);
+  }
+  constexpr bool kExactUp = !std::is_same<OutT, __bf16>::value, kExactDown = std::is_same<OutT, float>::value;
+  int height = (int)ctx().block_gemm_rows;
+  const int64_t slots = tokens * x.top_k;
+  const bool direct = height == 0 ? experts_direct(slots, x.experts, x.hidden, x.inter) : height == 16;
+  if (direct && slots <= kMostDirectSlots && direct_smem(x) <= kDirectSmem) return run_direct<OutT>(x, tokens, st);
   const int64_t pass = std::min(tokens, std::max<int64_t>(1, kPassSlots / x.top_k));
-  const int height = pass * x.top_k <= 24 * (int64_t)x.experts ? 16 : 32;
-  const Scratch s(pass, x, height);
+  if (height < 64) height = choose_expert_rows(pass * x.top_k, x.experts, x.hidden, x.inter, kExactUp, kExactDown);
+  if (kExactUp) height = std::min(height, 128);
+  const Scratch s(pass, x, height, kExactUp ? 4 : 2);
   void* ws = nullptr;
   const int rc = workspace(s.bytes, &ws);
   if (rc) return rc;

@@ -281,4 +281,91 @@ inline int64_t attn_partition_align(int64_t pairs, int64_t max_ctx, int64_t bloc
   return align;
 }
 
+// Products of e4m3 operands with a scale for each block of 128 (block_gemm8.h, block_tiled8.h).
+struct BlockTile {
+  int rows, cols;  // tile; rows 16: the form that reads straight to registers, of cols channels a workgroup
+  int per_split;   // blocks of k of a range, 0: unsplit
+};
+struct BlockTileCost {
+  int rows, cols;
+  double block, loaded, start;  // us of a block of k, more of it with all CUs at work, start and stores of a tile
+};
+// [exact]: codes widened to bf16.  Fitted to 1800 timings of six to ten weight shapes (512 x 20000 to 16384 x 1024) at 1 to 4096 rows,
+// every tile and 1 to 16 ranges of k: off by 11 % in the mean.
+constexpr BlockTileCost kBlockTiles[2][5] = {
+    {{64, 64, 0.193, 0.071, 3.9}, {64, 128, 0.283, 0.096, 4.5}, {64, 256, 0.512, 0.182, 4.6}, {128, 256, 0.826, 0.272, 6.2}, {256, 256, 1.332, 0.440, 11.6}},
+    {{64, 64, 0.246, 0.050, 4.8}, {64, 128, 0.439, 0.081, 5.5}, {64, 256, 0.818, 0.192, 5.7}, {128, 256, 1.413, 0.381, 7.0}, {0, 0, 0.0, 0.0, 0.0}}};
+
+// The form with the least estimated time of a product of m rows, n channels and kb blocks of k.  Timed against every tile and count of
+// ranges, the one it picks among the tiles is 3 % from the best in the mean.  rows, cols, splits: given, or 0.
+// Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, or, with few channels
+// and a long k, 16 of eight (11008 x 4096 at one row 19.4 -> 10.0 us, 16384 x 1024 20.6 -> 12.2; 4096 x 14336 the other way 13.6 -> 19.5).
+inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact, int64_t num_cu, int rows, int cols, int splits) {
+  const double weights_mb = (double)n * (double)kb * 128e-6;
+  double best = 1e30;
+  BlockTile pick{128, 256, 0};
+  if ((rows == 0 && m <= 16 && splits == 0) || rows == 16) {
+    const double stream = 2.3 + weights_mb / 5.2 * (1.0 + 0.02 * (double)m);
+    const double wide = std::max(stream, 3.0 + (double)kb / 4 * (0.6 + 0.012 * (double)m));
+    best = wide;
+    pick = BlockTile{16, 32, 0};
+    if (n <= 16 * num_cu) {
+      const double few = std::max(stream, 3.0 + (double)kb / 8 * (0.55 + 0.045 * (double)m));
+      if (few < wide) {
+        best = few;
+        pick = BlockTile{16, 16, 0};
+      }
+    }
+    if (rows == 16) return pick;
+  }
+  for (const BlockTileCost& t : kBlockTiles[exact]) {
+    if (t.rows == 0 || (rows > 0 && t.rows != (exact ? std::min(rows, 128) : rows)) || (cols > 0 && t.rows == 64 && t.cols != cols)) continue;
+    const int64_t tiles = ((m + t.rows - 1) / t.rows) * ((n + t.cols - 1) / t.cols), groups = 256 / t.cols;  // groups of wavefronts along k
+    for (int64_t sp = 1; sp <= 16; ++sp) {
+      if (splits > 0 ? sp != std::min<int64_t>(splits, kb) : sp > 1 && kb / sp < 8) continue;
+      const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per, wgs = tiles * ranges;
+      const double load = std::min(1.0, (double)wgs / (double)num_cu);
+      double us = (double)((wgs + num_cu - 1) / num_cu) * ((double)((per + groups - 1) / groups * groups) * (t.block + t.loaded * load) + t.start);
+      us = std::max(us, 4.0 + weights_mb / 4.2);
+      if (ranges > 1) us += 4.1 + (double)ranges * (double)m * (double)n * 8e-6 / 4.6;
+      if (us < best) {
+        best = us;
+        pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0};
+      }
+    }
+  }
+  return pick;
+}
+
+// Whether the experts' FFN of so many slots reads every slot's matrices for itself instead of planning tiles (experts.hip), by the
+// bytes that either form reads and what it starts with.  Measured, one token on, us direct / tiles: 8 of 64 experts of 4096 x
+// 1408 41 / 54, 73 / 70, 107 / 95; 4 of 60 of 2048 x 1024 16 / 32, 22 / 36, 30 / 37, 35 / 39, 51 / 42 at six; 8 of 128 of 1024 x 512 14 / 27 to 31
+// / 36 at eight, 46 / 43 at twelve; 2 of 8 of 5120 x 4096 42 / 73, 72 / 77, 100 / 81.
+inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
+  const double mb = 3e-6 * (double)hidden * (double)inter;
+  double unused = (double)experts;
+  for (int64_t i = 0; i < slots && i < 4096; ++i) unused *= 1.0 - 1.0 / (double)experts;
+  return 5.0 + (double)slots * mb / 4.0 < 26.0 + ((double)experts - unused) * mb / 5.2;
+}
+
+// Tile height of both products of the experts' FFN: the least sum over the tiles of what they cost, an expert's rows filling up half a tile in the
+// mean.  8 of 64 experts of 4096 x 1408, 64 / 128 / 256 rows, us: 256 tokens 248 / 254 / 307, 512 304 / 288 / 331, 1024 414 / 384 / 384, 4096 1279 / 1036 / 946.
+inline int choose_expert_rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, bool exact_up, bool exact_down) {
+  const double used = (double)std::min(slots, experts), each = (double)slots / used;
+  double best = 1e30;
+  int pick = 64;
+  for (int i = 2; i < 5; ++i) {
+    const BlockTileCost &up = kBlockTiles[exact_up][i], &down = kBlockTiles[exact_down][i];
+    if (up.rows == 0 || down.rows == 0) continue;
+    const double tiles = used * std::max(1.0, each / up.rows + 0.5);
+    auto cost = [](const BlockTileCost& t, int64_t kb) { return (double)kb * (t.block + t.loaded) + t.start; };
+    const double us = tiles * ((double)(inter / 128) * cost(up, hidden / 128) + (double)((hidden + 255) / 256) * cost(down, inter / 128));
+    if (us < best) {
+      best = us;
+      pick = up.rows;
+    }
+  }
+  return pick;
+}
+
 }  // namespace pto_hip

@@ -29,4 +29,12 @@ __device__ __forceinline__ void to_lds(uint32_t voff, const void* sbase, uint32_
 #pragma clang diagnostic pop
 }
 
+// One 4-byte request per lane from sbase + voff to the 256 bytes of LDS at lds_w (wave-uniform).
+__device__ __forceinline__ void to_lds_dword(uint32_t voff, const void* sbase, uint32_t lds_w) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_w) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
 }  // namespace pto_hip

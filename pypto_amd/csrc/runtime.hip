@@ -1273,7 +1273,13 @@ int pto_hip_set_option(const char* name, int64_t value) {
   } else if (!std::strcmp(name, "w8a16_gemm_rows")) {
     PTO_CHECK_ARG(value >= 0 && value <= (1 << 20), "w8a16_gemm_rows must be in [0, 2^20]");
     c.w8a16_gemm_rows = value;
-
+  } else if (!std::strcmp(name, "block_gemm_rows")) {
+    PTO_CHECK_ARG(value == 0 || value == 16 || value == 64 || value == 128 || value == 256,
+                  "block_gemm_rows must be 0, 16, 64, 128 or 256");
+    c.block_gemm_rows = value;
+  } else if (!std::strcmp(name, "block_gemm_cols")) {
+    PTO_CHECK_ARG(value == 0 || value == 64 || value == 128 || value == 256, "block_gemm_cols must be 0, 64, 128 or 256");
+    c.block_gemm_cols = value;
   } else {
     return fail(PTO_HIP_ERR_NOT_FOUND, "unknown option '%s'", name);
   }
@@ -1337,6 +1343,8 @@ int pto_hip_get_option(const char* name, int64_t* value) {
   else if (!std::strcmp(name, "skinny_fused")) *value = c.skinny_fused;
   else if (!std::strcmp(name, "w8a16_wide")) *value = c.w8a16_wide;
   else if (!std::strcmp(name, "w8a16_gemm_rows")) *value = c.w8a16_gemm_rows;
+  else if (!std::strcmp(name, "block_gemm_rows")) *value = c.block_gemm_rows;
+  else if (!std::strcmp(name, "block_gemm_cols")) *value = c.block_gemm_cols;
   else return fail(PTO_HIP_ERR_NOT_FOUND, "unknown option '%s'", name);
   return PTO_HIP_OK;
 }

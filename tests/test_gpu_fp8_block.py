@@ -164,13 +164,32 @@ def _product(worker, a, sa, w, sw, dtype):
     return out.t
 
 
+@pytest.fixture(params=[0, 16, 64, 128, 256])
+def rows(request, worker):
+    """Every height of a product's tiles, the library's own choice first."""
+    worker.set_option("block_gemm_rows", request.param)
+    yield request.param
+    worker.set_option("block_gemm_rows", 0)
+
+
+# ... and, of a projection's, every width and several ranges of k
+@pytest.fixture(params=[(0, 0, 0), (16, 0, 0), (64, 64, 0), (64, 128, 0), (64, 256, 0), (128, 0, 0), (256, 0, 0), (64, 64, 3), (64, 128, 2), (64, 256, 4),
+                        (128, 0, 3), (256, 0, 2)], ids=str)
+def tile(request, worker):
+    for name, value in zip(("block_gemm_rows", "block_gemm_cols", "gemm_splits"), request.param):
+        worker.set_option(name, value)
+    yield request.param
+    for name in ("block_gemm_rows", "block_gemm_cols", "gemm_splits"):
+        worker.set_option(name, 0)
+
+
 @pytest.mark.parametrize("m,k,n", PRODUCT_SHAPES)
-def test_product_is_exact_on_whole_numbers_and_stays_inside(worker, m, k, n):
+def test_product_is_exact_on_whole_numbers_and_stays_inside(worker, tile, m, k, n):
     """Whole numbers up to 8 and scales of 2^-8 and 2^-7: every sum is a multiple of 2^-16 below 64 * 4224 * 2^-14, which
     fp32 holds exactly in any order.  Past the operands' ends lie NaN codes."""
     g = torch.Generator().manual_seed(m + k + n)
-    num = lambda rows: torch.randint(-8, 9, (rows, k), generator=g).float()
-    scale = lambda rows: torch.exp2(-7.0 - torch.randint(0, 2, (rows, k // 128), generator=g).float())
+    num = lambda count: torch.randint(-8, 9, (count, k), generator=g).float()
+    scale = lambda count: torch.exp2(-7.0 - torch.randint(0, 2, (count, k // 128), generator=g).float())
     a, w, sa, sw = num(m), num(n), scale(m), scale(-(-n // 128))
     want = ob.projection(a.cuda(), sa.cuda(), w.cuda(), sw.cuda())
     fenced = lambda t: _Fenced(t.shape, torch.float32, fill=0xFF, inside=t).t  # all ones: a NaN
@@ -187,7 +206,7 @@ def _operands(g, m, k, n):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,k,n", [(1, 4096, 515), (24, 2816, 96), (130, 4096, 256), (300, 11008, 300), (600, 1024, 900)])
-def test_product_on_quantised_values(worker, m, k, n, dtype):
+def test_product_on_quantised_values(worker, tile, m, k, n, dtype):
     """fp32 sums of k products in any order: at most (128 + k / 128 + 4) roundings in a row, each of the sum of magnitudes."""
     a, sa, w, sw = _operands(_gen(k + n), m, k, n)
     got = _product(worker, a, sa, w, sw, dtype).double()
@@ -197,7 +216,7 @@ def test_product_on_quantised_values(worker, m, k, n, dtype):
     assert ((got - want).abs() <= bound + (want.abs() + bound) * HALF_STEP[dtype] + TINY[dtype]).all()
 
 
-def test_product_rows_do_not_depend_on_their_batch(worker):
+def test_product_rows_do_not_depend_on_their_batch(worker, tile):
     """A row's scales and codes are its own: NaN in one row stays in that row."""
     a, sa, w, sw = _operands(_gen(9), 70, 1024, 260)
     want = _product(worker, a, sa, w, sw, torch.float32)
@@ -361,14 +380,14 @@ EXPERT_SHAPES = [(1, 256, 128, 4, 2), (1, 1024, 1408, 16, 8), (2, 128, 256, 8, 1
 
 
 @pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", EXPERT_SHAPES)
-def test_experts(worker, tokens, hidden, inter, experts, top_k):
+def test_experts(worker, rows, tokens, hidden, inter, experts, top_k):
     args = _experts_case(tokens + hidden, tokens, hidden, inter, experts, top_k)
     for dtype in (torch.bfloat16, torch.float16, torch.float32):
         _check_experts(worker, args, dtype)
 
 
 @pytest.mark.parametrize("tokens", [1, 5, 90, 600])
-def test_experts_on_uneven_routes(worker, tokens):
+def test_experts_on_uneven_routes(worker, rows, tokens):
     """Slots without an expert, tokens without any, one expert for all, the same expert twice in a row."""
     args = _experts_case(tokens, tokens, 384, 256, 12, 4)
     ids = args[2]
@@ -396,7 +415,7 @@ def test_an_expert_that_there_is_not_is_left_out_and_reported(worker):
     assert ((out.double() - want).abs() <= slack + want.abs() * 2.0 ** -24).all()
 
 
-def test_a_token_s_result_does_not_depend_on_its_batch(worker):
+def test_a_token_s_result_does_not_depend_on_its_batch(worker, rows):
     """NaN and infinities of one token, and weights that nobody asked for, reach no other token."""
     args = _experts_case(8, 50, 512, 256, 16, 3)
     args[2].clamp_(max=14)
