@@ -43,7 +43,7 @@ def _codes_of(values):
 
 # ---- norm and quantiser --------------------------------------------------------------------------------
 
-NORM_SHAPES = [(1, 8), (3, 120), (2, 128), (5, 136), (7, 1000), (4, 2048), (3, 2056), (2, 4104), (33, 5120), (3, 8200), (2, 16384)]
+NORM_SHAPES = [(2100, 8200), (1, 8), (3, 120), (2, 128), (5, 136), (7, 1000), (4, 2048), (3, 2056), (2, 4104), (33, 5120), (3, 8200), (2, 16384)]
 
 
 def _check_codes(codes, scale, n, slack):
