@@ -59,7 +59,7 @@ struct TiledShape {
   static constexpr int kScaleRow8 = 264;                 // bytes of a request of those
   static constexpr int kScaleBuf = BM / 8 * kScaleRow8;
   static constexpr int kScales = RING * kStage, kChannelScales = kScales + 2 * kScaleBuf;
-  static size_t smem(int kb) { return (size_t)kChannelScales + 2 * (size_t)kb * sizeof(float); }
+  static constexpr size_t smem(int kb) { return (size_t)kChannelScales + 2 * (size_t)((kb + 63) / 64 * 64) * sizeof(float); }
   static_assert(KG == 1 || PH == 1, "groups along k have one half of rows");
 };
 
@@ -91,16 +91,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int n0 = tn * (GATE ? kBlock : BN);
   const int nk = SPLIT && p.per_split ? min(p.per_split, p.kb - k0) : p.kb;
 
-  // ---- the channels' scales, all of k ----
-  lds_float* const s_cols = (lds_float*)(lds0 + S::kChannelScales);  // [2][nk]: two blocks of channels, or gate and up
+  // ---- the channels' scales, all of k: two blocks of channels, or gate and up ----
+  const int nk64 = (nk + 63) / 64 * 64;  // a request brings 64
+  lds_float* const s_cols = (lds_float*)(lds0 + S::kChannelScales);  // [2][nk64]
+  const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds0);
   {
     const int blocks_n = (p.n + kBlock - 1) / kBlock, at = tile.expert * blocks_n;
     const float* c0 = p.sb0 + (size_t)(at + n0 / kBlock) * p.kb + k0;
     const float* c1 = (GATE ? p.sb1 : p.sb0) + (size_t)(at + (GATE ? n0 / kBlock : min(n0 / kBlock + 1, blocks_n - 1))) * p.kb + k0;
-    for (int i = tid; i < nk; i += 512) {
-      s_cols[i] = c0[i];
-      s_cols[nk + i] = c1[i];
-    }
+    for (int i = (wave >> 1) * 64; i < nk; i += 256)
+      to_lds_dword((uint32_t)min(i + lane, nk - 1) * 4u, wave & 1 ? c1 : c0, lds_base + S::kChannelScales + ((wave & 1) * nk64 + i) * 4);
   }
 
   // ---- requests: instruction e of a part brings its rows 64 e + 8 wave + lane / 8; rows and channels past the end are clamped
@@ -129,7 +129,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // scales: request e of wavefront w brings rows 8 (e * 8 + w) .. +8, block lane % 8 of eight
 #pragma unroll
   for (int e = 0; e < S::NS; ++e) vs[e] = row_at((e * 8 + wave) * 8 + (lane >> 3)) * (uint32_t)p.kb;
-  const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds0);
   const uint32_t lds_w = lds_base + wave * 1024;
   // the first half (all, if there is one) or the second of the rows, and the channels, of stage t (past the last one: the last block)
   auto request_a = [&](auto half_c, int t, uint32_t slot) {
@@ -307,7 +306,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // not finite has made the same results NaN already).
     const int block = S::KG == 1 ? t : min(t * S::KG + kg, nk - 1);
     const bool spare = S::KG > 1 && t * S::KG + kg >= nk;
-    float s0 = s_cols[(GATE ? 0 : wn / 2) * nk + block], s1 = GATE ? s_cols[nk + block] : 0.f;
+    float s0 = s_cols[(GATE ? 0 : wn / 2) * nk64 + block], s1 = GATE ? s_cols[nk64 + block] : 0.f;
     const uint32_t s_at = s_off + ((block >> 3) & 1) * S::kScaleBuf + (block & 7) * 4;
     auto one = [&](auto i_c) {
       constexpr int I = decltype(i_c)::value, H = I / S::HF, ROW = H * (BM / S::PH) + (I % S::HF) * 32;
@@ -349,13 +348,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int r = 0; r < 16; ++r) sums[((wave - 2 * S::WN) * 32 + j * 16 + r) * 64 + lane] = acc[0][j][r];
     }
     __syncthreads();
-    if (kg > 0) return;
+    if (kg == 0) {
 #pragma unroll
-    for (int g = 0; g < S::KG - 1; ++g)
+      for (int g = 0; g < S::KG - 1; ++g)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[0][j][r] += sums[((g * 2 * S::WN + wave) * 32 + j * 16 + r) * 64 + lane];
+          for (int r = 0; r < 16; ++r) acc[0][j][r] += sums[((g * 2 * S::WN + wave) * 32 + j * 16 + r) * 64 + lane];
+    }
+    __syncthreads();
   }
 
   // ---- epilogue: acc[i][j][r] is row r0 + lane % 32 of the tile, channel 32 j + (r / 4) * 8 + hi * 4 + r % 4 of the wavefront's 64 ----
@@ -393,53 +394,75 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const int row = u >> 3;
       *reinterpret_cast<i32x4*>(codes + (size_t)tile.c_row(row) * p.n + n0 + (u & 7) * 16) = *reinterpret_cast<const i32x4*>(smem + u * 16);
     }
-  } else if constexpr (MAP == kDown && std::is_same<OutT, _Float16>::value) {
-    // rows for the sum over a token's experts: fp16 with a power of two per row and 128 channels that puts the largest below 2^15
-    lds_float* const top = (lds_float*)(lds0 + S::kScales);  // [4][BM]
-#pragma unroll
-    for (int i = 0; i < S::MF; ++i) {
-      float amax = 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) amax = fmaxf(amax, finite_size(acc[i][j][r]));
-      amax = fmaxf(amax, __shfl_xor(amax, 32));
-      if (hi == 0) top[wn * BM + row_of(i)] = amax;
-    }
-    __syncthreads();
-    const int group = n0 / kBlock + wn / 2;
-#pragma unroll
-    for (int i = 0; i < S::MF; ++i) {
-      const int row = row_of(i);
-      if (row >= tile.rows || group * kBlock >= p.n) continue;
-      const size_t at = tile.c_row(row);
-      const int e = half_exponent(fmaxf(top[(wn & ~1) * BM + row], top[(wn | 1) * BM + row]));
-      if ((wn & 1) == 0 && hi == 0) p.c_scale[at * (p.n / kBlock) + group] = __builtin_ldexpf(1.f, e);
-      _Float16* const dst = reinterpret_cast<_Float16*>(p.c) + at * p.n + n0 + wn * 64 + hi * 4;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          f32x4 y;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = __builtin_ldexpf(acc[i][j][4 * v + r], -e);
-          store_upto4(dst + j * 32 + v * 8, y, 4);
-        }
-    }
   } else {
-    OutT* const c = reinterpret_cast<OutT*>(p.c) + (size_t)range * p.m * p.n;
+    // Rows go through LDS, a half of them at a time, so that they are written in whole lines: straight from the accumulators a wavefront's
+    // store has 16 bytes of each of 32 rows.
+    constexpr bool SCALED = MAP == kDown && std::is_same<OutT, _Float16>::value;
+    constexpr int ROWS = BM / S::PH, PITCH = BN * (int)sizeof(OutT) + 16;  // bytes; the padding spreads rows over the banks
+    static_assert(ROWS * PITCH <= (SCALED ? (int)S::kScales : (int)S::kChannelScales), "a half of the rows fits");
+    int e[S::MF];  // SCALED: rows for the sum over a token's experts, fp16 with a power of two per row and 128 channels that puts the largest below 2^15
 #pragma unroll
-    for (int i = 0; i < S::MF; ++i) {
-      const int row = row_of(i);
-      if (row >= tile.rows) continue;
-      OutT* const dst = c + (size_t)tile.c_row(row) * p.n;
+    for (int i = 0; i < S::MF; ++i) e[i] = 0;
+    if constexpr (SCALED) {
+      lds_float* const top = (lds_float*)(lds0 + S::kScales);  // [4][BM]
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int i = 0; i < S::MF; ++i) {
+        float amax = 0.f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int col = n0 + wn * 64 + j * 32 + v * 8 + hi * 4;
-          if (col < p.n) store_upto4(dst + col, f32x4{acc[i][j][4 * v], acc[i][j][4 * v + 1], acc[i][j][4 * v + 2], acc[i][j][4 * v + 3]}, p.n - col);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) amax = fmaxf(amax, finite_size(acc[i][j][r]));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        if (hi == 0) top[wn * BM + row_of(i)] = amax;
+      }
+      __syncthreads();
+      const int group = n0 / kBlock + wn / 2;
+#pragma unroll
+      for (int i = 0; i < S::MF; ++i) {
+        const int row = row_of(i);
+        e[i] = half_exponent(fmaxf(top[(wn & ~1) * BM + row], top[(wn | 1) * BM + row]));
+        if ((wn & 1) == 0 && hi == 0 && row < tile.rows && group * kBlock < p.n)
+          p.c_scale[(size_t)tile.c_row(row) * (p.n / kBlock) + group] = __builtin_ldexpf(1.f, e[i]);
+      }
+    }
+    OutT* const c = reinterpret_cast<OutT*>(p.c) + (size_t)range * p.m * p.n + n0;
+    const int cols = min(BN, p.n - n0);
+    const bool whole = p.n % (16 / (int)sizeof(OutT)) == 0 && (uintptr_t)p.c % 16 == 0 && ((size_t)range * p.m * p.n * sizeof(OutT)) % 16 == 0;
+#pragma unroll
+    for (int h = 0; h < S::PH; ++h) {
+      if (kg == 0) {
+#pragma unroll
+        for (int f = 0; f < S::HF; ++f) {
+          const int i = h * S::HF + f;
+          uint8_t* const dst = smem + (row_of(i) - h * ROWS) * PITCH + (wn * 64 + hi * 4) * (int)sizeof(OutT);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              typedef __attribute__((__vector_size__(4 * sizeof(OutT)))) OutT vec4;
+              vec4 y;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) y[r] = (OutT)(SCALED ? __builtin_ldexpf(acc[i][j][4 * v + r], -e[i]) : acc[i][j][4 * v + r]);
+              *reinterpret_cast<vec4*>(dst + (j * 32 + v * 8) * (int)sizeof(OutT)) = y;
+            }
         }
+      }
+      __syncthreads();
+      const int rows = min(ROWS, tile.rows - h * ROWS);
+      if (whole) {
+        constexpr int VEC = 16 / (int)sizeof(OutT), PER_ROW = BN / VEC;
+        for (int u = tid; u < rows * PER_ROW; u += 512) {
+          const int row = u / PER_ROW, at = u % PER_ROW;
+          if (at * VEC < cols)
+            *reinterpret_cast<i32x4*>(c + (size_t)tile.c_row(h * ROWS + row) * p.n + at * VEC) = *reinterpret_cast<const i32x4*>(smem + row * PITCH + at * 16);
+        }
+      } else {
+        for (int u = tid; u < rows * BN; u += 512) {
+          const int row = u / BN, at = u % BN;
+          if (at < cols) c[(size_t)tile.c_row(h * ROWS + row) * p.n + at] = reinterpret_cast<const OutT*>(smem + row * PITCH)[at];
+        }
+      }
+      if (h + 1 < S::PH) __syncthreads();
     }
   }
 }

@@ -290,14 +290,14 @@ struct BlockTileCost {
   int rows, cols;
   double block, loaded, start;  // us of a block of k, more of it with all CUs at work, start and stores of a tile
 };
-// [exact]: codes widened to bf16.  Fitted to 1800 timings of six to ten weight shapes (512 x 20000 to 16384 x 1024) at 1 to 4096 rows,
-// every tile and 1 to 16 ranges of k: off by 11 % in the mean.
+// [exact]: codes widened to bf16.  Fitted to 1560 timings of ten weight shapes (512 x 20000 to 16384 x 1024) at 24 to 4096 rows,
+// every tile and 1 to 8 ranges of k: off by 7 % in the mean, exact 5 %.
 constexpr BlockTileCost kBlockTiles[2][5] = {
-    {{64, 64, 0.193, 0.071, 3.9}, {64, 128, 0.283, 0.096, 4.5}, {64, 256, 0.512, 0.182, 4.6}, {128, 256, 0.826, 0.272, 6.2}, {256, 256, 1.332, 0.440, 11.6}},
-    {{64, 64, 0.246, 0.050, 4.8}, {64, 128, 0.439, 0.081, 5.5}, {64, 256, 0.818, 0.192, 5.7}, {128, 256, 1.413, 0.381, 7.0}, {0, 0, 0.0, 0.0, 0.0}}};
+    {{64, 64, 0.217, 0.044, 3.6}, {64, 128, 0.299, 0.081, 3.8}, {64, 256, 0.533, 0.173, 3.6}, {128, 256, 0.847, 0.228, 5.4}, {256, 256, 1.308, 0.444, 6.9}},
+    {{64, 64, 0.254, 0.051, 4.7}, {64, 128, 0.440, 0.098, 5.2}, {64, 256, 0.826, 0.212, 5.3}, {128, 256, 1.429, 0.327, 7.1}, {0, 0, 0.0, 0.0, 0.0}}};
 
 // The form with the least estimated time of a product of m rows, n channels and kb blocks of k.  Timed against every tile and count of
-// ranges, the one it picks among the tiles is 3 % from the best in the mean.  rows, cols, splits: given, or 0.
+// ranges, the one it picks among the tiles is 1.4 % from the best in the mean and 22 % at worst, exact 0.3 % and 9 %.  rows, cols, splits: given, or 0.
 // Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, or, with few channels
 // and a long k, 16 of eight (11008 x 4096 at one row 19.4 -> 10.0 us, 16384 x 1024 20.6 -> 12.2; 4096 x 14336 the other way 13.6 -> 19.5).
 inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact, int64_t num_cu, int rows, int cols, int splits) {
@@ -326,8 +326,8 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
       const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per, wgs = tiles * ranges;
       const double load = std::min(1.0, (double)wgs / (double)num_cu);
       double us = (double)((wgs + num_cu - 1) / num_cu) * ((double)((per + groups - 1) / groups * groups) * (t.block + t.loaded * load) + t.start);
-      us = std::max(us, 4.0 + weights_mb / 4.2);
-      if (ranges > 1) us += 4.1 + (double)ranges * (double)m * (double)n * 8e-6 / 4.6;
+      us = std::max(us, 4.0 + weights_mb / 4.5);
+      if (ranges > 1) us += 4.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
       if (us < best) {
         best = us;
         pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0};
