@@ -368,7 +368,7 @@ PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* sca
 
 /* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
  * codes = e4m3(n / scale), round to nearest even; sum_out = x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every
- * output is rounded once.  residual, gamma, sum_out and normed_out may each be NULL; sum_out may be x or residual itself.  NaN
+ * output is rounded once (a row whose sum of squares passes fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out may each be NULL; sum_out may be x or residual itself.  NaN
  * elements are left out of amax and give NaN codes.  cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the
  * last group may be shorter).  quantize_fp8_block: codes and scales of x itself. */
 PTO_HIP_API int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out,
@@ -380,7 +380,7 @@ PTO_HIP_API int pto_hip_quantize_fp8_block(const void* x, void* codes, float* sc
 /* out[m, n] = sum_kb a_scale[m, kb] * w_scale[n / 128, kb] * sum_{k in block kb} a8[m, k] * w8[n, k], any M and N; K a multiple
  * of 128 and at most 65536 (PTO_HIP_ERR_UNSUPPORTED otherwise).  out FP32, BF16 or FP16.  Blocks are added in fp32.  Inside a block the
  * 8-bit matrix instructions drop what lies 2^-13 below the largest of eight products, 1.4e-5 of the result in norm; with FP32
- * results, and up to 16 rows, the codes are widened and nothing is dropped. */
+ * results, and in the form for few rows, the codes are widened and nothing is dropped.  The form is chosen by M, N and K. */
 PTO_HIP_API int pto_hip_projection_fp8_block(const void* a8, const float* a_scale, const void* w8, const float* w_scale, void* out,
                                              int64_t m, int64_t k, int64_t n, int out_dtype, void* stream);
 
@@ -401,9 +401,10 @@ PTO_HIP_API int pto_hip_route_experts(const void* logits, const float* bias, int
  * experts' half of a mixture layer behind pto_hip_rms_norm_fp8_block and pto_hip_route_experts.  Products as
  * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 as pto_hip_quantize_fp8_block does, the sum over a token's
  * experts is fp32.  A negative id leaves its slot out (a token without any gives zeros); an id of an expert that there is
- * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  Where out is BF16 both products are as
- * pto_hip_projection_fp8_block's of 16-bit results, where it is FP16 the second one is; the widened form has the rest.  With
- * BF16 results the experts' rows are added from fp16 with a power of two per 128 channels.  H and I multiples of 128 and at most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the
+ * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  With BF16 results of many
+ * tokens both products are as pto_hip_projection_fp8_block's of 16-bit results, and the experts' rows are added from fp16 with a
+ * power of two per 128 channels; with FP16 results the second product is; the widened form has the rest.  H and I multiples of 128
+ * and at most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the
  * other: w_gate8, w_up8 [E, I, H], w_down8 [E, H, I].  out FP32, BF16 or FP16. */
 PTO_HIP_API int pto_hip_experts_ffn_fp8_block(const void* x8, const float* x_scale, const int32_t* expert_ids,
                                               const float* expert_weights, const void* w_gate8, const float* w_gate_scale,

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 namespace pto_hip {
@@ -343,8 +344,7 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
 // / 36 at eight, 46 / 43 at twelve; 2 of 8 of 5120 x 4096 42 / 73, 72 / 77, 100 / 81.
 inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
   const double mb = 3e-6 * (double)hidden * (double)inter;
-  double unused = (double)experts;
-  for (int64_t i = 0; i < slots && i < 4096; ++i) unused *= 1.0 - 1.0 / (double)experts;
+  const double unused = (double)experts * std::pow(1.0 - 1.0 / (double)experts, (double)slots);
   return 5.0 + (double)slots * mb / 4.0 < 26.0 + ((double)experts - unused) * mb / 5.2;
 }
 

@@ -14,6 +14,7 @@
 // 2048 31.6 / 25.7 and 44.2 / 38.5; but 1024 x 4096 9.3 / 8.2 and 20.9 / 22.4, 512 x 4096 8.3 / 7.6 and 18.8 / 20.7.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "block_fp8.h"
@@ -29,6 +30,7 @@ using pto_hip::block8::kBlock;
 constexpr int kThreads = 256;
 constexpr int kVecs = 8;  // most groups of eight columns a thread holds
 constexpr int64_t kStreamBytes = 32 << 20;
+constexpr int64_t kLaunchRows = 1 << 23;  // a launch holds fewer than 2^32 threads
 
 template <bool STREAM, typename V>
 __device__ __forceinline__ void store(V* to, const V& v) {
@@ -160,8 +162,15 @@ int run(const char* what, bool norm, const void* x, const void* residual, const 
   PTO_CHECK_ARG(!sum_out || sum_out != normed_out, "%s: sum_out and normed_out are the same tensor", what);
   const bool stream = rows * cols * (1 + 2 * (sum_out != nullptr) + 2 * (normed_out != nullptr)) > kStreamBytes;
   auto go = [&](auto type, auto norm_c, auto stream_c) {
-    return launch<decltype(type), decltype(norm_c)::value, decltype(stream_c)::value>(x, residual, gamma, sum_out, normed_out, codes, scale, rows,
-                                                                                     cols, eps, st);
+    auto from = [&](auto* p, int64_t bytes) { return p ? reinterpret_cast<decltype(p)>((uintptr_t)p + bytes) : nullptr; };
+    for (int64_t r = 0; r < rows; r += kLaunchRows) {
+      const int64_t at = r * cols;
+      const int rc = launch<decltype(type), decltype(norm_c)::value, decltype(stream_c)::value>(
+          from(x, 2 * at), from(residual, 2 * at), gamma, from(sum_out, 2 * at), from(normed_out, 2 * at), from(codes, at),
+          scale + r * ((cols + block8::kBlock - 1) / block8::kBlock), std::min(kLaunchRows, rows - r), cols, eps, st);
+      if (rc) return rc;
+    }
+    return (int)PTO_HIP_OK;
   };
   auto typed = [&](auto type) {
     if (norm) return stream ? go(type, std::true_type{}, std::true_type{}) : go(type, std::true_type{}, std::false_type{});

@@ -14,12 +14,15 @@
 // best of a wavefront is an integer maximum.  Bound by the chain of top_k maxima (six lane exchanges each), not by memory.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxGroups = 64, kMaxTopK = 64;
 constexpr int kWaves = 4;  // tokens of a workgroup
+constexpr int64_t kLaunchTokens = 1 << 25;  // a launch holds fewer than 2^32 threads
 
 struct Params {
   const void* logits;
@@ -356,12 +359,18 @@ extern "C" int pto_hip_route_experts(const void* logits, const float* bias, int3
                 "route_experts: misaligned operand");
   int group_lanes = 64;
   while (group_lanes * n_groups > 64) group_lanes /= 2;
-  const Params p{logits, bias, expert_ids, expert_weights, (int)tokens, (int)experts, (int)top_k, (int)n_groups, (int)topk_groups,
-                 (int)(experts / n_groups), group_lanes, score_fn == PTO_HIP_SCORE_SIGMOID, renormalize != 0, scale};
+  Params p{logits, bias, expert_ids, expert_weights, (int)tokens, (int)experts, (int)top_k, (int)n_groups, (int)topk_groups,
+           (int)(experts / n_groups), group_lanes, score_fn == PTO_HIP_SCORE_SIGMOID, renormalize != 0, scale};
   hipStream_t st = (hipStream_t)stream;
-  if (logits_dtype == PTO_HIP_FP32) bias ? launch<float, true>(p, st) : launch<float, false>(p, st);
-  else if (logits_dtype == PTO_HIP_BF16) bias ? launch<__bf16, true>(p, st) : launch<__bf16, false>(p, st);
-  else bias ? launch<_Float16, true>(p, st) : launch<_Float16, false>(p, st);
+  for (int64_t t = 0; t < tokens; t += kLaunchTokens) {
+    p.logits = reinterpret_cast<const char*>(logits) + t * experts * dtype_bytes(logits_dtype);
+    p.ids = expert_ids + t * top_k;
+    p.weights = expert_weights + t * top_k;
+    p.tokens = (int)std::min(kLaunchTokens, tokens - t);
+    if (logits_dtype == PTO_HIP_FP32) bias ? launch<float, true>(p, st) : launch<float, false>(p, st);
+    else if (logits_dtype == PTO_HIP_BF16) bias ? launch<__bf16, true>(p, st) : launch<__bf16, false>(p, st);
+    else bias ? launch<_Float16, true>(p, st) : launch<_Float16, false>(p, st);
+  }
   PTO_CHECK_HIP(hipGetLastError());
   return PTO_HIP_OK;
 }

@@ -534,3 +534,149 @@ def test_a_captured_layer_on_another_stream(worker, tokens):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(layer.results(), want)), i
     worker.sync()
+
+
+# ---- the ends of what is allowed -----------------------------------------------------------------------
+
+
+def test_norm_of_more_rows_than_a_launch_holds(worker):
+    """The last rows have the bits of a call on them alone."""
+    rows, cols, last = (1 << 23) + 5, 8, 9
+    g = _gen(1)
+    x, r, gamma = _randn(g, rows, cols).bfloat16(), _randn(g, rows, cols).bfloat16(), 1 + 0.1 * _randn(g, cols)
+
+    def call(x, r):
+        n = len(x)
+        outs = [torch.empty((n, cols), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        outs += [torch.empty((n, cols), dtype=F8, device="cuda"), torch.empty((n, 1), device="cuda")]
+        worker.run(runtime.add_rms_norm_fp8_block_normed, x, r, gamma, *outs, 1e-6)
+        worker.sync()
+        outs[2] = outs[2].view(torch.uint8)
+        return outs
+
+    for got, want in zip(call(x, r), call(x[-last:].contiguous(), r[-last:].contiguous())):
+        assert torch.equal(got[-last:], want)
+
+
+def test_router_of_more_tokens_than_a_launch_holds(worker):
+    tokens, last = (1 << 25) + 3, 7
+    logits = torch.randint(-100, 100, (tokens, 3), dtype=torch.int8, device="cuda", generator=_gen(2)).bfloat16()
+    bias = torch.tensor([0.0, 0.1, -0.1], device="cuda")
+
+    def call(logits):
+        ids, weights = torch.empty((len(logits), 2), dtype=torch.int32, device="cuda"), torch.empty((len(logits), 2), device="cuda")
+        worker.run(runtime.route_experts_biased, logits, bias, ids, weights, 1, 1, 1, 1, 1.0)
+        worker.sync()
+        return ids, weights
+
+    for got, want in zip(call(logits), call(logits[-last:].contiguous())):
+        assert torch.equal(got[-last:], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m", [3, 16, 70])
+def test_product_of_the_longest_rows(worker, tile, m, dtype):
+    a, sa, w, sw = _operands(_gen(m), m, 65536, 130)
+    got = _product(worker, a, sa, w, sw, dtype).double()
+    want = ob.projection(a, sa, w, sw)
+    sizes = ob.dequantize_rows(a, sa).abs() @ ob.dequantize_matrix(w, sw).abs().t()
+    bound = sizes * (132 + 512) * 2.0 ** -24
+    assert ((got - want).abs() <= bound + (want.abs() + bound) * HALF_STEP[dtype] + TINY[dtype]).all()
+
+
+@pytest.mark.parametrize("m,k,n", [(5, 384, 100), (130, 640, 256), (300, 1024, 512)])
+def test_product_on_scales_and_results_aligned_to_their_elements(worker, tile, m, k, n):
+    """One element behind a 16-byte boundary: the bits of the call on aligned ones."""
+    a, sa, w, sw = _operands(_gen(k), m, k, n)
+    shifted = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    want = _product(worker, a, sa, w, sw, torch.float32)
+    out = _Fenced((m * n + 1,), torch.float32)
+    worker.run(runtime.projection_fp8_block, a, shifted(sa), w, shifted(sw), out.t[1:].view(m, n))
+    worker.sync()
+    assert torch.equal(out.t[1:].view(m, n), want) and out.intact()
+
+
+@pytest.mark.parametrize("tile", [(0, 0, 0), (64, 64, 0), (64, 128, 0), (64, 256, 0), (128, 0, 0), (256, 0, 0)], ids=str, indirect=True)
+def test_product_past_32_bits(worker, tile):
+    """Rows that lie beyond the first 4 GB of codes, and results beyond the first 4 GB."""
+    m, k, n, last = (1 << 18) + 33, 16512, 8320, 40
+    a = torch.empty((m, k), dtype=torch.uint8, device="cuda")
+    sa = torch.empty((m, k // 128), device="cuda")
+    tail, scales, w, sw = _operands(_gen(3), last, k, n)
+    a[:], sa[:] = 0, 1
+    a[-last:], sa[-last:] = tail.view(torch.uint8), scales
+    out = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    worker.run(runtime.projection_fp8_block, a.view(F8), sa, w, sw, out)
+    worker.sync()
+    want = ob.projection(tail, scales, w, sw)
+    bound = (ob.dequantize_rows(tail, scales).abs() @ ob.dequantize_matrix(w, sw).abs().t()) * (132 + k // 128) * 2.0 ** -24
+    assert ((out[-last:].double() - want).abs() <= bound + (want.abs() + bound) * 2.0 ** -8 + 2.0 ** -134).all()
+    assert (out[:-last].view(torch.int16) == 0).all()
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,experts,top_k", [(4200, 256, 128, 16, 8), (2, 128, 128, 1024, 64), (40, 128, 256, 1024, 64), (520, 128, 128, 1024, 64),
+                                                               (2, 65536, 128, 2, 2), (70, 65536, 128, 2, 1), (2, 128, 65536, 2, 1), (70, 128, 65536, 2, 1)])
+def test_experts_at_the_ends(worker, tokens, hidden, inter, experts, top_k):
+    """Several passes, the most experts and slots of a token, the longest rows; recorded and replayed with the bits of the eager call."""
+    args = _experts_case(tokens + hidden, tokens, hidden, inter, experts, top_k)
+    run = worker.register(runtime.experts_ffn_fp8_block)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        want = _check_experts(worker, args, dtype)
+        out, graph = torch.empty_like(want), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(*args, out, stream=torch.cuda.current_stream().cuda_stream)
+        for _ in range(3):
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    worker.sync()
+
+
+@pytest.mark.parametrize("tokens", [2, 100])
+def test_experts_past_32_bits(worker, tokens):
+    """The last of 66 experts, whose matrices lie beyond the first 4 GB: the bits of a call that has it alone."""
+    experts, hidden, inter = 66, 8192, 8320
+    alone = _experts_case(4, tokens, hidden, inter, 1, 1)
+    args = list(alone)
+    for i in range(4, 10):
+        args[i] = torch.empty((experts, *alone[i].shape[1:]), dtype=alone[i].dtype, device="cuda")
+        args[i][-1].view(torch.uint8 if i % 2 == 0 else torch.float32).copy_(alone[i][0].view(torch.uint8 if i % 2 == 0 else torch.float32))
+    args[2] = torch.full_like(alone[2], experts - 1)
+    outs = []
+    worker.set_option("block_gemm_rows", 16 if tokens < 16 else 64)
+    try:
+        for case in (args, alone):
+            outs.append(torch.empty((tokens, hidden), dtype=torch.float32, device="cuda"))
+            worker.run(runtime.experts_ffn_fp8_block, *case, outs[-1])
+            worker.sync()
+    finally:
+        worker.set_option("block_gemm_rows", 0)
+    assert outs[1].isfinite().all() and outs[1].abs().max() > 0 and torch.equal(*outs)
+
+
+def test_two_threads_on_one_stream(worker):
+    """Calls of two threads are issued one after the other: each has the results of its own call."""
+    import threading
+
+    cases = [_experts_case(i, 300 + 40 * i, 512, 256, 16, 4) for i in range(2)]
+    want = [_check_experts(worker, c, torch.bfloat16) for c in cases]
+    outs = [[torch.empty_like(w) for _ in range(20)] for w in want]
+    run, errors = worker.register(runtime.experts_ffn_fp8_block), []
+
+    def work(i):
+        try:
+            for out in outs[i]:
+                run(*cases[i], out)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    worker.sync()
+    assert not errors
+    assert all(torch.equal(out, w) for outs_i, w in zip(outs, want) for out in outs_i)
