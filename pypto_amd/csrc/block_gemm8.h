@@ -33,7 +33,7 @@ struct Params {
   int per_split;
   // Experts: the rows of a tile belong to one expert and are listed by the plan (experts.hip).
   const int4* tiles;       // {expert, first place, rows, 0}
-  const int* n_tiles;
+  const int* n_tiles;      // of each height
   const int32_t* order;    // slot (token * top_k + j) of each place
   int top_k;
 };

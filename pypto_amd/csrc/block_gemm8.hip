@@ -27,18 +27,17 @@ __global__ __launch_bounds__(256) void sum_ranges_kernel(const float* __restrict
 
 template <int BM, int BN, bool EXACT, typename OutT>
 int launch_tiles(Params p, int per_split, hipStream_t st) {
-  const int tiles_m = (p.m + BM - 1) / BM;
-  if (per_split <= 0 || per_split >= p.kb) return launch_tiled<kPlain, BM, BN, EXACT, OutT>(p, tiles_m, st);
+  if (per_split <= 0 || per_split >= p.kb) return launch_tiled<BM, BN, EXACT, OutT>(p, st);
   const int ranges = (p.kb + per_split - 1) / per_split;
   const int64_t count = (int64_t)p.m * p.n;
   void* slabs = nullptr;
   int rc = gemm_slabs((size_t)ranges * count * sizeof(float), st, &slabs);
   if (rc) return rc;
-  if (!slabs) return launch_tiled<kPlain, BM, BN, EXACT, OutT>(p, tiles_m, st);
+  if (!slabs) return launch_tiled<BM, BN, EXACT, OutT>(p, st);
   OutT* const out = reinterpret_cast<OutT*>(p.c);
   p.c = slabs;
   p.per_split = per_split;
-  rc = launch_tiled<kPlain, BM, BN, EXACT, float>(p, tiles_m, st);
+  rc = launch_tiled<BM, BN, EXACT, float>(p, st);
   if (rc) return rc;
   hipLaunchKernelGGL(sum_ranges_kernel<OutT>, dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, st, reinterpret_cast<const float*>(slabs),
                      ranges, count, out);

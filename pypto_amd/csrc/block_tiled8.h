@@ -19,6 +19,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -63,30 +64,31 @@ struct TiledShape {
   static_assert(KG == 1 || PH == 1, "groups along k have one half of rows");
 };
 
-template <int MAP, int BM, int BN, bool EXACT, typename OutT>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tiled_kernel(Params p, int tiles_m, int tiles_n) {
+// A workgroup's place among the tiles: bands of eight row tiles, rows first, so that an XCD's 32 consecutive ids are 8 row tiles x 4
+// column tiles.
+struct Place {
+  int tm, tn;
+  __device__ __forceinline__ Place(int logical, int tiles_m, int tiles_n) {
+    const int per_band = 8 * tiles_n;
+    const int band = logical / per_band, idx = logical - band * per_band;
+    const int band_rows = min(8, tiles_m - band * 8);
+    tn = idx / band_rows, tm = band * 8 + (idx - tn * band_rows);
+  }
+};
+
+// STREAM: the weights are read with the non-temporal hint.
+template <int MAP, int BM, int BN, bool EXACT, bool STREAM, typename OutT>
+__device__ __forceinline__ void work_tile(const Params& p, int tm, int tn, int range, uint8_t* smem) {
   typedef TiledShape<BM, BN> S;
   constexpr bool GATE = MAP == kGateUp;
   static_assert(!GATE || BN == 256, "a gate/up tile holds whole groups of h");
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   lds_char* const lds0 = (lds_char*)smem;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave & 1, wn = (wave >> 1) % S::WN, kg = (wave >> 1) / S::WN;
-  // bands of eight row tiles, rows first: an XCD's 32 consecutive ids are 8 row tiles x 4 column tiles
-  if (MAP != kPlain) tiles_m = __builtin_amdgcn_readfirstlane(*p.n_tiles);
   constexpr bool SPLIT = MAP == kPlain && std::is_same<OutT, float>::value;
-  const int ranges = SPLIT && p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1;
-  if ((int)blockIdx.x >= tiles_m * tiles_n * ranges) return;
-  int logical = xcd_remap(blockIdx.x, tiles_m * tiles_n * ranges);
-  const int range = SPLIT ? logical / (tiles_m * tiles_n) : 0;
-  logical -= range * tiles_m * tiles_n;
   const int k0 = range * p.per_split;  // first block of k
-  const int per_band = 8 * tiles_n;
-  const int band = logical / per_band, idx = logical - band * per_band;
-  const int band_rows = min(8, tiles_m - band * 8);
-  const int tn = idx / band_rows, tm = band * 8 + (idx - tn * band_rows);
   const Tile<MAP> tile(p, tm, BM);
   const int n0 = tn * (GATE ? kBlock : BN);
   const int nk = SPLIT && p.per_split ? min(p.per_split, p.kb - k0) : p.kb;
@@ -145,11 +147,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int g = 0; g < S::KG; ++g) {
       const uint8_t* src = base_b + min(t * S::KG + g, nk - 1) * kBlock;
       const uint32_t dst = lds_w + slot + g * S::kBlockBytes;
-      to_lds<BM * kBlock>(vb[0], src, dst);
-      if constexpr (S::NB > 1) to_lds<BM * kBlock + 8192>(vb[1], src, dst);
+      to_lds<BM * kBlock, STREAM>(vb[0], src, dst);
+      if constexpr (S::NB > 1) to_lds<BM * kBlock + 8192, STREAM>(vb[1], src, dst);
       if constexpr (S::NB > 2) {
-        to_lds<BM * kBlock + 16384>(vb[2], src, dst);
-        to_lds<BM * kBlock + 24576>(vb[3], src, dst);
+        to_lds<BM * kBlock + 16384, STREAM>(vb[2], src, dst);
+        to_lds<BM * kBlock + 24576, STREAM>(vb[3], src, dst);
       }
     }
   };
@@ -467,22 +469,77 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   }
 }
 
-template <int MAP, int BM, int BN, bool EXACT, typename OutT>
-int launch_tiled(const Params& p, int tiles_m, hipStream_t st) {
-  typedef TiledShape<BM, BN> S;
-  auto kern = tiled_kernel<MAP, BM, BN, EXACT, OutT>;
-  const int tiles_n = MAP == kGateUp ? p.n / kBlock : (p.n + BN - 1) / BN;
-  static std::atomic<bool> attr_set{false};  // per instantiation; callers hold the dispatch lock
-  if (!attr_set.load(std::memory_order_acquire)) {
-    PTO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)S::smem(kMaxK / kBlock)));
+template <int BM, int BN, bool EXACT, typename OutT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tiled_kernel(Params p, int tiles_m, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tiles = tiles_m * tiles_n;
+  int logical = xcd_remap(blockIdx.x, (int)gridDim.x);
+  const int range = std::is_same<OutT, float>::value ? logical / tiles : 0;
+  logical -= range * tiles;
+  const Place at(logical, tiles_m, tiles_n);
+  work_tile<kPlain, BM, BN, EXACT, false, OutT>(p, at.tm, at.tn, range, smem);
+}
+
+// Tiles of experts: heights BM, BM / 2 and BM / 4 (64 at least) lie one behind the other in the plan's list, p.n_tiles[] of each.  Each
+// height is dealt to the XCDs by itself, the highest first, so that the lower ones fill up what the higher leave.  With tiles of 64 rows most
+// experts have one, whose weights nobody else reads: with the non-temporal hint gate and up of 128 tokens for 8 of 64 experts of 4096 x 1408
+// took 129 us for 140, of 40 tokens for 4 of 60 of 2048 x 1024 41 for 45; with 512 tokens of the former, several tiles an expert, 186 for 182.
+// (A projection's weights are left to the caches: 48 rows of 4096 x 14336 that the last-level cache holds 14.3 us for 17.2, from memory 18.5
+// for 17.5.)
+template <int MAP, int BM, bool EXACT, typename OutT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tiled_experts_kernel(Params p, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  int id = blockIdx.x, first = 0;
+  auto work = [&](auto height_c, int which) {
+    constexpr int H = decltype(height_c)::value;
+    const int tiles = __builtin_amdgcn_readfirstlane(p.n_tiles[which]);
+    if (id < tiles * tiles_n) {
+      const Place at(xcd_remap(id, tiles * tiles_n), tiles, tiles_n);
+      work_tile<MAP, H, 256, EXACT, BM == 64, OutT>(p, first + at.tm, at.tn, 0, smem);
+      return true;
+    }
+    id -= tiles * tiles_n;
+    first += tiles;
+    return false;
+  };
+  if (work(IntConst<BM>{}, 0)) return;
+  if constexpr (BM >= 128) {
+    if (work(IntConst<BM / 2>{}, 1)) return;
+  }
+  if constexpr (BM >= 256) work(IntConst<BM / 4>{}, 2);
+}
+
+template <typename K, typename... Args>
+int launch_tiles_of(K kern, std::atomic<bool>& attr_set, int most_smem, int64_t wgs, size_t smem, hipStream_t st, const Params& p, Args... args) {
+  if (!attr_set.load(std::memory_order_acquire)) {  // callers hold the dispatch lock
+    PTO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, most_smem));
     attr_set.store(true, std::memory_order_release);
   }
-  const int64_t wgs = (int64_t)tiles_m * tiles_n * (p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1);
   if (wgs >= (1 << 23)) return fail(PTO_HIP_ERR_UNSUPPORTED, "a product of %lld tiles is more than one launch holds", (long long)wgs);
-  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(512), S::smem(p.kb), st, p, tiles_m, tiles_n);
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(512), smem, st, p, args...);
   PTO_CHECK_HIP(hipGetLastError());
   return PTO_HIP_OK;
+}
+
+template <int BM, int BN, bool EXACT, typename OutT>
+int launch_tiled(const Params& p, hipStream_t st) {
+  typedef TiledShape<BM, BN> S;
+  static std::atomic<bool> attr_set{false};  // per instantiation
+  const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
+  const int64_t wgs = (int64_t)tiles_m * tiles_n * (p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1);
+  return launch_tiles_of(tiled_kernel<BM, BN, EXACT, OutT>, attr_set, (int)S::smem(kMaxK / kBlock), wgs, S::smem(p.kb), st, p, tiles_m, tiles_n);
+}
+
+// most_tiles: as many row tiles as the plan may have.
+template <int MAP, int BM, bool EXACT, typename OutT>
+int launch_tiled_experts(const Params& p, int most_tiles, hipStream_t st) {
+  static std::atomic<bool> attr_set{false};
+  auto smem = [](int kb) {
+    return std::max(TiledShape<BM, 256>::smem(kb), std::max(TiledShape<std::max(BM / 2, 64), 256>::smem(kb), TiledShape<64, 256>::smem(kb)));
+  };
+  const int tiles_n = MAP == kGateUp ? p.n / kBlock : (p.n + 255) / 256;
+  return launch_tiles_of(tiled_experts_kernel<MAP, BM, EXACT, OutT>, attr_set, (int)smem(kMaxK / kBlock), (int64_t)most_tiles * tiles_n, smem(p.kb),
+                         st, p, tiles_n);
 }
 
 }  // namespace block8

@@ -25,28 +25,31 @@ constexpr int kPlanThreads = 1024;
 constexpr int64_t kPassSlots = 32768;
 constexpr int64_t kMostDirectSlots = 1024;
 
-// The plan: slots by expert, and tiles of `height` rows of one expert each.  One workgroup; a slot with a negative expert is in no
-// tile, one with an expert that there is not is reported.  Each wavefront counts for itself ([wavefronts][experts] in LDS), so that the
+// The plan: slots by expert, and tiles of one expert each: of `height` rows, and what an expert has left in a tile of the least of height,
+// height / 2 and height / 4 rows (64 at least) that holds it.  The heights lie one behind the other, n_tiles[] of each.  One workgroup; a
+// slot with a negative expert is in no tile, one with an expert that there is not is reported.  Each wavefront counts for itself ([wavefronts][experts] in LDS), so that the
 // counters of a busy expert are shared by 64 lanes and not by all, and a slot's rank in its wavefront's count is its place: with
-// one set of counters and a second round of atomics for the places 16384 slots of 64 experts took 19 us.  The order of the ranks is
-// that of the atomics: which row of which tile a slot becomes changes no bit of its result.
+// one set of counters and a second round of atomics for the places 16384 slots of 64 experts took 19 us.  The sorted slots are put together in
+// LDS: written one by one, each to a line of its own, they took 8 of 17 us.  The order of the ranks is that of the atomics: which row of which tile a slot becomes changes no bit of its result.
+template <int EACH>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __restrict__ ids, int slots, int experts, int height,
                                                             int32_t* __restrict__ order, int4* __restrict__ tiles, int* __restrict__ n_tiles,
                                                             int* __restrict__ flag) {
-  constexpr int kWaves = kPlanThreads / 64, kEach = kPassSlots / kPlanThreads;  // slots of a thread
-  extern __shared__ int count[];  // [kWaves][experts]
+  constexpr int kWaves = kPlanThreads / 64;
+  extern __shared__ int count[];  // [kWaves][experts], then the slots by expert
+  uint16_t* const sorted = reinterpret_cast<uint16_t*>(count + kWaves * experts);
   __shared__ int sums[2][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < kWaves * experts; i += kPlanThreads) count[i] = 0;
-  int e[kEach], rank[kEach];
+  int e[EACH], rank[EACH];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     const int s = i * kPlanThreads + tid;
     e[i] = s < slots ? ids[s] : -1;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
+  for (int i = 0; i < EACH; ++i) {
     if (e[i] >= experts) {
       *flag = 1;
       e[i] = -1;
@@ -58,8 +61,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
   int rows = 0;
   if (tid < experts)
     for (int w = 0; w < kWaves; ++w) rows += count[w * experts + tid];
-  const int mine = (rows + height - 1) / height;
-  int sum[2] = {rows, mine};
+  int mine[3] = {rows / height, 0, 0};
+  const int rest = rows - mine[0] * height;
+  const int rest_height = height >= 256 && rest <= height / 4 ? 2 : height >= 128 && rest <= height / 2 ? 1 : 0;
+#pragma unroll
+  for (int q = 0; q < 3; ++q) mine[q] += rest > 0 && rest_height == q;
+  // two sums in a word: rows (at most 2^15) and tiles of height / 4 (at most kMaxExperts), tiles of height and of height / 2
+  const int each[2] = {rows | mine[2] << 16, mine[0] | mine[1] << 16};
+  int sum[2] = {each[0], each[1]};
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
 #pragma unroll
@@ -70,26 +79,38 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
     if (lane == 63) sums[q][wave] = sum[q];
   }
   __syncthreads();
-  int before[2] = {sum[0] - rows, sum[1] - mine};
-  for (int w = 0; w < wave; ++w) {
-    before[0] += sums[0][w];
-    before[1] += sums[1][w];
-  }
+  int before[2] = {sum[0] - each[0], sum[1] - each[1]}, all[2] = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (w < wave) before[q] += sums[q][w];
+      all[q] += sums[q][w];
+    }
   if (tid < experts) {
-    for (int i = 0; i < mine; ++i) tiles[before[1] + i] = int4{tid, before[0] + i * height, min(height, rows - i * height), 0};
-    int at = before[0];
+    int at = before[0] & 0xffff;
+    const int full = before[1] & 0xffff, all_full = all[1] & 0xffff;
+    for (int i = 0; i < rows / height; ++i) tiles[full + i] = int4{tid, at + i * height, height, 0};
+    if (rest > 0) {
+      const int place = rest_height == 0 ? full + rows / height : all_full + (rest_height == 1 ? before[1] >> 16 : (all[1] >> 16) + (before[0] >> 16));
+      tiles[place] = int4{tid, at + rows - rest, rest, 0};
+    }
     for (int w = 0; w < kWaves; ++w) {
       const int here = count[w * experts + tid];
       count[w * experts + tid] = at;
       at += here;
     }
   }
-  if (tid == kPlanThreads - 1) *n_tiles = before[1] + mine;
+  if (tid < 3) n_tiles[tid] = tid == 0 ? all[1] & 0xffff : tid == 1 ? all[1] >> 16 : all[0] >> 16;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    if (e[i] >= 0) order[count[wave * experts + e[i]] + rank[i]] = i * kPlanThreads + tid;
+  for (int i = 0; i < EACH; ++i)
+    if (e[i] >= 0) sorted[count[wave * experts + e[i]] + rank[i]] = (uint16_t)(i * kPlanThreads + tid);
+  __syncthreads();
+  for (int i = tid; i < (all[0] & 0xffff); i += kPlanThreads) order[i] = sorted[i];
 }
+
+size_t plan_smem(int64_t slots, int experts) { return (size_t)(kPlanThreads / 64) * experts * sizeof(int) + (size_t)slots * sizeof(uint16_t); }
 
 // out[t] = sum over j of weights[t, j] * y[t * top_k + j], the slots without an expert left out.  Y _Float16: times the row's power
 // of two of each 128 channels.  One workgroup per token and 2048 channels, eight a thread.
@@ -357,7 +378,7 @@ struct Scratch {
     };
     order = take((size_t)slots * 4);
     tiles = take((size_t)max_tiles * sizeof(int4));
-    n_tiles = take(sizeof(int));
+    n_tiles = take(3 * sizeof(int));
     h = take((size_t)slots * x.inter);
     h_scale = take((size_t)slots * (x.inter / kBlock) * 4);
     y = take((size_t)slots * x.hidden * y_bytes);
@@ -377,9 +398,15 @@ int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, cha
   int32_t* order = reinterpret_cast<int32_t*>(ws + s.order);
   int4* tiles = reinterpret_cast<int4*>(ws + s.tiles);
   int* n_tiles = reinterpret_cast<int*>(ws + s.n_tiles);
-  const size_t counters = (size_t)(kPlanThreads / 64) * x.experts * sizeof(int);
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), counters, st, x.ids, (int)(tokens * x.top_k), x.experts, height, order, tiles,
-                     n_tiles, ctx().flags + 3);
+  const int slots = (int)(tokens * x.top_k);
+  auto plan = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(1), dim3(kPlanThreads), plan_smem(slots, x.experts), st, x.ids, slots, x.experts, height, order, tiles, n_tiles,
+                       ctx().flags + 3);
+  };
+  if (slots <= kPlanThreads) plan(plan_kernel<1>);
+  else if (slots <= 8 * kPlanThreads) plan(plan_kernel<8>);
+  else if (slots <= 16 * kPlanThreads) plan(plan_kernel<16>);
+  else plan(plan_kernel<kPassSlots / kPlanThreads>);
   Params p{};
   p.tiles = tiles;
   p.n_tiles = n_tiles;
@@ -397,9 +424,9 @@ int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, cha
   p.k = x.hidden;
   p.kb = x.hidden / kBlock;
   int rc;
-  if (height == 64) rc = launch_tiled<kGateUp, 64, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
-  else if (height == 128 || kExactUp) rc = launch_tiled<kGateUp, 128, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
-  else rc = launch_tiled<kGateUp, kExactUp ? 128 : 256, 256, kExactUp, uint8_t>(p, s.max_tiles, st);
+  if (height == 64) rc = launch_tiled_experts<kGateUp, 64, kExactUp, uint8_t>(p, s.max_tiles, st);
+  else if (height == 128 || kExactUp) rc = launch_tiled_experts<kGateUp, 128, kExactUp, uint8_t>(p, s.max_tiles, st);
+  else rc = launch_tiled_experts<kGateUp, kExactUp ? 128 : 256, kExactUp, uint8_t>(p, s.max_tiles, st);
   if (rc) return rc;
   Params d = p;
   d.a = reinterpret_cast<const uint8_t*>(ws + s.h);
@@ -411,9 +438,9 @@ int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, cha
   d.n = x.hidden;
   d.k = x.inter;
   d.kb = x.inter / kBlock;
-  if (height == 64) rc = launch_tiled<kDown, 64, 256, kExactDown, Y>(d, s.max_tiles, st);
-  else if (height == 128 || kExactUp) rc = launch_tiled<kDown, 128, 256, kExactDown, Y>(d, s.max_tiles, st);
-  else rc = launch_tiled<kDown, kExactUp ? 128 : 256, 256, kExactDown, Y>(d, s.max_tiles, st);
+  if (height == 64) rc = launch_tiled_experts<kDown, 64, kExactDown, Y>(d, s.max_tiles, st);
+  else if (height == 128 || kExactUp) rc = launch_tiled_experts<kDown, 128, kExactDown, Y>(d, s.max_tiles, st);
+  else rc = launch_tiled_experts<kDown, kExactUp ? 128 : 256, kExactDown, Y>(d, s.max_tiles, st);
   if (rc) return rc;
   hipLaunchKernelGGL((combine_kernel<Y, OutT>), dim3((unsigned)((x.hidden + 2047) / 2048), (unsigned)tokens), dim3(256), 0, st,
                      reinterpret_cast<const Y*>(ws + s.y), reinterpret_cast<const float*>(ws + s.y_scale), x.ids, x.weights,
@@ -426,8 +453,9 @@ template <typename OutT>
 int run_experts(Experts x, int64_t tokens, hipStream_t st) {
   static std::atomic<bool> attr_set{false};  // callers hold the dispatch lock
   if (!attr_set.load(std::memory_order_acquire)) {
-    PTO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      kPlanThreads / 64 * kMaxExperts * (int)sizeof(int)));
+    for (const void* kern : {reinterpret_cast<const void*>(plan_kernel<1>), reinterpret_cast<const void*>(plan_kernel<8>),
+                             reinterpret_cast<const void*>(plan_kernel<16>), reinterpret_cast<const void*>(plan_kernel<kPassSlots / kPlanThreads>)})
+      PTO_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kPassSlots, kMaxExperts)));
     attr_set.store(true, std::memory_order_release);
   }
   constexpr bool kExactUp = !std::is_same<OutT, __bf16>::value, kExactDown = std::is_same<OutT, float>::value;
@@ -436,7 +464,7 @@ int run_experts(Experts x, int64_t tokens, hipStream_t st) {
   const bool direct = height == 0 ? experts_direct(slots, x.experts, x.hidden, x.inter) : height == 16;
   if (direct && slots <= kMostDirectSlots && direct_smem(x) <= kDirectSmem) return run_direct<OutT>(x, tokens, st);
   const int64_t pass = std::min(tokens, std::max<int64_t>(1, kPassSlots / x.top_k));
-  if (height < 64) height = choose_expert_rows(pass * x.top_k, x.experts, x.hidden, x.inter, kExactUp, kExactDown);
+  if (height < 64) height = choose_expert_rows(pass * x.top_k, x.experts, x.hidden, x.inter, kExactUp, kExactDown, ctx().num_cu);
   if (kExactUp) height = std::min(height, 128);
   const Scratch s(pass, x, height, kExactUp ? 4 : 2);
   void* ws = nullptr;

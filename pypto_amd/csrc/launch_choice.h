@@ -298,7 +298,7 @@ constexpr BlockTileCost kBlockTiles[2][5] = {
     {{64, 64, 0.254, 0.051, 4.7}, {64, 128, 0.440, 0.098, 5.2}, {64, 256, 0.826, 0.212, 5.3}, {128, 256, 1.429, 0.327, 7.1}, {0, 0, 0.0, 0.0, 0.0}}};
 
 // The form with the least estimated time of a product of m rows, n channels and kb blocks of k.  Timed against every tile and count of
-// ranges, the one it picks among the tiles is 1.4 % from the best in the mean and 22 % at worst, exact 0.3 % and 9 %.  rows, cols, splits: given, or 0.
+// ranges, the one it picks among the tiles is 0.9 % from the best in the mean and 13 % at worst, exact 0.3 % and 9 %.  rows, cols, splits: given, or 0.
 // Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, or, with few channels
 // and a long k, 16 of eight (11008 x 4096 at one row 19.4 -> 10.0 us, 16384 x 1024 20.6 -> 12.2; 4096 x 14336 the other way 13.6 -> 19.5).
 inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact, int64_t num_cu, int rows, int cols, int splits) {
@@ -327,7 +327,8 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
       const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per, wgs = tiles * ranges;
       const double load = std::min(1.0, (double)wgs / (double)num_cu);
       double us = (double)((wgs + num_cu - 1) / num_cu) * ((double)((per + groups - 1) / groups * groups) * (t.block + t.loaded * load) + t.start);
-      us = std::max(us, 4.0 + weights_mb / 4.5);
+      const double memory = 4.0 + weights_mb / 5.0;
+      us = std::max(us, memory) + 0.1 * std::min(us, memory);
       if (ranges > 1) us += 4.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
       if (us < best) {
         best = us;
@@ -348,21 +349,40 @@ inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64
   return 5.0 + (double)slots * mb / 4.0 < 26.0 + ((double)experts - unused) * mb / 5.2;
 }
 
-// Tile height of both products of the experts' FFN: the least sum over the tiles of what they cost, an expert's rows filling up half a tile in the
-// mean.  8 of 64 experts of 4096 x 1408, 64 / 128 / 256 rows, us: 256 tokens 248 / 254 / 307, 512 304 / 288 / 331, 1024 414 / 384 / 384, 4096 1279 / 1036 / 946.
-inline int choose_expert_rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, bool exact_up, bool exact_down) {
-  const double used = (double)std::min(slots, experts), each = (double)slots / used;
+// The highest tiles of both products of the experts' FFN; what an expert has left goes to lower ones (experts.hip).  The least sum over
+// the two products of their tiles' costs, spread over the CUs but never below one tile's, with experts of 0.2 to 2.3 times the mean rows, as
+// routers leave them.  Over 88 timings of five layers at 16 to 4096 tokens the pick is 0.6 % from the best height in the mean and 21 % at
+// worst.  8 of 64 experts of 4096 x 1408, 64 / 128 / 256 rows, us: 128 tokens 261 / 262 / 262, 512 320 / 309 / 296, 1024 413 / 417 / 362, 4096
+// 1163 / 993 / 872; with one height for all of an expert's tiles 512 tokens took 304 / 288 / 331, 4096 1279 / 1036 / 946.
+inline int choose_expert_rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, bool exact_up, bool exact_down, int64_t num_cu) {
+  const double used = (double)experts * (1.0 - std::pow(1.0 - 1.0 / (double)experts, (double)slots)), each = (double)slots / used;
+  // us of a tile of the height kBlockTiles[][i]
+  auto cost = [](bool exact, int i, int64_t kb) {
+    const BlockTileCost& t = kBlockTiles[exact][i];
+    return (double)kb * (t.block + t.loaded) + t.start;
+  };
   double best = 1e30;
   int pick = 64;
-  for (int i = 2; i < 5; ++i) {
-    const BlockTileCost &up = kBlockTiles[exact_up][i], &down = kBlockTiles[exact_down][i];
-    if (up.rows == 0 || down.rows == 0) continue;
-    const double tiles = used * std::max(1.0, each / up.rows + 0.5);
-    auto cost = [](const BlockTileCost& t, int64_t kb) { return (double)kb * (t.block + t.loaded) + t.start; };
-    const double us = tiles * ((double)(inter / 128) * cost(up, hidden / 128) + (double)((hidden + 255) / 256) * cost(down, inter / 128));
+  for (int i = 2; i < (exact_up ? 4 : 5); ++i) {
+    const int height = kBlockTiles[0][i].rows;
+    double us = 0.0;
+    for (int pass = 0; pass < 2; ++pass) {
+      const bool exact = pass ? exact_down : exact_up;
+      const int64_t kb = (pass ? inter : hidden) / 128, tiles_n = pass ? (hidden + 255) / 256 : inter / 128;
+      double work = 0.0, longest = 0.0;
+      for (const double share : {0.2, 0.5, 0.8, 1.2, 2.3}) {
+        const double rows = std::max(1.0, each * share), full = std::floor(rows / height), rest = rows - full * height;
+        int low = 2;  // the least height that holds the rest
+        while (kBlockTiles[0][low].rows < rest) ++low;
+        const double high_us = full > 0.0 ? cost(exact, i, kb) : 0.0, low_us = rest > 0.0 ? cost(exact, low, kb) : 0.0;
+        work += (full * high_us + low_us) / 5.0;
+        longest = std::max(longest, std::max(high_us, low_us));
+      }
+      us += std::max(longest, used * (double)tiles_n * work / (double)num_cu);
+    }
     if (us < best) {
       best = us;
-      pick = up.rows;
+      pick = height;
     }
   }
   return pick;

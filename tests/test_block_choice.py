@@ -16,7 +16,7 @@ extern "C" void tile(int64_t m, int64_t n, int64_t kb, int exact, int rows, int 
 }
 extern "C" int direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) { return pto_hip::experts_direct(slots, experts, hidden, inter); }
 extern "C" int rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, int up, int down) {
-  return pto_hip::choose_expert_rows(slots, experts, hidden, inter, up != 0, down != 0);
+  return pto_hip::choose_expert_rows(slots, experts, hidden, inter, up != 0, down != 0, 256);
 }
 """
 
@@ -81,5 +81,5 @@ def test_measured_sides(choice):
     assert _tile(choice, 4096, 14336, 32)[0] == 256 and _tile(choice, 4096, 14336, 32, exact=True)[0] == 128
     assert choice.direct(8, 64, 4096, 1408) and not choice.direct(32, 64, 4096, 1408)
     assert choice.direct(64, 128, 1024, 512) and not choice.direct(128, 128, 1024, 512)
-    assert choice.rows(2048, 64, 4096, 1408, 0, 0) == 64 and choice.rows(32768, 64, 4096, 1408, 0, 0) == 256
+    assert choice.rows(320, 64, 4096, 1408, 0, 0) == 64 and choice.rows(32768, 64, 4096, 1408, 0, 0) == 256
     assert choice.rows(32768, 64, 4096, 1408, 1, 0) == 128
