@@ -40,19 +40,19 @@ struct Params {
 
 enum RowMap { kPlain = 0, kGateUp = 1, kDown = 2 };
 
-// A tile's rows: row r of it is row a_row(r) of the activations and row c_row(r) of the result.
+// A tile's rows: row r of it is row a_row(r) of the activations and row c_row(r) of the result.  `at`: its first row, experts: its index.
 template <int MAP>
 struct Tile {
   int expert, first, rows;
   const int32_t* order;
   int top_k;
-  __device__ __forceinline__ Tile(const Params& p, int index, int height) : order(p.order), top_k(p.top_k) {
+  __device__ __forceinline__ Tile(const Params& p, int at, int height) : order(p.order), top_k(p.top_k) {
     if constexpr (MAP == kPlain) {
       expert = 0;
-      first = index * height;
+      first = at;
       rows = min(height, p.m - first);
     } else {
-      const int4 t = p.tiles[index];
+      const int4 t = p.tiles[at];
       expert = t.x;
       first = t.y;
       rows = t.z;

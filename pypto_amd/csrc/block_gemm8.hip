@@ -25,19 +25,20 @@ __global__ __launch_bounds__(256) void sum_ranges_kernel(const float* __restrict
   store_upto4(out + at, sum, here);
 }
 
-template <int BM, int BN, bool EXACT, typename OutT>
-int launch_tiles(Params p, int per_split, hipStream_t st) {
-  if (per_split <= 0 || per_split >= p.kb) return launch_tiled<BM, BN, EXACT, OutT>(p, st);
+// `launch` with p, or with ranges of k into slabs that are summed behind it.  launch(p, type of the results)
+template <typename OutT, typename F>
+int launch_ranges(Params p, int per_split, hipStream_t st, F launch) {
+  if (per_split <= 0 || per_split >= p.kb) return launch(p, OutT{});
   const int ranges = (p.kb + per_split - 1) / per_split;
   const int64_t count = (int64_t)p.m * p.n;
   void* slabs = nullptr;
   int rc = gemm_slabs((size_t)ranges * count * sizeof(float), st, &slabs);
   if (rc) return rc;
-  if (!slabs) return launch_tiled<BM, BN, EXACT, OutT>(p, st);
+  if (!slabs) return launch(p, OutT{});
   OutT* const out = reinterpret_cast<OutT*>(p.c);
   p.c = slabs;
   p.per_split = per_split;
-  rc = launch_tiled<BM, BN, EXACT, float>(p, st);
+  rc = launch(p, float{});
   if (rc) return rc;
   hipLaunchKernelGGL(sum_ranges_kernel<OutT>, dim3((unsigned)((count + 1023) / 1024)), dim3(256), 0, st, reinterpret_cast<const float*>(slabs),
                      ranges, count, out);
@@ -60,13 +61,16 @@ int launch_projection(const Params& p, hipStream_t st) {
     PTO_CHECK_HIP(hipGetLastError());
     return PTO_HIP_OK;
   }
-  if (t.rows == 64 && t.cols == 64) return launch_tiles<64, 64, kExact, OutT>(p, t.per_split, st);
-  if (t.rows == 64 && t.cols == 128) return launch_tiles<64, 128, kExact, OutT>(p, t.per_split, st);
-  if (t.rows == 64) return launch_tiles<64, 256, kExact, OutT>(p, t.per_split, st);
-  if constexpr (!kExact) {
-    if (t.rows == 256) return launch_tiles<256, 256, false, OutT>(p, t.per_split, st);
-  }
-  return launch_tiles<128, 256, kExact, OutT>(p, t.per_split, st);
+  return launch_ranges<OutT>(p, t.per_split, st, [&](const Params& q, auto type) {
+    typedef decltype(type) C;
+    if (t.cols == 64) return launch_tiled<64, kExact, C>(q, st);
+    if (t.cols == 128) return launch_tiled<128, kExact, C>(q, st);
+    if (t.rows == 64) return launch_tiled_rows<64, kExact, C>(q, t.tiles, st);
+    if constexpr (!kExact) {
+      if (t.rows == 256) return launch_tiled_rows<256, kExact, C>(q, t.tiles, st);
+    }
+    return launch_tiled_rows<128, kExact, C>(q, t.tiles, st);
+  });
 }
 
 }  // namespace block8

@@ -78,7 +78,7 @@ struct Place {
 
 // STREAM: the weights are read with the non-temporal hint.
 template <int MAP, int BM, int BN, bool EXACT, bool STREAM, typename OutT>
-__device__ __forceinline__ void work_tile(const Params& p, int tm, int tn, int range, uint8_t* smem) {
+__device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int range, uint8_t* smem) {
   typedef TiledShape<BM, BN> S;
   constexpr bool GATE = MAP == kGateUp;
   static_assert(!GATE || BN == 256, "a gate/up tile holds whole groups of h");
@@ -89,7 +89,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int tm, int tn, int r
   const int wm = wave & 1, wn = (wave >> 1) % S::WN, kg = (wave >> 1) / S::WN;
   constexpr bool SPLIT = MAP == kPlain && std::is_same<OutT, float>::value;
   const int k0 = range * p.per_split;  // first block of k
-  const Tile<MAP> tile(p, tm, BM);
+  const Tile<MAP> tile(p, at, BM);
   const int n0 = tn * (GATE ? kBlock : BN);
   const int nk = SPLIT && p.per_split ? min(p.per_split, p.kb - k0) : p.kb;
 
@@ -98,9 +98,9 @@ __device__ __forceinline__ void work_tile(const Params& p, int tm, int tn, int r
   lds_float* const s_cols = (lds_float*)(lds0 + S::kChannelScales);  // [2][nk64]
   const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds0);
   {
-    const int blocks_n = (p.n + kBlock - 1) / kBlock, at = tile.expert * blocks_n;
-    const float* c0 = p.sb0 + (size_t)(at + n0 / kBlock) * p.kb + k0;
-    const float* c1 = (GATE ? p.sb1 : p.sb0) + (size_t)(at + (GATE ? n0 / kBlock : min(n0 / kBlock + 1, blocks_n - 1))) * p.kb + k0;
+    const int blocks_n = (p.n + kBlock - 1) / kBlock, first = tile.expert * blocks_n;
+    const float* c0 = p.sb0 + (size_t)(first + n0 / kBlock) * p.kb + k0;
+    const float* c1 = (GATE ? p.sb1 : p.sb0) + (size_t)(first + (GATE ? n0 / kBlock : min(n0 / kBlock + 1, blocks_n - 1))) * p.kb + k0;
     for (int i = (wave >> 1) * 64; i < nk; i += 256)
       to_lds_dword((uint32_t)min(i + lane, nk - 1) * 4u, wave & 1 ? c1 : c0, lds_base + S::kChannelScales + ((wave & 1) * nk64 + i) * 4);
   }
@@ -469,7 +469,8 @@ __device__ __forceinline__ void work_tile(const Params& p, int tm, int tn, int r
   }
 }
 
-template <int BM, int BN, bool EXACT, typename OutT>
+// The rows of a product in tiles of one height of 64 or 128 channels, groups of wavefronts along k.
+template <int BN, bool EXACT, typename OutT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tiled_kernel(Params p, int tiles_m, int tiles_n) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tiles = tiles_m * tiles_n;
@@ -477,11 +478,39 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int range = std::is_same<OutT, float>::value ? logical / tiles : 0;
   logical -= range * tiles;
   const Place at(logical, tiles_m, tiles_n);
-  work_tile<kPlain, BM, BN, EXACT, false, OutT>(p, at.tm, at.tn, range, smem);
+  work_tile<kPlain, 64, BN, EXACT, false, OutT>(p, at.tm * 64, at.tn, range, smem);
 }
 
-// Tiles of experts: heights BM, BM / 2 and BM / 4 (64 at least) lie one behind the other in the plan's list, p.n_tiles[] of each.  Each
-// height is dealt to the XCDs by itself, the highest first, so that the lower ones fill up what the higher leave.  With tiles of 64 rows most
+// Tiles of 256 channels and up to three heights: `high` row tiles of BM rows, then `half` of BM / 2 and the rest of BM / 4 (64 at least).
+// Each height is dealt to the XCDs by itself, the highest first, so that the lower ones fill up what the higher leave.
+template <int BM, bool EXACT, typename OutT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void tiled_rows_kernel(Params p, int high, int half, int quarter, int tiles_n) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int ranges = std::is_same<OutT, float>::value && p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1;
+  int id = blockIdx.x, first = 0;
+  auto work = [&](auto height_c, int tiles_m) {
+    constexpr int H = decltype(height_c)::value;
+    const int tiles = tiles_m * tiles_n;
+    if (id < tiles * ranges) {
+      int logical = xcd_remap(id, tiles * ranges);
+      const int range = logical / tiles;
+      logical -= range * tiles;
+      const Place at(logical, tiles_m, tiles_n);
+      work_tile<kPlain, H, 256, EXACT, false, OutT>(p, first + at.tm * H, at.tn, range, smem);
+      return true;
+    }
+    id -= tiles * ranges;
+    first += tiles_m * H;
+    return false;
+  };
+  if (work(IntConst<BM>{}, high)) return;
+  if constexpr (BM >= 128) {
+    if (work(IntConst<BM / 2>{}, half)) return;
+  }
+  if constexpr (BM >= 256) work(IntConst<BM / 4>{}, quarter);
+}
+
+// The same for tiles of experts, which lie in the plan's list by height, p.n_tiles[] of each.  With tiles of 64 rows most
 // experts have one, whose weights nobody else reads: with the non-temporal hint gate and up of 128 tokens for 8 of 64 experts of 4096 x 1408
 // took 129 us for 140, of 40 tokens for 4 of 60 of 2048 x 1024 41 for 45; with 512 tokens of the former, several tiles an expert, 186 for 182.
 // (A projection's weights are left to the caches: 48 rows of 4096 x 14336 that the last-level cache holds 14.3 us for 17.2, from memory 18.5
@@ -521,25 +550,39 @@ int launch_tiles_of(K kern, std::atomic<bool>& attr_set, int most_smem, int64_t 
   return PTO_HIP_OK;
 }
 
-template <int BM, int BN, bool EXACT, typename OutT>
+template <int BM>
+constexpr size_t mixed_smem(int kb) {
+  return std::max(TiledShape<BM, 256>::smem(kb), std::max(TiledShape<std::max(BM / 2, 64), 256>::smem(kb), TiledShape<64, 256>::smem(kb)));
+}
+
+inline int64_t ranges_of(const Params& p) { return p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1; }
+
+template <int BN, bool EXACT, typename OutT>
 int launch_tiled(const Params& p, hipStream_t st) {
-  typedef TiledShape<BM, BN> S;
+  typedef TiledShape<64, BN> S;
   static std::atomic<bool> attr_set{false};  // per instantiation
-  const int tiles_m = (p.m + BM - 1) / BM, tiles_n = (p.n + BN - 1) / BN;
-  const int64_t wgs = (int64_t)tiles_m * tiles_n * (p.per_split ? (p.kb + p.per_split - 1) / p.per_split : 1);
-  return launch_tiles_of(tiled_kernel<BM, BN, EXACT, OutT>, attr_set, (int)S::smem(kMaxK / kBlock), wgs, S::smem(p.kb), st, p, tiles_m, tiles_n);
+  const int tiles_m = (p.m + 63) / 64, tiles_n = (p.n + BN - 1) / BN;
+  return launch_tiles_of(tiled_kernel<BN, EXACT, OutT>, attr_set, (int)S::smem(kMaxK / kBlock), tiles_m * ranges_of(p) * tiles_n, S::smem(p.kb), st, p,
+                         tiles_m, tiles_n);
+}
+
+// tiles: of BM, BM / 2 and BM / 4 rows
+template <int BM, bool EXACT, typename OutT>
+int launch_tiled_rows(const Params& p, const int (&tiles)[3], hipStream_t st) {
+  static std::atomic<bool> attr_set{false};
+  const int tiles_n = (p.n + 255) / 256;
+  return launch_tiles_of(tiled_rows_kernel<BM, EXACT, OutT>, attr_set, (int)mixed_smem<BM>(kMaxK / kBlock),
+                         ((int64_t)tiles[0] + tiles[1] + tiles[2]) * ranges_of(p) * tiles_n, mixed_smem<BM>(p.kb), st, p, tiles[0], tiles[1], tiles[2],
+                         tiles_n);
 }
 
 // most_tiles: as many row tiles as the plan may have.
 template <int MAP, int BM, bool EXACT, typename OutT>
 int launch_tiled_experts(const Params& p, int most_tiles, hipStream_t st) {
   static std::atomic<bool> attr_set{false};
-  auto smem = [](int kb) {
-    return std::max(TiledShape<BM, 256>::smem(kb), std::max(TiledShape<std::max(BM / 2, 64), 256>::smem(kb), TiledShape<64, 256>::smem(kb)));
-  };
   const int tiles_n = MAP == kGateUp ? p.n / kBlock : (p.n + 255) / 256;
-  return launch_tiles_of(tiled_experts_kernel<MAP, BM, EXACT, OutT>, attr_set, (int)smem(kMaxK / kBlock), (int64_t)most_tiles * tiles_n, smem(p.kb),
-                         st, p, tiles_n);
+  return launch_tiles_of(tiled_experts_kernel<MAP, BM, EXACT, OutT>, attr_set, (int)mixed_smem<BM>(kMaxK / kBlock),
+                         (int64_t)most_tiles * tiles_n, mixed_smem<BM>(p.kb), st, p, tiles_n);
 }
 
 }  // namespace block8

@@ -286,6 +286,7 @@ inline int64_t attn_partition_align(int64_t pairs, int64_t max_ctx, int64_t bloc
 struct BlockTile {
   int rows, cols;  // tile; rows 16: the form that reads straight to registers, of cols channels a workgroup
   int per_split;   // blocks of k of a range, 0: unsplit
+  int tiles[3];    // 256 channels: row tiles of `rows`, half and a quarter of it, one behind the other
 };
 struct BlockTileCost {
   int rows, cols;
@@ -297,42 +298,106 @@ constexpr BlockTileCost kBlockTiles[2][5] = {
     {{64, 64, 0.217, 0.044, 3.6}, {64, 128, 0.299, 0.081, 3.8}, {64, 256, 0.533, 0.173, 3.6}, {128, 256, 0.847, 0.228, 5.4}, {256, 256, 1.308, 0.444, 6.9}},
     {{64, 64, 0.254, 0.051, 4.7}, {64, 128, 0.440, 0.098, 5.2}, {64, 256, 0.826, 0.212, 5.3}, {128, 256, 1.429, 0.327, 7.1}, {0, 0, 0.0, 0.0, 0.0}}};
 
+// us until the last of jobs[c] workgroups of us[c] each is done, which are started in their order, the long ones first, on the CUs of an
+// XCD (they are dealt to the XCDs in turn).
+inline double makespan(const int64_t (&jobs)[3], const double (&us)[3], int64_t num_cu) {
+  constexpr int kXcds = 8;
+  struct Free {
+    double at;
+    int64_t cus;
+  } free[8] = {{0.0, std::max<int64_t>(1, num_cu / kXcds)}};  // by time
+  int n = 1;
+  double last = 0.0;
+  for (int c = 0; c < 3; ++c)
+    for (int64_t left = (jobs[c] + kXcds - 1) / kXcds; left > 0;) {
+      const Free f = free[0];
+      const int64_t now = std::min(left, f.cus);
+      // as many rounds as the first CUs have before others are free
+      int64_t rounds = left / f.cus;
+      if (n > 1) rounds = std::min<int64_t>(rounds, (int64_t)((free[1].at - f.at) / us[c]));
+      rounds = std::max<int64_t>(rounds, 1);
+      const Free later{f.at + (double)rounds * us[c], now};
+      left -= now * rounds;
+      last = std::max(last, later.at);
+      if (now < f.cus && n < 8) {
+        free[0].cus -= now;
+      } else {
+        for (int i = 1; i < n; ++i) free[i - 1] = free[i];
+        --n;
+      }
+      int at = n++;
+      for (; at > 0 && free[at - 1].at > later.at; --at) free[at] = free[at - 1];
+      free[at] = later;
+    }
+  return last;
+}
+
 // The form with the least estimated time of a product of m rows, n channels and kb blocks of k.  Timed against every tile and count of
 // ranges, the one it picks among the tiles is 0.9 % from the best in the mean and 13 % at worst, exact 0.3 % and 9 %.  rows, cols, splits: given, or 0.
+// Tiles of 256 channels share the rows among several heights where one height leaves its last round part empty: 11008 channels of 4096, us
+// with one height / several: 1300 rows 78 / 64, 1600 106 / 91, 2048 115 / 101, 4096 185 / 186; 5003 of 5120 4096 rows 149 / 125.
+// The estimate itself takes 1 us of the caller's time, none where up to 16 rows are bound by memory.
 // Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, or, with few channels
 // and a long k, 16 of eight (11008 x 4096 at one row 19.4 -> 10.0 us, 16384 x 1024 20.6 -> 12.2; 4096 x 14336 the other way 13.6 -> 19.5).
 inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact, int64_t num_cu, int rows, int cols, int splits) {
   const double weights_mb = (double)n * (double)kb * 128e-6;
+  const double memory = 4.0 + weights_mb / 5.0;
   double best = 1e30;
-  BlockTile pick{128, 256, 0};
+  BlockTile pick{64, 256, 0, {(int)((m + 63) / 64), 0, 0}};
   if ((rows == 0 && m <= 16 && splits == 0) || rows == 16) {
     const double stream = 2.3 + weights_mb / 5.2 * (1.0 + 0.02 * (double)m);
     const double wide = std::max(stream, 3.0 + (double)kb / 4 * (0.6 + 0.012 * (double)m));
     best = wide;
-    pick = BlockTile{16, 32, 0};
+    pick = BlockTile{16, 32, 0, {}};
     if (n <= 16 * num_cu) {
       const double few = std::max(stream, 3.0 + (double)kb / 8 * (0.55 + 0.045 * (double)m));
       if (few < wide) {
         best = few;
-        pick = BlockTile{16, 16, 0};
+        pick = BlockTile{16, 16, 0, {}};
       }
     }
-    if (rows == 16) return pick;
+    if (rows == 16 || best <= memory) return pick;
   }
-  for (const BlockTileCost& t : kBlockTiles[exact]) {
-    if (t.rows == 0 || (rows > 0 && t.rows != (exact ? std::min(rows, 128) : rows)) || (cols > 0 && t.rows == 64 && t.cols != cols)) continue;
-    const int64_t tiles = ((m + t.rows - 1) / t.rows) * ((n + t.cols - 1) / t.cols), groups = 256 / t.cols;  // groups of wavefronts along k
+  for (int form = 0; form < (exact ? 4 : 5); ++form) {
+    const BlockTileCost& t = kBlockTiles[exact][form];
+    if ((rows > 0 && t.rows != (exact ? std::min(rows, 128) : rows)) || (cols > 0 && t.rows == 64 && t.cols != cols)) continue;
+    const int64_t tiles_n = (n + t.cols - 1) / t.cols, groups = 256 / t.cols;  // groups of wavefronts along k
+    const int64_t least_tiles = (m + t.rows - 1) / t.rows * tiles_n;
     for (int64_t sp = 1; sp <= 16; ++sp) {
-      if (splits > 0 ? sp != std::min<int64_t>(splits, kb) : sp > 1 && kb / sp < 8) continue;
-      const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per, wgs = tiles * ranges;
-      const double load = std::min(1.0, (double)wgs / (double)num_cu);
-      double us = (double)((wgs + num_cu - 1) / num_cu) * ((double)((per + groups - 1) / groups * groups) * (t.block + t.loaded * load) + t.start);
-      const double memory = 4.0 + weights_mb / 5.0;
-      us = std::max(us, memory) + 0.1 * std::min(us, memory);
-      if (ranges > 1) us += 4.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
-      if (us < best) {
-        best = us;
-        pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0};
+      if (splits > 0 && sp != std::min<int64_t>(splits, kb)) continue;
+      if (splits == 0 && sp > 1 && (kb / sp < 8 || least_tiles * (sp - 1) >= 2 * num_cu)) break;  // short ranges, or CUs enough without them
+      const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per;
+      auto consider = [&](int64_t high, int64_t half, int64_t quarter) {
+        const int64_t jobs[3] = {high * tiles_n * ranges, half * tiles_n * ranges, quarter * tiles_n * ranges};
+        const double load = std::min(1.0, (double)(jobs[0] + jobs[1] + jobs[2]) / (double)num_cu);
+        double each[3] = {0.0, 0.0, 0.0};
+        for (int c = 0; c < 3; ++c) {
+          const BlockTileCost& l = kBlockTiles[exact][std::max(form - c, std::min(form, 2))];
+          each[c] = (double)((per + groups - 1) / groups * groups) * (l.block + l.loaded * load) + l.start;
+        }
+        double us = makespan(jobs, each, num_cu);
+        us = std::max(us, memory) + 0.1 * std::min(us, memory);
+        if (ranges > 1) us += 4.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
+        if (us < best) {
+          best = us;
+          pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0, {(int)high, (int)half, (int)quarter}};
+        }
+      };
+      const int64_t whole = m / t.rows, all = (m + t.rows - 1) / t.rows;
+      if (t.rows == 64) {
+        consider(all, 0, 0);
+        continue;
+      }
+      // so many tiles of the full height, the rows behind them in lower ones
+      for (int64_t high = rows > 0 ? whole : std::max<int64_t>(1, whole - 5); high <= (rows > 0 ? whole : all); ++high) {
+        const int64_t rest = std::max<int64_t>(0, m - high * t.rows);
+        if (t.rows == 128) {
+          consider(high, (rest + 63) / 64, 0);
+          continue;
+        }
+        const int64_t half = rest / 128, end = rest - half * 128;
+        if (end <= 64) consider(high, half, end > 0);
+        if (end > 0) consider(high, half + 1, 0);
       }
     }
   }

@@ -1,6 +1,8 @@
 """The forms the host picks for products of block-scaled operands (CPU: the header is compiled for the host and called)."""
 
 import ctypes as C
+import heapq
+import random
 import subprocess
 from pathlib import Path
 
@@ -13,7 +15,9 @@ _SOURCE = """
 extern "C" void tile(int64_t m, int64_t n, int64_t kb, int exact, int rows, int cols, int splits, int* out) {
   const pto_hip::BlockTile t = pto_hip::choose_block_tile(m, n, kb, exact != 0, 256, rows, cols, splits);
   out[0] = t.rows, out[1] = t.cols, out[2] = t.per_split;
+  for (int i = 0; i < 3; ++i) out[3 + i] = t.tiles[i];
 }
+extern "C" double span(int64_t a, int64_t b, int64_t c, double x, double y, double z, int64_t cus) { return pto_hip::makespan({a, b, c}, {x, y, z}, cus); }
 extern "C" int direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) { return pto_hip::experts_direct(slots, experts, hidden, inter); }
 extern "C" int rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, int up, int down) {
   return pto_hip::choose_expert_rows(slots, experts, hidden, inter, up != 0, down != 0, 256);
@@ -29,15 +33,25 @@ def choice(tmp_path_factory):
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", f"-I{CSRC}", str(d / "choice.cpp"), "-o", str(so)], check=True)
     lib = C.CDLL(str(so))
     lib.tile.argtypes = [C.c_int64] * 3 + [C.c_int] * 4 + [C.POINTER(C.c_int)]
+    lib.span.argtypes, lib.span.restype = [C.c_int64] * 3 + [C.c_double] * 3 + [C.c_int64], C.c_double
     lib.direct.argtypes = [C.c_int64] * 4
     lib.rows.argtypes = [C.c_int64] * 4 + [C.c_int] * 2
     return lib
 
 
 def _tile(lib, m, n, kb, exact=False, rows=0, cols=0, splits=0):
-    out = (C.c_int * 3)()
+    out = (C.c_int * 6)()
     lib.tile(m, n, kb, exact, rows, cols, splits, out)
-    return tuple(out)
+    if out[1] == 256:  # every tile starts inside the rows, and they hold all of them
+        heights = [out[0], out[0] // 2, out[0] // 4]
+        last, first = 0, 0
+        for tiles, height in zip(out[3:], heights):
+            assert tiles >= 0 and (tiles == 0 or height >= 64)
+            if tiles:
+                last = first + (tiles - 1) * height
+                first += tiles * height
+        assert last < m <= first
+    return tuple(out[:3])
 
 
 FORMS = {(16, 16), (16, 32), (64, 64), (64, 128), (64, 256), (128, 256), (256, 256)}
@@ -54,6 +68,37 @@ def test_every_size_gets_a_form_that_there_is(choice):
                     # a launch's work items stay below 2^32
                     wgs = -(-m // rows) * -(-n // cols) * (-(-kb // per) if per else 1)
                     assert wgs * 512 < 1 << 32 or m * n > 1 << 34
+
+
+def test_tiles_of_several_heights_hold_all_rows(choice):
+    for m in [*range(1, 1100), 2047, 2048, 2049, 4097, 100000]:
+        for n in (200, 5003, 11008):
+            for exact in (False, True):
+                _tile(choice, m, n, 32, exact)
+        for rows in (64, 128, 256):
+            _tile(choice, m, 2048, 32, rows=rows, cols=256)
+            _tile(choice, m, 2048, 32, exact=True, rows=rows, cols=256, splits=2)
+    # 11008 channels: 43 tiles; 2048 rows as 8 x 256 or 16 x 128 leave the second or third round of tiles a third full
+    assert _tile(choice, 2048, 11008, 32)[:2] == (256, 256)
+
+
+def _greedy(jobs, us, cus):
+    """The same by handing out the workgroups of one XCD one after the other."""
+    free = [0.0] * (cus // 8)
+    heapq.heapify(free)
+    for n, t in zip(jobs, us):
+        for _ in range(-(-n // 8)):
+            heapq.heappush(free, heapq.heappop(free) + t)
+    return max(free)
+
+
+def test_makespan(choice):
+    rng = random.Random(4)
+    for _ in range(2000):
+        jobs = [rng.randint(0, 3000) if rng.random() < 0.7 else 0 for _ in range(3)]
+        us = sorted((rng.uniform(5, 100) for _ in range(3)), reverse=True)
+        got, want = choice.span(*jobs, *us, 256), _greedy(jobs, us, 256)
+        assert abs(got - want) < 1e-6 * max(1.0, want), (jobs, us, got, want)
 
 
 def test_forms_that_are_asked_for(choice):
