@@ -11,7 +11,9 @@
 // 32-bit keys' error: about one token in a hundred.  NaN counts as -inf; equal infinities share a softmax's mass evenly.
 //
 // One wavefront per token, expert e in lane e % 64.  Keys are mapped to unsigned integers of the same order, so that the
-// best of a wavefront is an integer maximum.  Bound by the chain of top_k maxima (six lane exchanges each), not by memory.
+// best of a wavefront is an integer maximum.  Bound by instructions, not by memory: 4096 tokens, eight of 256 experts in four of eight groups,
+// sigmoid and bias, 9.0 us a call, where the 4.5 MB take 1 us; 11.6 us with loads waited for one by one, the lanes' best looked for again
+// behind every choice and groups ranked on exact keys, 14.7 with the whole choice on 64-bit keys.  One token 7 us, the call's own time.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -48,7 +50,7 @@ __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cas
 
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t max_with(uint32_t v) {
-  return max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xf, false));
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true));  // one instruction: 0 where no lane is read
 }
 // The largest of a wavefront's values (wave-uniform): along rows of 16 lanes, then from row to row; lane 63 has seen all.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
@@ -91,16 +93,18 @@ __device__ __forceinline__ V wave_sum(V v) {
   return of_lane(v, 63);
 }
 
-// The lane with the best key of a wavefront, ties to the lowest expert; `top` is that key.
+// The lane with the best key of a wavefront, ties to the lowest expert (ANY: to any); `top` is that key.
+template <bool ANY>
 __device__ __forceinline__ int best_lane(uint32_t key, int expert, uint32_t* top) {
   *top = wave_max(key);
   uint64_t equal = __ballot(key == *top);
-  if (__builtin_expect((equal & (equal - 1)) != 0, 0)) {
+  if (!ANY && __builtin_expect((equal & (equal - 1)) != 0, 0)) {
     const uint32_t lowest = wave_max(key == *top ? ~(uint32_t)expert : 0u);  // all lanes take part
     equal = __ballot(~(uint32_t)expert == lowest);
   }
   return __builtin_ctzll(equal);
 }
+template <bool ANY>
 __device__ __forceinline__ int best_lane(uint64_t key, int expert, uint64_t* top) {
   const uint32_t hi = wave_max((uint32_t)(key >> 32));
   const bool first = (uint32_t)(key >> 32) == hi;
@@ -204,19 +208,28 @@ __device__ __forceinline__ bool choose(const Params& p, const float (&logit)[J],
     }
     V worth = BIAS && p.group_size > 1 ? best + second : best;
     if (!(worth == worth)) worth = -INFINITY;
-    const Key own = g < p.groups ? ordered(worth) : Key(0);
-    int ahead = 0;
-    bool close = false;
-    for (int o = 0; o < p.groups; ++o) {
-      const V other = of_lane(worth, o * p.group_lanes);
-      const Key k = ordered(other);
-      ahead += k > own || (k == own && o < g);
-      if (kNear && o != g && !(fabsf((float)(other - worth)) > 2.f * margin((float)worth, p.sigmoid))) close = true;  // (equal infinities give NaN)
+    bool stays;
+    if constexpr (kNear) {
+      // how many of the others are surely better, and how many may be; one between the two can change sides
+      const float here = fminf(fmaxf(worth, -3e38f), 3e38f), reach = 2.f * margin(here, p.sigmoid);
+      int surely = 0, maybe = -1;  // (itself)
+      for (int o = 0; o < p.groups; ++o) {
+        const float other = of_lane(here, o * p.group_lanes);
+        surely += other > here + reach;
+        maybe += other >= here - reach;
+      }
+      stays = g < p.groups && maybe < p.kept;
+      if (__ballot(g < p.groups && !stays && surely < p.kept)) near = true;
+    } else {
+      const Key own = g < p.groups ? ordered(worth) : Key(0);
+      int ahead = 0;
+      for (int o = 0; o < p.groups; ++o) {
+        const Key k = ordered(of_lane(worth, o * p.group_lanes));
+        ahead += k > own || (k == own && o < g);
+      }
+      stays = g < p.groups && ahead < p.kept;
     }
-    const bool stays = g < p.groups && ahead < p.kept;
     const uint64_t stay = __ballot(stays);
-    // only a group next to the line between those that stay and those that do not can change sides: the last that stays, the first that does not
-    if (kNear && p.kept < p.groups && __ballot(g < p.groups && close && (ahead == p.kept - 1 || ahead == p.kept))) near = true;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int e = lane + 64 * j;
@@ -228,40 +241,68 @@ __device__ __forceinline__ bool choose(const Params& p, const float (&logit)[J],
     }
     __builtin_amdgcn_wave_barrier();
   }
-  Key best = 0;
-  int at = 0;
-  auto look = [&] {  // this lane's best
-    best = key[0];
-    at = 0;
+  // Up to four keys a lane are put in descending order first, the lower expert first among equal ones; of more the best is looked for
+  // again behind every choice (sorting sixteen takes longer than that).
+  constexpr bool kSorted = J <= 4;
+  int at[J];
 #pragma unroll
-    for (int j = 1; j < J; ++j)
-      if (key[j] > best) {
-        best = key[j];
-        at = j;
+  for (int j = 0; j < J; ++j) at[j] = lane + 64 * j;
+  if constexpr (kSorted) {
+#pragma unroll
+    for (int end = J - 1; end > 0; --end)
+#pragma unroll
+      for (int j = 0; j < end; ++j) {
+        const bool swap = key[j + 1] > key[j];
+        const Key high = swap ? key[j + 1] : key[j], low = swap ? key[j] : key[j + 1];
+        const int high_at = swap ? at[j + 1] : at[j], low_at = swap ? at[j] : at[j + 1];
+        key[j] = high, key[j + 1] = low, at[j] = high_at, at[j + 1] = low_at;
       }
+  }
+  Key best = 0;  // this lane's
+  int best_at = 0;
+  auto look = [&] {
+    best = key[0];
+    best_at = at[0];
+    if constexpr (!kSorted) {
+#pragma unroll
+      for (int j = 1; j < J; ++j)
+        if (key[j] > best) {
+          best = key[j];
+          best_at = at[j];
+        }
+    }
   };
   look();
-  Key last = 0;
-  const int picks = kNear ? p.top_k + 1 : p.top_k;  // one more to know how far the first left out is
-  for (int i = 0; i < picks; ++i) {
+  Key taken = 0;  // lane i: key of the i-th expert
+  for (int i = 0; i < p.top_k; ++i) {
     Key first;
-    const int winner = best_lane(best, lane + 64 * at, &first);
-    if constexpr (kNear) {
-      if (first == 0) break;  // nothing is left out
-      const float a = value_of(last), b = value_of(first);
-      if (i > 0 && !(a - b > margin(a, p.sigmoid))) near = true;
-      if (near) break;
-      last = first;
-      if (i == p.top_k) break;
+    const int winner = best_lane<kNear>(best, best_at, &first);
+    const int e = __builtin_amdgcn_readlane(best_at, winner);
+    if (lane == i) {
+      *mine = e;
+      taken = first;
     }
-    const int e = __builtin_amdgcn_readlane(lane + 64 * at, winner);
-    if (lane == i) *mine = e;
     if (lane == winner) {
+      if constexpr (kSorted) {
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (j == at) key[j] = 0;
+        for (int j = 0; j + 1 < J; ++j) {
+          key[j] = key[j + 1];
+          at[j] = at[j + 1];
+        }
+        key[J - 1] = 0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (at[j] == best_at) key[j] = 0;
+      }
       look();
     }
+  }
+  if constexpr (kNear) {
+    const uint32_t left_out = wave_max(best);  // 0: nothing is
+    const uint32_t next = (uint32_t)__shfl_down((int)taken, 1);
+    const float a = value_of(taken), b = value_of(lane + 1 < p.top_k ? next : left_out);
+    if (__ballot(lane < p.top_k && (lane + 1 < p.top_k || left_out) && !(a - b > margin(a, p.sigmoid)))) near = true;
   }
   return !near;
 }
@@ -277,11 +318,13 @@ __global__ __launch_bounds__(kWaves * 64) void route_kernel(Params p) {
   float top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const int e = lane + 64 * j;
-    const float v = e < p.experts ? (float)row[e] : -INFINITY;
-    logit[j] = v == v ? v : -INFINITY;
-    bias[j] = BIAS && e < p.experts ? p.bias[e] : 0.f;
+    const int e = min(lane + 64 * j, p.experts - 1);  // (all are asked for at once)
+    logit[j] = (float)row[e];
+    bias[j] = BIAS ? p.bias[e] : 0.f;
   }
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (lane + 64 * j >= p.experts || !(logit[j] == logit[j])) logit[j] = -INFINITY;
 #pragma unroll
   for (int j = 0; j < J; ++j) top = fmaxf(top, logit[j]);
   top = value_of(wave_max(ordered(top)));

@@ -680,3 +680,24 @@ def test_two_threads_on_one_stream(worker):
     worker.sync()
     assert not errors
     assert all(torch.equal(out, w) for outs_i, w in zip(outs, want) for out in outs_i)
+
+
+@pytest.mark.parametrize("experts,top_k,groups,kept", [(256, 8, 8, 4), (64, 6, 1, 1), (512, 10, 32, 5)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_router_of_many_tokens(worker, experts, top_k, groups, kept, sigmoid):
+    """Enough of them that some choices fall between keys, and groups, that 32 bits do not tell apart."""
+    g = _gen(experts)
+    logits = _randn(g, 5000, experts).bfloat16()
+    _check_route(worker, logits, 0.01 * _randn(g, experts), top_k, groups, kept, sigmoid=sigmoid)
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("big", [1e6, 3e38, float("inf"), float("-inf")])
+def test_router_on_biases_that_swallow_the_scores(worker, sigmoid, big):
+    g = _gen(6)
+    logits = _randn(g, 40, 96)
+    bias = torch.zeros(96, device="cuda")
+    bias[[3, 17, 50, 51, 52, 80]] = big
+    bias[48:60] = -abs(big)
+    for groups, kept in ((1, 1), (8, 3), (8, 5)):
+        _check_route(worker, logits, bias, 7, groups, kept, sigmoid=sigmoid)
