@@ -40,7 +40,7 @@ struct Params {
 
 enum RowMap { kPlain = 0, kGateUp = 1, kDown = 2 };
 
-// A tile's rows: row r of it is row a_row(r) of the activations and row c_row(r) of the result.  `at`: its first row, experts: its index.
+// A tile's rows: row r of it is row a_row(r) of the activations.  `at`: its first row, experts: its index.
 template <int MAP>
 struct Tile {
   int expert, first, rows;
@@ -59,7 +59,6 @@ struct Tile {
     }
   }
   __device__ __forceinline__ int a_row(int r) const { return MAP == kGateUp ? order[first + r] / top_k : first + r; }
-  __device__ __forceinline__ int c_row(int r) const { return MAP == kDown ? order[first + r] : first + r; }
 };
 
 // SiLU with the hardware's 1-ulp reciprocal (as the other e4m3 FFN's).

@@ -34,6 +34,7 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) const i32x4 lds_ci32x4;
 typedef __attribute__((address_space(3))) float lds_float;
+typedef __attribute__((address_space(3))) int lds_int;
 
 constexpr int kXcds = 8;
 // Consecutive logical ids to one XCD: workgroups are dealt to the XCDs in turn.
@@ -59,7 +60,7 @@ struct TiledShape {
   static constexpr int NS = BM / 64;                     // ... for eight blocks' row scales
   static constexpr int kScaleRow8 = 264;                 // bytes of a request of those
   static constexpr int kScaleBuf = BM / 8 * kScaleRow8;
-  static constexpr int kScales = RING * kStage, kChannelScales = kScales + 2 * kScaleBuf;
+  static constexpr int kScales = RING * kStage, kRows = kScales + 2 * kScaleBuf, kChannelScales = kRows + BM * 4;
   static constexpr size_t smem(int kb) { return (size_t)kChannelScales + 2 * (size_t)((kb + 63) / 64 * 64) * sizeof(float); }
   static_assert(KG == 1 || PH == 1, "groups along k have one half of rows");
 };
@@ -104,6 +105,14 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
     for (int i = (wave >> 1) * 64; i < nk; i += 256)
       to_lds_dword((uint32_t)min(i + lane, nk - 1) * 4u, wave & 1 ? c1 : c0, lds_base + S::kChannelScales + ((wave & 1) * nk64 + i) * 4);
   }
+
+  // ---- down pass: where the rows go, for the epilogue (asked for there, one after the other between the stores, they took 8 us a tile) ----
+  lds_int* const s_rows = (lds_int*)(lds0 + S::kRows);
+  if constexpr (MAP == kDown) {
+    if (wave < BM / 64)
+      to_lds_dword((uint32_t)min(wave * 64 + lane, tile.rows - 1) * 4u, p.order + tile.first, lds_base + S::kRows + wave * 256);
+  }
+  auto c_row = [&](int r) { return (size_t)(MAP == kDown ? s_rows[r] : tile.first + r); };
 
   // ---- requests: instruction e of a part brings its rows 64 e + 8 wave + lane / 8; rows and channels past the end are clamped
   // (their products are not stored) ----
@@ -388,20 +397,20 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
       for (int v = 0; v < 4; ++v)
         *reinterpret_cast<uint32_t*>(smem + row * kBlock + wn * 32 + v * 8 + hi * 4) =
             codes4(q(y[i][4 * v]), q(y[i][4 * v + 1]), q(y[i][4 * v + 2]), q(y[i][4 * v + 3]));
-      if (wn == 0 && hi == 0 && row < tile.rows) p.c_scale[(size_t)tile.c_row(row) * (p.n / kBlock) + tn] = s;
+      if (wn == 0 && hi == 0 && row < tile.rows) p.c_scale[c_row(row) * (p.n / kBlock) + tn] = s;
     }
     __syncthreads();
     uint8_t* const codes = reinterpret_cast<uint8_t*>(p.c);
     for (int u = tid; u < tile.rows * 8; u += 512) {
       const int row = u >> 3;
-      *reinterpret_cast<i32x4*>(codes + (size_t)tile.c_row(row) * p.n + n0 + (u & 7) * 16) = *reinterpret_cast<const i32x4*>(smem + u * 16);
+      *reinterpret_cast<i32x4*>(codes + c_row(row) * p.n + n0 + (u & 7) * 16) = *reinterpret_cast<const i32x4*>(smem + u * 16);
     }
   } else {
     // Rows go through LDS, a half of them at a time, so that they are written in whole lines: straight from the accumulators a wavefront's
     // store has 16 bytes of each of 32 rows.
     constexpr bool SCALED = MAP == kDown && std::is_same<OutT, _Float16>::value;
     constexpr int ROWS = BM / S::PH, PITCH = BN * (int)sizeof(OutT) + 16;  // bytes; the padding spreads rows over the banks
-    static_assert(ROWS * PITCH <= (SCALED ? (int)S::kScales : (int)S::kChannelScales), "a half of the rows fits");
+    static_assert(ROWS * PITCH <= (SCALED ? (int)S::kScales : (int)S::kRows), "a half of the rows fits");
     int e[S::MF];  // SCALED: rows for the sum over a token's experts, fp16 with a power of two per row and 128 channels that puts the largest below 2^15
 #pragma unroll
     for (int i = 0; i < S::MF; ++i) e[i] = 0;
@@ -424,7 +433,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
         const int row = row_of(i);
         e[i] = half_exponent(fmaxf(top[(wn & ~1) * BM + row], top[(wn | 1) * BM + row]));
         if ((wn & 1) == 0 && hi == 0 && row < tile.rows && group * kBlock < p.n)
-          p.c_scale[(size_t)tile.c_row(row) * (p.n / kBlock) + group] = __builtin_ldexpf(1.f, e[i]);
+          p.c_scale[c_row(row) * (p.n / kBlock) + group] = __builtin_ldexpf(1.f, e[i]);
       }
     }
     OutT* const c = reinterpret_cast<OutT*>(p.c) + (size_t)range * p.m * p.n + n0;
@@ -456,12 +465,12 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
         for (int u = tid; u < rows * PER_ROW; u += 512) {
           const int row = u / PER_ROW, at = u % PER_ROW;
           if (at * VEC < cols)
-            *reinterpret_cast<i32x4*>(c + (size_t)tile.c_row(h * ROWS + row) * p.n + at * VEC) = *reinterpret_cast<const i32x4*>(smem + row * PITCH + at * 16);
+            *reinterpret_cast<i32x4*>(c + c_row(h * ROWS + row) * p.n + at * VEC) = *reinterpret_cast<const i32x4*>(smem + row * PITCH + at * 16);
         }
       } else {
         for (int u = tid; u < rows * BN; u += 512) {
           const int row = u / BN, at = u % BN;
-          if (at < cols) c[(size_t)tile.c_row(h * ROWS + row) * p.n + at] = reinterpret_cast<const OutT*>(smem + row * PITCH)[at];
+          if (at < cols) c[c_row(h * ROWS + row) * p.n + at] = reinterpret_cast<const OutT*>(smem + row * PITCH)[at];
         }
       }
       if (h + 1 < S::PH) __syncthreads();

@@ -26,11 +26,12 @@ constexpr int64_t kPassSlots = 32768;
 constexpr int64_t kMostDirectSlots = 1024;
 
 // The plan: slots by expert, and tiles of one expert each: of `height` rows, and what an expert has left in a tile of the least of height,
-// height / 2 and height / 4 rows (64 at least) that holds it.  The heights lie one behind the other, n_tiles[] of each.  One workgroup; a
-// slot with a negative expert is in no tile, one with an expert that there is not is reported.  Each wavefront counts for itself ([wavefronts][experts] in LDS), so that the
-// counters of a busy expert are shared by 64 lanes and not by all, and a slot's rank in its wavefront's count is its place: with
-// one set of counters and a second round of atomics for the places 16384 slots of 64 experts took 19 us.  The sorted slots are put together in
-// LDS: written one by one, each to a line of its own, they took 8 of 17 us.  The order of the ranks is that of the atomics: which row of which tile a slot becomes changes no bit of its result.
+// height / 2 and height / 4 rows (64 at least) that holds it.  The heights lie one behind the other, n_tiles[] of each.  One workgroup, EACH
+// slots a thread; a slot with a negative expert is in no tile, one with an expert that there is not is reported.  Each wavefront counts for
+// itself ([wavefronts][experts] in LDS), so that the counters of a busy expert are shared by 64 lanes and not by all, and a slot's rank in its
+// wavefront's count is its place.  The sorted slots are put together in LDS: written one by one, each to a line of its own, they took 5 us
+// more.  The order of the ranks is that of the atomics: which row of which tile a slot becomes changes no bit of its result.
+// Bound by the LDS atomics: 160 slots 4.7 us, 4096 6, 16384 12, 32768 16.
 template <int EACH>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __restrict__ ids, int slots, int experts, int height,
                                                             int32_t* __restrict__ order, int4* __restrict__ tiles, int* __restrict__ n_tiles,
@@ -41,26 +42,30 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
   __shared__ int sums[2][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int i = tid; i < kWaves * experts; i += kPlanThreads) count[i] = 0;
-  int e[EACH], rank[EACH];
+  int place[EACH];  // the slot's expert, then with its rank behind the experts' bits; -1: none
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int s = i * kPlanThreads + tid;
-    e[i] = s < slots ? ids[s] : -1;
+    const int id = ids[(uint32_t)min(s, slots - 1)];
+    place[i] = s < slots ? id : -1;
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    if (e[i] >= experts) {
-      *flag = 1;
-      e[i] = -1;
-    }
-    rank[i] = e[i] >= 0 ? atomicAdd(&count[wave * experts + e[i]], 1) : 0;
+    const int e = place[i];
+    if (e >= experts) *flag = 1;
+    int rank = 0;
+    if ((unsigned)e < (unsigned)experts) rank = atomicAdd(&count[wave * experts + e], 1);
+    place[i] = (unsigned)e < (unsigned)experts ? e | rank * kMaxExperts : -1;
   }
   __syncthreads();
   // thread t: expert t's rows and tiles, exclusive sums over the experts in front, then over its wavefronts
-  int rows = 0;
-  if (tid < experts)
-    for (int w = 0; w < kWaves; ++w) rows += count[w * experts + tid];
+  int rows = 0, counted[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    counted[w] = tid < experts ? count[w * experts + tid] : 0;
+    rows += counted[w];
+  }
   int mine[3] = {rows / height, 0, 0};
   const int rest = rows - mine[0] * height;
   const int rest_height = height >= 256 && rest <= height / 4 ? 2 : height >= 128 && rest <= height / 2 ? 1 : 0;
@@ -95,17 +100,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
       const int place = rest_height == 0 ? full + rows / height : all_full + (rest_height == 1 ? before[1] >> 16 : (all[1] >> 16) + (before[0] >> 16));
       tiles[place] = int4{tid, at + rows - rest, rest, 0};
     }
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const int here = count[w * experts + tid];
       count[w * experts + tid] = at;
-      at += here;
+      at += counted[w];
     }
   }
   if (tid < 3) n_tiles[tid] = tid == 0 ? all[1] & 0xffff : tid == 1 ? all[1] >> 16 : all[0] >> 16;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
-    if (e[i] >= 0) sorted[count[wave * experts + e[i]] + rank[i]] = (uint16_t)(i * kPlanThreads + tid);
+    if (place[i] >= 0)
+      sorted[count[wave * experts + (unsigned)place[i] % kMaxExperts] + (unsigned)place[i] / kMaxExperts] = (uint16_t)(i * kPlanThreads + tid);
   __syncthreads();
   for (int i = tid; i < (all[0] & 0xffff); i += kPlanThreads) order[i] = sorted[i];
 }
