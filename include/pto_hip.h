@@ -399,7 +399,7 @@ PTO_HIP_API int pto_hip_route_experts(const void* logits, const float* bias, int
 
 /* out[t] = sum_j expert_weights[t, j] * (SiLU(x Wg_e) * (x Wu_e)) Wd_e with e = expert_ids[t, j] and x the token's values: the
  * experts' half of a mixture layer behind pto_hip_rms_norm_fp8_block and pto_hip_route_experts.  Products as
- * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 as pto_hip_quantize_fp8_block does, the sum over a token's
+ * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 with those scales, the sum over a token's
  * experts is fp32.  A negative id leaves its slot out (a token without any gives zeros); an id of an expert that there is
  * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  With BF16 results of many
  * tokens both products are as pto_hip_projection_fp8_block's of 16-bit results, and the experts' rows are added from fp16 with a

@@ -32,15 +32,16 @@ __device__ __forceinline__ float finite_size(float v) { return fabsf(v) <= 3.402
 // The power of two that, divided out, puts a largest size of amax into [2^14, 2^15); 0 for none, and within what fp32 holds.
 __device__ __forceinline__ int half_exponent(float amax) { return amax > 0.f ? max(ilogbf(amax) - 14, -126) : 0; }
 
-// v / scale, correctly rounded, as often as a group has elements: the reciprocal is refined once to half an ulp, the quotient
-// twice by its exact remainder (as in ffn_fp8.hip's row quantiser).  No quotient of a finite group leaves +-448 (1 + 2^-23), which rounds to a code
-// without a clamp; an infinite scale (an infinite element) takes the division itself.
+// v / scale as often as a group has elements.
 struct GroupQuotient {
   float s, r;
   __device__ __forceinline__ explicit GroupQuotient(float scale) : s(scale) {
     r = __builtin_amdgcn_rcpf(s);
     r = fmaf(fmaf(-s, r, 1.f), r, r);
   }
+  // Correctly rounded: the reciprocal is refined once to half an ulp, the quotient twice by its exact remainder (as in ffn_fp8.hip's row
+  // quantiser).  No quotient of a finite group leaves +-448 (1 + 2^-23), which rounds to a code without a clamp; an infinite scale (an infinite
+  // element) takes the division itself.
   __device__ __forceinline__ float operator()(float v) const {
     if (__builtin_expect(!(s <= 3.4028234664e38f), 0)) return v / s;
     const float q0 = v * r;
@@ -48,6 +49,9 @@ struct GroupQuotient {
     const float q2 = fmaf(fmaf(-q1, s, v), r, q1);
     return v == 0.f ? v : q2;  // a zero keeps its sign
   }
+  // Within an ulp and a half, for values that are further off themselves (h, whose exponential and reciprocal are off by 2^-17); of an
+  // infinite scale the same as the division, zeros and NaN.
+  __device__ __forceinline__ float near(float v) const { return v * (s <= 3.4028234664e38f ? r : 0.f); }
 };
 
 // Four quotients as codes, the first in the lowest byte (round to nearest even; NaN stays NaN).

@@ -106,7 +106,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
       to_lds_dword((uint32_t)min(i + lane, nk - 1) * 4u, wave & 1 ? c1 : c0, lds_base + S::kChannelScales + ((wave & 1) * nk64 + i) * 4);
   }
 
-  // ---- down pass: where the rows go, for the epilogue (asked for there, one after the other between the stores, they took 8 us a tile) ----
+  // ---- down pass: where the rows go, for the epilogue (asked for there, between the stores, they took 3 us a tile) ----
   lds_int* const s_rows = (lds_int*)(lds0 + S::kRows);
   if constexpr (MAP == kDown) {
     if (wave < BM / 64)
@@ -396,7 +396,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
 #pragma unroll
       for (int v = 0; v < 4; ++v)
         *reinterpret_cast<uint32_t*>(smem + row * kBlock + wn * 32 + v * 8 + hi * 4) =
-            codes4(q(y[i][4 * v]), q(y[i][4 * v + 1]), q(y[i][4 * v + 2]), q(y[i][4 * v + 3]));
+            codes4(q.near(y[i][4 * v]), q.near(y[i][4 * v + 1]), q.near(y[i][4 * v + 2]), q.near(y[i][4 * v + 3]));
       if (wn == 0 && hi == 0 && row < tile.rows) p.c_scale[c_row(row) * (p.n / kBlock) + tn] = s;
     }
     __syncthreads();
@@ -422,7 +422,14 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) amax = fmaxf(amax, finite_size(acc[i][j][r]));
+          for (int r = 0; r < 16; ++r) amax = fmaxf(amax, fabsf(acc[i][j][r]));
+        if (__builtin_expect(__ballot(!(amax <= 3.4028234664e38f)) != 0, 0)) {  // infinities aside
+          amax = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) amax = fmaxf(amax, finite_size(acc[i][j][r]));
+        }
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         if (hi == 0) top[wn * BM + row_of(i)] = amax;
       }

@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kDirectDown * 64) void direct_down_kernel(Experts x
       const float s = group_scale(amax);
       const GroupQuotient q(s);
       if (u < units) {  // rows and groups lie one behind the other in units' order
-        *reinterpret_cast<uint32_t*>(codes + u * kBlock + 4 * lane32) = codes4(q(v[i].x), q(v[i].y), q(v[i].z), q(v[i].w));
+        *reinterpret_cast<uint32_t*>(codes + u * kBlock + 4 * lane32) = codes4(q.near(v[i].x), q.near(v[i].y), q.near(v[i].z), q.near(v[i].w));
         if (lane32 == 0) scales[u] = s * weight[i];
       }
     }
