@@ -374,6 +374,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
   auto row_of = [&](int i) { return (i / S::HF) * (BM / S::PH) + wm * (BM / S::PH / 2) + (i % S::HF) * 32 + (lane & 31); };
   if constexpr (GATE) {
     // the wavefront's 32 outputs of a row, the largest of the row's 128 through LDS, codes staged there for whole rows' stores
+    constexpr int PITCH = kBlock + 16;  // bytes; with rows of 128 the 32 lanes of a store were in one bank, 4 us of a 256-row tile
     lds_float* const top = (lds_float*)(lds0 + S::kScales);  // [4][BM]
     f32x16 y[S::MF];
 #pragma unroll
@@ -395,7 +396,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
       const GroupQuotient q(s);
 #pragma unroll
       for (int v = 0; v < 4; ++v)
-        *reinterpret_cast<uint32_t*>(smem + row * kBlock + wn * 32 + v * 8 + hi * 4) =
+        *reinterpret_cast<uint32_t*>(smem + row * PITCH + wn * 32 + v * 8 + hi * 4) =
             codes4(q.near(y[i][4 * v]), q.near(y[i][4 * v + 1]), q.near(y[i][4 * v + 2]), q.near(y[i][4 * v + 3]));
       if (wn == 0 && hi == 0 && row < tile.rows) p.c_scale[c_row(row) * (p.n / kBlock) + tn] = s;
     }
@@ -403,7 +404,7 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
     uint8_t* const codes = reinterpret_cast<uint8_t*>(p.c);
     for (int u = tid; u < tile.rows * 8; u += 512) {
       const int row = u >> 3;
-      *reinterpret_cast<i32x4*>(codes + c_row(row) * p.n + n0 + (u & 7) * 16) = *reinterpret_cast<const i32x4*>(smem + u * 16);
+      *reinterpret_cast<i32x4*>(codes + c_row(row) * p.n + n0 + (u & 7) * 16) = *reinterpret_cast<const i32x4*>(smem + row * PITCH + (u & 7) * 16);
     }
   } else {
     // Rows go through LDS, a half of them at a time, so that they are written in whole lines: straight from the accumulators a wavefront's
