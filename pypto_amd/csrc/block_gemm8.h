@@ -104,7 +104,7 @@ __device__ __forceinline__ f32x4 block_product(const i32x4 (&w)[2], const i32x4 
 
 // Up to 16 rows a tile: 16 rows x 16 CT channels, both operands straight from memory to registers; the workgroup's KW wavefronts take
 // the steps of 128 codes in turn, NS of them in flight, and sum through LDS in wavefront order.  Bound by the stream of the weights and what
-// starts it: 25 MB of 4096 x 6144 at one row 8.4 us a call (an empty call 6.8, the stream 4.8), 45 MB of 11008 x 4096 10.
+// starts it: 25 MB of 4096 x 6144 at one row 8.0 us a call (an empty call 6.8, the stream 4.8), 45 MB of 11008 x 4096 10.
 template <int CT, int KW, int NS, typename OutT>
 __global__ __launch_bounds__(KW * 64) void narrow_kernel(Params p, int tiles_n) {
   __shared__ __attribute__((aligned(16))) f32x4 red[KW][CT][64];

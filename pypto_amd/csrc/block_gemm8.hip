@@ -57,6 +57,7 @@ int launch_projection(const Params& p, hipStream_t st) {
     if (wgs >= (1 << 23)) return fail(PTO_HIP_ERR_UNSUPPORTED, "a product of %lld tiles is more than one launch holds", (long long)wgs);
     const dim3 grid((unsigned)wgs);
     if (t.cols == 16) hipLaunchKernelGGL((narrow_kernel<1, 8, 4, OutT>), grid, dim3(512), 0, st, p, tiles_n);
+    else if (t.tiles[0] == 8) hipLaunchKernelGGL((narrow_kernel<2, 8, 3, OutT>), grid, dim3(512), 0, st, p, tiles_n);
     else hipLaunchKernelGGL((narrow_kernel<2, 4, 3, OutT>), grid, dim3(256), 0, st, p, tiles_n);
     PTO_CHECK_HIP(hipGetLastError());
     return PTO_HIP_OK;

@@ -286,7 +286,7 @@ inline int64_t attn_partition_align(int64_t pairs, int64_t max_ctx, int64_t bloc
 struct BlockTile {
   int rows, cols;  // tile; rows 16: the form that reads straight to registers, of cols channels a workgroup
   int per_split;   // blocks of k of a range, 0: unsplit
-  int tiles[3];    // 256 channels: row tiles of `rows`, half and a quarter of it, one behind the other
+  int tiles[3];    // 256 channels: row tiles of `rows`, half and a quarter of it, one behind the other; rows 16: wavefronts of a workgroup
 };
 struct BlockTileCost {
   int rows, cols;
@@ -333,12 +333,14 @@ inline double makespan(const int64_t (&jobs)[3], const double (&us)[3], int64_t 
 }
 
 // The form with the least estimated time of a product of m rows, n channels and kb blocks of k.  Timed against every tile and count of
-// ranges, the one it picks among the tiles is 0.9 % from the best in the mean and 13 % at worst, exact 0.3 % and 9 %.  rows, cols, splits: given, or 0.
+// ranges, the one it picks among the tiles is 0.9 % from the best in the mean and 13 % at worst, exact 0.4 % and 7 %.  rows, cols, splits: given, or 0.
 // Tiles of 256 channels share the rows among several heights where one height leaves its last round part empty: 11008 channels of 4096, us
 // with one height / several: 1300 rows 78 / 64, 1600 106 / 91, 2048 115 / 101, 4096 185 / 186; 5003 of 5120 4096 rows 149 / 125.
 // The estimate itself takes 1 us of the caller's time, none where up to 16 rows are bound by memory.
-// Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, or, with few channels
-// and a long k, 16 of eight (11008 x 4096 at one row 19.4 -> 10.0 us, 16384 x 1024 20.6 -> 12.2; 4096 x 14336 the other way 13.6 -> 19.5).
+// Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, of eight where
+// there is at most one of them for a CU, 16 of eight where that leaves half of the CUs without one.  One row, us, four / eight / 16 of eight: 4096 x
+// 14336 14.0 / 16.4 / 19.6, 4096 x 6144 9.6 / 8.8 / 10.7, 5120 x 5003 11.6 / 8.8 / 10.8, 8192 x 8192 22.1 / 18.7 / 16.6, 11008 x 4096 - / 16.4 / 12.7, 16384 x 1024
+// - / 19.1 / 12.2.
 inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact, int64_t num_cu, int rows, int cols, int splits) {
   const double weights_mb = (double)n * (double)kb * 128e-6;
   const double memory = 4.0 + weights_mb / 5.0;
@@ -346,16 +348,10 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
   BlockTile pick{64, 256, 0, {(int)((m + 63) / 64), 0, 0}};
   if ((rows == 0 && m <= 16 && splits == 0) || rows == 16) {
     const double stream = 2.3 + weights_mb / 5.2 * (1.0 + 0.02 * (double)m);
-    const double wide = std::max(stream, 3.0 + (double)kb / 4 * (0.6 + 0.012 * (double)m));
-    best = wide;
-    pick = BlockTile{16, 32, 0, {}};
-    if (n <= 16 * num_cu) {
-      const double few = std::max(stream, 3.0 + (double)kb / 8 * (0.55 + 0.045 * (double)m));
-      if (few < wide) {
-        best = few;
-        pick = BlockTile{16, 16, 0, {}};
-      }
-    }
+    const int channels = n <= 16 * num_cu ? 16 : 32, waves = n <= 32 * num_cu ? 8 : 4;
+    const double step = channels == 16 ? 0.55 + 0.045 * (double)m : 0.6 + 0.012 * (double)m;
+    best = std::max(stream, 3.0 + (double)kb / waves * step);
+    pick = BlockTile{16, channels, 0, {waves}};
     if (rows == 16 || best <= memory) return pick;
   }
   for (int form = 0; form < (exact ? 4 : 5); ++form) {
@@ -377,7 +373,7 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
         }
         double us = makespan(jobs, each, num_cu);
         us = std::max(us, memory) + 0.1 * std::min(us, memory);
-        if (ranges > 1) us += 4.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
+        if (ranges > 1) us += 5.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
         if (us < best) {
           best = us;
           pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0, {(int)high, (int)half, (int)quarter}};

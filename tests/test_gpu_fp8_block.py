@@ -198,6 +198,18 @@ def test_product_is_exact_on_whole_numbers_and_stays_inside(worker, tile, m, k, 
         assert torch.equal(got, want.float().to(dtype)), dtype
 
 
+@pytest.mark.parametrize("tile", [(0, 0, 0), (16, 0, 0)], ids=str, indirect=True)
+@pytest.mark.parametrize("m,k,n", [(1, 256, 4200), (16, 1152, 4097), (3, 3968, 5003), (5, 640, 8192), (1, 128, 8193), (16, 1408, 8300), (9, 4096, 9000), (40, 512, 8200)])
+def test_product_of_few_rows_and_many_channels(worker, tile, m, k, n):
+    """16 or 32 channels a workgroup, four or eight wavefronts: their steps end unevenly."""
+    a, sa, w, sw = _operands(_gen(k + n), m, k, n)
+    for dtype in (torch.float32, torch.float16):
+        got = _product(worker, a, sa, w, sw, dtype).double()
+        want = ob.projection(a, sa, w, sw)
+        bound = (ob.dequantize_rows(a, sa).abs() @ ob.dequantize_matrix(w, sw).abs().t()) * (132 + k // 128) * 2.0 ** -24
+        assert ((got - want).abs() <= bound + (want.abs() + bound) * HALF_STEP[dtype] + TINY[dtype]).all()
+
+
 def _operands(g, m, k, n):
     a, sa = ob.quantize_rows(_randn(g, m, k))
     w, sw = ob.quantize_matrix(_randn(g, n, k) * k ** -0.5)
