@@ -713,3 +713,37 @@ def test_router_on_biases_that_swallow_the_scores(worker, sigmoid, big):
     bias[48:60] = -abs(big)
     for groups, kept in ((1, 1), (8, 3), (8, 5)):
         _check_route(worker, logits, bias, 7, groups, kept, sigmoid=sigmoid)
+
+
+def test_two_graphs_that_share_scratch(worker):
+    """Recorded one behind the other, replayed in turn on one stream: each has the bits of its eager call, whichever ran before."""
+    stream = torch.cuda.Stream()
+    cases = [_experts_case(20 + i, t, 512, 384, 16, 4) for i, t in enumerate((5, 90, 700))]
+    a, sa, w, sw = _operands(_gen(30), 40, 8192, 512)  # few tiles, a long k: ranges in slabs
+    run, product = worker.register(runtime.experts_ffn_fp8_block), worker.register(runtime.projection_fp8_block)
+    outs = [torch.empty((len(c[0]), 512), dtype=torch.bfloat16, device="cuda") for c in cases] + [torch.empty((40, 512), dtype=torch.float16, device="cuda")]
+
+    def call(i, st):
+        if i < 3:
+            run(*cases[i], outs[i], stream=st)
+        else:
+            product(a, sa, w, sw, outs[i], stream=st)
+
+    want, graphs = [], []
+    for i in range(4):
+        call(i, 0)
+        worker.sync()
+        want.append(outs[i].clone())
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            call(i, torch.cuda.current_stream().cuda_stream)
+    for order in ((0, 1, 2, 3), (3, 1, 0, 2), (2, 0, 3, 1)):
+        for out in outs:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for i in order:
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, w) for out, w in zip(outs, want)), order
+    worker.sync()
