@@ -364,13 +364,15 @@ PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* sca
 /* ---- e4m3 operands with a scale for each block of 128 (none has a counterpart in the reference) ----
  * Activations: codes [rows, cols] with one fp32 scale per 128 columns of a row, [rows, ceil(cols / 128)].  Weights: codes one row per
  * OUTPUT channel with k contiguous, [n, k], with one fp32 scale per block of 128 x 128, [ceil(n / 128), k / 128].  A value is its
- * code times its scale; scales may be any fp32 values. */
+ * code times its scale; scales may be any fp32 values.  Results lie apart from the operands and from each other, unless said otherwise
+ * (PTO_HIP_ERR_INVALID_VALUE). */
 
 /* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
  * codes = e4m3(n / scale), round to nearest even; sum_out = x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every
- * output is rounded once (a row whose sum of squares passes fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out may each be NULL; sum_out may be x or residual itself.  NaN
- * elements are left out of amax and give NaN codes.  cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the
- * last group may be shorter).  quantize_fp8_block: codes and scales of x itself. */
+ * output is rounded once (a row whose sum of squares passes fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out
+ * may each be NULL; sum_out and normed_out may be x or residual themselves.  NaN elements are left out of amax and give NaN codes.
+ * cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the last group may be shorter).
+ * quantize_fp8_block: codes and scales of x itself. */
 PTO_HIP_API int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out,
                                            void* codes, float* scale, int64_t rows, int64_t cols, float eps, int x_dtype,
                                            void* stream);

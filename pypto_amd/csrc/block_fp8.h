@@ -15,6 +15,12 @@ namespace block8 {
 constexpr int kBlock = 128;  // elements that share a scale
 constexpr int kMaxK = 65536;  // longest rows of the products: byte offsets inside a tile stay far below 2^31
 
+// Whether two ranges of bytes have any in common (null: none).
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+  return a && b && pa < pb + (uintptr_t)b_bytes && pb < pa + (uintptr_t)a_bytes;
+}
+
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4;
 typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
 

@@ -94,6 +94,11 @@ extern "C" int pto_hip_projection_fp8_block(const void* a8, const float* a_scale
   PTO_CHECK_ARG(((uintptr_t)a8 | (uintptr_t)w8) % 16 == 0 && ((uintptr_t)a_scale | (uintptr_t)w_scale) % 4 == 0 &&
                     (uintptr_t)out % (size_t)dtype_bytes(out_dtype) == 0,
                 "projection_fp8_block: codes must be 16-byte aligned, scales and out to their elements");
+  const int64_t kb = k / block8::kBlock, out_bytes = m * n * dtype_bytes(out_dtype);
+  PTO_CHECK_ARG(!block8::overlap(out, out_bytes, a8, m * k) && !block8::overlap(out, out_bytes, a_scale, m * kb * 4) &&
+                    !block8::overlap(out, out_bytes, w8, n * k) &&
+                    !block8::overlap(out, out_bytes, w_scale, (n + block8::kBlock - 1) / block8::kBlock * kb * 4),
+                "projection_fp8_block: out overlaps an operand");
   block8::Params p{};
   p.a = reinterpret_cast<const uint8_t*>(a8);
   p.sa = a_scale;

@@ -526,6 +526,17 @@ extern "C" int pto_hip_experts_ffn_fp8_block(const void* x8, const float* x_scal
                     ((uintptr_t)x_scale | (uintptr_t)expert_ids | (uintptr_t)expert_weights | (uintptr_t)w_gate_scale |
                      (uintptr_t)w_up_scale | (uintptr_t)w_down_scale) % 4 == 0,
                 "experts_ffn_fp8_block: codes and out must be 16-byte aligned, scales, ids and weights to their elements");
+  {
+    const int64_t hb = hidden / block8::kBlock, ib = intermediate / block8::kBlock, matrix = experts * hidden * intermediate;
+    const struct {
+      const void* at;
+      int64_t bytes;
+    } operands[] = {{x8, tokens * hidden}, {x_scale, tokens * hb * 4}, {expert_ids, tokens * top_k * 4}, {expert_weights, tokens * top_k * 4},
+                    {w_gate8, matrix}, {w_up8, matrix}, {w_down8, matrix}, {w_gate_scale, experts * hb * ib * 4}, {w_up_scale, experts * hb * ib * 4},
+                    {w_down_scale, experts * hb * ib * 4}};
+    for (const auto& o : operands)
+      PTO_CHECK_ARG(!block8::overlap(out, tokens * hidden * dtype_bytes(out_dtype), o.at, o.bytes), "experts_ffn_fp8_block: out overlaps an operand");
+  }
   const block8::Experts x{reinterpret_cast<const uint8_t*>(x8), x_scale, expert_ids, expert_weights, reinterpret_cast<const uint8_t*>(w_gate8),
                           reinterpret_cast<const uint8_t*>(w_up8), reinterpret_cast<const uint8_t*>(w_down8), w_gate_scale, w_up_scale,
                           w_down_scale, out, (int)hidden, (int)intermediate, (int)experts, (int)top_k};

@@ -159,7 +159,21 @@ int run(const char* what, bool norm, const void* x, const void* residual, const 
   PTO_CHECK_ARG(((uintptr_t)x | (uintptr_t)residual | (uintptr_t)gamma | (uintptr_t)sum_out | (uintptr_t)normed_out) % 16 == 0 &&
                     (uintptr_t)codes % 8 == 0 && (uintptr_t)scale % 4 == 0,
                 "%s: misaligned operand", what);
-  PTO_CHECK_ARG(!sum_out || sum_out != normed_out, "%s: sum_out and normed_out are the same tensor", what);
+  {
+    using block8::overlap;
+    const int64_t row_bytes = 2 * rows * cols, scale_bytes = rows * ((cols + kBlock - 1) / kBlock) * 4, gamma_bytes = cols * 4;
+    auto apart = [&](const void* o, int64_t bytes, bool in_place) {  // an output from the inputs; in_place: it may be one of the rows themselves
+      return !overlap(o, bytes, gamma, gamma_bytes) && ((in_place && o == x) || !overlap(o, bytes, x, row_bytes)) &&
+             ((in_place && o == residual) || !overlap(o, bytes, residual, row_bytes));
+    };
+    PTO_CHECK_ARG(apart(sum_out, row_bytes, true) && apart(normed_out, row_bytes, true) && apart(codes, rows * cols, false) &&
+                      apart(scale, scale_bytes, false),
+                  "%s: an output overlaps an input (sum_out and normed_out may be x or residual as a whole)", what);
+    PTO_CHECK_ARG(!overlap(sum_out, row_bytes, normed_out, row_bytes) && !overlap(codes, rows * cols, scale, scale_bytes) &&
+                      !overlap(codes, rows * cols, sum_out, row_bytes) && !overlap(codes, rows * cols, normed_out, row_bytes) &&
+                      !overlap(scale, scale_bytes, sum_out, row_bytes) && !overlap(scale, scale_bytes, normed_out, row_bytes),
+                  "%s: two outputs overlap", what);
+  }
   const bool stream = rows * cols * (1 + 2 * (sum_out != nullptr) + 2 * (normed_out != nullptr)) > kStreamBytes;
   auto go = [&](auto type, auto norm_c, auto stream_c) {
     auto from = [&](auto* p, int64_t bytes) { return p ? reinterpret_cast<decltype(p)>((uintptr_t)p + bytes) : nullptr; };

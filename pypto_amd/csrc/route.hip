@@ -18,6 +18,7 @@
 
 #include <algorithm>
 
+#include "block_fp8.h"
 #include "common.h"
 
 namespace {
@@ -400,6 +401,14 @@ extern "C" int pto_hip_route_experts(const void* logits, const float* bias, int3
   PTO_CHECK_ARG(((uintptr_t)bias | (uintptr_t)expert_ids | (uintptr_t)expert_weights) % 4 == 0 &&
                     (uintptr_t)logits % (size_t)dtype_bytes(logits_dtype) == 0,
                 "route_experts: misaligned operand");
+  {
+    using block8::overlap;
+    const int64_t chosen = tokens * top_k * 4, all = tokens * experts * dtype_bytes(logits_dtype);
+    PTO_CHECK_ARG(!overlap(expert_ids, chosen, expert_weights, chosen) && !overlap(expert_ids, chosen, logits, all) &&
+                      !overlap(expert_weights, chosen, logits, all) && !overlap(expert_ids, chosen, bias, experts * 4) &&
+                      !overlap(expert_weights, chosen, bias, experts * 4),
+                  "route_experts: the results overlap an operand or each other");
+  }
   int group_lanes = 64;
   while (group_lanes * n_groups > 64) group_lanes /= 2;
   Params p{logits, bias, expert_ids, expert_weights, (int)tokens, (int)experts, (int)top_k, (int)n_groups, (int)topk_groups,

@@ -747,3 +747,38 @@ def test_two_graphs_that_share_scratch(worker):
         torch.cuda.synchronize()
         assert all(torch.equal(out, w) for out, w in zip(outs, want)), order
     worker.sync()
+
+
+def test_results_over_operands_are_refused(worker):
+    raw = lambda n: torch.zeros(n, dtype=torch.uint8, device="cuda")
+    buf = raw(1 << 16)
+    part = lambda at, dtype, *shape: buf[at:at + torch.Size(shape).numel() * torch.empty(0, dtype=dtype).element_size()].view(dtype).view(shape)
+    # product: out from the last byte of the codes on, and over the scales
+    a, sa, w, sw = part(0, F8, 4, 256), part(2048, torch.float32, 4, 2), part(4096, F8, 16, 256), part(16384, torch.float32, 1, 2)
+    for at in (1008, 2064, 4096 + 4080, 16384):
+        with pytest.raises(ValueError, match="out overlaps an operand"):
+            worker.run(runtime.projection_fp8_block, a, sa, w, sw, part(at, torch.float32, 4, 16))
+    worker.run(runtime.projection_fp8_block, a, sa, w, sw, part(1024, torch.float32, 4, 16))  # right behind the codes
+    # router
+    logits, ids = part(0, torch.float32, 4, 8), part(1024, torch.int32, 4, 2)
+    with pytest.raises(ValueError, match="overlap"):
+        worker.run(runtime.route_experts, logits, ids, part(112, torch.float32, 4, 2), 1, 1, 0, 1, 1.0)
+    with pytest.raises(ValueError, match="overlap"):
+        worker.run(runtime.route_experts, logits, ids, part(1028, torch.float32, 4, 2), 1, 1, 0, 1, 1.0)
+    # norm: a shifted sum, codes over the rows, two outputs in one place
+    x, gamma, codes, scale = part(0, torch.bfloat16, 4, 128), part(2048, torch.float32, 128), part(4096, F8, 4, 128), part(8192, torch.float32, 4, 1)
+    other, free = part(16384, torch.bfloat16, 4, 128), part(20480, torch.bfloat16, 4, 128)
+    run = lambda *args: worker.run(runtime.add_rms_norm_fp8_block_normed, *args, 1e-6)
+    for args in ((x, other, gamma, part(256, torch.bfloat16, 4, 128), free, codes, scale), (x, other, gamma, free, other, part(512, F8, 4, 128), scale),
+                 (x, other, gamma, free, x, codes, part(2048, torch.float32, 4, 1))):
+        with pytest.raises(ValueError, match="overlaps an input"):
+            run(*args)
+    for args in ((x, other, gamma, free, free, codes, scale), (x, other, gamma, x, x, codes, scale), (x, other, gamma, free, x, codes, part(4608 - 16, torch.float32, 4, 1))):
+        with pytest.raises(ValueError, match="two outputs overlap"):
+            run(*args)
+    run(x, other, gamma, other, x, codes, scale)
+    # experts
+    args = _experts_case(1, 2, 128, 128, 2, 1)
+    with pytest.raises(ValueError, match="out overlaps an operand"):
+        worker.run(runtime.experts_ffn_fp8_block, *args, args[4].view(torch.uint8).flatten()[:512].view(torch.bfloat16).view(2, 128))
+    worker.sync()
