@@ -475,7 +475,7 @@ int run_experts(Experts x, int64_t tokens, hipStream_t st) {
   constexpr bool kExactUp = !std::is_same<OutT, __bf16>::value, kExactDown = std::is_same<OutT, float>::value;
   int height = (int)ctx().block_gemm_rows;
   const int64_t slots = tokens * x.top_k;
-  const bool direct = height == 0 ? experts_direct(slots, x.experts, x.hidden, x.inter) : height == 16;
+  const bool direct = height == 0 ? experts_direct(slots, x.experts, x.hidden, x.inter, kExactUp) : height == 16;
   if (direct && slots <= kMostDirectSlots && direct_smem(x) <= kDirectSmem) return run_direct<OutT>(x, tokens, st);
   const int64_t pass = std::min(tokens, std::max<int64_t>(1, kPassSlots / x.top_k));
   if (height < 64) height = choose_expert_rows(pass * x.top_k, x.experts, x.hidden, x.inter, kExactUp, kExactDown, ctx().num_cu);

@@ -400,14 +400,17 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
   return pick;
 }
 
-// Whether the experts' FFN of so many slots reads every slot's matrices for itself instead of planning tiles (experts.hip), by the
-// bytes that either form reads and what it starts with.  Measured, one token on, us direct / tiles: 8 of 64 experts of 4096 x
-// 1408 41 / 54, 73 / 70, 107 / 95; 4 of 60 of 2048 x 1024 16 / 32, 22 / 36, 30 / 37, 35 / 39, 51 / 42 at six; 8 of 128 of 1024 x 512 14 / 27 to 31
-// / 36 at eight, 46 / 43 at twelve; 2 of 8 of 5120 x 4096 42 / 73, 72 / 77, 100 / 81.
-inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) {
+// Whether the experts' FFN of so many slots reads every slot's matrices for itself instead of planning tiles (experts.hip): the stream of them,
+// against that of the used experts' and the chain of a tile's blocks, whichever is longer (as sides of a triangle; both forms start with 10 us).
+// Measured, us direct / tiles: 8 of 64 experts of 4096 x 1408, one token on, 32 / 49, 55 / 62, 77 / 84, 98 / 112; 4 of 60 of 2048 x 1024 13 / 32, 16 / 33,
+// at six 33 / 36, at eight 43 / 38; 8 of 128 of 1024 x 512 11 / 26, at twelve 29 / 38; 2 of 8 of 5120 x 4096 33 / 69, 51 / 72, 70 / 74, 90 / 82; 8 of
+// 256 of 7168 x 2048 67 / 78, 128 / 121.
+inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, bool exact) {
   const double mb = 3e-6 * (double)hidden * (double)inter;
-  const double unused = (double)experts * std::pow(1.0 - 1.0 / (double)experts, (double)slots);
-  return 5.0 + (double)slots * mb / 4.0 < 26.0 + ((double)experts - unused) * mb / 5.2;
+  const double used = (double)experts * (1.0 - std::pow(1.0 - 1.0 / (double)experts, (double)slots));
+  const BlockTileCost &up = kBlockTiles[exact][2], &down = kBlockTiles[0][2];
+  const double chain = (double)(hidden / 128) * up.block + up.start + (double)(inter / 128) * down.block + down.start, stream = used * mb / 5.3;
+  return (double)slots * mb / 6.3 < std::sqrt(chain * chain + stream * stream);
 }
 
 // The highest tiles of both products of the experts' FFN; what an expert has left goes to lower ones (experts.hip).  The least sum over

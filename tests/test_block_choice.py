@@ -18,7 +18,7 @@ extern "C" void tile(int64_t m, int64_t n, int64_t kb, int exact, int rows, int 
   for (int i = 0; i < 3; ++i) out[3 + i] = t.tiles[i];
 }
 extern "C" double span(int64_t a, int64_t b, int64_t c, double x, double y, double z, int64_t cus) { return pto_hip::makespan({a, b, c}, {x, y, z}, cus); }
-extern "C" int direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) { return pto_hip::experts_direct(slots, experts, hidden, inter); }
+extern "C" int direct(int64_t slots, int64_t experts, int64_t hidden, int64_t inter) { return pto_hip::experts_direct(slots, experts, hidden, inter, false); }
 extern "C" int rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, int up, int down) {
   return pto_hip::choose_expert_rows(slots, experts, hidden, inter, up != 0, down != 0, 256);
 }
@@ -124,7 +124,7 @@ def test_measured_sides(choice):
     rows, cols, per = _tile(choice, 64, 4096, 86)
     assert rows == 64 and per
     assert _tile(choice, 4096, 14336, 32)[0] == 256 and _tile(choice, 4096, 14336, 32, exact=True)[0] == 128
-    assert choice.direct(8, 64, 4096, 1408) and not choice.direct(32, 64, 4096, 1408)
+    assert choice.direct(8, 64, 4096, 1408) and choice.direct(24, 64, 4096, 1408) and not choice.direct(64, 64, 4096, 1408)
     assert choice.direct(64, 128, 1024, 512) and not choice.direct(128, 128, 1024, 512)
     assert choice.rows(320, 64, 4096, 1408, 0, 0) == 64 and choice.rows(32768, 64, 4096, 1408, 0, 0) == 256
     assert choice.rows(32768, 64, 4096, 1408, 1, 0) == 128
