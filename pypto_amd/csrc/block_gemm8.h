@@ -66,9 +66,10 @@ __device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcp
 
 template <typename T>
 __device__ __forceinline__ void store_upto4(T* dst, const f32x4& v, int count) {
-  if (count >= 4 && ((uintptr_t)dst & (4 * sizeof(T) - 1)) == 0) {
+  if (count >= 4) {
     typedef __attribute__((__vector_size__(4 * sizeof(T)))) T vec4;
-    *reinterpret_cast<vec4*>(dst) = vec4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    const vec4 all = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    __builtin_memcpy(dst, &all, sizeof(all));  // one store, at any element
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)

@@ -18,9 +18,13 @@ __global__ __launch_bounds__(256) void sum_ranges_kernel(const float* __restrict
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   for (int r = 0; r < ranges; ++r) {
     const float* src = slabs + r * count + at;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < here) sum[e] += src[e];
+    if (here == 4) {
+      f32x4 v;
+      __builtin_memcpy(&v, src, sizeof(v));
+      sum += v;
+    } else {
+      for (int e = 0; e < here; ++e) sum[e] += src[e];
+    }
   }
   store_upto4(out + at, sum, here);
 }

@@ -453,7 +453,6 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
     }
     OutT* const c = reinterpret_cast<OutT*>(p.c) + (size_t)range * p.m * p.n + n0;
     const int cols = min(BN, p.n - n0);
-    const bool whole = p.n % (16 / (int)sizeof(OutT)) == 0 && (uintptr_t)p.c % 16 == 0 && ((size_t)range * p.m * p.n * sizeof(OutT)) % 16 == 0;
 #pragma unroll
     for (int h = 0; h < S::PH; ++h) {
       if (kg == 0) {
@@ -475,17 +474,15 @@ __device__ __forceinline__ void work_tile(const Params& p, int at, int tn, int r
       }
       __syncthreads();
       const int rows = min(ROWS, tile.rows - h * ROWS);
-      if (whole) {
-        constexpr int VEC = 16 / (int)sizeof(OutT), PER_ROW = BN / VEC;
-        for (int u = tid; u < rows * PER_ROW; u += 512) {
-          const int row = u / PER_ROW, at = u % PER_ROW;
-          if (at * VEC < cols)
-            *reinterpret_cast<i32x4*>(c + c_row(h * ROWS + row) * p.n + at * VEC) = *reinterpret_cast<const i32x4*>(smem + row * PITCH + at * 16);
-        }
-      } else {
-        for (int u = tid; u < rows * BN; u += 512) {
-          const int row = u / BN, at = u % BN;
-          if (at < cols) c[c_row(h * ROWS + row) * p.n + at] = reinterpret_cast<const OutT*>(smem + row * PITCH)[at];
+      constexpr int VEC = 16 / (int)sizeof(OutT), PER_ROW = BN / VEC;
+      for (int u = tid; u < rows * PER_ROW; u += 512) {
+        const int row = u / PER_ROW, at = u % PER_ROW * VEC;
+        OutT* const dst = c + c_row(h * ROWS + row) * p.n + at;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(smem + row * PITCH + at * (int)sizeof(OutT));
+        if (at + VEC <= cols) {
+          __builtin_memcpy(dst, &v, 16);  // (rows may start at any element)
+        } else {
+          for (int i = 0; at + i < cols; ++i) dst[i] = reinterpret_cast<const OutT*>(smem + row * PITCH)[at + i];
         }
       }
       if (h + 1 < S::PH) __syncthreads();
