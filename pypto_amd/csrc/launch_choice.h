@@ -414,10 +414,10 @@ inline bool experts_direct(int64_t slots, int64_t experts, int64_t hidden, int64
 }
 
 // The highest tiles of both products of the experts' FFN; what an expert has left goes to lower ones (experts.hip).  The least sum over
-// the two products of their tiles' costs, spread over the CUs but never below one tile's, with experts of 0.2 to 2.3 times the mean rows, as
-// routers leave them.  Over 88 timings of five layers at 16 to 4096 tokens the pick is 0.6 % from the best height in the mean and 21 % at
-// worst.  8 of 64 experts of 4096 x 1408, 64 / 128 / 256 rows, us: 128 tokens 261 / 262 / 262, 512 320 / 309 / 296, 1024 413 / 417 / 362, 4096
-// 1163 / 993 / 872; with one height for all of an expert's tiles 512 tokens took 304 / 288 / 331, 4096 1279 / 1036 / 946.
+// the two products of what takes longest: their tiles' costs spread over the CUs, one tile's, the weights that the tiles read, and three quarters of
+// the rounds that the expected tiles make; with experts of 0.2 to 2.3 times the mean rows, as routers leave them.  Over 88 timings of five layers at 16 to 4096 tokens the pick is 0.04 % from the best height in
+// the mean and 1.5 % at worst.  8 of 64 experts of 4096 x 1408, 64 / 128 / 256 rows, us: 128 tokens 261 / 262 / 262, 512 320 / 309 / 296, 1024 413 / 417 /
+// 362, 4096 1163 / 993 / 872; with one height for all of an expert's tiles 512 tokens took 304 / 288 / 331, 4096 1279 / 1036 / 946.
 inline int choose_expert_rows(int64_t slots, int64_t experts, int64_t hidden, int64_t inter, bool exact_up, bool exact_down, int64_t num_cu) {
   const double used = (double)experts * (1.0 - std::pow(1.0 - 1.0 / (double)experts, (double)slots)), each = (double)slots / used;
   // us of a tile of the height kBlockTiles[][i]
@@ -433,16 +433,22 @@ inline int choose_expert_rows(int64_t slots, int64_t experts, int64_t hidden, in
     for (int pass = 0; pass < 2; ++pass) {
       const bool exact = pass ? exact_down : exact_up;
       const int64_t kb = (pass ? inter : hidden) / 128, tiles_n = pass ? (hidden + 255) / 256 : inter / 128;
-      double work = 0.0, longest = 0.0;
+      double work = 0.0, longest = 0.0, tiles[3] = {0.0, 0.0, 0.0}, each_us[3] = {0.0, 0.0, 0.0};  // of the height, half and a quarter of it
+      for (int c = 0; c < 3 && i - c >= 2; ++c) each_us[c] = cost(exact, i - c, kb);
       for (const double share : {0.2, 0.5, 0.8, 1.2, 2.3}) {
         const double rows = std::max(1.0, each * share), full = std::floor(rows / height), rest = rows - full * height;
-        int low = 2;  // the least height that holds the rest
-        while (kBlockTiles[0][low].rows < rest) ++low;
-        const double high_us = full > 0.0 ? cost(exact, i, kb) : 0.0, low_us = rest > 0.0 ? cost(exact, low, kb) : 0.0;
-        work += (full * high_us + low_us) / 5.0;
-        longest = std::max(longest, std::max(high_us, low_us));
+        tiles[0] += full / 5.0;
+        if (rest > 0.0) tiles[height >= 256 && rest <= height / 4 ? 2 : height >= 128 && rest <= height / 2 ? 1 : 0] += 0.2;
       }
-      us += std::max(longest, used * (double)tiles_n * work / (double)num_cu);
+      int64_t jobs[3];
+      for (int c = 0; c < 3; ++c) {
+        const double all = used * (double)tiles_n * tiles[c];
+        jobs[c] = (int64_t)std::ceil(all);
+        work += all * each_us[c];
+        if (tiles[c] > 0.0) longest = std::max(longest, each_us[c]);
+      }
+      const double memory = used * (double)tiles_n * (tiles[0] + tiles[1] + tiles[2]) * 256.0 * 128e-6 * (double)kb / 5.3;  // every tile reads its weights
+      us += std::max({longest, work / (double)num_cu, memory, 0.75 * makespan(jobs, each_us, num_cu)});
     }
     if (us < best) {
       best = us;
