@@ -368,8 +368,9 @@ PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* sca
  * (PTO_HIP_ERR_INVALID_VALUE). */
 
 /* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
- * codes = e4m3(n / scale), round to nearest even; sum_out = x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every
- * output is rounded once (a row whose sum of squares passes fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out
+ * codes = e4m3(n / scale), round to nearest even, decided on 64 bits where 32 might pass a border between two codes; sum_out =
+ * x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every output is rounded once (a row whose sum of squares passes
+ * fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out
  * may each be NULL; sum_out and normed_out may be x or residual themselves.  NaN elements are left out of amax and give NaN codes.
  * cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the last group may be shorter).
  * quantize_fp8_block: codes and scales of x itself. */

@@ -3,7 +3,10 @@
 //   s = x + residual      n = s * rsqrt(mean s^2 + eps) * gamma      scale = amax_group |n| / 448      codes = e4m3(n / scale)
 //
 // and, where asked for, s (the next residual) and n in the 16-bit type of x.  s and n stay in 32 bits from the loads to the
-// outputs, so that each output is rounded once: the codes are those of n itself, not of its 16-bit copy.
+// outputs, so that each output is rounded once: the codes are those of n itself, not of its 16-bit copy.  n / scale is 448 t / max t with
+// t = s gamma: the row's statistic cancels, and the quotient's 32-bit roundings (2^-22) matter only next to a border between two codes.
+// There, 13 values in a million, the group is done again in 64 bits: the codes are the exact rows' (a plain evaluation in 32 bits has one in a
+// million wrong).
 // Without the norm the same kernel is the quantiser of activations that come from elsewhere.
 //
 // Bound by memory: 2 bytes an element for x and for each of residual, sum and normed, 1 for the codes.  One workgroup holds a row in
@@ -12,6 +15,7 @@
 // is still to be read; smaller ones stay there for who reads them next.  All outputs of bf16 rows, us without / with it, and with a
 // product of the codes behind: 4096 x 8192 63.3 / 54.3 (302 MB: 5.6 TB/s) and 113.5 / 108.5, 2048 x 5120 25.8 / 16.8 and 45.0 / 39.5, 8192 x
 // 2048 31.6 / 25.7 and 44.2 / 38.5; but 1024 x 4096 9.3 / 8.2 and 20.9 / 22.4, 512 x 4096 8.3 / 7.6 and 18.8 / 20.7.
+// With the weights asked for ahead of the row's statistic 4096 x 8192 takes 50 us in a loop of its own (6.1 TB/s), 4096 x 16384 95.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -36,6 +40,25 @@ template <bool STREAM, typename V>
 __device__ __forceinline__ void store(V* to, const V& v) {
   if constexpr (STREAM) __builtin_nontemporal_store(v, to);
   else *to = v;
+}
+
+// The quotients s g inv / scale of a group in 64 bits, rounded to 32 so that they stay on their side of every border between two codes (to
+// zero, the last bit set where anything is lost).  top: the group's largest |n|; all lanes of the group take part.
+__device__ __forceinline__ void exact_quotients(const float (&s)[8], const float (&g)[8], float inv, float top, float scale, float (&q)[8]) {
+  double amax = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs((double)s[e] * (double)g[e]));
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
+  // (no scale but 1 for a row normalised to zeros, none below the smallest normal number)
+  const bool least = top < 448.f * 0x1p-126f;
+  const double factor = !(top > 0.f) ? 0.0 : (least ? (double)inv : 448.0) / (least ? (double)scale : amax);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double v = (double)s[e] * (double)g[e] * factor;
+    const float f = __double2float_rz(v);
+    q[e] = (double)f == v || !(v == v) ? f : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) | 1u);
+  }
 }
 
 // sum_out and normed_out may be x or residual themselves: a thread writes the columns that it alone has read.
@@ -80,7 +103,18 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
       if (i < nvec) store<STREAM>(out + i, v);
     }
   }
+  float inv = 1.f, g[VECS][8];  // NORM: the columns' weights
   if constexpr (NORM) {
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+      const int i = threadIdx.x + u * kThreads;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[u][e] = 1.f;
+      if (gamma && i < nvec) {
+        *reinterpret_cast<float4*>(&g[u][0]) = reinterpret_cast<const float4*>(gamma)[2 * i];
+        *reinterpret_cast<float4*>(&g[u][4]) = reinterpret_cast<const float4*>(gamma)[2 * i + 1];
+      }
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
@@ -88,25 +122,7 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
     float tot = red[0];
 #pragma unroll
     for (int w = 1; w < kThreads / 64; ++w) tot += red[w];
-    const float inv = rsqrtf(tot / (float)cols + eps);
-#pragma unroll
-    for (int u = 0; u < VECS; ++u) {
-      const int i = threadIdx.x + u * kThreads;
-      if (i < nvec) {
-        float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-        if (gamma) {
-          *reinterpret_cast<float4*>(&g[0]) = reinterpret_cast<const float4*>(gamma)[2 * i];
-          *reinterpret_cast<float4*>(&g[4]) = reinterpret_cast<const float4*>(gamma)[2 * i + 1];
-        }
-        vec8 v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          s[u][e] = s[u][e] * inv * g[e];
-          v[e] = (T)s[u][e];
-        }
-        if (normed_out) store<STREAM>(reinterpret_cast<vec8*>(normed_out + row * cols) + i, v);
-      }
-    }
+    inv = rsqrtf(tot / (float)cols + eps);
   }
   typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
   u32x2* crow = reinterpret_cast<u32x2*>(codes + row * cols);
@@ -114,15 +130,39 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
     const int i = threadIdx.x + u * kThreads;
-    float amax = 0.f;
+    float t[8], q[8], amax = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(s[u][e]));
+    for (int e = 0; e < 8; ++e) {
+      t[e] = NORM ? s[u][e] * g[u][e] : s[u][e];
+      amax = fmaxf(amax, fabsf(t[e]));
+    }
+    if (NORM && normed_out) {
+      vec8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = (T)(t[e] * inv);
+      if (i < nvec) store<STREAM>(reinterpret_cast<vec8*>(normed_out + row * cols) + i, v);
+    }
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-    const float sc = group_scale(amax);
-    const GroupQuotient q(sc);
+    const float top = NORM ? amax * inv : amax, sc = group_scale(top);
+    if constexpr (NORM) {
+      // n / scale is 448 t / max t: the row's statistic cancels
+      const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : 0.f;
+      bool exact = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f && top >= 448.f * 0x1p-126f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        q[e] = t[e] * r;
+        // within 6 steps of the 24-bit format of a border between two codes: the roundings so far, 2^-22 together, are up to 4
+        exact |= ((__builtin_bit_cast(uint32_t, q[e]) & 0xfffffu) - (0x80000u - 6u)) <= 12u;
+      }
+      if (__builtin_expect(__ballot(exact) != 0, 0)) exact_quotients(s[u], g[u], inv, top, sc, q);
+    } else {
+      const GroupQuotient quotient(sc);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = quotient(t[e]);
+    }
     if (i < nvec) {
-      store<STREAM>(crow + i, u32x2{codes4(q(s[u][0]), q(s[u][1]), q(s[u][2]), q(s[u][3])), codes4(q(s[u][4]), q(s[u][5]), q(s[u][6]), q(s[u][7]))});
+      store<STREAM>(crow + i, u32x2{codes4(q[0], q[1], q[2], q[3]), codes4(q[4], q[5], q[6], q[7])});
       if (i % 16 == 0) srow[i / 16] = sc;
     }
   }

@@ -782,3 +782,28 @@ def test_results_over_operands_are_refused(worker):
     with pytest.raises(ValueError, match="out overlaps an operand"):
         worker.run(runtime.experts_ffn_fp8_block, *args, args[4].view(torch.uint8).flatten()[:512].view(torch.bfloat16).view(2, 128))
     worker.sync()
+
+
+@pytest.mark.parametrize("rows,cols", [(700, 4096), (300, 8200), (900, 752), (64, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_codes_are_those_of_the_exact_rows(worker, rows, cols, dtype):
+    """n / scale is decided on 64 bits wherever 32 might pass a border between two codes: every code that is not subnormal is the exact one."""
+    g = _gen(rows + cols)
+    x = _randn(g, rows, cols) * torch.where(torch.rand(cols, device="cuda", generator=g) < 0.02, 20.0, 1.0)
+    big, small = (1e15, 1e-36) if dtype == torch.bfloat16 else (100.0, 1e-5)
+    x[0:3] *= big
+    x[3:6] *= small
+    if dtype == torch.bfloat16:
+        x[6:9] *= 1e-39
+    x = x.to(dtype)
+    gamma = 1 + 0.3 * _randn(g, cols)
+    gamma[5], gamma[7] = 0.0, -2.0
+    codes, scale = torch.empty((rows, cols), dtype=F8, device="cuda"), torch.empty((rows, -(-cols // 128)), device="cuda")
+    worker.run(runtime.rms_norm_fp8_block, x, gamma, codes, scale, 1e-6)
+    worker.sync()
+    n = ob.rms_norm(x, None, gamma, 1e-6)[1]
+    want, exact_scale = ob.quantize_rows(n)
+    ratio = n / exact_scale.repeat_interleave(128, -1)[:, :cols]
+    regular = (ratio.abs() >= 2.0 ** -6) & (exact_scale.repeat_interleave(128, -1)[:, :cols] > 2.0 ** -125)
+    assert torch.equal(codes.double()[regular], want[regular])
+    _check_codes(codes, scale, n, 2.0 ** -17)
