@@ -52,7 +52,7 @@ __device__ __forceinline__ void exact_quotients(const float (&s)[8], const float
   for (int off = 8; off > 0; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
   // (no scale but 1 for a row normalised to zeros, none below the smallest normal number)
   const bool least = top < 448.f * 0x1p-126f;
-  const double factor = !(top > 0.f) ? 0.0 : (least ? (double)inv : 448.0) / (least ? (double)scale : amax);
+  const double factor = !(top > 0.f) ? (double)inv * 0.0 : (least ? (double)inv : 448.0) / (least ? (double)scale : amax);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const double v = (double)s[e] * (double)g[e] * factor;
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
     const float top = NORM ? amax * inv : amax, sc = group_scale(top);
     if constexpr (NORM) {
       // n / scale is 448 t / max t: the row's statistic cancels
-      const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : 0.f;
+      const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : inv * 0.f;  // (a statistic that is not finite: NaN)
       bool exact = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f && top >= 448.f * 0x1p-126f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

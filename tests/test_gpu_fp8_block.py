@@ -807,3 +807,53 @@ def test_norm_codes_are_those_of_the_exact_rows(worker, rows, cols, dtype):
     regular = (ratio.abs() >= 2.0 ** -6) & (exact_scale.repeat_interleave(128, -1)[:, :cols] > 2.0 ** -125)
     assert torch.equal(codes.double()[regular], want[regular])
     _check_codes(codes, scale, n, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("cols", [128, 1000, 4104])
+def test_norm_of_rows_that_are_not_finite(worker, cols):
+    """A NaN makes its row NaN; an infinity leaves a NaN of itself and zeros; neither reaches another row, and every scale is 1."""
+    inf, nan = float("inf"), float("nan")
+    x = _randn(_gen(cols), 6, cols).bfloat16()
+    clean = x.clone()
+    x[1, 3], x[2, cols - 1], x[3, 0], x[4, 5], x[4, 6] = nan, inf, -inf, inf, nan
+    gamma = 1 + 0.1 * _randn(_gen(1), cols)
+
+    def call(x):
+        outs = [torch.empty((6, cols), dtype=torch.bfloat16, device="cuda"), torch.empty((6, cols), dtype=F8, device="cuda"), torch.empty((6, -(-cols // 128)), device="cuda")]
+        worker.run(runtime.rms_norm_fp8_block_normed, x, gamma, *outs, 1e-6)
+        worker.sync()
+        return outs[0].float(), outs[1].float(), outs[2]
+
+    normed, codes, scale = call(x)
+    want = call(clean)
+    for got, w in zip((normed, codes, scale), want):
+        assert torch.equal(got[[0, 5]], w[[0, 5]])
+    assert (scale[1:5] == 1).all()
+    for values in (normed, codes):
+        assert values[1].isnan().all() and values[4].isnan().all()
+        for row, at in ((2, cols - 1), (3, 0)):
+            rest = torch.arange(cols, device="cuda") != at
+            assert values[row, at].isnan() and (values[row, rest] == 0).all()
+    # no eps, no values: 0 / 0
+    zeros = torch.zeros((6, cols), dtype=torch.bfloat16, device="cuda")
+    out, codes, scale = torch.empty_like(zeros), torch.empty((6, cols), dtype=F8, device="cuda"), torch.empty((6, -(-cols // 128)), device="cuda")
+    worker.run(runtime.rms_norm_fp8_block_normed, zeros, gamma, out, codes, scale, 0.0)
+    worker.sync()
+    assert out.isnan().all() and codes.float().isnan().all() and (scale == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_infinite_results_of_an_expert_stay_in_their_channels(worker, rows, dtype):
+    """One block of an expert's down scales is infinite: 128 channels of its tokens are lost, everything else keeps its bits."""
+    args = _experts_case(12, 90, 384, 256, 6, 2)
+    want = _check_experts(worker, args, dtype)
+    args[9][3, 1, 0] = float("inf")  # expert 3, channels 128 to 255
+    out = torch.empty_like(want)
+    worker.run(runtime.experts_ffn_fp8_block, *args, out)
+    worker.sync()
+    hit = (args[2] == 3).any(-1)
+    assert hit.any() and not hit.all()
+    assert not out[hit, 128:256].isfinite().any()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[hit, 128:256] = False
+    assert torch.equal(out[keep], want[keep])
