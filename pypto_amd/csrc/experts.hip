@@ -27,6 +27,7 @@ namespace block8 {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kPlanThreads = 1024;
+constexpr int kFewSlots = 1024, kFewThreads = 256;  // a plan of few slots and experts: 192 slots of 16 experts 2.8 us for 3.6, 1024 of 250 3.4 for 4.6
 // Tokens are worked through in passes of so many slots, so that the scratch stays below a gigabyte or two and every index inside 32 bits.
 constexpr int64_t kPassSlots = 32768;
 constexpr int64_t kMostDirectSlots = 1024;
@@ -37,21 +38,21 @@ constexpr int64_t kMostDirectSlots = 1024;
 // itself ([wavefronts][experts] in LDS), so that the counters of a busy expert are shared by 64 lanes and not by all, and a slot's rank in its
 // wavefront's count is its place.  The sorted slots are put together in LDS: written one by one, each to a line of its own, they took 5 us
 // more.  The order of the ranks is that of the atomics: which row of which tile a slot becomes changes no bit of its result.
-// Bound by the LDS atomics: 160 slots 4.7 us, 4096 6, 16384 12, 32768 16.
-template <int EACH>
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __restrict__ ids, int slots, int experts, int height,
+// Bound by the LDS atomics: 192 slots 2.8 us (4.8 behind a stream that has emptied the caches), 4096 6, 16384 12, 32768 16.
+template <int EACH, int THREADS>
+__global__ __launch_bounds__(THREADS) void plan_kernel(const int32_t* __restrict__ ids, int slots, int experts, int height,
                                                             int32_t* __restrict__ order, int4* __restrict__ tiles, int* __restrict__ n_tiles,
                                                             int* __restrict__ flag) {
-  constexpr int kWaves = kPlanThreads / 64;
+  constexpr int kWaves = THREADS / 64;
   extern __shared__ int count[];  // [kWaves][experts], then the slots by expert
   uint16_t* const sorted = reinterpret_cast<uint16_t*>(count + kWaves * experts);
   __shared__ int sums[2][kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int i = tid; i < kWaves * experts; i += kPlanThreads) count[i] = 0;
+  for (int i = tid; i < kWaves * experts; i += THREADS) count[i] = 0;
   int place[EACH];  // the slot's expert, then with its rank behind the experts' bits; -1: none
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
-    const int s = i * kPlanThreads + tid;
+    const int s = i * THREADS + tid;
     const int id = ids[(uint32_t)min(s, slots - 1)];
     place[i] = s < slots ? id : -1;
   }
@@ -117,12 +118,12 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const int32_t* __res
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
     if (place[i] >= 0)
-      sorted[count[wave * experts + (unsigned)place[i] % kMaxExperts] + (unsigned)place[i] / kMaxExperts] = (uint16_t)(i * kPlanThreads + tid);
+      sorted[count[wave * experts + (unsigned)place[i] % kMaxExperts] + (unsigned)place[i] / kMaxExperts] = (uint16_t)(i * THREADS + tid);
   __syncthreads();
-  for (int i = tid; i < (all[0] & 0xffff); i += kPlanThreads) order[i] = sorted[i];
+  for (int i = tid; i < (all[0] & 0xffff); i += THREADS) order[i] = sorted[i];
 }
 
-size_t plan_smem(int64_t slots, int experts) { return (size_t)(kPlanThreads / 64) * experts * sizeof(int) + (size_t)slots * sizeof(uint16_t); }
+size_t plan_smem(int64_t slots, int experts, int threads) { return (size_t)(threads / 64) * experts * sizeof(int) + (size_t)slots * sizeof(uint16_t); }
 
 // out[t] = sum over j of weights[t, j] * y[t * top_k + j], the slots without an expert left out.  Y _Float16: times the row's power
 // of two of each 128 channels.  One workgroup per token and 2048 channels, eight a thread.  Bound by memory: 16384 rows of 4096 in fp16 30 us (140 MB
@@ -413,14 +414,14 @@ int run_pass(const Experts& x, int64_t tokens, const Scratch& s, int height, cha
   int4* tiles = reinterpret_cast<int4*>(ws + s.tiles);
   int* n_tiles = reinterpret_cast<int*>(ws + s.n_tiles);
   const int slots = (int)(tokens * x.top_k);
-  auto plan = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(1), dim3(kPlanThreads), plan_smem(slots, x.experts), st, x.ids, slots, x.experts, height, order, tiles, n_tiles,
+  auto plan = [&](auto kern, int threads) {
+    hipLaunchKernelGGL(kern, dim3(1), dim3(threads), plan_smem(slots, x.experts, threads), st, x.ids, slots, x.experts, height, order, tiles, n_tiles,
                        ctx().flags + 3);
   };
-  if (slots <= kPlanThreads) plan(plan_kernel<1>);
-  else if (slots <= 8 * kPlanThreads) plan(plan_kernel<8>);
-  else if (slots <= 16 * kPlanThreads) plan(plan_kernel<16>);
-  else plan(plan_kernel<kPassSlots / kPlanThreads>);
+  if (slots <= kFewSlots && x.experts <= kFewThreads) plan(plan_kernel<kFewSlots / kFewThreads, kFewThreads>, kFewThreads);
+  else if (slots <= 8 * kPlanThreads) plan(plan_kernel<8, kPlanThreads>, kPlanThreads);
+  else if (slots <= 16 * kPlanThreads) plan(plan_kernel<16, kPlanThreads>, kPlanThreads);
+  else plan(plan_kernel<kPassSlots / kPlanThreads, kPlanThreads>, kPlanThreads);
   Params p{};
   p.tiles = tiles;
   p.n_tiles = n_tiles;
@@ -467,9 +468,9 @@ template <typename OutT>
 int run_experts(Experts x, int64_t tokens, hipStream_t st) {
   static std::atomic<bool> attr_set{false};  // callers hold the dispatch lock
   if (!attr_set.load(std::memory_order_acquire)) {
-    for (const void* kern : {reinterpret_cast<const void*>(plan_kernel<1>), reinterpret_cast<const void*>(plan_kernel<8>),
-                             reinterpret_cast<const void*>(plan_kernel<16>), reinterpret_cast<const void*>(plan_kernel<kPassSlots / kPlanThreads>)})
-      PTO_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kPassSlots, kMaxExperts)));
+    for (const void* kern : {reinterpret_cast<const void*>(plan_kernel<8, kPlanThreads>), reinterpret_cast<const void*>(plan_kernel<16, kPlanThreads>),
+                             reinterpret_cast<const void*>(plan_kernel<kPassSlots / kPlanThreads, kPlanThreads>)})
+      PTO_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kPassSlots, kMaxExperts, kPlanThreads)));
     attr_set.store(true, std::memory_order_release);
   }
   constexpr bool kExactUp = !std::is_same<OutT, __bf16>::value, kExactDown = std::is_same<OutT, float>::value;

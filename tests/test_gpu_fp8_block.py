@@ -857,3 +857,9 @@ def test_infinite_results_of_an_expert_stay_in_their_channels(worker, rows, dtyp
     keep = torch.ones_like(out, dtype=torch.bool)
     keep[hit, 128:256] = False
     assert torch.equal(out[keep], want[keep])
+
+
+@pytest.mark.parametrize("rows", [64, 256], indirect=True)
+@pytest.mark.parametrize("tokens,experts", [(128, 256), (128, 257), (129, 256), (1, 256), (1025, 40), (2050, 1000)])
+def test_experts_at_the_borders_of_the_plan_s_forms(worker, rows, tokens, experts):
+    _check_experts(worker, _experts_case(tokens + experts, tokens, 128, 128, experts, 8), torch.bfloat16)
