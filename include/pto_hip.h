@@ -671,11 +671,11 @@ PTO_HIP_API int pto_hip_backend_handler_query(const char* hook, int32_t arg, cha
  *                               input RMSNorm, 2 = SwiGLU of the pair in front, 4 = the merge of the attention
  *                               partials (a sum of these; default 7, 0 = never)
  *  "skinny_fused"               read only: which of these the last decoder layer or FFN block (pto_hip_ffn_swiglu) took
- *  "block_gemm_rows"            tile height of the products of block-scaled e4m3 operands (pto_hip_projection_fp8_block and both
+ *  "block_gemm_rows"            highest tiles of the products of block-scaled e4m3 operands (pto_hip_projection_fp8_block and both
  *                               products of pto_hip_experts_ffn_fp8_block): 0 = by estimate (default); 16 = operands straight to
  *                               registers (experts: every slot for itself, up to 1024 of them); 64, 128, 256 = tiles through LDS
- *                               (256 only where the codes are multiplied as they are, 128 otherwise).  "gemm_splits" gives
- *                               the ranges of k of the projection's tiles
+ *                               (256 only where the codes are multiplied as they are, 128 otherwise), the rows that are left in lower
+ *                               ones.  "gemm_splits" gives the ranges of k of the projection's tiles
  *  "block_gemm_cols"            channels of the projection's tiles of 64 rows: 0 = by estimate (default), 64, 128, 256
  *  "w8a16_gemm_rows"            rows from which the int8 projections run as one tiled GEMM (codes
  *                               widened inside the kernel, weights read once) instead of 32-row
