@@ -365,7 +365,8 @@ PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* sca
  * Activations: codes [rows, cols] with one fp32 scale per 128 columns of a row, [rows, ceil(cols / 128)].  Weights: codes one row per
  * OUTPUT channel with k contiguous, [n, k], with one fp32 scale per block of 128 x 128, [ceil(n / 128), k / 128].  A value is its
  * code times its scale; scales may be any fp32 values.  Results lie apart from the operands and from each other, unless said otherwise
- * (PTO_HIP_ERR_INVALID_VALUE). */
+ * (PTO_HIP_ERR_INVALID_VALUE).  The experts' FFN, and a product whose k is cut into ranges, use the library's scratch: like all calls
+ * that do, they are ordered on one stream, or synchronised, and a size is called once eagerly before it is captured. */
 
 /* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
  * codes = e4m3(n / scale), round to nearest even, decided on 64 bits where 32 might pass a border between two codes; sum_out =
