@@ -122,8 +122,9 @@ __device__ __forceinline__ int best_lane(uint64_t key, int expert, uint64_t* top
 
 // How far apart two 32-bit keys have to be for their order to be the 64-bit keys'.  A sigmoid's exponential is off by (|v| + 2) 2^-24 of itself,
 // which moves the score by at most 2^-23, as do sum and quotient: 2^-21 together with room.  A softmax's sum of up to 16 + 6 steps is off by
-// 2^-19 of itself.  The sum with the bias adds 2^-24 of its size.  Both keys are off; a group's key is the sum of two.
-__device__ __forceinline__ float margin(float key, bool sigmoid) { return (sigmoid ? 0x1p-20f : 0x1p-17f) + 0x1p-21f * fabsf(key); }
+// 2^-19 of itself.  The sum with the bias adds 2^-24 of its size.  Both keys are off.  A group's key is the sum of two, off by as much as both:
+// size is that of the keys' roundings, |best| + |second|, whatever is left of them in the sum; this is then how far the one group's key may be off.
+__device__ __forceinline__ float margin(float size, bool sigmoid) { return (sigmoid ? 0x1p-20f : 0x1p-17f) + 0x1p-21f * fabsf(size); }
 
 template <typename V>
 struct KeyOf {
@@ -212,12 +213,12 @@ __device__ __forceinline__ bool choose(const Params& p, const float (&logit)[J],
     bool stays;
     if constexpr (kNear) {
       // how many of the others are surely better, and how many may be; one between the two can change sides
-      const float here = fminf(fmaxf(worth, -3e38f), 3e38f), reach = 2.f * margin(here, p.sigmoid);
+      const float size = fminf(p.group_size > 1 ? fabsf(best) + fabsf(second) : fabsf(best), 3e38f), off = margin(size, p.sigmoid);
+      const float here = fminf(fmaxf(worth, -3e38f), 3e38f), least = here - off, most = here + off;
       int surely = 0, maybe = -1;  // (itself)
       for (int o = 0; o < p.groups; ++o) {
-        const float other = of_lane(here, o * p.group_lanes);
-        surely += other > here + reach;
-        maybe += other >= here - reach;
+        surely += of_lane(least, o * p.group_lanes) > most;
+        maybe += of_lane(most, o * p.group_lanes) >= least;
       }
       stays = g < p.groups && maybe < p.kept;
       if (__ballot(g < p.groups && !stays && surely < p.kept)) near = true;

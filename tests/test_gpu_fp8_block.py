@@ -863,3 +863,23 @@ def test_infinite_results_of_an_expert_stay_in_their_channels(worker, rows, dtyp
 @pytest.mark.parametrize("tokens,experts", [(128, 256), (128, 257), (129, 256), (1, 256), (1025, 40), (2050, 1000)])
 def test_experts_at_the_borders_of_the_plan_s_forms(worker, rows, tokens, experts):
     _check_experts(worker, _experts_case(tokens + experts, tokens, 128, 128, experts, 8), torch.bfloat16)
+
+
+@pytest.mark.parametrize("sigmoid,big", [(True, 32.0), (True, 64.0), (True, 1024.0), (False, 1024.0), (True, 1e6), (False, 1e6)])
+@pytest.mark.parametrize("size", [2, 4, 32])
+def test_router_on_groups_whose_two_best_keys_cancel(worker, sigmoid, big, size):
+    """A group's best key is biased up and its second down: their sum is small, the roundings of 32-bit keys are those of the summands.  The
+    groups' logits differ by about as much, so that the order of the sums falls between them."""
+    g = _gen(size)
+    bias = torch.full((2, size), -2.0 * big, device="cuda")
+    bias[:, 0], bias[:, 1] = big, -big
+    logits = _randn(g, 6000, 1, size).expand(-1, 2, -1) + big * 2.0 ** -24 * _randn(g, 6000, 2, size)
+    _check_route(worker, logits.flatten(1).contiguous(), bias.flatten(), 2, 2, 1, sigmoid=sigmoid)
+
+
+def test_router_on_biases_of_both_signs(worker):
+    """Ordinary logits; in every group some experts are pushed up and the others down."""
+    g = _gen(7)
+    bias = torch.where(torch.rand(256, device="cuda", generator=g) < 0.03, 1024.0, -1024.0)
+    bias.view(8, 32)[:, 5] = 1024.0
+    _check_route(worker, _randn(g, 20000, 256), bias, 8, 8, 4, sigmoid=True)
