@@ -52,10 +52,11 @@ __device__ __forceinline__ void exact_quotients(const float (&s)[8], const float
   for (int off = 8; off > 0; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
   // (no scale but 1 for a row normalised to zeros, none below the smallest normal number)
   const bool least = top < 448.f * 0x1p-126f;
-  const double factor = !(top > 0.f) ? (double)inv * 0.0 : (least ? (double)inv : 448.0) / (least ? (double)scale : amax);
+  // 448 s g has at most 51 bits: a quotient that is a tie between two codes is one here too, as it is divided last
+  const double factor = !(top > 0.f) ? (double)inv * 0.0 : least ? (double)inv : 448.0, over = !(top > 0.f) ? 1.0 : least ? (double)scale : amax;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double v = (double)s[e] * (double)g[e] * factor;
+    const double v = (double)s[e] * (double)g[e] * factor / over;
     const float f = __double2float_rz(v);
     q[e] = (double)f == v || !(v == v) ? f : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) | 1u);
   }

@@ -883,3 +883,23 @@ def test_router_on_biases_of_both_signs(worker):
     bias = torch.where(torch.rand(256, device="cuda", generator=g) < 0.03, 1024.0, -1024.0)
     bias.view(8, 32)[:, 5] = 1024.0
     _check_route(worker, _randn(g, 20000, 256), bias, 8, 8, 4, sigmoid=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [512, 4104])
+def test_norm_codes_on_ties(worker, dtype, cols):
+    """x is 3/4 of its group's largest value, or 3/32: 448 times which is 21/16 of a power of two, a tie that goes to 20/16.  The groups' weights
+    leave it one, whatever their own last bits and the statistic's are."""
+    g = _gen(cols)
+    rows, groups = 300, -(-cols // 128)
+    whole = torch.randint(32, 64, (rows, groups, 1), device="cuda", generator=g).float()  # six bits: 3/4 of it has eight
+    which = torch.rand((rows, groups, 128), device="cuda", generator=g)
+    which[..., 0] = 1
+    ratio = torch.where(which < 0.5, 0.75, torch.where(which < 0.75, -0.75 / 8, 1.0))
+    x = (whole * ratio).flatten(1)[:, :cols].to(dtype).contiguous()
+    gamma = (1 + torch.rand((groups, 1), device="cuda", generator=g)).expand(-1, 128).flatten()[:cols].contiguous()
+    codes, scale = torch.empty((rows, cols), dtype=F8, device="cuda"), torch.empty((rows, groups), device="cuda")
+    worker.run(runtime.rms_norm_fp8_block, x, gamma, codes, scale, 1e-6)
+    worker.sync()
+    want = torch.where(ratio == 0.75, 320.0, torch.where(ratio < 0, -40.0, 448.0)).flatten(1)[:, :cols]
+    assert torch.equal(codes.float(), want)
