@@ -150,12 +150,17 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
       // n / scale is 448 t / max t: the row's statistic cancels
       const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : inv * 0.f;  // (a statistic that is not finite: NaN)
       bool exact = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f && top >= 448.f * 0x1p-126f);
+      // Within 6 steps of the 24-bit format of a border between two codes: the roundings so far, 2^-22 together, are up to 4.  A border lies
+      // where the last 20 bits are 0x80000; below 2^-6, where codes lie 2^-9 apart, of 32 |q| + 1/2 (larger ones are 1 there: no border).
+      constexpr uint32_t kReach = 6;
+      auto past = [](float v) { return (__builtin_bit_cast(uint32_t, v) << 12) - ((0x80000u - kReach) << 12); };
+      uint32_t nearest = ~0u;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         q[e] = t[e] * r;
-        // within 6 steps of the 24-bit format of a border between two codes: the roundings so far, 2^-22 together, are up to 4
-        exact |= ((__builtin_bit_cast(uint32_t, q[e]) & 0xfffffu) - (0x80000u - 6u)) <= 12u;
+        nearest = min(nearest, min(past(q[e]), past(__builtin_amdgcn_fmed3f(fmaf(fabsf(q[e]), 32.f, 0.5f), 0.f, 1.f))));
       }
+      exact |= nearest <= (2 * kReach) << 12;
       if (__builtin_expect(__ballot(exact) != 0, 0)) exact_quotients(s[u], g[u], inv, top, sc, q);
     } else {
       const GroupQuotient quotient(sc);

@@ -903,3 +903,30 @@ def test_norm_codes_on_ties(worker, dtype, cols):
     worker.sync()
     want = torch.where(ratio == 0.75, 320.0, torch.where(ratio < 0, -40.0, 448.0)).flatten(1)[:, :cols]
     assert torch.equal(codes.float(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_codes_below_the_smallest_normal_code(worker, dtype, residual):
+    """Groups of one large value and many whose codes are subnormal, steps of 2^-9: random ones, and 2^-16 of the large one, which is
+    448 * 2^-16 = 3.5 steps, a tie that goes to the fourth, whatever row, weight and statistic are."""
+    g = _gen(11)
+    rows, cols = 600, 4096
+    x = _randn(g, rows, cols // 128, 128) * 2.0 ** -16
+    top = 1 + torch.rand((rows, cols // 128), device="cuda", generator=g)
+    x[..., 0] = top
+    x = (x * 256).to(dtype)
+    x[..., 64:] = x[..., :1] * 2.0 ** -16
+    gamma = 1 + 0.3 * torch.rand((cols // 128, 128), device="cuda", generator=g)
+    gamma[:, 64:] = gamma[:, :1]
+    x, gamma = x.flatten(1).contiguous(), gamma.flatten()
+    codes, scale = torch.empty((rows, cols), dtype=F8, device="cuda"), torch.empty((rows, cols // 128), device="cuda")
+    r, sums = torch.zeros_like(x), torch.empty_like(x)
+    if residual:
+        worker.run(runtime.add_rms_norm_fp8_block, x, r, gamma, sums, codes, scale, 1e-6)
+    else:
+        worker.run(runtime.rms_norm_fp8_block, x, gamma, codes, scale, 1e-6)
+    worker.sync()
+    want, _ = ob.quantize_rows(ob.rms_norm(x, None, gamma, 1e-6)[1])
+    assert (want.unflatten(-1, (-1, 128))[..., 64:] == 4 * 2.0 ** -9).all()
+    assert torch.equal(codes.double(), want)
