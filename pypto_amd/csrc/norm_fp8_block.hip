@@ -42,14 +42,22 @@ __device__ __forceinline__ void store(V* to, const V& v) {
   else *to = v;
 }
 
-// The quotients s g inv / scale of a group in 64 bits, rounded to 32 so that they stay on their side of every border between two codes (to
-// zero, the last bit set where anything is lost).  top: the group's largest |n|; all lanes of the group take part.
-__device__ __forceinline__ void exact_quotients(const float (&s)[8], const float (&g)[8], float inv, float top, float scale, float (&q)[8]) {
+// A group in 64 bits: its quotients s g inv / scale, rounded to 32 so that they stay on their side of every border between two codes (to
+// zero, the last bit set where anything is lost).  wide: s g may lie outside of what fp32 holds well, and its largest value and n are made here
+// as well.  top: the group's largest |n|; all lanes of the group take part.
+__device__ __forceinline__ void exact_group(const float (&s)[8], const float (&g)[8], float inv, bool wide, float& top, float& scale, float (&n)[8],
+                                            float (&q)[8]) {
   double amax = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs((double)s[e] * (double)g[e]));
 #pragma unroll
   for (int off = 8; off > 0; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
+  if (wide) {
+    top = (float)(amax * (double)inv);
+    scale = group_scale(top);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) n[e] = (float)((double)s[e] * (double)g[e] * (double)inv);
+  }
   // (no scale but 1 for a row normalised to zeros, none below the smallest normal number)
   const bool least = top < 448.f * 0x1p-126f;
   // 448 s g has at most 51 bits: a quotient that is a tie between two codes is one here too, as it is divided last
@@ -137,19 +145,21 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
       t[e] = NORM ? s[u][e] * g[u][e] : s[u][e];
       amax = fmaxf(amax, fabsf(t[e]));
     }
-    if (NORM && normed_out) {
+    auto store_normed = [&](const float (&n)[8], float times) {
       vec8 v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)(t[e] * inv);
+      for (int e = 0; e < 8; ++e) v[e] = (T)(n[e] * times);
       if (i < nvec) store<STREAM>(reinterpret_cast<vec8*>(normed_out + row * cols) + i, v);
-    }
+    };
+    if (NORM && normed_out) store_normed(t, inv);
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-    const float top = NORM ? amax * inv : amax, sc = group_scale(top);
+    float top = NORM ? amax * inv : amax, sc = group_scale(top);
     if constexpr (NORM) {
       // n / scale is 448 t / max t: the row's statistic cancels
       const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : inv * 0.f;  // (a statistic that is not finite: NaN)
-      bool exact = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f && top >= 448.f * 0x1p-126f);
+      const bool wide = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f);
+      bool exact = amax > 0.f && (wide || !(top >= 448.f * 0x1p-126f));
       // Within 6 steps of the 24-bit format of a border between two codes: the roundings so far, 2^-22 together, are up to 4.  A border lies
       // where the last 20 bits are 0x80000; below 2^-6, where codes lie 2^-9 apart, of 32 |q| + 1/2 (larger ones are 1 there: no border).
       constexpr uint32_t kReach = 6;
@@ -161,7 +171,10 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
         nearest = min(nearest, min(past(q[e]), past(__builtin_amdgcn_fmed3f(fmaf(fabsf(q[e]), 32.f, 0.5f), 0.f, 1.f))));
       }
       exact |= nearest <= (2 * kReach) << 12;
-      if (__builtin_expect(__ballot(exact) != 0, 0)) exact_quotients(s[u], g[u], inv, top, sc, q);
+      if (__builtin_expect(__ballot(exact) != 0, 0)) {
+        exact_group(s[u], g[u], inv, wide, top, sc, t, q);
+        if (normed_out && wide) store_normed(t, 1.f);  // over the one above
+      }
     } else {
       const GroupQuotient quotient(sc);
 #pragma unroll

@@ -930,3 +930,27 @@ def test_norm_codes_below_the_smallest_normal_code(worker, dtype, residual):
     want, _ = ob.quantize_rows(ob.rms_norm(x, None, gamma, 1e-6)[1])
     assert (want.unflatten(-1, (-1, 128))[..., 64:] == 4 * 2.0 ** -9).all()
     assert torch.equal(codes.double(), want)
+
+
+@pytest.mark.parametrize("cols", [256, 1000, 8200])
+def test_norm_where_the_weighted_sum_leaves_fp32_and_its_norm_does_not(worker, cols):
+    """s * gamma overflows, or is too small for 24 bits, while s * rsqrt(..) * gamma is an ordinary number."""
+    g = _gen(cols)
+    out, codes, scale = torch.empty((4, cols), dtype=torch.bfloat16, device="cuda"), torch.empty((4, cols), dtype=F8, device="cuda"), torch.empty(
+        (4, -(-cols // 128)), device="cuda")
+
+    def check(x, gamma):
+        worker.run(runtime.rms_norm_fp8_block_normed, x, gamma, out, codes, scale, 0.0)
+        worker.sync()
+        n = ob.rms_norm(x, None, gamma, 0.0)[1]
+        _check_codes(codes, scale, n, 2.0 ** -17)
+        assert ((out.double() - n).abs() <= n.abs() * (HALF_STEP[torch.bfloat16] + 2.0 ** -17) + TINY[torch.bfloat16]).all()
+
+    x = _randn(g, 4, cols)
+    check((x * 1e16).bfloat16(), 1e24 * (1 + 0.2 * _randn(g, cols)))
+    check((x * 1e-16).bfloat16(), 1e-26 * (1 + 0.2 * _randn(g, cols)))
+    # a row whose sum of squares passes fp32 is normalised to zeros, in 16 bits as in codes
+    gamma = 2 + 0.1 * torch.rand(cols, device="cuda", generator=g)
+    worker.run(runtime.rms_norm_fp8_block_normed, (x.sign() * 3e38).bfloat16(), gamma, out, codes, scale, 1e-6)
+    worker.sync()
+    assert (out == 0).all() and (codes.float() == 0).all() and (scale == 1).all()
