@@ -4,9 +4,9 @@
 //
 // and, where asked for, s (the next residual) and n in the 16-bit type of x.  s and n stay in 32 bits from the loads to the
 // outputs, so that each output is rounded once: the codes are those of n itself, not of its 16-bit copy.  n / scale is 448 t / max t with
-// t = s gamma: the row's statistic cancels, and the quotient's 32-bit roundings (2^-22) matter only next to a border between two codes.
-// There, 13 values in a million, the group is done again in 64 bits: the codes are the exact rows' (a plain evaluation in 32 bits has one in a
-// million wrong).
+// t = s gamma: the row's statistic cancels, and the quotient's 32-bit roundings (7 * 2^-24) matter only next to a border between two codes.
+// There, some 15 values in a million, the group is done again in 64 bits from its inputs, read once more: the codes are the exact rows' (a plain evaluation
+// in 32 bits has one in a million wrong), but in groups whose scale is the least there is, 2^-126, where the statistic does not cancel.
 // Without the norm the same kernel is the quantiser of activations that come from elsewhere.
 //
 // Bound by memory: 2 bytes an element for x and for each of residual, sum and normed, 1 for the codes.  One workgroup holds a row in
@@ -15,7 +15,8 @@
 // is still to be read; smaller ones stay there for who reads them next.  All outputs of bf16 rows, us without / with it, and with a
 // product of the codes behind: 4096 x 8192 63.3 / 54.3 (302 MB: 5.6 TB/s) and 113.5 / 108.5, 2048 x 5120 25.8 / 16.8 and 45.0 / 39.5, 8192 x
 // 2048 31.6 / 25.7 and 44.2 / 38.5; but 1024 x 4096 9.3 / 8.2 and 20.9 / 22.4, 512 x 4096 8.3 / 7.6 and 18.8 / 20.7.
-// With the weights asked for ahead of the row's statistic 4096 x 8192 takes 50 us in a loop of its own (6.1 TB/s), 4096 x 16384 95.
+// With the weights asked for ahead of the row's statistic 4096 x 8192 takes 49 us in a loop of its own (6.1 TB/s), 4096 x 16384 99.
+// Rows of up to 4096 columns have 64 registers, so that a SIMD holds eight of their wavefronts: 2048 x 4096 13.3 us, with 70 of them 13.9.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -29,6 +30,7 @@ namespace {
 using pto_hip::block8::codes4;
 using pto_hip::block8::group_scale;
 using pto_hip::block8::GroupQuotient;
+using pto_hip::block8::i32x4;
 using pto_hip::block8::kBlock;
 
 constexpr int kThreads = 256;
@@ -42,37 +44,91 @@ __device__ __forceinline__ void store(V* to, const V& v) {
   else *to = v;
 }
 
-// A group in 64 bits: its quotients s g inv / scale, rounded to 32 so that they stay on their side of every border between two codes (to
-// zero, the last bit set where anything is lost).  wide: s g may lie outside of what fp32 holds well, and its largest value and n are made here
-// as well.  top: the group's largest |n|; all lanes of the group take part.
-__device__ __forceinline__ void exact_group(const float (&s)[8], const float (&g)[8], float inv, bool wide, float& top, float& scale, float (&n)[8],
-                                            float (&q)[8]) {
+// v of the lane N further round in the 16 that hold a group.
+template <int N>
+__device__ __forceinline__ uint32_t rotated(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, true);
+}
+template <int N>
+__device__ __forceinline__ float rotated(float v) {
+  return __builtin_bit_cast(float, rotated<N>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int N>
+__device__ __forceinline__ double rotated(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)rotated<N>((uint32_t)(b >> 32)) << 32 | rotated<N>((uint32_t)b));
+}
+// The group's largest value, in all of its lanes.
+template <typename V>
+__device__ __forceinline__ V group_max(V v) {
+  v = fmax(v, rotated<8>(v));
+  v = fmax(v, rotated<4>(v));
+  v = fmax(v, rotated<2>(v));
+  return fmax(v, rotated<1>(v));
+}
+
+// The codes of a group of p inv / scale, p = s gamma, in 64 bits, from its inputs (x + residual may not fit 32).  A quotient 448 p / max p is first made in 32 bits;
+// which side of the border between the two codes around it the exact one lies on, or whether on the border itself, is the sign of
+// 448 p - border max p, exact where s has 24 bits.  wide: p may lie outside of what fp32 holds well, and the group's largest |n| and its scale are
+// made here as well.  All lanes of the group take part.
+// Products are made for each use, and one code after the other: whatever is held here are registers of the whole kernel.
+template <typename T>
+__device__ __forceinline__ void exact_codes(i32x4 x, i32x4 residual, bool add, const float (&g)[8], float inv, bool wide, float& top, float& scale,
+                                            uint32_t (&codes)[2]) {
+  auto product = [&](int e) {
+    typedef __attribute__((__vector_size__(8 * sizeof(T)))) T vec8;
+    const double a = (double)(float)__builtin_bit_cast(vec8, x)[e], b = (double)(float)__builtin_bit_cast(vec8, residual)[e];
+    float weight = g[e];
+    asm volatile("" : "+v"(weight));
+    return (add ? a + b : a) * (double)weight;
+  };
   double amax = 0.0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs((double)s[e] * (double)g[e]));
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
+  for (int e = 0; e < 8; ++e) amax = fmax(amax, fabs(product(e)));
+  amax = group_max(amax);
   if (wide) {
-    top = (float)(amax * (double)inv);
+    float by = inv;
+    asm volatile("" : "+v"(by));
+    top = (float)(amax * (double)by);
     scale = group_scale(top);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) n[e] = (float)((double)s[e] * (double)g[e] * (double)inv);
   }
-  // (no scale but 1 for a row normalised to zeros, none below the smallest normal number)
-  const bool least = top < 448.f * 0x1p-126f;
-  // 448 s g has at most 51 bits: a quotient that is a tie between two codes is one here too, as it is divided last
-  const double factor = !(top > 0.f) ? (double)inv * 0.0 : least ? (double)inv : 448.0, over = !(top > 0.f) ? 1.0 : least ? (double)scale : amax;
+  // A row that is normalised to zeros or to NaN, and one that is divided by the least scale that there is: p times so much and 2^126.
+  const bool none = !(top > 0.f) || amax > 0x1.fffffffffffffp1023, special = none || top < 448.f * 0x1p-126f;
+  const float times = none ? inv * 0.f : inv;
+  const int exponent = none ? 0 : __builtin_amdgcn_frexp_exp(amax);
+  amax = ldexp(amax, -exponent);  // 1/2 to 1
+  const float r = 448.f * GroupQuotient((float)amax).r;
+  auto quotient = [&](int e) {
+    asm volatile("" : "+v"(x), "+v"(residual));
+    __builtin_amdgcn_sched_barrier(0);
+    const double v = product(e);
+    if (special) {
+      float by = times;
+      asm volatile("" : "+v"(by));
+      return (float)(ldexp(v, 126) * (double)by);
+    }
+    const double size = ldexp(fabs(v), -exponent);
+    const float near = (float)size * r;
+    const bool low = near < 0x1p-6f;  // (there 32 |q| + 1/2 has the borders where larger ones have them)
+    float border = low ? fminf(fmaf(near, 32.f, 0.5f), 0x1.fffffep-1f) : near;
+    border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, border) & ~0xfffffu) | 0x80000u);
+    border = low ? (border - 0.5f) * 0x1p-5f : border;
+    const double past = fma(448.0, size, -((double)border * amax));
+    const uint32_t side = __builtin_bit_cast(uint32_t, border) + (uint32_t)(past > 0.0) - (uint32_t)(past < 0.0);
+    return copysignf(__builtin_bit_cast(float, side), (float)v);
+  };
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double v = (double)s[e] * (double)g[e] * factor / over;
-    const float f = __double2float_rz(v);
-    q[e] = (double)f == v || !(v == v) ? f : __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, f) | 1u);
+  for (int h = 0; h < 2; ++h) {
+    const float q0 = quotient(4 * h), q1 = quotient(4 * h + 1);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q0, q1, 0, false);
+    const float q2 = quotient(4 * h + 2), q3 = quotient(4 * h + 3);
+    codes[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q2, q3, w, true);
   }
 }
 
-// sum_out and normed_out may be x or residual themselves: a thread writes the columns that it alone has read.
+// sum_out and normed_out may be x or residual themselves: a thread writes the columns that it alone reads, behind its last use of them.
 template <typename T, bool NORM, bool STREAM, int VECS>
-__global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, const T* residual, const float* __restrict__ gamma,
+__global__ __launch_bounds__(kThreads, VECS <= 2 ? 8 : 2) void norm_fp8_block_kernel(const T* x, const T* residual, const float* __restrict__ gamma,
                                                                   T* sum_out, T* normed_out, uint8_t* __restrict__ codes,
                                                                   float* __restrict__ scale, int cols, float eps) {
   typedef __attribute__((__vector_size__(8 * sizeof(T)))) T vec8;
@@ -101,16 +157,17 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
       ss += s[u][e] * s[u][e];
     }
   }
-  if (sum_out) {
-    vec8* out = reinterpret_cast<vec8*>(sum_out + row * cols);
+  auto store_sum = [&](int u) {
+    const int i = threadIdx.x + u * kThreads;
+    vec8 v;
 #pragma unroll
-    for (int u = 0; u < VECS; ++u) {
-      const int i = threadIdx.x + u * kThreads;
-      vec8 v;
+    for (int e = 0; e < 8; ++e) v[e] = (T)s[u][e];
+    if (i < nvec) store<STREAM>(reinterpret_cast<vec8*>(sum_out + row * cols) + i, v);
+  };
+  const bool in_place = sum_out == x || sum_out == residual;  // the exact codes read both again
+  if (NORM && sum_out && !in_place) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)s[u][e];
-      if (i < nvec) store<STREAM>(out + i, v);
-    }
+    for (int u = 0; u < VECS; ++u) store_sum(u);
   }
   float inv = 1.f, g[VECS][8];  // NORM: the columns' weights
   if constexpr (NORM) {
@@ -145,24 +202,17 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
       t[e] = NORM ? s[u][e] * g[u][e] : s[u][e];
       amax = fmaxf(amax, fabsf(t[e]));
     }
-    auto store_normed = [&](const float (&n)[8], float times) {
-      vec8 v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (T)(n[e] * times);
-      if (i < nvec) store<STREAM>(reinterpret_cast<vec8*>(normed_out + row * cols) + i, v);
-    };
-    if (NORM && normed_out) store_normed(t, inv);
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+    amax = group_max(amax);
     float top = NORM ? amax * inv : amax, sc = group_scale(top);
+    uint32_t word[2];
     if constexpr (NORM) {
       // n / scale is 448 t / max t: the row's statistic cancels
       const float r = amax > 0.f ? 448.f * GroupQuotient(amax).r : inv * 0.f;  // (a statistic that is not finite: NaN)
       const bool wide = amax > 0.f && !(amax > 0x1p-90f && amax < 0x1p90f);
       bool exact = amax > 0.f && (wide || !(top >= 448.f * 0x1p-126f));
-      // Within 6 steps of the 24-bit format of a border between two codes: the roundings so far, 2^-22 together, are up to 4.  A border lies
+      // Within 7 steps of the 24-bit format of a border between two codes: the roundings so far, seven of 2^-24, are less.  A border lies
       // where the last 20 bits are 0x80000; below 2^-6, where codes lie 2^-9 apart, of 32 |q| + 1/2 (larger ones are 1 there: no border).
-      constexpr uint32_t kReach = 6;
+      constexpr uint32_t kReach = 7;
       auto past = [](float v) { return (__builtin_bit_cast(uint32_t, v) << 12) - ((0x80000u - kReach) << 12); };
       uint32_t nearest = ~0u;
 #pragma unroll
@@ -171,17 +221,39 @@ __global__ __launch_bounds__(kThreads) void norm_fp8_block_kernel(const T* x, co
         nearest = min(nearest, min(past(q[e]), past(__builtin_amdgcn_fmed3f(fmaf(fabsf(q[e]), 32.f, 0.5f), 0.f, 1.f))));
       }
       exact |= nearest <= (2 * kReach) << 12;
+      word[0] = codes4(q[0], q[1], q[2], q[3]), word[1] = codes4(q[4], q[5], q[6], q[7]);
       if (__builtin_expect(__ballot(exact) != 0, 0)) {
-        exact_group(s[u], g[u], inv, wide, top, sc, t, q);
-        if (normed_out && wide) store_normed(t, 1.f);  // over the one above
+        const i32x4 *xa = reinterpret_cast<const i32x4*>(xr), *ra = reinterpret_cast<const i32x4*>(rr);
+        asm volatile("" : "+s"(xa), "+s"(ra));  // (read again: kept since the start they would be registers of the whole kernel)
+        i32x4 a = {}, b = {};
+        if (i < nvec) {
+          a = xa[i];
+          if (ra) b = ra[i];
+        }
+        exact_codes<T>(a, b, rr != nullptr, g[u], inv, wide, top, sc, word);
+      }
+      if (normed_out) {
+        vec8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          asm volatile("" : "+v"(s[u][e]));  // (not held over the branch)
+          v[e] = (T)(s[u][e] * g[u][e] * inv);
+        }
+        if (__builtin_expect(__ballot(wide) != 0, 0)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = wide ? (T)(float)((double)s[u][e] * (double)inv * (double)g[u][e]) : v[e];
+        }
+        if (i < nvec) store<STREAM>(reinterpret_cast<vec8*>(normed_out + row * cols) + i, v);
       }
     } else {
       const GroupQuotient quotient(sc);
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[e] = quotient(t[e]);
+      word[0] = codes4(q[0], q[1], q[2], q[3]), word[1] = codes4(q[4], q[5], q[6], q[7]);
     }
+    if (NORM && sum_out && in_place) store_sum(u);
     if (i < nvec) {
-      store<STREAM>(crow + i, u32x2{codes4(q[0], q[1], q[2], q[3]), codes4(q[4], q[5], q[6], q[7])});
+      store<STREAM>(crow + i, u32x2{word[0], word[1]});
       if (i % 16 == 0) srow[i / 16] = sc;
     }
   }

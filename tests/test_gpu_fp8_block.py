@@ -954,3 +954,53 @@ def test_norm_where_the_weighted_sum_leaves_fp32_and_its_norm_does_not(worker, c
     worker.run(runtime.rms_norm_fp8_block_normed, (x.sign() * 3e38).bfloat16(), gamma, out, codes, scale, 1e-6)
     worker.sync()
     assert (out == 0).all() and (codes.float() == 0).all() and (scale == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [512, 2048, 4104, 16384])
+def test_norm_codes_are_those_of_the_exact_sums(worker, dtype, cols):
+    """x is 3/4 of its group's largest value or an eighth of that, 448 times which is a tie between two codes; the residual, too small for the
+    fp32 sum to show it, decides."""
+    g = _gen(cols)
+    rows = 300
+    whole = torch.randint(32, 64, (rows, -(-cols // 128), 1), device="cuda", generator=g).float()  # six bits: 3/4 of it has eight
+    which = torch.rand((rows, -(-cols // 128), 128), device="cuda", generator=g)
+    x = torch.where(which < 0.5, whole * 0.75, torch.where(which < 0.75, whole * 0.75 / 8, whole))
+    x[..., 0] = whole[..., 0]
+    small = 2.0 ** -26 if dtype == torch.bfloat16 else 2.0 ** -20  # of up to 64: below the last of its 24 bits
+    r = torch.where(torch.rand(x.shape, device="cuda", generator=g) < 0.5, -small, small)
+    r = torch.where(x == whole, 0.0, r)
+    x, r = (t.flatten(1)[:, :cols].to(dtype).contiguous() for t in (x, r))
+    gamma = torch.full((cols,), 0.5, device="cuda")
+    codes, scale = torch.empty((rows, cols), dtype=F8, device="cuda"), torch.empty((rows, -(-cols // 128)), device="cuda")
+    sums = torch.empty_like(x)
+    worker.run(runtime.add_rms_norm_fp8_block, x, r, gamma, sums, codes, scale, 1e-6)
+    worker.sync()
+    s, n = ob.rms_norm(x, r, gamma, 1e-6)
+    want, _ = ob.quantize_rows(n)
+    assert torch.equal(sums, s.to(dtype)) and not torch.equal(want, ob.quantize_rows(ob.rms_norm(x, None, gamma, 1e-6)[1])[0])
+    assert torch.equal(codes.double(), want)
+    # the sum over the residual and the norm over x, as a loop that keeps its buffers calls it
+    got, again, normed = torch.empty_like(codes), torch.empty_like(scale), x.clone()
+    worker.run(runtime.add_rms_norm_fp8_block_normed, normed, r, gamma, r, normed, got, again, 1e-6)
+    worker.sync()
+    assert torch.equal(got.double(), want) and torch.equal(again, scale) and torch.equal(r, sums)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_codes_around_the_smallest_normal_code(worker, dtype):
+    """2^-12 of a largest value of 7 is a code of 2^-6 itself, whichever side of it 32 bits see; ties next to it send the group to 64 bits."""
+    g = _gen(21)
+    rows, groups = 64, 64
+    x = torch.full((rows, groups, 128), 7.0, device="cuda")
+    x[..., 1:50] = 2.0 ** -12
+    x[..., 50:90] = -15 / 16 * 2.0 ** -12  # 7.5 of the steps of 2^-9 that 2^-6 has eight of
+    x[..., 90:100] = 5.25
+    x = x.flatten(1).to(dtype)
+    gamma = (1 + torch.rand((groups, 1), device="cuda", generator=g)).expand(-1, 128).flatten().contiguous()
+    codes, scale = torch.empty(x.shape, dtype=F8, device="cuda"), torch.empty((rows, groups), device="cuda")
+    worker.run(runtime.rms_norm_fp8_block, x, gamma, codes, scale, 1e-6)
+    worker.sync()
+    want = torch.full((128,), 448.0, device="cuda")
+    want[1:50], want[50:90], want[90:100] = 2.0 ** -6, -(2.0 ** -6), 320.0
+    assert (codes.float().unflatten(-1, (-1, 128)) == want).all()
