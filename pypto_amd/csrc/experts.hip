@@ -28,8 +28,8 @@ namespace block8 {
 constexpr int kMaxExperts = 1024;
 constexpr int kPlanThreads = 1024;
 constexpr int kFewSlots = 1024, kFewThreads = 256;  // a plan of few slots and experts: 192 slots of 16 experts 2.8 us for 3.6, 1024 of 250 3.4 for 4.6
-// Tokens are worked through in passes of so many slots, so that the scratch stays below a gigabyte or two and every index inside 32 bits.
-constexpr int64_t kPassSlots = 32768;
+// Tokens are worked through in passes of at most so many slots (expert_pass_tokens), so that the scratch stays small and every index inside 32 bits.
+constexpr int64_t kPassSlots = kExpertPassSlots;
 constexpr int64_t kMostDirectSlots = 1024;
 
 // The plan: slots by expert, and tiles of one expert each: of `height` rows, and what an expert has left in a tile of the least of height,
@@ -478,7 +478,7 @@ int run_experts(Experts x, int64_t tokens, hipStream_t st) {
   const int64_t slots = tokens * x.top_k;
   const bool direct = height == 0 ? experts_direct(slots, x.experts, x.hidden, x.inter, kExactUp) : height == 16;
   if (direct && slots <= kMostDirectSlots && direct_smem(x) <= kDirectSmem) return run_direct<OutT>(x, tokens, st);
-  const int64_t pass = std::min(tokens, std::max<int64_t>(1, kPassSlots / x.top_k));
+  const int64_t pass = expert_pass_tokens(tokens, x.top_k, x.hidden, x.inter, kExactUp ? 4 : 2);
   if (height < 64) height = choose_expert_rows(pass * x.top_k, x.experts, x.hidden, x.inter, kExactUp, kExactDown, ctx().num_cu);
   if (kExactUp) height = std::min(height, 128);
   const Scratch s(pass, x, height, kExactUp ? 4 : 2);

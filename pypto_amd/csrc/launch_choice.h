@@ -400,6 +400,15 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
   return pick;
 }
 
+// Tokens of a pass of the experts' FFN (experts.hip): as many slots as its plan holds, fewer where the pass's scratch (h as codes, the second product's
+// rows of y_bytes an element, their scales) would be more than 2 GB: 32768 rows of 65536 in fp32 are 8.6.
+constexpr int64_t kExpertPassSlots = 32768;
+constexpr int64_t kExpertPassBytes = 2ll << 30;
+inline int64_t expert_pass_tokens(int64_t tokens, int64_t top_k, int64_t hidden, int64_t inter, int64_t y_bytes) {
+  const int64_t slot = 4 + inter + inter / 32 + hidden * y_bytes + hidden / 32;
+  return std::min(tokens, std::max<int64_t>(1, std::min(kExpertPassSlots, kExpertPassBytes / slot) / top_k));
+}
+
 // Whether the experts' FFN of so many slots reads every slot's matrices for itself instead of planning tiles (experts.hip): the stream of them,
 // against that of the used experts' and the chain of a tile's blocks, whichever is longer (as sides of a triangle; both forms start with 10 us).
 // Measured, us direct / tiles: 8 of 64 experts of 4096 x 1408, one token on, 32 / 49, 55 / 62, 77 / 84, 98 / 112; 4 of 60 of 2048 x 1024 13 / 32, 16 / 33,

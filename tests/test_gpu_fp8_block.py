@@ -1004,3 +1004,23 @@ def test_norm_codes_around_the_smallest_normal_code(worker, dtype):
     want = torch.full((128,), 448.0, device="cuda")
     want[1:50], want[50:90], want[90:100] = 2.0 ** -6, -(2.0 ** -6), 320.0
     assert (codes.float().unflatten(-1, (-1, 128)) == want).all()
+
+
+def test_experts_whose_rows_would_not_fit_the_scratch_at_once(worker):
+    """500 tokens of 64 slots of 65536 channels, whose rows would be 8 GB in fp32: several passes.  Tokens of the first, the second and the last have the bits of a
+    call of theirs alone, and the library's scratch has not grown by those rows."""
+    args = _experts_case(5, 500, 65536, 128, 2, 64)
+    some = [0, 1, 130, 498, 499]
+    few = [t[some].contiguous() for t in args[:4]] + args[4:]
+    out, want = torch.empty((500, 65536), device="cuda"), torch.empty((5, 65536), device="cuda")
+    worker.set_option("block_gemm_rows", 64)
+    try:
+        worker.run(runtime.experts_ffn_fp8_block, *few, want)
+        worker.sync()
+        free = torch.cuda.mem_get_info()[0]
+        worker.run(runtime.experts_ffn_fp8_block, *args, out)
+        worker.sync()
+        assert free - torch.cuda.mem_get_info()[0] < 6e9
+    finally:
+        worker.set_option("block_gemm_rows", 0)
+    assert torch.equal(out[some], want) and want.isfinite().all() and want.abs().amax() > 0
