@@ -310,6 +310,18 @@ inline double makespan(const int64_t (&jobs)[3], const double (&us)[3], int64_t 
   double last = 0.0;
   for (int c = 0; c < 3; ++c)
     for (int64_t left = (jobs[c] + kXcds - 1) / kXcds; left > 0;) {
+      // all free within one workgroup's time of each other: every CU takes one in turn, for as many turns as all of them do
+      if (n > 1 && free[n - 1].at - free[0].at < us[c]) {
+        int64_t cus = 0;
+        for (int i = 0; i < n; ++i) cus += free[i].cus;
+        const int64_t turns = left / cus;
+        if (turns > 0) {
+          for (int i = 0; i < n; ++i) free[i].at += (double)turns * us[c];
+          last = std::max(last, free[n - 1].at);
+          left -= turns * cus;
+          continue;
+        }
+      }
       const Free f = free[0];
       const int64_t now = std::min(left, f.cus);
       // as many rounds as the first CUs have before others are free
@@ -336,7 +348,7 @@ inline double makespan(const int64_t (&jobs)[3], const double (&us)[3], int64_t 
 // ranges, the one it picks among the tiles is 0.9 % from the best in the mean and 13 % at worst, exact 0.4 % and 7 %.  rows, cols, splits: given, or 0.
 // Tiles of 256 channels share the rows among several heights where one height leaves its last round part empty: 11008 channels of 4096, us
 // with one height / several: 1300 rows 78 / 64, 1600 106 / 91, 2048 115 / 101, 4096 185 / 186; 5003 of 5120 4096 rows 149 / 125.
-// The estimate itself takes 1 us of the caller's time, none where up to 16 rows are bound by memory.
+// The estimate itself takes 0.5 us of the caller's time in the mean of 7500 sizes and 4 at most, none where up to 16 rows are bound by memory.
 // Up to 16 rows the form that reads straight to registers is a candidate: 32 channels a workgroup of four wavefronts, of eight where
 // there is at most one of them for a CU, 16 of eight where that leaves half of the CUs without one.  One row, us, four / eight / 16 of eight: 4096 x
 // 14336 14.0 / 16.4 / 19.6, 4096 x 6144 9.6 / 8.8 / 10.7, 5120 x 5003 11.6 / 8.8 / 10.8, 8192 x 8192 22.1 / 18.7 / 16.6, 11008 x 4096 - / 16.4 / 12.7, 16384 x 1024
@@ -363,6 +375,7 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
       if (splits > 0 && sp != std::min<int64_t>(splits, kb)) continue;
       if (splits == 0 && sp > 1 && (kb / sp < 8 || least_tiles * (sp - 1) >= 2 * num_cu)) break;  // short ranges, or CUs enough without them
       const int64_t per = (kb + sp - 1) / sp, ranges = (kb + per - 1) / per;
+      const double slabs = ranges > 1 ? 5.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4 : 0.0;
       auto consider = [&](int64_t high, int64_t half, int64_t quarter) {
         const int64_t jobs[3] = {high * tiles_n * ranges, half * tiles_n * ranges, quarter * tiles_n * ranges};
         const double load = std::min(1.0, (double)(jobs[0] + jobs[1] + jobs[2]) / (double)num_cu);
@@ -371,9 +384,15 @@ inline BlockTile choose_block_tile(int64_t m, int64_t n, int64_t kb, bool exact,
           const BlockTileCost& l = kBlockTiles[exact][std::max(form - c, std::min(form, 2))];
           each[c] = (double)((per + groups - 1) / groups * groups) * (l.block + l.loaded * load) + l.start;
         }
-        double us = makespan(jobs, each, num_cu);
-        us = std::max(us, memory) + 0.1 * std::min(us, memory);
-        if (ranges > 1) us += 5.0 + (double)ranges * (double)m * (double)n * 8e-6 / 5.4;
+        auto in_all = [&](double us) { return std::max(us, memory) + 0.1 * std::min(us, memory) + slabs; };
+        // no schedule takes less than the tiles' costs spread over the CUs, nor less than one tile
+        double least = 0.0, spread = 0.0;
+        for (int c = 0; c < 3; ++c) {
+          spread += (double)jobs[c] * each[c];
+          if (jobs[c] > 0) least = std::max(least, each[c]);
+        }
+        if (in_all(std::max(least, (1.0 - 1e-9) * spread / (double)num_cu)) >= best) return;
+        const double us = in_all(makespan(jobs, each, num_cu));
         if (us < best) {
           best = us;
           pick = BlockTile{t.rows, t.cols, ranges > 1 ? (int)per : 0, {(int)high, (int)half, (int)quarter}};
