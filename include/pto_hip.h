@@ -364,17 +364,18 @@ PTO_HIP_API int pto_hip_quantize_rows_fp8(const void* x, void* codes, float* sca
 /* ---- e4m3 operands with a scale for each block of 128 (none has a counterpart in the reference) ----
  * Activations: codes [rows, cols] with one fp32 scale per 128 columns of a row, [rows, ceil(cols / 128)].  Weights: codes one row per
  * OUTPUT channel with k contiguous, [n, k], with one fp32 scale per block of 128 x 128, [ceil(n / 128), k / 128].  A value is its
- * code times its scale; scales may be any fp32 values.  Results lie apart from the operands and from each other, unless said otherwise
- * (PTO_HIP_ERR_INVALID_VALUE).  The experts' FFN, and a product whose k is cut into ranges, use the library's scratch: like all calls
+ * code times its scale; scales may be any fp32 values, but the product of the two scales of a block is formed in fp32 before the sum of its codes
+ * is multiplied: below 2^-126 it loses bits, beyond 2^128 it is infinite.  Results lie apart from the operands and from each other, unless said
+ * otherwise (PTO_HIP_ERR_INVALID_VALUE).  The experts' FFN, and a product whose k is cut into ranges, use the library's scratch: like all calls
  * that do, they are ordered on one stream, or synchronised, and a size is called once eagerly before it is captured. */
 
 /* s = x + residual; n = s * rsqrt(mean s^2 + eps) * gamma; scale[t, g] = max(amax_g |n| / 448, 2^-126), 1 for a group of zeros;
- * codes = e4m3(n / scale), round to nearest even, decided on 64 bits where 32 might pass a border between two codes; sum_out =
- * x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every output is rounded once (a row whose sum of squares passes
- * fp32 is normalised to zeros).  residual, gamma, sum_out and normed_out
+ * codes = e4m3(n / scale), round to nearest even, decided on 64 bits, from x + residual itself, where 32 might pass a border between two codes:
+ * those of the exact rows, but for groups whose scale is 2^-126; sum_out = x_dtype(s), normed_out = x_dtype(n).  s and n are kept in fp32: every
+ * output is rounded once (a row whose sum of squares passes fp32 is normalised to zeros; a group whose s * gamma are all below 2^-150 counts as zeros).  residual, gamma, sum_out and normed_out
  * may each be NULL; sum_out and normed_out may be x or residual themselves.  NaN elements are left out of amax and give NaN codes.
  * cols a multiple of 8 and at most 16384 (PTO_HIP_ERR_UNSUPPORTED otherwise; the last group may be shorter).
- * quantize_fp8_block: codes and scales of x itself. */
+ * quantize_fp8_block: codes and scales of x itself, codes = e4m3(fp32(x / scale)). */
 PTO_HIP_API int pto_hip_rms_norm_fp8_block(const void* x, const void* residual, const float* gamma, void* sum_out, void* normed_out,
                                            void* codes, float* scale, int64_t rows, int64_t cols, float eps, int x_dtype,
                                            void* stream);
@@ -405,7 +406,8 @@ PTO_HIP_API int pto_hip_route_experts(const void* logits, const float* bias, int
  * experts' half of a mixture layer behind pto_hip_rms_norm_fp8_block and pto_hip_route_experts.  Products as
  * pto_hip_projection_fp8_block; h = SiLU(g) * u is quantised from fp32 with those scales, the sum over a token's
  * experts is fp32.  A negative id leaves its slot out (a token without any gives zeros); an id of an expert that there is
- * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  With BF16 results of many
+ * not does so too and is reported by the next pto_hip_sync.  An expert may be named twice by a token.  The form is chosen by all T * top_k slots,
+ * with an expert or without.  With BF16 results of many
  * tokens both products are as pto_hip_projection_fp8_block's of 16-bit results, and the experts' rows are added from fp16 with a
  * power of two per 128 channels; with FP16 results the second product is; the widened form has the rest.  H and I multiples of 128
  * and at most 65536, at most 1024 experts and top_k 64 (PTO_HIP_ERR_UNSUPPORTED otherwise).  Matrices of all experts lie one behind the

@@ -12,7 +12,7 @@
 //
 // One wavefront per token, expert e in lane e % 64.  Keys are mapped to unsigned integers of the same order, so that the
 // best of a wavefront is an integer maximum.  Bound by instructions, not by memory: 4096 tokens, eight of 256 experts in four of eight groups,
-// sigmoid and bias, 9.0 us a call, where the 4.5 MB take 1 us; 11.6 us with loads waited for one by one, the lanes' best looked for again
+// sigmoid and bias, 8.7 us a call, where the 4.5 MB take 1 us; 11.6 us with loads waited for one by one, the lanes' best looked for again
 // behind every choice and groups ranked on exact keys, 14.7 with the whole choice on 64-bit keys.  One token 7 us, the call's own time.
 #include <hip/hip_runtime.h>
 
