@@ -223,14 +223,14 @@ __global__ __launch_bounds__(kThreads, VECS <= 2 ? 8 : 2) void norm_fp8_block_ke
       exact |= nearest <= (2 * kReach) << 12;
       word[0] = codes4(q[0], q[1], q[2], q[3]), word[1] = codes4(q[4], q[5], q[6], q[7]);
       if (__builtin_expect(__ballot(exact) != 0, 0)) {
-        const i32x4 *xa = reinterpret_cast<const i32x4*>(xr), *ra = reinterpret_cast<const i32x4*>(rr);
+        const vec8 *xa = xr, *ra = rr;
         asm volatile("" : "+s"(xa), "+s"(ra));  // (read again: kept since the start they would be registers of the whole kernel)
-        i32x4 a = {}, b = {};
+        vec8 a = {}, b = {};
         if (i < nvec) {
           a = xa[i];
           if (ra) b = ra[i];
         }
-        exact_codes<T>(a, b, rr != nullptr, g[u], inv, wide, top, sc, word);
+        exact_codes<T>(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), rr != nullptr, g[u], inv, wide, top, sc, word);
       }
       if (normed_out) {
         vec8 v;
