@@ -16,7 +16,8 @@
 // product of the codes behind: 4096 x 8192 63.3 / 54.3 (302 MB: 5.6 TB/s) and 113.5 / 108.5, 2048 x 5120 25.8 / 16.8 and 45.0 / 39.5, 8192 x
 // 2048 31.6 / 25.7 and 44.2 / 38.5; but 1024 x 4096 9.3 / 8.2 and 20.9 / 22.4, 512 x 4096 8.3 / 7.6 and 18.8 / 20.7.
 // With the weights asked for ahead of the row's statistic 4096 x 8192 takes 49 us in a loop of its own (6.1 TB/s), 4096 x 16384 99.
-// Rows of up to 4096 columns have 64 registers, so that a SIMD holds eight of their wavefronts: 2048 x 4096 13.3 us, with 70 of them 13.9.
+// Rows of up to 4096 columns have 64 registers, so that a SIMD holds eight of their wavefronts: 2048 x 4096 12.8 us, with 70 of them 13.9.
+// Where every weight is the same, ties are common and most wavefronts go through the 64 bits: 4096 x 8192 53 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -71,7 +72,7 @@ __device__ __forceinline__ V group_max(V v) {
 // which side of the border between the two codes around it the exact one lies on, or whether on the border itself, is the sign of
 // 448 p - border max p, exact where s has 24 bits.  wide: p may lie outside of what fp32 holds well, and the group's largest |n| and its scale are
 // made here as well.  All lanes of the group take part.
-// Products are made for each use, and one code after the other: whatever is held here are registers of the whole kernel.
+// Products are made for each use: whatever is held here are registers of the whole kernel.
 template <typename T>
 __device__ __forceinline__ void exact_codes(i32x4 x, i32x4 residual, bool add, const float (&g)[8], float inv, bool wide, float& top, float& scale,
                                             uint32_t (&codes)[2]) {
@@ -92,37 +93,38 @@ __device__ __forceinline__ void exact_codes(i32x4 x, i32x4 residual, bool add, c
     top = (float)(amax * (double)by);
     scale = group_scale(top);
   }
-  // A row that is normalised to zeros or to NaN, and one that is divided by the least scale that there is: p times so much and 2^126.
+  auto encode = [&](auto quotient) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      asm volatile("" : "+v"(x), "+v"(residual));
+      const float q0 = quotient(4 * h), q1 = quotient(4 * h + 1), q2 = quotient(4 * h + 2), q3 = quotient(4 * h + 3);
+      codes[h] = codes4(q0, q1, q2, q3);
+    }
+  };
+  // a row that is normalised to zeros or to NaN, and one that is divided by the least scale that there is
   const bool none = !(top > 0.f) || amax > 0x1.fffffffffffffp1023, special = none || top < 448.f * 0x1p-126f;
-  const float times = none ? inv * 0.f : inv;
-  const int exponent = none ? 0 : __builtin_amdgcn_frexp_exp(amax);
-  amax = ldexp(amax, -exponent);  // 1/2 to 1
-  const float r = 448.f * GroupQuotient((float)amax).r;
-  auto quotient = [&](int e) {
-    asm volatile("" : "+v"(x), "+v"(residual));
-    __builtin_amdgcn_sched_barrier(0);
-    const double v = product(e);
-    if (special) {
+  if (!special) {
+    const int exponent = __builtin_amdgcn_frexp_exp(amax);
+    amax = ldexp(amax, -exponent);  // 1/2 to 1
+    const float r = 448.f * GroupQuotient((float)amax).r;
+    encode([&](int e) {
+      const double v = product(e), size = ldexp(fabs(v), -exponent);
+      const float near = (float)size * r;
+      const bool low = near < 0x1p-6f;  // (there 32 |q| + 1/2 has the borders where larger ones have them)
+      float border = low ? fminf(fmaf(near, 32.f, 0.5f), 0x1.fffffep-1f) : near;
+      border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, border) & ~0xfffffu) | 0x80000u);
+      border = low ? (border - 0.5f) * 0x1p-5f : border;
+      const double past = fma(448.0, size, -((double)border * amax));
+      const uint32_t side = __builtin_bit_cast(uint32_t, border) + (uint32_t)(past > 0.0) - (uint32_t)(past < 0.0);
+      return copysignf(__builtin_bit_cast(float, side), (float)v);
+    });
+  } else {
+    const float times = none ? inv * 0.f : inv;
+    encode([&](int e) {
       float by = times;
       asm volatile("" : "+v"(by));
-      return (float)(ldexp(v, 126) * (double)by);
-    }
-    const double size = ldexp(fabs(v), -exponent);
-    const float near = (float)size * r;
-    const bool low = near < 0x1p-6f;  // (there 32 |q| + 1/2 has the borders where larger ones have them)
-    float border = low ? fminf(fmaf(near, 32.f, 0.5f), 0x1.fffffep-1f) : near;
-    border = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, border) & ~0xfffffu) | 0x80000u);
-    border = low ? (border - 0.5f) * 0x1p-5f : border;
-    const double past = fma(448.0, size, -((double)border * amax));
-    const uint32_t side = __builtin_bit_cast(uint32_t, border) + (uint32_t)(past > 0.0) - (uint32_t)(past < 0.0);
-    return copysignf(__builtin_bit_cast(float, side), (float)v);
-  };
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float q0 = quotient(4 * h), q1 = quotient(4 * h + 1);
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q0, q1, 0, false);
-    const float q2 = quotient(4 * h + 2), q3 = quotient(4 * h + 3);
-    codes[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q2, q3, w, true);
+      return (float)(ldexp(product(e), 126) * (double)by);
+    });
   }
 }
 
