@@ -154,6 +154,21 @@ PTO_HIP_API int pto_hip_sync(void* stream);
  *  "experts_ffn_fp8_block"  the chosen experts' FFN (no counterpart in the reference)
  *      tensors: x8[T,H] e4m3, x_scale[T,H/128] fp32, expert_ids[T,top_k] i32, expert_weights[T,top_k] fp32, w_gate8[E,I,H],
  *               w_gate_scale[E,I/128,H/128], w_up8, w_up_scale, w_down8[E,H,I], w_down_scale[E,H/128,I/128], out[T,H]
+ *  "rope_append_tokens"   several new tokens of every sequence rotated and appended to a paged cache (one token each:
+ *                      "rope_kv_cache_update"; examples/models/qwen3_jit/kernels/attention.py:39-102)
+ *      tensors: qkv[T,(Hq+2Hkv)*D] fp32|bf16|fp16, positions[T] i32, token_starts[B+1] i32, context_lens[B] i32, rope_cos[max_pos,R/2] or
+ *               [max_pos,D], rope_sin, [gamma_q[D] fp32, gamma_k[D] fp32,] block_table[B,max_blocks] i32, key_cache (INOUT), value_cache (INOUT),
+ *               q_out[T*Hq,D];  scalars: num_heads, kv_head_num, head_dim, block_size [, eps (f32 bits) with the gammas]
+ *  "rope_append_tokens_fp8"  the same with FP8E4M3FN caches, quantised on write
+ *      tensors: ..., key_cache (INOUT), value_cache (INOUT), k_scale[pool,Hkv] fp32 (INOUT), v_scale (INOUT), q_out
+ *  "tree_attention"    attention of the new tokens of every sequence over its paged cache and over each other, by a mask (one token each:
+ *                      "paged_attention")
+ *      tensors: query[T*Hq,D] bf16|fp16, key_cache[pool*Hkv*bs,D], value_cache, block_table[B,max_blocks] i32, context_lens[B] i32,
+ *               token_starts[B+1] i32, tree_mask[T,W] i32, out[T*Hq,D] (dtype of query) [, k_scale[pool,Hkv] fp32, v_scale]
+ *      scalars: num_heads, kv_head_num, head_dim, block_size, scale (f32 bits)
+ *  "sample_tokens"     the next token of every row of logits (no counterpart in the reference)
+ *      tensors: logits[R,V] fp32|bf16|fp16, temperature[R] fp32, top_k[R] i32, top_p[R] fp32, min_p[R] fp32, uniform[R] fp32,
+ *               tokens[R] i32, probs[R] fp32
  *  "llama_mini"        examples/models/08_llama_mini.py:384-483
  *      tensors: hidden[S,D], causal_mask[S,S], cos_emb[S,D/2], sin_emb[S,D/2], wq, wk, wv, w_dense, w_gate, w_up,
  *               w_down [D,D], w_lm[D,V], logits[S,V], all fp32
@@ -475,6 +490,89 @@ PTO_HIP_API int pto_hip_rope_kv_cache_update_fp8(const float* qkv, const int32_t
                                                  int64_t kv_head_num, int64_t head_dim, int64_t block_size,
                                                  int64_t max_num_blocks_per_req, int64_t max_pos,
                                                  int64_t pool_blocks, int q_dtype, void* stream);
+
+/* ---- a step that verifies drafted tokens: several new tokens per sequence (none has a counterpart in the reference) ----
+ * Sequence b's new tokens are rows token_starts[b] .. token_starts[b+1] - 1 of the ragged batch (rising, token_starts[B] <= T; rows outside of
+ * [token_starts[0], token_starts[B]) belong to nobody and what they would write is left as it was).  Its i-th new token lies at index
+ * context_lens[b] + i of its cache, found through block_table; context_lens counts the tokens in front of the new ones.  The calls read these tensors
+ * on the device: a captured call serves any lengths that fit its T, B and table. */
+
+/* q = rope(norm(q) gamma_q), k = rope(norm(k) gamma_k), v as it is, of every new token; norm(x) = x / sqrt(mean x^2 + eps) over a head's D
+ * elements, left out where the gammas are NULL.  rope turns elements i and i + R/2 by the angle of row positions[t] of the tables, R = 2 *
+ * rope_table_width <= D; elements from R on stay as they are (rope_table_width = D: the reference's tables, R = D, low-half and high-half factors
+ * side by side).  positions are the caller's: a drafted token's is that of its depth in the tree, not of its index.  All of it in fp32; k and v go to
+ * the cache and q to q_out, rounded once.  A position outside the tables, or an index outside the block table or the cache, leaves its token out
+ * and is reported by the next pto_hip_sync.
+ * FP8E4M3FN caches have one scale per (block, KV head).  All new rows of a block are taken together: where the first of them is the block's first row,
+ * scale = max |new rows| / 448 (1 for zeros); otherwise the scale only grows to that, and where it does the block's rows in front are coded
+ * again.  Infinite and NaN elements are left out of the maximum; infinite ones give codes of 448.  head_dim a multiple of 8 and R of 16, at most 512 (PTO_HIP_ERR_UNSUPPORTED otherwise).
+ * A block that a call appends to belongs to one sequence.  At most 2^20 tokens. */
+typedef struct PtoHipRopeAppendArgs {
+  const void* qkv;              /* [T, (Hq + 2 Hkv) D]: q heads, k heads, v heads */
+  const int32_t* positions;     /* [T] rows of the rope tables */
+  const int32_t* token_starts;  /* [B + 1] */
+  const int32_t* context_lens;  /* [B] */
+  const float* rope_cos;        /* [max_pos, rope_table_width] */
+  const float* rope_sin;
+  const float* gamma_q;         /* [D], or both NULL */
+  const float* gamma_k;
+  const int32_t* block_table;   /* [B, max_num_blocks_per_req] */
+  void* key_cache;              /* [pool_blocks * Hkv * block_size, D], updated in place */
+  void* value_cache;
+  float* k_scale;               /* [pool_blocks, Hkv], updated in place (e4m3 caches only) */
+  float* v_scale;
+  void* q_out;                  /* [T * Hq, D] dtype */
+  int64_t tokens, batch, num_heads, kv_head_num, head_dim;
+  int64_t block_size, max_num_blocks_per_req, max_pos, pool_blocks;
+  float eps;
+  int32_t qkv_dtype;            /* PTO_HIP_FP32, PTO_HIP_BF16 or PTO_HIP_FP16 */
+  int32_t dtype;                /* of q_out, and of the caches unless kv_dtype says otherwise: PTO_HIP_BF16 or PTO_HIP_FP16 */
+  int32_t kv_dtype;             /* 0 = caches hold `dtype`; PTO_HIP_FP8E4M3FN */
+  int32_t rope_table_width;     /* 0 = D / 2 */
+} PtoHipRopeAppendArgs;
+PTO_HIP_API int pto_hip_rope_append_tokens(const PtoHipRopeAppendArgs* args, void* stream);
+
+/* out[t, h] = softmax(scale q k^T) v of the keys that row t sees: the first context_lens[b] of its sequence, and of the sequence's new tokens - whose
+ * keys and values lie behind those in the cache - number j where bit j % 32 of tree_mask[t, j / 32] is set (a tree: a token's ancestors and
+ * itself; a chain: all up to itself).  Bits of tokens that the sequence does not have say nothing; a sequence with more new tokens than 32
+ * mask_words is reported by the next pto_hip_sync, its tokens from there on seen by nobody.  A row that sees nothing gives zeros; what a row does not
+ * see has no part in it, infinities and NaN among it.  Scores, their sums and out are kept in fp32; probabilities are rounded to the query's type in front
+ * of their product with the values, and summed as rounded; out is rounded once.  A table entry outside the cache reads block 0
+ * and is reported by the next pto_hip_sync.  Uses the library's scratch: like all calls that do, calls are ordered on one stream, or synchronised,
+ * and a size is called once eagerly before it is captured.  head_dim 64, 128 and 256 with blocks of a multiple of 16 tokens (32 for FP8E4M3FN caches)
+ * run on matrix instructions, any other head_dim up to 256 and block_size on a plain kernel (beyond: PTO_HIP_ERR_UNSUPPORTED).  At most 2^20 tokens,
+ * mask_words 32. */
+typedef struct PtoHipTreeAttentionArgs {
+  const void* query;            /* [T * Hq, D] dtype */
+  const void* key_cache;        /* [pool_blocks * Hkv * block_size, D] */
+  const void* value_cache;
+  const float* k_scale;         /* [pool_blocks, Hkv] (e4m3 caches only) */
+  const float* v_scale;
+  const int32_t* block_table;   /* [B, max_num_blocks_per_req] */
+  const int32_t* context_lens;  /* [B] */
+  const int32_t* token_starts;  /* [B + 1] */
+  const int32_t* tree_mask;     /* [T, mask_words] */
+  void* out;                    /* [T * Hq, D] dtype */
+  int64_t tokens, batch, num_heads, kv_head_num, head_dim;
+  int64_t block_size, max_num_blocks_per_req, pool_blocks, mask_words;
+  float scale;
+  int32_t dtype;                /* PTO_HIP_BF16 or PTO_HIP_FP16 */
+  int32_t kv_dtype;             /* 0 = caches hold `dtype`; PTO_HIP_FP8E4M3FN */
+} PtoHipTreeAttentionArgs;
+PTO_HIP_API int pto_hip_tree_attention(const PtoHipTreeAttentionArgs* args, void* stream);
+
+/* The next token of every row of logits, from a random number of the row's own.  weight = exp((logit - largest) / temperature); the order is by logit,
+ * of equal ones the lower index first.  Kept are the first top_k tokens (0 or less: all), of those the fewest from the front whose weights reach
+ * top_p of all of theirs (1 or more, or NaN: all; the best one always), of those the ones whose weight is at least min_p (at most 1; 0 or less, or
+ * NaN: all).  The token is the first, in the order of indices, at which the running sum of the kept weights passes `uniform` times their sum
+ * (uniform in [0, 1); below 2^-25 it counts as that), probs its share of that sum.  A temperature that is not above 0 takes the largest logit, with
+ * probability 1.  A NaN logit counts as -inf, which is never kept; infinite ones share everything evenly; a row without any other gives token -1 and
+ * probability 0.  Weights are added exactly, as integers in units of 2^-44 of the largest (below 2^-45 of it they are none): the result does not
+ * depend on how the work is split.  top_k, top_p, min_p and probs may be NULL.  At most 2^19 logits a row (PTO_HIP_ERR_UNSUPPORTED otherwise).
+ * Uses the library's scratch (ordered on one stream, and called once eagerly before it is captured). */
+PTO_HIP_API int pto_hip_sample_tokens(const void* logits, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                                      const float* uniform, int32_t* tokens, float* probs, int64_t rows, int64_t vocab, int logits_dtype,
+                                      void* stream);
 
 /* One decoder layer, one new token per sequence (examples/models/qwen3_jit/qwen3_decode.py:47-113):
  * RMSNorm -> QKV -> RoPE + K/V append -> paged attention -> o_proj + residual -> RMSNorm ->

@@ -34,7 +34,7 @@ EXPORTS = (
     "pto_hip_ffn_swiglu_fp8", "pto_hip_quantize_rows_fp8", "pto_hip_rms_norm_quantize_fp8",
     "pto_hip_gate_up_swiglu_fp8", "pto_hip_projection_fp8", "pto_hip_llama_mini",
     "pto_hip_rms_norm_fp8_block", "pto_hip_quantize_fp8_block", "pto_hip_projection_fp8_block", "pto_hip_route_experts",
-    "pto_hip_experts_ffn_fp8_block",
+    "pto_hip_experts_ffn_fp8_block", "pto_hip_rope_append_tokens", "pto_hip_tree_attention", "pto_hip_sample_tokens",
     "pto_hip_write_manifest", "pto_hip_backend_info", "pto_hip_backend_op_name", "pto_hip_backend_op_info",
     "pto_hip_backend_codegen", "pto_hip_backend_check_ops", "pto_hip_backend_program_ops",
     "pto_hip_backend_mem_path", "pto_hip_backend_handler_query",
@@ -87,6 +87,26 @@ class DeviceInfo(C.Structure):
         ("hbm_bytes", C.c_int64),
         ("arch", C.c_char * 32),
     ]
+
+
+class RopeAppendArgs(C.Structure):
+    """PtoHipRopeAppendArgs."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("qkv", "positions", "token_starts", "context_lens", "rope_cos", "rope_sin", "gamma_q", "gamma_k",
+                                          "block_table", "key_cache", "value_cache", "k_scale", "v_scale", "q_out")] \
+        + [(n, C.c_int64) for n in ("tokens", "batch", "num_heads", "kv_head_num", "head_dim", "block_size", "max_num_blocks_per_req", "max_pos",
+                                    "pool_blocks")] \
+        + [("eps", C.c_float), ("qkv_dtype", C.c_int32), ("dtype", C.c_int32), ("kv_dtype", C.c_int32), ("rope_table_width", C.c_int32)]
+
+
+class TreeAttentionArgs(C.Structure):
+    """PtoHipTreeAttentionArgs."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("query", "key_cache", "value_cache", "k_scale", "v_scale", "block_table", "context_lens", "token_starts",
+                                          "tree_mask", "out")] \
+        + [(n, C.c_int64) for n in ("tokens", "batch", "num_heads", "kv_head_num", "head_dim", "block_size", "max_num_blocks_per_req",
+                                    "pool_blocks", "mask_words")] \
+        + [("scale", C.c_float), ("dtype", C.c_int32), ("kv_dtype", C.c_int32)]
 
 
 _lib = None
@@ -142,6 +162,9 @@ def load() -> C.CDLL:
         "pto_hip_projection_fp8_block": [vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, vp],
         "pto_hip_route_experts": [vp, vp, vp, vp, i64, i64, i64, i64, i64, C.c_int, C.c_int, C.c_float, C.c_int, vp],
         "pto_hip_experts_ffn_fp8_block": [vp] * 11 + [i64] * 5 + [C.c_int, vp],
+        "pto_hip_rope_append_tokens": [C.POINTER(RopeAppendArgs), vp],
+        "pto_hip_tree_attention": [C.POINTER(TreeAttentionArgs), vp],
+        "pto_hip_sample_tokens": [vp] * 8 + [i64, i64, C.c_int, vp],
         "pto_hip_llama_mini": [vp] * 13 + [i64, i64, i64, C.c_float, vp],
         "pto_hip_w8a16_matmul": [vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, C.c_int, C.c_int, vp],
         "pto_hip_w8a16_swiglu": [vp, vp, vp, vp, vp, vp, i64, i64, i64, C.c_int, C.c_int, vp],

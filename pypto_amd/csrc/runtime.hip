@@ -120,6 +120,10 @@ enum ProgramKind {
   kProjectionFp8Block,
   kRouteExperts,
   kExpertsFfnFp8Block,
+  kRopeAppendTokens,
+  kRopeAppendTokensFp8,
+  kTreeAttention,
+  kSampleTokens,
   kNumPrograms
 };
 
@@ -128,7 +132,8 @@ const char* const kProgramNames[kNumPrograms] = {
     "w8a16_matmul",    "w8a16_swiglu",  "rope_kv_cache_update", "rope_kv_cache_update_fp8",
     "decoder_layer_decode", "projection", "gate_up_swiglu", "ffn_block_fp8", "llama_mini",
     "paged_attention_batch", "paged_attention_dynamic", "paged_attention_spmd", "ffn_gelu", "ffn_relu",
-    "rms_norm_fp8_block", "quantize_fp8_block", "projection_fp8_block", "route_experts", "experts_ffn_fp8_block"};
+    "rms_norm_fp8_block", "quantize_fp8_block", "projection_fp8_block", "route_experts", "experts_ffn_fp8_block",
+    "rope_append_tokens", "rope_append_tokens_fp8", "tree_attention", "sample_tokens"};
 
 std::mutex g_mu;
 std::vector<int> g_callables;  // callable id -> ProgramKind, -1 once unregistered
@@ -825,6 +830,184 @@ int run_rope_kv(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hi
                                       numel(t[2]) / rope_w, rope_w, numel(t[5]) / d, (int)t[5].dtype, stream);
 }
 
+// ---- a step that verifies drafted tokens ----
+// token_starts[B+1], context_lens[B] and block_table[B, max_blocks] of a ragged batch.
+int check_ragged(const char* prog, const PtoHipChipTensor& starts, const PtoHipChipTensor& lens, const PtoHipChipTensor& table) {
+  PTO_CHECK_ARG(starts.dtype == PTO_HIP_INT32 && lens.dtype == PTO_HIP_INT32 && table.dtype == PTO_HIP_INT32,
+                "%s: token_starts, context_lens and block_table must be INT32", prog);
+  PTO_CHECK_ARG(starts.ndims == 1 && lens.ndims == 1 && numel(starts) == numel(lens) + 1,
+                "%s: token_starts must have an entry more than context_lens (one per sequence), got %lld and %lld", prog, (long long)numel(starts),
+                (long long)numel(lens));
+  PTO_CHECK_ARG(table.ndims == 2 && table.shapes[0] == lens.shapes[0] && (table.shapes[1] > 0 || lens.shapes[0] == 0),
+                "%s: block_table must be [B=%lld, max_blocks]", prog, (long long)numel(lens));
+  return PTO_HIP_OK;
+}
+// Four positive scalars num_heads, kv_head_num, head_dim, block_size, none so large that a product of them with a tensor's size overflows.
+int check_heads(const char* prog, const uint64_t* s) {
+  for (int i = 0; i < 4; ++i) PTO_CHECK_ARG(s[i] > 0 && s[i] < 1ull << 20, "%s: scalar %d must be in [1, 2^20), got %lld", prog, i, (long long)s[i]);
+  return PTO_HIP_OK;
+}
+// Caches of equal shape, whole blocks [pool * Hkv * bs, D]; with scales FP8E4M3FN ones.
+int check_caches(const char* prog, const PtoHipChipTensor& kc, const PtoHipChipTensor& vc, const PtoHipChipTensor* ks, const PtoHipChipTensor* vs,
+                 int dtype, int64_t hkv, int64_t bs, int64_t d, int64_t* pool) {
+  PTO_CHECK_ARG(kc.dtype == vc.dtype && numel(kc) == numel(vc) && numel(kc) > 0 && numel(kc) % (hkv * bs * d) == 0,
+                "%s: key/value cache must be equal-shaped [pool*Hkv*bs, D]", prog);
+  *pool = numel(kc) / (hkv * bs * d);
+  if (!ks) {
+    PTO_CHECK_ARG((int)kc.dtype == dtype, "%s: caches of %s beside queries of %s (FP8E4M3FN ones come with scales)", prog, dtype_name(kc.dtype),
+                  dtype_name(dtype));
+    return PTO_HIP_OK;
+  }
+  PTO_CHECK_ARG(kc.dtype == PTO_HIP_FP8E4M3FN, "%s: caches with scales must be FP8E4M3FN, got %s", prog, dtype_name(kc.dtype));
+  PTO_CHECK_ARG(ks->dtype == PTO_HIP_FP32 && vs->dtype == PTO_HIP_FP32 && numel(*ks) == *pool * hkv && numel(*vs) == *pool * hkv,
+                "%s: k_scale/v_scale must be FP32 [pool_blocks, Hkv]", prog);
+  return PTO_HIP_OK;
+}
+
+int run_rope_append(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hipStream_t stream, bool fp8) {
+  const char* prog = fp8 ? "rope_append_tokens_fp8" : "rope_append_tokens";
+  const int plain = fp8 ? 12 : 10;
+  const bool normed = nt == plain + 2;
+  PTO_CHECK_ARG((nt == plain || normed) && ns == (normed ? 5 : 4),
+                "%s: expected qkv, positions, token_starts, context_lens, rope_cos, rope_sin, [gamma_q, gamma_k,] block_table, key_cache, value_cache, "
+                "%sq_out + scalars num_heads, kv_head_num, head_dim, block_size [, eps]; got %d + %d", prog, fp8 ? "k_scale, v_scale, " : "", nt, ns);
+  static const char* const names[14] = {"qkv", "positions", "token_starts", "context_lens", "rope_cos", "rope_sin", "gamma_q", "gamma_k",
+                                        "block_table", "key_cache", "value_cache", "k_scale", "v_scale", "q_out"};
+  const PtoHipChipTensor* at[14];
+  for (int i = 0, from = 0; i < 14; ++i) {
+    const bool there = i == 6 || i == 7 ? normed : i == 11 || i == 12 ? fp8 : true;
+    at[i] = there ? &t[from++] : nullptr;
+    if (!there) continue;
+    const int rc = check_tensor(prog, names[i], *at[i], 1, 2, dtype_bytes(at[i]->dtype) ? dtype_bytes(at[i]->dtype) : 1);
+    if (rc) return rc;
+  }
+  int rc = check_heads(prog, s);
+  if (!rc) rc = check_ragged(prog, *at[2], *at[3], *at[8]);
+  if (rc) return rc;
+  const int64_t hq = (int64_t)s[0], hkv = (int64_t)s[1], d = (int64_t)s[2], bs = (int64_t)s[3];
+  const PtoHipChipTensor &qkv = *at[0], &cos = *at[4], &sin = *at[5], &q_out = *at[13];
+  PTO_CHECK_ARG(qkv.ndims == 2 && qkv.shapes[1] == (hq + 2 * hkv) * d, "%s: qkv must be [T, (Hq+2Hkv)*D=%lld]", prog, (long long)((hq + 2 * hkv) * d));
+  const int64_t tokens = qkv.shapes[0];
+  PTO_CHECK_ARG(at[1]->dtype == PTO_HIP_INT32 && numel(*at[1]) == tokens, "%s: positions must be INT32 [T=%lld]", prog, (long long)tokens);
+  PTO_CHECK_ARG(cos.dtype == PTO_HIP_FP32 && sin.dtype == PTO_HIP_FP32 && cos.ndims == 2 && sin.ndims == 2 && cos.shapes[0] == sin.shapes[0] &&
+                    cos.shapes[1] == sin.shapes[1],
+                "%s: rope_cos and rope_sin must be FP32 [max_pos, width] alike", prog);
+  PTO_CHECK_ARG(cos.shapes[0] > 0 && cos.shapes[1] > 0, "%s: empty rope tables", prog);
+  if (normed)
+    PTO_CHECK_ARG(at[6]->dtype == PTO_HIP_FP32 && at[7]->dtype == PTO_HIP_FP32 && numel(*at[6]) == d && numel(*at[7]) == d,
+                  "%s: gamma_q and gamma_k must be FP32 with %lld elements", prog, (long long)d);
+  PTO_CHECK_ARG((q_out.dtype == PTO_HIP_BF16 || q_out.dtype == PTO_HIP_FP16) && numel(q_out) == tokens * hq * d,
+                "%s: q_out must be BF16 or FP16 [T*Hq, D]", prog);
+  int64_t pool = 0;
+  rc = check_caches(prog, *at[9], *at[10], at[11], at[12], (int)q_out.dtype, hkv, bs, d, &pool);
+  if (rc) return rc;
+  auto f32 = [&](int i) { return at[i] ? reinterpret_cast<float*>(tptr_mut(*at[i])) : nullptr; };
+  auto i32 = [&](int i) { return reinterpret_cast<const int32_t*>(tptr(*at[i])); };
+  PtoHipRopeAppendArgs a{};
+  a.qkv = tptr(qkv);
+  a.positions = i32(1);
+  a.token_starts = i32(2);
+  a.context_lens = i32(3);
+  a.rope_cos = f32(4);
+  a.rope_sin = f32(5);
+  a.gamma_q = f32(6);
+  a.gamma_k = f32(7);
+  a.block_table = i32(8);
+  a.key_cache = tptr_mut(*at[9]);
+  a.value_cache = tptr_mut(*at[10]);
+  a.k_scale = f32(11);
+  a.v_scale = f32(12);
+  a.q_out = tptr_mut(q_out);
+  a.tokens = tokens;
+  a.batch = numel(*at[3]);
+  a.num_heads = hq;
+  a.kv_head_num = hkv;
+  a.head_dim = d;
+  a.block_size = bs;
+  a.max_num_blocks_per_req = std::max<int64_t>(1, at[8]->shapes[1]);
+  a.max_pos = cos.shapes[0];
+  a.pool_blocks = pool;
+  a.eps = normed ? scalar_f32(s[4]) : 0.f;
+  a.qkv_dtype = (int32_t)qkv.dtype;
+  a.dtype = (int32_t)q_out.dtype;
+  a.kv_dtype = fp8 ? PTO_HIP_FP8E4M3FN : 0;
+  PTO_CHECK_ARG(cos.shapes[1] <= (uint32_t)d, "%s: rope tables of width %u for a head_dim of %lld", prog, cos.shapes[1], (long long)d);
+  a.rope_table_width = (int32_t)cos.shapes[1];
+  return pto_hip_rope_append_tokens(&a, stream);
+}
+
+// query, key_cache, value_cache, block_table, context_lens, token_starts, tree_mask, out [, k_scale, v_scale]
+int run_tree_attention(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hipStream_t stream) {
+  const char* prog = "tree_attention";
+  PTO_CHECK_ARG((nt == 8 || nt == 10) && ns == 5,
+                "%s: expected query, key_cache, value_cache, block_table, context_lens, token_starts, tree_mask, out [, k_scale, v_scale] + scalars "
+                "num_heads, kv_head_num, head_dim, block_size, scale; got %d + %d", prog, nt, ns);
+  static const char* const names[10] = {"query", "key_cache", "value_cache", "block_table", "context_lens", "token_starts", "tree_mask", "out",
+                                        "k_scale", "v_scale"};
+  for (int i = 0; i < nt; ++i) {
+    const int rc = check_tensor(prog, names[i], t[i], 1, 2, t[i].dtype == PTO_HIP_FP32 ? 4 : 0);
+    if (rc) return rc;
+  }
+  const bool fp8 = nt == 10;
+  int rc = check_heads(prog, s);
+  if (!rc) rc = check_ragged(prog, t[5], t[4], t[3]);
+  if (rc) return rc;
+  const int64_t hq = (int64_t)s[0], hkv = (int64_t)s[1], d = (int64_t)s[2], bs = (int64_t)s[3];
+  const PtoHipChipTensor &q = t[0], &mask = t[6], &out = t[7];
+  PTO_CHECK_ARG(numel(q) % (hq * d) == 0 && numel(out) == numel(q) && out.dtype == q.dtype, "%s: query and out must be [T*Hq, D] of one dtype", prog);
+  const int64_t tokens = numel(q) / (hq * d);
+  PTO_CHECK_ARG(mask.dtype == PTO_HIP_INT32 && mask.ndims == 2 && mask.shapes[0] == tokens && mask.shapes[1] > 0,
+                "%s: tree_mask must be INT32 [T=%lld, words]", prog, (long long)tokens);
+  int64_t pool = 0;
+  rc = check_caches(prog, t[1], t[2], fp8 ? &t[8] : nullptr, fp8 ? &t[9] : nullptr, (int)q.dtype, hkv, bs, d, &pool);
+  if (rc) return rc;
+  auto i32 = [&](int i) { return reinterpret_cast<const int32_t*>(tptr(t[i])); };
+  PtoHipTreeAttentionArgs a{};
+  a.query = tptr(q);
+  a.key_cache = tptr(t[1]);
+  a.value_cache = tptr(t[2]);
+  a.k_scale = fp8 ? reinterpret_cast<const float*>(tptr(t[8])) : nullptr;
+  a.v_scale = fp8 ? reinterpret_cast<const float*>(tptr(t[9])) : nullptr;
+  a.block_table = i32(3);
+  a.context_lens = i32(4);
+  a.token_starts = i32(5);
+  a.tree_mask = i32(6);
+  a.out = tptr_mut(out);
+  a.tokens = tokens;
+  a.batch = numel(t[4]);
+  a.num_heads = hq;
+  a.kv_head_num = hkv;
+  a.head_dim = d;
+  a.block_size = bs;
+  a.max_num_blocks_per_req = std::max<int64_t>(1, t[3].shapes[1]);
+  a.pool_blocks = pool;
+  a.mask_words = mask.shapes[1];
+  a.scale = scalar_f32(s[4]);
+  a.dtype = (int32_t)q.dtype;
+  a.kv_dtype = fp8 ? PTO_HIP_FP8E4M3FN : 0;
+  return pto_hip_tree_attention(&a, stream);
+}
+
+// logits, temperature, top_k, top_p, min_p, uniform, tokens, probs
+int run_sample_tokens(const PtoHipChipTensor* t, int nt, const uint64_t*, int ns, hipStream_t stream) {
+  const char* prog = "sample_tokens";
+  PTO_CHECK_ARG(nt == 8 && ns == 0, "%s: expected logits, temperature, top_k, top_p, min_p, uniform, tokens, probs and no scalars, got %d + %d", prog, nt, ns);
+  static const char* const names[8] = {"logits", "temperature", "top_k", "top_p", "min_p", "uniform", "tokens", "probs"};
+  for (int i = 0; i < nt; ++i) {
+    const int rc = check_tensor(prog, names[i], t[i], i == 0 ? 2 : 1, 2, dtype_bytes(t[i].dtype) ? dtype_bytes(t[i].dtype) : 1);
+    if (rc) return rc;
+  }
+  const int64_t rows = t[0].shapes[0], vocab = t[0].shapes[1];
+  for (int i = 1; i < nt; ++i) {
+    const bool whole = i == 2 || i == 6;
+    PTO_CHECK_ARG(t[i].dtype == (whole ? PTO_HIP_INT32 : PTO_HIP_FP32) && numel(t[i]) == rows, "%s: %s must be %s with %lld elements", prog, names[i],
+                  whole ? "INT32" : "FP32", (long long)rows);
+  }
+  auto f32 = [&](int i) { return reinterpret_cast<float*>(tptr_mut(t[i])); };
+  return pto_hip_sample_tokens(tptr(t[0]), f32(1), reinterpret_cast<const int32_t*>(tptr(t[2])), f32(3), f32(4), f32(5),
+                               reinterpret_cast<int32_t*>(tptr_mut(t[6])), f32(7), rows, vocab, (int)t[0].dtype, stream);
+}
+
 int run_decoder_layer(const PtoHipChipTensor* t, int nt, const uint64_t* s, int ns, hipStream_t stream) {
   PTO_CHECK_ARG((nt == 20 || nt == 22 || nt == 15 || nt == 17) && ns == 5,
                 "decoder_layer_decode: expected 20 tensors with INT8 weights and their scales or 15 with 16-bit "
@@ -941,6 +1124,10 @@ int dispatch(int kind, const PtoHipChipTensor* t, int nt, const uint64_t* s, int
     case kProjectionFp8Block: return run_projection_fp8_block(t, nt, s, ns, stream);
     case kRouteExperts: return run_route_experts(t, nt, s, ns, stream);
     case kExpertsFfnFp8Block: return run_experts_ffn_fp8_block(t, nt, s, ns, stream);
+    case kRopeAppendTokens: return run_rope_append(t, nt, s, ns, stream, false);
+    case kRopeAppendTokensFp8: return run_rope_append(t, nt, s, ns, stream, true);
+    case kTreeAttention: return run_tree_attention(t, nt, s, ns, stream);
+    case kSampleTokens: return run_sample_tokens(t, nt, s, ns, stream);
     case kLlamaMini: return run_llama_mini(t, nt, s, ns, stream);
     case kW8a16Matmul: return run_w8a16_matmul(t, nt, s, ns, stream);
     case kProjection: return run_projection(t, nt, s, ns, stream);
@@ -1110,9 +1297,9 @@ int pto_hip_sync(void* stream) {
   PTO_DISPATCH_LOCK();
   if (!ctx().initialized) return fail(PTO_HIP_ERR_NOT_INITIALIZED, "the library was closed during the wait");
   // Device-side argument errors of launches that do not block are reported here.
-  int flags[4] = {0, 0, 0, 0};
+  int flags[6] = {0, 0, 0, 0, 0, 0};
   PTO_CHECK_HIP(hipMemcpy(flags, ctx().flags, sizeof(flags), hipMemcpyDeviceToHost));
-  if (flags[0] || flags[1] || flags[2] || flags[3]) {
+  if (flags[0] || flags[1] || flags[2] || flags[3] || flags[4] || flags[5]) {
     PTO_CHECK_HIP(hipMemset(ctx().flags, 0, sizeof(flags)));
     if (flags[0])
       return fail(PTO_HIP_ERR_INVALID_VALUE,
@@ -1121,6 +1308,12 @@ int pto_hip_sync(void* stream) {
       return fail(PTO_HIP_ERR_INVALID_VALUE,
                   "rope_kv_cache_update: a decode position lies outside the rope table, the block table or the cache");
     if (flags[3]) return fail(PTO_HIP_ERR_INVALID_VALUE, "experts_ffn_fp8_block: an expert id names an expert that there is not");
+    if (flags[4])
+      return fail(PTO_HIP_ERR_INVALID_VALUE,
+                  "rope_append_tokens: a position lies outside the rope tables, or a token's index outside the block table or the cache");
+    if (flags[5])
+      return fail(PTO_HIP_ERR_INVALID_VALUE,
+                  "tree_attention: a sequence has more tokens than its mask has bits or its block table room, or a block outside the cache");
     return fail(PTO_HIP_ERR_INVALID_VALUE,
                 "paged_attention: a block_table entry a sequence uses addresses a block outside the cache");
   }

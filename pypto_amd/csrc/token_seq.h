@@ -1,0 +1,53 @@
+// Ragged batches: which sequence a token belongs to, from the rising list of the sequences' first tokens.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace pto_hip {
+
+// The device that a call's pointers belong to is the library's; the caller's current one may be another, and is again afterwards.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    if (hipGetDevice(&before_) != hipSuccess || before_ == device) return;
+    changed_ = hipSetDevice(device) == hipSuccess;
+  }
+  ~DeviceScope() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+struct TokenSeq {
+  int seq;    // -1: the token belongs to nobody
+  int first;  // the sequence's first token
+  int count;  // and how many it has
+};
+
+// The last sequence that starts at `token` or in front of it, looked for by a whole wavefront: 64 starts a step, so that 64 sequences take one
+// trip to memory and 4096 two.  starts[0 .. batch]; whatever they hold, no other element is read and the answer lies in the batch.
+__device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch, int token, int lane) {
+  int lo = 0, n = batch;
+  while (n > 64) {
+    const int step = (n + 63) / 64;
+    const int at = lo + lane * step;
+    const uint64_t in_front = __ballot(lane * step < n && starts[min(at, batch)] <= token);
+    const int k = max((int)__popcll(in_front) - 1, 0);  // below the number of lanes that voted: lo stays in the batch
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  const int at = min(lo + lane, batch);
+  const int start = starts[at], next = starts[min(at + 1, batch)];
+  const int k = max((int)__popcll(__ballot(lane < n && start <= token)) - 1, 0);
+  const int first = __shfl(start, k), end = __shfl(next, k);
+  return TokenSeq{first <= token && token < end ? lo + k : -1, first, end - first};
+}
+
+}  // namespace pto_hip

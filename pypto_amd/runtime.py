@@ -98,6 +98,22 @@ route_experts_biased = HipProgram("route_experts", (IN, IN, OUT, OUT),
 # x8, x_scale, expert_ids, expert_weights, then (codes [E, out, in], scales [E, out/128, in/128]) for gate, up and down
 experts_ffn_fp8_block = HipProgram("experts_ffn_fp8_block", (IN,) * 10 + (OUT,))
 
+# a step that verifies drafted tokens, several new ones per sequence: qkv, positions, token_starts, context_lens, rope_cos, rope_sin,
+# [gamma_q, gamma_k,] block_table, key_cache, value_cache, [k_scale, v_scale,] q_out
+rope_append_tokens = HipProgram("rope_append_tokens", (IN,) * 7 + (INOUT, INOUT, OUT),
+                                scalars=("num_heads", "kv_head_num", "head_dim", "block_size"))
+rope_append_tokens_normed = HipProgram("rope_append_tokens", (IN,) * 9 + (INOUT, INOUT, OUT),
+                                       scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "eps"))
+rope_append_tokens_fp8 = HipProgram("rope_append_tokens_fp8", (IN,) * 7 + (INOUT,) * 4 + (OUT,),
+                                    scalars=("num_heads", "kv_head_num", "head_dim", "block_size"))
+rope_append_tokens_fp8_normed = HipProgram("rope_append_tokens_fp8", (IN,) * 9 + (INOUT,) * 4 + (OUT,),
+                                           scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "eps"))
+# query, key_cache, value_cache, block_table, context_lens, token_starts, tree_mask, out [, k_scale, v_scale]
+tree_attention = HipProgram("tree_attention", (IN,) * 7 + (OUT, IN, IN), optional=2,
+                            scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "scale"))
+# logits, temperature, top_k, top_p, min_p, uniform, tokens, probs
+sample_tokens = HipProgram("sample_tokens", (IN,) * 6 + (OUT, OUT))
+
 # the reference's minimal single-head LLaMA forward: hidden, causal_mask, cos, sin, 7 x [D,D], w_lm, logits
 llama_mini = HipProgram("llama_mini", (IN,) * 12 + (OUT,))
 
@@ -133,7 +149,8 @@ decoder_layer_decode_w16_fp8kv = HipProgram(
 PROGRAMS = {p.name: p for p in (paged_attention, paged_attention_batch, paged_attention_dynamic, paged_attention_spmd,
                                 paged_gather, rms_norm, ffn_swiglu, ffn_gelu, ffn_relu, ffn_block, ffn_block_fp8,
                                 rms_norm_fp8_block, quantize_fp8_block, projection_fp8_block, route_experts,
-                                experts_ffn_fp8_block, llama_mini,
+                                experts_ffn_fp8_block, rope_append_tokens, rope_append_tokens_fp8, tree_attention, sample_tokens,
+                                llama_mini,
                                 projection, gate_up_swiglu,
                                 w8a16_matmul,
                                 w8a16_swiglu, rope_kv_cache_update, rope_kv_cache_update_fp8,
