@@ -50,6 +50,7 @@ FLAGS = [
 # the GEMM keeps the default AGPR form.
 EXTRA_FLAGS = {
     "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "tree_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "block_gemm8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "experts.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
