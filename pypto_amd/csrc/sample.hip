@@ -4,9 +4,15 @@
 //   kept: the first top_k; of those the fewest from the front whose sum reaches top_p of all of theirs; of those the w_i >= min_p
 //   token: the first index at which the running sum of the kept w, in the order of indices, passes u times their sum
 //
-// The kept tokens are what lies in front of a border (key, number of tokens of that key), and a filter only moves the border forward; min_p asks each
-// weight by itself.  Weights are integers, w in units of 2^-44: their sums are exact in any order, so that a row's token does not depend on how
+// The kept tokens are what lies in front of a border in that order, and a filter only moves the border forward; min_p asks each weight by itself.
+// Weights are integers, w in units of 2^-44: their sums are exact in any order, so that a row's token does not depend on how
 // the work is split, and next to a border or the random number the decision is that of the definition in 64 bits up to 2^-45 a token.
+//
+// Four kernels, the first three over slices of the rows so that few rows fill the chip too: the largest logit; of rows with top_k or top_p, how many
+// tokens and how much weight lie in each of 1472 intervals of 2^(1/32) below it; the sum of what each slice surely keeps, and the tokens of the border's
+// interval; and, a workgroup a row, those tokens in order, the border among them, the slice in which the random number falls and the token in it.
+// Where more tokens share the border's interval than are collected (thousands of nearly equal logits), the last kernel looks for the border in the row
+// itself, eleven bits of the key a pass.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,7 +27,6 @@ constexpr int kMaxVocab = 1 << 19;  // sums of 2^19 weights of 2^44 stay below 2
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kTiles = kMaxVocab / kThreads;
 constexpr int kUnit = 44;  // a weight of 1 is 2^44
 constexpr uint64_t kOne = 1ull << kUnit;
 
@@ -45,39 +50,47 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
-// 2^-y for y >= 0, to 2^-50 or better of it: the fraction's power is its series in ln 2 times it.
-__device__ __forceinline__ double power_of_two(double y) {
-  const double n = rint(y);
-  const double f = (n - y) * 0.69314718055994530942;  // [-0.35, 0.35]
-  double s = 1.0 / 6227020800.0;
-  s = fma(s, f, 1.0 / 479001600.0);
-  s = fma(s, f, 1.0 / 39916800.0);
-  s = fma(s, f, 1.0 / 3628800.0);
-  s = fma(s, f, 1.0 / 362880.0);
-  s = fma(s, f, 1.0 / 40320.0);
-  s = fma(s, f, 1.0 / 5040.0);
-  s = fma(s, f, 1.0 / 720.0);
-  s = fma(s, f, 1.0 / 120.0);
-  s = fma(s, f, 1.0 / 24.0);
-  s = fma(s, f, 1.0 / 6.0);
-  s = fma(s, f, 0.5);
-  s = fma(s, f, 1.0);
-  s = fma(s, f, 1.0);
-  return ldexp(s, -(int)n);
+// 2^(-i / 64), kept in LDS by every workgroup.
+struct Powers {
+  double of[64];
+};
+__device__ __forceinline__ void fill(Powers& t) {  // and a barrier
+  if (threadIdx.x < 64) t.of[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0);
 }
+constexpr int kSteps = 46 * 64;          // weights end behind 45 of the 64ths of a power of two
+constexpr int kIntervals = kSteps / 2;
+
+// What a logit of a row weighs.  With z = 64 log2(best's weight / its own): z's whole part is a place in the table, the rest, below 1/64, five terms of
+// the exponential's series (off by 3e-15 of it).
 struct Weights {
-  float best;   // the largest logit
-  double rate;  // log2(e) / T
-  __device__ __forceinline__ double exponent(float v) const { return ((double)best - (double)v) * rate; }
-  // in units of 2^-44, rounded to the nearest
-  __device__ __forceinline__ uint64_t operator()(float v) const {
-    if (v == best) return kOne;
-    const double y = exponent(v);
-    if (!(y < kUnit + 1.0)) return 0;
-    const double big = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number
-    return __builtin_bit_cast(uint64_t, power_of_two(y) * (double)kOne + big) - __builtin_bit_cast(uint64_t, big);
+  float best;     // the largest logit
+  double rate;    // 64 log2(e) / T
+  const Powers* powers;
+  __device__ __forceinline__ double steps(float v) const { return v == best ? 0.0 : ((double)best - (double)v) * rate; }
+  __device__ __forceinline__ double series(double z, int whole) const {
+    const double f = (z - (double)whole) * (-0.69314718055994530942 / 64.0);
+    double s = 1.0 / 120.0;
+    s = fma(s, f, 1.0 / 24.0);
+    s = fma(s, f, 1.0 / 6.0);
+    s = fma(s, f, 0.5);
+    s = fma(s, f, 1.0);
+    s = fma(s, f, 1.0);
+    return s * powers->of[whole & 63];
   }
-  __device__ __forceinline__ double exact(float v) const { return v == best ? 1.0 : power_of_two(fmin(exponent(v), 1000.0)); }
+  // in units of 2^-44, rounded to the nearest; z in [0, kSteps)
+  __device__ __forceinline__ uint64_t at(double z) const {
+    const int whole = (int)z;
+    const double big = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number
+    return __builtin_bit_cast(uint64_t, ldexp(series(z, whole), kUnit - (whole >> 6)) + big) - __builtin_bit_cast(uint64_t, big);
+  }
+  __device__ __forceinline__ uint64_t operator()(float v) const {
+    const double z = steps(v);
+    return z < (double)kSteps ? at(z) : 0;  // NaN: nothing
+  }
+  __device__ __forceinline__ double exact(float v) const {
+    const double z = fmin(steps(v), 64000.0);
+    return ldexp(series(z, (int)z), -((int)z >> 6));
+  }
 };
 
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
@@ -125,8 +138,6 @@ struct Border {
 struct Shared {
   unsigned int count[kBins];
   unsigned long long weight[kBins];
-  unsigned long long tile_weight[kTiles];
-  unsigned int tile_ties[kTiles];
   unsigned long long waves[kWaves];
   unsigned long long found[4];
 };
@@ -154,7 +165,7 @@ __device__ bool find_border(Shared& sh, const T* row, int vocab, const Weights& 
       if (key < lo || key > hi) continue;
       const int bin = (hi - key) >> shift;
       atomicAdd(&sh.count[bin], 1u);
-      const uint64_t x = w(value_of(key));
+      const uint64_t x = w(v);
       if (x) atomicAdd(&sh.weight[bin], (unsigned long long)x);
     }
     __syncthreads();
@@ -193,23 +204,348 @@ __device__ bool find_border(Shared& sh, const T* row, int vocab, const Weights& 
   }
 }
 
+// A row's filters.
+struct Filters {
+  int k;        // 0: none
+  bool by_sum;  // top_p
+  double p;
+  uint64_t least;  // a chosen token's weight
+  __device__ __forceinline__ bool any() const { return k > 0 || by_sum; }
+};
+__device__ __forceinline__ Filters filters_of(const Params& p, int r) {
+  Filters f;
+  const int k = p.top_k ? p.top_k[r] : 0;
+  const float top_p = p.top_p ? p.top_p[r] : 1.f, min_p = p.min_p ? p.min_p[r] : 0.f;
+  f.k = k > 0 && k < p.vocab ? k : 0;
+  f.by_sum = top_p < 1.f;
+  f.p = fmax((double)top_p, 0.0);
+  f.least = min_p > 0.f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;  // weights of nothing are never chosen
+  return f;
+}
+__device__ __forceinline__ uint64_t needed(const Filters& f, uint64_t sum) { return max((uint64_t)ceil(f.p * (double)sum), (uint64_t)1); }
+
+// A token's place in the order, larger ones in front: its key, then its index.
+__device__ __forceinline__ uint64_t packed(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
+
+// The place of the last token that a row's filters keep, from the row alone (all threads of a workgroup of kThreads).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_kernel(Params p) {
-  __shared__ Shared sh;
-  const int r = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int vocab = p.vocab;
-  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * vocab;
-  // the best token: the largest key, of equal ones the lowest index
-  uint64_t best = 0;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const uint64_t k = (uint64_t)ordered(logit(row, i)) << 32 | (uint32_t)~i;
-    best = k > best ? k : best;
+__device__ __noinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, const Weights& w, const Filters& f) {
+  const uint32_t top = ordered(w.best);
+  Border border{kNone, 0};
+  uint64_t total = 0;
+  bool bounded = false;
+  if (f.k) bounded = find_border(sh, row, vocab, w, false, (uint64_t)f.k, kNone + 1, top, &border, &total);
+  if (f.by_sum) {
+    if (!bounded) {
+      for (int i = threadIdx.x; i < vocab; i += kThreads) total += w(logit(row, i));
+      unsigned long long all;
+      sum_in_front<unsigned long long>(total, sh.waves, &all);
+      total = all;
+    }
+    Border nearer;
+    uint64_t unused;
+    if (find_border(sh, row, vocab, w, true, needed(f, total), bounded ? border.key : kNone + 1, top, &nearer, &unused)) {
+      border = nearer;
+      bounded = true;
+    }
   }
+  if (!bounded) return (uint64_t)(kNone + 1) << 32;
+  // the index of the last of its ties
+  uint64_t before = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.found[0] = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < vocab && before < border.ties; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    const bool tie = i < vocab && ordered(logit(row, i)) == border.key;
+    unsigned long long all;
+    const uint64_t number = before + sum_in_front<unsigned long long>(tie, sh.waves, &all);
+    if (tie && number + 1 == border.ties) sh.found[0] = (uint32_t)~i;
+    before += all;
+  }
+  __syncthreads();
+  return (uint64_t)border.key << 32 | sh.found[0];
+}
+
+// ---- slices ----
+constexpr int kSliceThreads = 256;
+constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
+constexpr int kMaxSlice = 16384;
+constexpr int kCollected = 4096;
+
+// What the kernels leave for each other, a row of each a row.
+struct Scratch {
+  unsigned long long* best;    // [slices] places of the slices' largest logits
+  unsigned long long* weight;  // [kIntervals]
+  unsigned int* count;         // [kIntervals]
+  unsigned int* collected;     // [1] tokens of the border's intervals
+  unsigned long long* tokens;  // [kCollected] their places
+  unsigned long long* sums;    // [slices] weights surely kept
+  unsigned long long* front;   // [3] tokens and weights in front of the border's intervals, weights of all
+  int slices, slice;           // elements of a slice, a multiple of kStep
+};
+
+// Eight elements from i on, -inf behind the end.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8]) {
+  if constexpr (WIDE) {
+    if (i + 8 <= end) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(row + i)[0], b = reinterpret_cast<const float4*>(row + i)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        typedef T T8 __attribute__((ext_vector_type(8)));
+        const T8 a = *reinterpret_cast<const T8*>(row + i);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = (float)a[u];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : -INFINITY;
+}
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
+  __shared__ unsigned long long waves[kSliceThreads / 64];
+  const int slice = blockIdx.x, r = blockIdx.y;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  uint64_t best = 0;
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    float v[8];
+    load8<T, WIDE>(row, i, end, v);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint64_t k = packed(v[u], i + u);
+      best = k > best ? k : best;
+    }
+  }
+  // the histogram of the next kernel starts from nothing
+  const int per = (kIntervals + s.slices - 1) / s.slices;
+  for (int i = slice * per + threadIdx.x; i < min(kIntervals, (slice + 1) * per); i += kSliceThreads) {
+    s.weight[(size_t)r * kIntervals + i] = 0;
+    s.count[(size_t)r * kIntervals + i] = 0;
+  }
+  if (slice == 0 && threadIdx.x == 0) s.collected[r] = 0;
   best = wave_max(best);
-  if (lane == 0) sh.waves[wave] = best;
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = best;
   __syncthreads();
-  for (int i = 0; i < kWaves; ++i) best = sh.waves[i] > best ? sh.waves[i] : best;
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kSliceThreads / 64; ++w) best = waves[w] > best ? waves[w] : best;
+    s.best[(size_t)r * s.slices + slice] = best;
+  }
+}
+
+// The place of a row's largest logit, by every wavefront for itself.
+__device__ __forceinline__ uint64_t best_of_row(const Scratch& s, int r) {
+  uint64_t best = 0;
+  for (int i = threadIdx.x % 64; i < s.slices; i += 64) {
+    const uint64_t b = s.best[(size_t)r * s.slices + i];
+    best = b > best ? b : best;
+  }
+  return wave_max(best);
+}
+__device__ __forceinline__ Weights weights_of(uint64_t best, float temperature, const Powers* powers) {
+  return Weights{value_of((uint32_t)(best >> 32)), 64.0 * 1.4426950408889634074 / (double)temperature, powers};
+}
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scratch s) {
+  __shared__ Powers powers;
+  __shared__ unsigned long long weight[kIntervals];
+  __shared__ unsigned int count[kIntervals];
+  const int slice = blockIdx.x, r = blockIdx.y;
+  const Filters f = filters_of(p, r);
+  const float t = p.temperature[r];
+  if (!(t > 0.f) || !f.any()) return;
+  const uint64_t best = best_of_row(s, r);
+  if ((uint32_t)(best >> 32) <= kNone) return;
+  fill(powers);
+  for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads) {
+    weight[i] = 0;
+    count[i] = 0;
+  }
   __syncthreads();
+  const Weights w = weights_of(best, t, &powers);
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    float v[8];
+    load8<T, WIDE>(row, i0 + threadIdx.x * 8, end, v);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const double z = w.steps(v[u]);
+      if (z < (double)kSteps) {
+        const int at = (int)z >> 1;
+        atomicAdd(&count[at], 1u);
+        if (f.by_sum) atomicAdd(&weight[at], (unsigned long long)w.at(z));
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads)
+    if (count[i]) {
+      atomicAdd(&s.count[(size_t)r * kIntervals + i], count[i]);
+      if (f.by_sum) atomicAdd(&s.weight[(size_t)r * kIntervals + i], weight[i]);
+    }
+}
+
+// The intervals in which a row's border may lie: first and last, and what lies in front of the first.
+struct BorderIntervals {
+  int first, last;
+  uint64_t tokens_front, weight_front, weight_all;
+};
+// Each thread holds the sums of its kIntervals / kSliceThreads intervals.
+__device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int r, const Filters& f) {
+  constexpr int kOwn = (kIntervals + kSliceThreads - 1) / kSliceThreads;
+  __shared__ unsigned long long wave_n[kSliceThreads / 64], wave_w[kSliceThreads / 64];
+  __shared__ unsigned long long found[8];
+  uint64_t n[kOwn], x[kOwn], n_own = 0, x_own = 0;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int at = threadIdx.x * kOwn + i;
+    n[i] = at < kIntervals ? s.count[(size_t)r * kIntervals + at] : 0;
+    x[i] = at < kIntervals && f.by_sum ? s.weight[(size_t)r * kIntervals + at] : 0;
+    n_own += n[i];
+    x_own += x[i];
+  }
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  uint64_t n_to = n_own, x_to = x_own;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t a = __shfl_up((unsigned long long)n_to, off), b = __shfl_up((unsigned long long)x_to, off);
+    if (lane >= off) {
+      n_to += a;
+      x_to += b;
+    }
+  }
+  if (lane == 63) {
+    wave_n[wave] = n_to;
+    wave_w[wave] = x_to;
+  }
+  if (threadIdx.x < 8) found[threadIdx.x] = kIntervals;
+  __syncthreads();
+  uint64_t all = 0, n_front = n_to - n_own, x_front = x_to - x_own;
+  for (int i = 0; i < kSliceThreads / 64; ++i) {
+    if (i < wave) {
+      n_front += wave_n[i];
+      x_front += wave_w[i];
+    }
+    all += wave_w[i];
+  }
+  // of top_k: found[0] its interval, the weights in front of it and up to its end in [1] and [2], the tokens in front in [3]
+  if (f.k) {
+    uint64_t a = n_front, b = x_front;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (a < (uint64_t)f.k && a + n[i] >= (uint64_t)f.k) {
+        found[0] = threadIdx.x * kOwn + i;
+        found[1] = b;
+        found[2] = b + x[i];
+        found[3] = a;
+      }
+      a += n[i];
+      b += x[i];
+    }
+    __syncthreads();
+  }
+  const int k_at = (int)found[0];
+  BorderIntervals out{k_at, k_at, k_at < kIntervals ? found[3] : 0, k_at < kIntervals ? found[1] : 0, all};
+  if (f.by_sum) {
+    // the weights of what top_k keeps lie between those in front of its interval and those up to its end
+    const uint64_t lo = needed(f, k_at < kIntervals ? found[1] : all), hi = needed(f, k_at < kIntervals ? found[2] : all);
+    uint64_t a = n_front, b = x_front;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (b < lo && b + x[i] >= lo) {
+        found[4] = threadIdx.x * kOwn + i;
+        found[5] = a;
+        found[6] = b;
+      }
+      if (b < hi && b + x[i] >= hi) found[7] = threadIdx.x * kOwn + i;
+      a += n[i];
+      b += x[i];
+    }
+    __syncthreads();
+    out.first = (int)found[4];
+    out.tokens_front = found[5];
+    out.weight_front = found[6];
+    out.last = k_at < kIntervals ? k_at : (int)found[7];
+  }
+  return out;
+}
+
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratch s) {
+  __shared__ Powers powers;
+  __shared__ unsigned long long waves[kSliceThreads / 64];
+  const int slice = blockIdx.x, r = blockIdx.y;
+  const float t = p.temperature[r];
+  if (!(t > 0.f)) return;
+  const Filters f = filters_of(p, r);
+  const uint64_t best = best_of_row(s, r);
+  if ((uint32_t)(best >> 32) <= kNone) return;
+  fill(powers);
+  BorderIntervals at{kIntervals, kIntervals, 0, 0, 0};
+  if (f.any()) at = find_intervals(s, r, f);
+  if (slice == 0 && threadIdx.x == 0) {
+    s.front[3 * (size_t)r] = at.tokens_front;
+    s.front[3 * (size_t)r + 1] = at.weight_front;
+    s.front[3 * (size_t)r + 2] = at.weight_all;
+  }
+  __syncthreads();
+  const Weights w = weights_of(best, t, &powers);
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  const double z_first = 2.0 * at.first, z_behind = min(2.0 * (at.last + 1), (double)kSteps);
+  uint64_t sum = 0;
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    float v[8];
+    load8<T, WIDE>(row, i, end, v);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const double z = w.steps(v[u]);
+      if (z < z_first) {
+        const uint64_t x = w.at(z);
+        sum += x >= f.least ? x : 0;
+      } else if (z < z_behind) {
+        const unsigned int n = atomicAdd(&s.collected[r], 1u);
+        if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v[u], i + u);
+      }
+    }
+  }
+  sum = wave_sum((unsigned long long)sum);
+  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kSliceThreads / 64; ++i) sum += waves[i];
+    s.sums[(size_t)r * s.slices + slice] = sum;
+  }
+}
+
+struct DrawShared {
+  Powers powers;
+  unsigned long long tokens[kCollected];
+  unsigned long long sums[kMaxVocab / kStep];
+  union {
+    Shared row;
+    struct {
+      unsigned long long waves[kWaves];
+      unsigned long long found[4];
+    } draw;
+  };
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
+  __shared__ DrawShared sh;
+  const int r = blockIdx.x;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const uint64_t best = best_of_row(s, r);
   const uint32_t top = (uint32_t)(best >> 32);
   const float t = p.temperature[r];
   if (top <= kNone || !(t > 0.f)) {  // nothing to choose from, or no choice
@@ -219,92 +555,165 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(Params p) {
     }
     return;
   }
-  const Weights w{value_of(top), 1.4426950408889634074 / (double)t};
-  Border border{kNone, 0};
-  uint64_t total = 0;
-  bool bounded = false;
-  const int k = p.top_k ? p.top_k[r] : 0;
-  if (k > 0 && k < vocab) bounded = find_border(sh, row, vocab, w, false, (uint64_t)k, kNone + 1, top, &border, &total);
-  const float top_p = p.top_p ? p.top_p[r] : 1.f;
-  if (top_p < 1.f) {
-    if (!bounded) {
-      for (int i = threadIdx.x; i < vocab; i += kThreads) total += w(value_of(ordered(logit(row, i))));
-      unsigned long long all;
-      sum_in_front<unsigned long long>(total, sh.waves, &all);
-      total = all;
+  const Filters f = filters_of(p, r);
+  fill(sh.powers);
+  const Weights w = weights_of(best, t, &sh.powers);
+  for (int i = threadIdx.x; i < s.slices; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.slices + i];
+  const int n = f.any() ? (int)min(s.collected[r], (unsigned int)kCollected + 1) : 0;
+  uint64_t border = (uint64_t)(kNone + 1) << 32;
+  __syncthreads();
+  if (n > kCollected) {
+    border = border_of_row(sh.row, row, p.vocab, w, f);
+    // the slices' sums lack what the border's intervals keep
+    for (int i = threadIdx.x; i < s.slices; i += kThreads) sh.sums[i] = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < p.vocab; i0 += kThreads) {
+      const int i = i0 + threadIdx.x;
+      const float v = i < p.vocab ? logit(row, i) : -INFINITY;
+      uint64_t x = i < p.vocab && packed(v, i) >= border ? w(v) : 0;
+      x = wave_sum((unsigned long long)(x >= f.least ? x : 0));
+      if (threadIdx.x % 64 == 0 && x) atomicAdd(&sh.sums[i0 / s.slice], (unsigned long long)x);  // a slice is a multiple of kThreads
     }
-    const uint64_t need = max((uint64_t)ceil(fmax((double)top_p, 0.0) * (double)total), (uint64_t)1);
-    Border nearer;
-    uint64_t unused;
-    if (find_border(sh, row, vocab, w, true, need, bounded ? border.key : kNone + 1, top, &nearer, &unused)) border = nearer;
-  }
-  const float min_p = p.min_p ? p.min_p[r] : 0.f;
-  const uint64_t least = min_p > 0.f ? (uint64_t)ceil(fmin((double)min_p, 1.0) * (double)kOne) : 1;  // weights of nothing are never chosen
-
-  // kept weights and ties of each 1024 tokens, in the order of indices
-  const int tiles = (vocab + kThreads - 1) / kThreads;
-  for (int i = threadIdx.x; i < tiles; i += kThreads) {
-    sh.tile_weight[i] = 0;
-    sh.tile_ties[i] = 0;
+  } else if (n > 0) {
+    // in order, the last places filled up with nothing
+    int size = 1;
+    while (size < n) size *= 2;
+    for (int i = threadIdx.x; i < size; i += kThreads) sh.tokens[i] = i < n ? s.tokens[(size_t)r * kCollected + i] : 0;
+    __syncthreads();
+    for (int span = 2; span <= size; span *= 2)
+      for (int gap = span / 2; gap > 0; gap /= 2) {
+        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+          const int a = 2 * i - (i & (gap - 1)), b = a + gap;
+          const uint64_t va = sh.tokens[a], vb = sh.tokens[b];
+          if ((va < vb) == ((a & span) == 0)) {
+            sh.tokens[a] = vb;
+            sh.tokens[b] = va;
+          }
+        }
+        __syncthreads();
+      }
+    const uint64_t n_front = s.front[3 * (size_t)r], w_front = s.front[3 * (size_t)r + 1];
+    constexpr int kOwn = kCollected / kThreads;
+    uint64_t x[kOwn], own = 0;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = threadIdx.x * kOwn + u;
+      x[u] = i < n ? w(value_of((uint32_t)(sh.tokens[i] >> 32))) : 0;
+      own += x[u];
+    }
+    unsigned long long all;
+    const uint64_t in_front = sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
+    const bool by_count = f.k > 0 && n_front + n >= (uint64_t)f.k;
+    int kept = by_count ? (int)(f.k - n_front) : n;  // of them
+    if (f.by_sum) {
+      // what the first `kept` weigh, then how many of them reach the share
+      if (threadIdx.x == 0) sh.draw.found[0] = all;
+      __syncthreads();
+      uint64_t to = in_front;
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) {
+        to += x[u];
+        if (threadIdx.x * kOwn + u + 1 == kept) sh.draw.found[0] = to;
+      }
+      __syncthreads();
+      const uint64_t need = needed(f, by_count ? w_front + sh.draw.found[0] : s.front[3 * (size_t)r + 2]);
+      if (threadIdx.x == 0) sh.draw.found[1] = kept;
+      __syncthreads();
+      uint64_t a = w_front + in_front;
+#pragma unroll
+      for (int u = 0; u < kOwn; ++u) {
+        if (a < need && a + x[u] >= need) sh.draw.found[1] = threadIdx.x * kOwn + u + 1;
+        a += x[u];
+      }
+      __syncthreads();
+      kept = min(kept, (int)sh.draw.found[1]);
+    }
+    border = sh.tokens[kept - 1];
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = threadIdx.x * kOwn + u;
+      if (i < kept && x[u] >= f.least) atomicAdd(&sh.sums[(int)~(uint32_t)sh.tokens[i] / s.slice], (unsigned long long)x[u]);
+    }
   }
   __syncthreads();
-  const uint64_t tie = w(value_of(border.key)), tie_weight = border.key > kNone && tie >= least ? tie : 0;
-  for (int i = 0; i < tiles; ++i) {
-    const int at = i * kThreads + threadIdx.x;
-    const uint32_t key = at < vocab ? ordered(logit(row, at)) : 0;
-    uint64_t x = key > border.key ? w(value_of(key)) : 0;
-    x = wave_sum((unsigned long long)(x >= least ? x : 0));
-    const int ties = __popcll(__ballot(key == border.key));
-    if (lane == 0 && x) atomicAdd(&sh.tile_weight[i], (unsigned long long)x);
-    if (lane == 0 && ties) atomicAdd(&sh.tile_ties[i], (unsigned)ties);
-  }
-  __syncthreads();
-  // the sum, and the tile in which the running sum passes its share
-  uint64_t ties_front = 0, front = 0;
+  // the slice in which the running sum passes its share
   if (threadIdx.x == 0) {
-    uint64_t ties = 0, sum = 0;
-    for (int i = 0; i < tiles; ++i) {
-      sum += sh.tile_weight[i] + (min((uint64_t)border.ties, ties + sh.tile_ties[i]) - min((uint64_t)border.ties, ties)) * tie_weight;
-      ties += sh.tile_ties[i];
-    }
+    uint64_t sum = 0, front = 0;
+    for (int i = 0; i < s.slices; ++i) sum += sh.sums[i];
     const double u = fmin(fmax((double)p.uniform[r], 0x1p-25), 1.0 - 0x1p-24);
     const uint64_t target = (uint64_t)(u * (double)sum);
-    ties = 0;
     int at = 0;
-    for (; at < tiles - 1; ++at) {
-      const uint64_t more = sh.tile_weight[at] + (min((uint64_t)border.ties, ties + sh.tile_ties[at]) - min((uint64_t)border.ties, ties)) * tie_weight;
-      if (front + more > target) break;
-      front += more;
-      ties += sh.tile_ties[at];
-    }
-    sh.found[0] = at;
-    sh.found[1] = target;
-    sh.found[2] = front;
-    sh.found[3] = ties;
-    sh.weight[0] = sum;
+    while (at < s.slices - 1 && front + sh.sums[at] <= target) front += sh.sums[at++];
+    sh.draw.found[0] = at;
+    sh.draw.found[1] = target;
+    sh.draw.found[2] = front;
+    sh.draw.found[3] = sum;
   }
   __syncthreads();
-  const int tile = (int)sh.found[0];
-  const uint64_t target = sh.found[1], sum = sh.weight[0];
-  front = sh.found[2];
-  ties_front = sh.found[3];
-  const int at = tile * kThreads + threadIdx.x;
-  const uint32_t key = at < vocab ? ordered(logit(row, at)) : 0;
-  unsigned long long all;
-  const uint64_t tie_number = ties_front + sum_in_front<unsigned long long>(key == border.key, sh.waves, &all);
-  uint64_t x = key > border.key ? w(value_of(key)) : 0;
-  x = x >= least ? x : 0;
-  if (key == border.key && tie_number < border.ties) x = tie_weight;
-  front += sum_in_front<unsigned long long>(x, sh.waves, &all);
-  if (front <= target && front + x > target) {
-    p.tokens[r] = at;
-    if (p.probs) p.probs[r] = (float)(w.exact(value_of(key)) / ((double)sum * (1.0 / (double)kOne)));
+  const int slice = (int)sh.draw.found[0], first = slice * s.slice;
+  const uint64_t target = sh.draw.found[1], sum = sh.draw.found[3];
+  uint64_t front = sh.draw.found[2];
+  const int end = min(p.vocab, first + s.slice);
+  for (int i0 = first; i0 < end; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    const float v = i < end ? logit(row, i) : -INFINITY;
+    uint64_t x = i < end && packed(v, i) >= border ? w(v) : 0;
+    x = x >= f.least ? x : 0;
+    unsigned long long all;
+    const uint64_t before = front + sum_in_front<unsigned long long>(x, sh.draw.waves, &all);
+    if (before <= target && before + x > target) {
+      p.tokens[r] = i;
+      if (p.probs) p.probs[r] = (float)(w.exact(v) / ((double)sum * (1.0 / (double)kOne)));
+    }
+    front += all;
+    if (front > target) break;
   }
 }
 
+template <typename T, bool WIDE>
+void launch_slices(const Params& p, const Scratch& s, hipStream_t st) {
+  const dim3 grid(s.slices, p.rows), threads(kSliceThreads);
+  hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  hipLaunchKernelGGL((draw_kernel<T>), dim3(p.rows), dim3(kThreads), 0, st, p, s);
+}
+
+constexpr int64_t kRowsAtOnce = 1024;
 template <typename T>
-void launch(const Params& p, hipStream_t st) {
-  hipLaunchKernelGGL((sample_kernel<T>), dim3(p.rows), dim3(kThreads), 0, st, p);
+int launch(Params p, hipStream_t st) {
+  const int64_t rows = p.rows, at_once = std::min(rows, kRowsAtOnce);
+  // slices for some four workgroups a CU
+  const int64_t even = (at_once * p.vocab + 4 * pto_hip::ctx().num_cu - 1) / (4 * pto_hip::ctx().num_cu);
+  Scratch s{};
+  s.slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(kStep, (even + kStep - 1) / kStep * kStep));
+  s.slices = (p.vocab + s.slice - 1) / s.slice;
+  const size_t per_row = 8 * (2 * (size_t)s.slices + kIntervals + kCollected + 3) + 4 * (kIntervals + 2);
+  void* ws = nullptr;
+  const int rc = pto_hip::workspace(per_row * at_once, &ws);
+  if (rc) return rc;
+  s.best = reinterpret_cast<unsigned long long*>(ws);
+  s.sums = s.best + at_once * s.slices;
+  s.weight = s.sums + at_once * s.slices;
+  s.tokens = s.weight + at_once * kIntervals;
+  s.front = s.tokens + at_once * kCollected;
+  s.count = reinterpret_cast<unsigned int*>(s.front + 3 * at_once);
+  s.collected = s.count + at_once * kIntervals;
+  const bool wide = (uintptr_t)p.logits % 16 == 0 && (int64_t)p.vocab * sizeof(T) % 16 == 0;
+  const Params whole = p;
+  for (int64_t r = 0; r < rows; r += at_once) {
+    p.rows = (int)std::min(at_once, rows - r);
+    p.logits = reinterpret_cast<const T*>(whole.logits) + r * p.vocab;
+    p.temperature = whole.temperature + r;
+    p.top_k = whole.top_k ? whole.top_k + r : nullptr;
+    p.top_p = whole.top_p ? whole.top_p + r : nullptr;
+    p.min_p = whole.min_p ? whole.min_p + r : nullptr;
+    p.uniform = whole.uniform + r;
+    p.tokens = whole.tokens + r;
+    p.probs = whole.probs ? whole.probs + r : nullptr;
+    wide ? launch_slices<T, true>(p, s, st) : launch_slices<T, false>(p, s, st);
+  }
+  return PTO_HIP_OK;
 }
 
 }  // namespace
@@ -336,9 +745,8 @@ extern "C" int pto_hip_sample_tokens(const void* logits, const float* temperatur
   const DeviceScope scope(ctx().device);
   hipStream_t st = (hipStream_t)stream;
   const Params p{logits, temperature, top_k, top_p, min_p, uniform, tokens, probs, (int)rows, (int)vocab};
-  if (logits_dtype == PTO_HIP_FP32) launch<float>(p, st);
-  else if (logits_dtype == PTO_HIP_BF16) launch<__bf16>(p, st);
-  else launch<_Float16>(p, st);
+  const int rc = logits_dtype == PTO_HIP_FP32 ? launch<float>(p, st) : logits_dtype == PTO_HIP_BF16 ? launch<__bf16>(p, st) : launch<_Float16>(p, st);
+  if (rc) return rc;
   PTO_CHECK_HIP(hipGetLastError());
   return PTO_HIP_OK;
 }
