@@ -239,6 +239,8 @@ __device__ __forceinline__ float code_value(uint32_t word, int byte) {
   }
 }
 
+__device__ __forceinline__ float times(float v, double by) { return (float)((double)v * by); }
+
 // The new rows of one block and KV head, keys or values, by one workgroup: that of the block's first new token.  Their maximum first, then their codes,
 // from the rows read again; the rows in front are coded again where the scale grows.
 template <typename In, int LANES>
@@ -291,14 +293,21 @@ __global__ __launch_bounds__(kThreads) void append_fp8_kernel(Params p) {
   float* slot = (is_k ? p.k_scale : p.v_scale) + (size_t)block * p.hkv + h;
   const float before = *slot;
   float scale = pto_hip::block8::group_scale(most);
+  // Quotients are taken by the exact scale, most / 448, in 64 bits: a 16-bit value is often a tie between two codes, which the rounded scale would push to either
+  // side, and never so near one that 2^-52 matters.
+  double inverse = scale == 1.f || scale == 0x1p-126f ? 1.0 / (double)scale : (double)kE4m3Max / (double)most;
   if (place > 0) {
     scale = fmaxf(before, most / kE4m3Max);
-    if (scale > before) {
+    if (!(scale > before)) {
+      inverse = scale > 0.f ? 1.0 / (double)scale : 0.0;
+    } else {
+      inverse = (double)kE4m3Max / (double)most;
+      const double ratio = (double)before * inverse;
       uint32_t* words = reinterpret_cast<uint32_t*>(base);
       for (size_t w = threadIdx.x; w < (size_t)place * p.d / 4; w += kThreads) {
         const uint32_t c = words[w];
-        words[w] = codes4(code_value(c, 0) * before / scale, code_value(c, 1) * before / scale, code_value(c, 2) * before / scale,
-                          code_value(c, 3) * before / scale);
+        words[w] = codes4(times(code_value(c, 0), ratio), times(code_value(c, 1), ratio), times(code_value(c, 2), ratio),
+                          times(code_value(c, 3), ratio));
       }
     }
   }
@@ -306,8 +315,8 @@ __global__ __launch_bounds__(kThreads) void append_fp8_kernel(Params p) {
     float y[8];
     if (row(r, y) && inside) {
       uint32_t* dst = reinterpret_cast<uint32_t*>(base + (size_t)(place + r) * p.d + e0);
-      dst[0] = codes4(y[0] / scale, y[1] / scale, y[2] / scale, y[3] / scale);
-      dst[1] = codes4(y[4] / scale, y[5] / scale, y[6] / scale, y[7] / scale);
+      dst[0] = codes4(times(y[0], inverse), times(y[1], inverse), times(y[2], inverse), times(y[3], inverse));
+      dst[1] = codes4(times(y[4], inverse), times(y[5], inverse), times(y[6], inverse), times(y[7], inverse));
     }
   }
   __syncthreads();  // everybody has read the scale of before

@@ -50,47 +50,59 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
-// 2^(-i / 64), kept in LDS by every workgroup.
+// 2^(-i / 64), kept in LDS by every workgroup: 64 places in 64 banks, two at most in one.
 struct Powers {
   double of[64];
 };
 __device__ __forceinline__ void fill(Powers& t) {  // and a barrier
-  if (threadIdx.x < 64) t.of[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0);
+  if (threadIdx.x < 64) {
+    const int i = threadIdx.x;
+    double v = i & 1 ? 0x1.fa7c1819e90d8p-1 : 1.0;  // 2^(-1 / 64)
+    v *= i & 2 ? 0x1.f50765b6e4540p-1 : 1.0;
+    v *= i & 4 ? 0x1.ea4afa2a490dap-1 : 1.0;
+    v *= i & 8 ? 0x1.d5818dcfba487p-1 : 1.0;
+    v *= i & 16 ? 0x1.ae89f995ad3adp-1 : 1.0;
+    v *= i & 32 ? 0x1.6a09e667f3bcdp-1 : 1.0;
+    t.of[i] = v;
+  }
 }
 constexpr int kSteps = 46 * 64;          // weights end behind 45 of the 64ths of a power of two
 constexpr int kIntervals = kSteps / 2;
 
-// What a logit of a row weighs.  With z = 64 log2(best's weight / its own): z's whole part is a place in the table, the rest, below 1/64, five terms of
-// the exponential's series (off by 3e-15 of it).
+// What a logit of a row weighs.  With z = 64 log2(best's weight / its own): z's whole part is a place in the table and a power of two, the rest, below
+// 1 / 64 of one, six terms of the exponential's series (off by 3e-15 of it).
 struct Weights {
   float best;     // the largest logit
   double rate;    // 64 log2(e) / T
   const Powers* powers;
   __device__ __forceinline__ double steps(float v) const { return v == best ? 0.0 : ((double)best - (double)v) * rate; }
-  __device__ __forceinline__ double series(double z, int whole) const {
-    const double f = (z - (double)whole) * (-0.69314718055994530942 / 64.0);
-    double s = 1.0 / 120.0;
-    s = fma(s, f, 1.0 / 24.0);
-    s = fma(s, f, 1.0 / 6.0);
-    s = fma(s, f, 0.5);
-    s = fma(s, f, 1.0);
-    s = fma(s, f, 1.0);
-    return s * powers->of[whole & 63];
-  }
-  // in units of 2^-44, rounded to the nearest; z in [0, kSteps)
-  __device__ __forceinline__ uint64_t at(double z) const {
+  // w 2^up, as a number; z in [0, 2^31)
+  __device__ __forceinline__ double scaled(double z, int up) const {
     const int whole = (int)z;
+    constexpr double c = -0.69314718055994530942 / 64.0;
+    const double f = z - (double)whole;
+    double s = c * c * c * c * c / 120.0;
+    s = fma(s, f, c * c * c * c / 24.0);
+    s = fma(s, f, c * c * c / 6.0);
+    s = fma(s, f, c * c / 2.0);
+    s = fma(s, f, c);
+    s = fma(s, f, 1.0);
+    return ldexp(s * powers->of[whole & 63], up - (whole >> 6));
+  }
+  // in units of 2^-44, rounded to the nearest, as a number: sums of up to 2^9 of them are exact; z in [0, kSteps)
+  __device__ __forceinline__ double units(double z) const {
     const double big = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number
-    return __builtin_bit_cast(uint64_t, ldexp(series(z, whole), kUnit - (whole >> 6)) + big) - __builtin_bit_cast(uint64_t, big);
+    return (scaled(z, kUnit) + big) - big;
+  }
+  __device__ __forceinline__ uint64_t at(double z) const {
+    const double big = 4503599627370496.0;
+    return __builtin_bit_cast(uint64_t, scaled(z, kUnit) + big) - __builtin_bit_cast(uint64_t, big);
   }
   __device__ __forceinline__ uint64_t operator()(float v) const {
     const double z = steps(v);
     return z < (double)kSteps ? at(z) : 0;  // NaN: nothing
   }
-  __device__ __forceinline__ double exact(float v) const {
-    const double z = fmin(steps(v), 64000.0);
-    return ldexp(series(z, (int)z), -((int)z >> 6));
-  }
+  __device__ __forceinline__ double exact(float v) const { return scaled(fmin(steps(v), 64000.0), 0); }
 };
 
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
@@ -306,23 +318,38 @@ __device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8
   for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : -INFINITY;
 }
 
+// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; -inf behind the end.
+template <typename T, bool WIDE, typename F>
+__device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
+  for (int i0 = first; i0 < end; i0 += 2 * kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    float a[8], b[8];
+    load8<T, WIDE>(row, i, end, a);
+    load8<T, WIDE>(row, i + kStep, end, b);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f(a[u], i + u);
+    if (i0 + kStep < end) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f(b[u], i + kStep + u);
+    }
+  }
+}
+
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
   __shared__ unsigned long long waves[kSliceThreads / 64];
   const int slice = blockIdx.x, r = blockIdx.y;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
-  uint64_t best = 0;
-  for (int i0 = first; i0 < end; i0 += kStep) {
-    const int i = i0 + threadIdx.x * 8;
-    float v[8];
-    load8<T, WIDE>(row, i, end, v);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const uint64_t k = packed(v[u], i + u);
-      best = k > best ? k : best;
-    }
-  }
+  // a thread meets its elements by rising index: of equal ones the first stays
+  float most = -INFINITY;
+  int where = first;
+  in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
+    const bool more = v > most;
+    most = more ? v : most;
+    where = more ? i : where;
+  });
+  uint64_t best = packed(most, where);
   // the histogram of the next kernel starts from nothing
   const int per = (kIntervals + s.slices - 1) / s.slices;
   for (int i = slice * per + threadIdx.x; i < min(kIntervals, (slice + 1) * per); i += kSliceThreads) {
@@ -372,19 +399,14 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const Weights w = weights_of(best, t, &powers);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
-  for (int i0 = first; i0 < end; i0 += kStep) {
-    float v[8];
-    load8<T, WIDE>(row, i0 + threadIdx.x * 8, end, v);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const double z = w.steps(v[u]);
-      if (z < (double)kSteps) {
-        const int at = (int)z >> 1;
-        atomicAdd(&count[at], 1u);
-        if (f.by_sum) atomicAdd(&weight[at], (unsigned long long)w.at(z));
-      }
+  in_steps<T, WIDE>(row, first, end, [&](float v, int) {
+    const double z = w.steps(v);
+    if (z < (double)kSteps) {
+      const int at = (int)z >> 1;
+      atomicAdd(&count[at], 1u);
+      if (f.by_sum) atomicAdd(&weight[at], (unsigned long long)w.at(z));
     }
-  }
+  });
   __syncthreads();
   for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads)
     if (count[i]) {
@@ -501,23 +523,20 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const double z_first = 2.0 * at.first, z_behind = min(2.0 * (at.last + 1), (double)kSteps);
-  uint64_t sum = 0;
-  for (int i0 = first; i0 < end; i0 += kStep) {
-    const int i = i0 + threadIdx.x * 8;
-    float v[8];
-    load8<T, WIDE>(row, i, end, v);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const double z = w.steps(v[u]);
-      if (z < z_first) {
-        const uint64_t x = w.at(z);
-        sum += x >= f.least ? x : 0;
-      } else if (z < z_behind) {
-        const unsigned int n = atomicAdd(&s.collected[r], 1u);
-        if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v[u], i + u);
-      }
+  const double least = (double)f.least;
+  double own = 0.0;  // at most 64 elements': exact
+  static_assert(kMaxSlice / kSliceThreads <= 256, "a thread's sum has to stay exact");
+  in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
+    const double z = w.steps(v);
+    if (z < z_first) {
+      const double x = w.units(z);
+      own += x >= least ? x : 0.0;
+    } else if (z < z_behind) {
+      const unsigned int n = atomicAdd(&s.collected[r], 1u);
+      if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v, i);
     }
-  }
+  });
+  uint64_t sum = (uint64_t)own;
   sum = wave_sum((unsigned long long)sum);
   if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = sum;
   __syncthreads();
@@ -637,36 +656,65 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   }
   __syncthreads();
   // the slice in which the running sum passes its share
-  if (threadIdx.x == 0) {
-    uint64_t sum = 0, front = 0;
-    for (int i = 0; i < s.slices; ++i) sum += sh.sums[i];
+  if (threadIdx.x < 64) {
+    constexpr int kOwn = kMaxVocab / kStep / 64;
+    uint64_t x[kOwn], own = 0;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = threadIdx.x * kOwn + u;
+      x[u] = i < s.slices ? sh.sums[i] : 0;
+      own += x[u];
+    }
+    uint64_t to = own;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint64_t o = __shfl_up((unsigned long long)to, off);
+      if ((int)threadIdx.x >= off) to += o;
+    }
+    const uint64_t sum = __shfl((unsigned long long)to, 63);
     const double u = fmin(fmax((double)p.uniform[r], 0x1p-25), 1.0 - 0x1p-24);
     const uint64_t target = (uint64_t)(u * (double)sum);
-    int at = 0;
-    while (at < s.slices - 1 && front + sh.sums[at] <= target) front += sh.sums[at++];
-    sh.draw.found[0] = at;
-    sh.draw.found[1] = target;
-    sh.draw.found[2] = front;
-    sh.draw.found[3] = sum;
+    uint64_t front = to - own;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) {
+      if (front <= target && front + x[i] > target) {
+        sh.draw.found[0] = threadIdx.x * kOwn + i;
+        sh.draw.found[1] = target;
+        sh.draw.found[2] = front;
+        sh.draw.found[3] = sum;
+      }
+      front += x[i];
+    }
   }
   __syncthreads();
-  const int slice = (int)sh.draw.found[0], first = slice * s.slice;
+  const int first = (int)sh.draw.found[0] * s.slice, end = min(p.vocab, first + s.slice);
   const uint64_t target = sh.draw.found[1], sum = sh.draw.found[3];
+  // and the token in it: a thread has neighbouring ones
+  constexpr int kMost = kMaxSlice / kThreads;
+  const int per = s.slice / kThreads;
+  uint64_t x[kMost], own = 0;
+#pragma unroll
+  for (int u = 0; u < kMost; ++u) {
+    const int i = first + threadIdx.x * per + u;
+    const bool there = u < per && i < end;
+    const float v = there ? logit(row, i) : -INFINITY;
+    x[u] = there && packed(v, i) >= border ? w(v) : 0;
+    x[u] = x[u] >= f.least ? x[u] : 0;
+    own += x[u];
+  }
+  unsigned long long all;
   uint64_t front = sh.draw.found[2];
-  const int end = min(p.vocab, first + s.slice);
-  for (int i0 = first; i0 < end; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const float v = i < end ? logit(row, i) : -INFINITY;
-    uint64_t x = i < end && packed(v, i) >= border ? w(v) : 0;
-    x = x >= f.least ? x : 0;
-    unsigned long long all;
-    const uint64_t before = front + sum_in_front<unsigned long long>(x, sh.draw.waves, &all);
-    if (before <= target && before + x > target) {
-      p.tokens[r] = i;
-      if (p.probs) p.probs[r] = (float)(w.exact(v) / ((double)sum * (1.0 / (double)kOne)));
+  front += sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
+  if (front <= target && front + own > target) {
+#pragma unroll
+    for (int u = 0; u < kMost; ++u) {
+      if (front <= target && front + x[u] > target) {
+        const int i = first + threadIdx.x * per + u;
+        p.tokens[r] = i;
+        if (p.probs) p.probs[r] = (float)(w.exact(logit(row, i)) / ((double)sum * (1.0 / (double)kOne)));
+      }
+      front += x[u];
     }
-    front += all;
-    if (front > target) break;
   }
 }
 
