@@ -24,7 +24,7 @@
 namespace {
 
 constexpr int kMaxVocab = 1 << 19;  // sums of 2^19 weights of 2^44 stay below 2^64
-constexpr int kThreads = 1024;
+constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kUnit = 44;  // a weight of 1 is 2^44
@@ -181,20 +181,29 @@ __device__ bool find_border(Shared& sh, const T* row, int vocab, const Weights& 
       if (x) atomicAdd(&sh.weight[bin], (unsigned long long)x);
     }
     __syncthreads();
-    // two bins a thread
-    const int b0 = 2 * threadIdx.x;
-    const uint64_t n0 = sh.count[b0], n1 = sh.count[b0 + 1], w0 = sh.weight[b0], w1 = sh.weight[b0 + 1];
+    constexpr int kOwn = kBins / kThreads;
+    uint64_t n_own = 0, x_own = 0;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      n_own += sh.count[threadIdx.x * kOwn + u];
+      x_own += sh.weight[threadIdx.x * kOwn + u];
+    }
     unsigned long long all;
-    const uint64_t n_front = tokens_front + sum_in_front<unsigned long long>(n0 + n1, sh.waves, &all);
-    const uint64_t w_front = weight_front + sum_in_front<unsigned long long>(w0 + w1, sh.waves, &all);
+    uint64_t n_front = tokens_front + sum_in_front<unsigned long long>(n_own, sh.waves, &all);
+    uint64_t x_front = weight_front + sum_in_front<unsigned long long>(x_own, sh.waves, &all);
     if (threadIdx.x == 0) sh.found[0] = kBins;
     __syncthreads();
-    const uint64_t front = by_weight ? w_front : n_front, own0 = by_weight ? w0 : n0, own1 = by_weight ? w1 : n1;
-    if (front < need && front + own0 + own1 >= need) {
-      const bool second = front + own0 < need;
-      sh.found[0] = b0 + second;
-      sh.found[1] = n_front + (second ? n0 : 0);
-      sh.found[2] = w_front + (second ? w0 : 0);
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const uint64_t n = sh.count[threadIdx.x * kOwn + u], x = sh.weight[threadIdx.x * kOwn + u];
+      const uint64_t front = by_weight ? x_front : n_front;
+      if (front < need && front + (by_weight ? x : n) >= need) {
+        sh.found[0] = threadIdx.x * kOwn + u;
+        sh.found[1] = n_front;
+        sh.found[2] = x_front;
+      }
+      n_front += n;
+      x_front += x;
     }
     __syncthreads();
     const int bin = (int)sh.found[0];
@@ -241,7 +250,7 @@ __device__ __forceinline__ uint64_t packed(float v, int i) { return (uint64_t)or
 
 // The place of the last token that a row's filters keep, from the row alone (all threads of a workgroup of kThreads).
 template <typename T>
-__device__ __noinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, const Weights& w, const Filters& f) {
+__device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, const Weights& w, const Filters& f) {
   const uint32_t top = ordered(w.best);
   Border border{kNone, 0};
   uint64_t total = 0;
@@ -280,9 +289,9 @@ __device__ __noinline__ uint64_t border_of_row(Shared& sh, const T* row, int voc
 }
 
 // ---- slices ----
-constexpr int kSliceThreads = 256;
+constexpr int kSliceThreads = kThreads;
 constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
-constexpr int kMaxSlice = 16384;
+constexpr int kMaxSlice = 64 * kThreads;  // a wavefront has a lane for each of a thread's tokens
 constexpr int kCollected = 4096;
 
 // What the kernels leave for each other, a row of each a row.
@@ -525,7 +534,6 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   const double z_first = 2.0 * at.first, z_behind = min(2.0 * (at.last + 1), (double)kSteps);
   const double least = (double)f.least;
   double own = 0.0;  // at most 64 elements': exact
-  static_assert(kMaxSlice / kSliceThreads <= 256, "a thread's sum has to stay exact");
   in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
     const double z = w.steps(v);
     if (z < z_first) {
@@ -559,7 +567,7 @@ struct DrawShared {
   };
 };
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   __shared__ DrawShared sh;
   const int r = blockIdx.x;
@@ -689,32 +697,40 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   __syncthreads();
   const int first = (int)sh.draw.found[0] * s.slice, end = min(p.vocab, first + s.slice);
   const uint64_t target = sh.draw.found[1], sum = sh.draw.found[3];
-  // and the token in it: a thread has neighbouring ones
-  constexpr int kMost = kMaxSlice / kThreads;
-  const int per = s.slice / kThreads;
-  uint64_t x[kMost], own = 0;
-#pragma unroll
-  for (int u = 0; u < kMost; ++u) {
+  // the thread whose tokens hold it, neighbouring ones, and its wavefront looks for the token among them
+  const int per = s.slice / kThreads, lane = threadIdx.x % 64;
+  auto kept = [&](int i) -> uint64_t {
+    const float v = logit(row, i);
+    const uint64_t x = packed(v, i) >= border ? w(v) : 0;
+    return x >= f.least ? x : 0;
+  };
+  uint64_t own = 0;
+  for (int u = 0; u < per; u += 8) {
     const int i = first + threadIdx.x * per + u;
-    const bool there = u < per && i < end;
-    const float v = there ? logit(row, i) : -INFINITY;
-    x[u] = there && packed(v, i) >= border ? w(v) : 0;
-    x[u] = x[u] >= f.least ? x[u] : 0;
-    own += x[u];
+    float v[8];
+    load8<T, WIDE>(row, i, end, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint64_t x = i + e < end && packed(v[e], i + e) >= border ? w(v[e]) : 0;
+      own += x >= f.least ? x : 0;
+    }
   }
   unsigned long long all;
-  uint64_t front = sh.draw.found[2];
-  front += sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
-  if (front <= target && front + own > target) {
+  const uint64_t front = sh.draw.found[2] + sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
+  const uint64_t here = __ballot(front <= target && front + own > target);
+  if (!here) return;
+  const int from = __builtin_ctzll(here), i = first + ((int)(threadIdx.x & ~63u) + from) * per + lane;
+  const uint64_t x = lane < per && i < end ? kept(i) : 0;
+  uint64_t to = x;
 #pragma unroll
-    for (int u = 0; u < kMost; ++u) {
-      if (front <= target && front + x[u] > target) {
-        const int i = first + threadIdx.x * per + u;
-        p.tokens[r] = i;
-        if (p.probs) p.probs[r] = (float)(w.exact(logit(row, i)) / ((double)sum * (1.0 / (double)kOne)));
-      }
-      front += x[u];
-    }
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_up((unsigned long long)to, off);
+    if (lane >= off) to += o;
+  }
+  to += __shfl((unsigned long long)front, from);
+  if (to - x <= target && to > target) {
+    p.tokens[r] = i;
+    if (p.probs) p.probs[r] = (float)(w.exact(logit(row, i)) / ((double)sum * (1.0 / (double)kOne)));
   }
 }
 
@@ -724,7 +740,7 @@ void launch_slices(const Params& p, const Scratch& s, hipStream_t st) {
   hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
   if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
   hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-  hipLaunchKernelGGL((draw_kernel<T>), dim3(p.rows), dim3(kThreads), 0, st, p, s);
+  hipLaunchKernelGGL((draw_kernel<T, WIDE>), dim3(p.rows), dim3(kThreads), 0, st, p, s);
 }
 
 constexpr int64_t kRowsAtOnce = 1024;

@@ -50,4 +50,29 @@ __device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch
   return TokenSeq{first <= token && token < end ? lo + k : -1, first, end - first};
 }
 
+// Sums over a wavefront without a trip through LDS: along rows of 16 lanes, then from row to row; lane 63 has all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_from(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_from(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
+}
+// The sum of the lanes up to this one (of integers: exact).
+template <typename V>
+__device__ __forceinline__ V wave_running_sum(V v) {
+  v = add_from<0x111, 0xf>(v);
+  v = add_from<0x112, 0xf>(v);
+  v = add_from<0x114, 0xf>(v);
+  v = add_from<0x118, 0xf>(v);
+  v = add_from<0x142, 0xa>(v);
+  v = add_from<0x143, 0xc>(v);
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_total(V v) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_running_sum(v)), 63));
+}
+
 }  // namespace pto_hip

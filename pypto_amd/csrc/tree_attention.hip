@@ -138,13 +138,12 @@ __global__ __launch_bounds__(64) void tree_any_kernel(Params p) {
 // second product.  Maxima and sums per row run along (online softmax); parts are joined by a second kernel.
 //
 // The parts are cut on the device, where the lengths are known: with `total` keys times row blocks over all sequences and KV heads, a part has total / target
-// keys (a multiple of 64, at least `least`), so that target workgroups and at most one more per row block have work that lasts alike.
+// keys or somewhat more (at least `least`), so that the workgroups that a GPU holds at once have work that lasts alike.
 // ---------------------------------------------------------------------------------------------
 using pto_hip::attn::f32x4;
 using pto_hip::attn::fp8x8_widen;
 using pto_hip::attn::kMinMax;
 using pto_hip::attn::mfma16;
-using pto_hip::attn::round_pack;
 using pto_hip::attn::u32x4;
 typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
 
@@ -171,122 +170,140 @@ __device__ __forceinline__ Work work_of(const Params& p, int b, int rows) {
   }
   return w;
 }
-__device__ __forceinline__ int64_t wave_total(int64_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor((long long)v, off);
-  return v;
-}
-// Sum of the lanes up to this one.
-__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t o = __shfl_up((long long)v, off);
-    if (lane >= off) v += o;
-  }
-  return v;
-}
-// Keys of a part (wave-uniform).
+__device__ __forceinline__ int parts_of(const Work& w, int keys) { return w.blocks ? max(1, (w.end + keys - 1) / keys) : 0; }
+
+// Keys of a part (wave-uniform): total / target, or a few eighths more, the least with which the workgroups are no more than target; twice as many where none of
+// these will do, as with short sequences.
 __device__ __forceinline__ int part_keys(const Params& p, int rows, int lane, const Work& first64) {
-  int64_t total = 0;
+  using pto_hip::wave_total;
+  float total = 0.f;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
-    total += (int64_t)w.end * w.blocks;
+    total += wave_total((float)w.end * (float)w.blocks);
   }
-  total = wave_total(total) * p.hkv;
-  const int64_t even = (total / p.target + 64) & ~63ll;
-  return (int)min(max(even, (int64_t)p.least), (int64_t)1 << 30);
+  total *= (float)p.hkv * 1.0001f / (float)p.target;  // not below the exact quotient: the room for partial results counts on it
+  constexpr int kTries = 8;
+  int keys[kTries];
+  float count[kTries];
+#pragma unroll
+  for (int i = 0; i < kTries; ++i) {
+    const float even = fminf(total * (1.f + 0.125f * i), 1e9f);
+    keys[i] = max(((int)even + kChunk) & ~(kChunk - 1), p.least);
+    count[i] = 0;
+  }
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
+#pragma unroll
+    for (int i = 0; i < kTries; ++i) count[i] += wave_total((float)parts_of(w, keys[i]) * (float)w.blocks);
+  }
+  int found = keys[kTries - 1];
+#pragma unroll
+  for (int i = kTries - 2; i >= 0; --i) found = count[i] * (float)p.hkv <= (float)p.target ? keys[i] : found;
+  return found;
 }
-__device__ __forceinline__ int parts_of(const Work& w, int keys) { return w.blocks ? max(1, (w.end + keys - 1) / keys) : 0; }
 
 struct Share {
   int seq;  // -1: nothing to do
-  int first, count, ctx, end;
+  Work w;
   int parts, part, block, h;
-  int64_t slot;  // of the sequence's first token in its first part
+  int slot;  // of the sequence's first token in its first part
 };
-__device__ __forceinline__ int64_t from_lane(int64_t v, int lane) { return __shfl((long long)v, lane); }
+// A sequence's partial results, in tokens: none where it has one part.  No more than there can be room for, so that sums over 64 of them stay in 32 bits.
+__device__ __forceinline__ int held_of(const Params& p, const Work& w, int parts) { return parts > 1 ? (int)min((int64_t)parts * w.count, (int64_t)p.slots + 1) : 0; }
+__device__ __forceinline__ Work work_in_lane(const Work& w, int k) {
+  return Work{__builtin_amdgcn_readlane(w.first, k), __builtin_amdgcn_readlane(w.count, k), __builtin_amdgcn_readlane(w.ctx, k),
+              __builtin_amdgcn_readlane(w.end, k), __builtin_amdgcn_readlane(w.blocks, k)};
+}
 // What workgroup `id` does.  Parts of a sequence follow each other, in each the row blocks, in each the KV heads: the blocks that read the same keys are a
 // multiple of the KV heads apart, on one XCD where these are a multiple of eight.
-__device__ __forceinline__ Share share_of(const Params& p, int rows, int64_t id, int lane) {
+__device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int lane) {
   const Work first64 = work_of(p, lane, rows);
   const int keys = part_keys(p, rows, lane, first64);
-  int64_t ids = 0, slots = 0;
+  int ids = 0, slots = 0;
+  Share s{};
+  s.seq = -1;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
     const int parts = parts_of(w, keys);
-    const int64_t mine = (int64_t)parts * w.blocks * p.hkv, held = parts > 1 ? (int64_t)parts * w.count : 0;
-    const int64_t to = ids + wave_scan(mine, lane), slot_to = slots + wave_scan(held, lane);
+    const int mine = parts * w.blocks * p.hkv, held = held_of(p, w, parts);
+    const int to = pto_hip::wave_running_sum(mine) + ids, slot_to = pto_hip::wave_running_sum(held) + slots;
     const uint64_t behind = __ballot(to > id);
     if (behind) {
       const int k = __builtin_ctzll(behind);
-      Share s;
       s.seq = b0 + k;
-      s.first = __shfl(w.first, k);
-      s.count = __shfl(w.count, k);
-      s.ctx = __shfl(w.ctx, k);
-      s.end = __shfl(w.end, k);
-      s.parts = __shfl(parts, k);
-      s.slot = from_lane(slot_to - held, k);
-      const int blocks = __shfl(w.blocks, k);
-      int at = (int)(id - from_lane(to - mine, k));
+      s.w = work_in_lane(w, k);
+      s.parts = __builtin_amdgcn_readlane(parts, k);
+      s.slot = __builtin_amdgcn_readlane(slot_to - held, k);
+      int at = id - __builtin_amdgcn_readlane(to - mine, k);
       s.h = at % p.hkv;
       at /= p.hkv;
-      s.block = at % blocks;
-      s.part = at / blocks;
-      if (s.parts > 1 && s.slot + (int64_t)s.parts * s.count > p.slots) s.seq = -1;  // only where the starts do not rise
+      s.block = at % s.w.blocks;
+      s.part = at / s.w.blocks;
+      if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) s.seq = -1;  // only where the starts do not rise
       return s;
     }
-    ids = from_lane(to, 63);
-    slots = from_lane(slot_to, 63);
+    ids = __builtin_amdgcn_readlane(to, 63);
+    slots = min(__builtin_amdgcn_readlane(slot_to, 63), p.slots + 1);
   }
-  Share none{};
-  none.seq = -1;
-  return none;
+  return s;
 }
 
-// LDS of a stage: K rows and V rows, 16 bytes apart from each other beyond their length, so that 16 rows read at one column lie in different banks.
-template <int D, bool FP8>
+// LDS of a stage: K rows and V rows as 16-bit values, 16 bytes apart from each other beyond their length, so that 16 rows read at one column lie in
+// different banks.
+template <int D>
 struct Stage {
-  static constexpr int kRow = FP8 ? D : 2 * D;
+  static constexpr int kRow = 2 * D;
   static constexpr int kPitch = kRow + 16;
   static constexpr int kBytes = 2 * kChunk * kPitch;
-  static constexpr int kItems = kChunk * kRow / 16;  // 16-byte pieces of K, and of V
 };
 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Whether any of a piece's values is infinite or NaN.
-template <bool BF16, bool FP8>
-__device__ __forceinline__ bool any_unbounded(u32x4 v) {
-  bool bad = false;
+// Zeros in the place of those of eight 16-bit values that are infinite or NaN; whether there were any.
+template <bool BF16>
+__device__ __forceinline__ bool drop_unbounded(u32x4& v) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  bool any = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (FP8) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) bad |= (v[i] >> (8 * k) & 0x7fu) == 0x7fu;
-    } else {
-      constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-      bad |= (v[i] & e) == e || (v[i] >> 16 & e) == e;
-    }
+    const bool low = (v[i] & e) == e, high = (v[i] >> 16 & e) == e;
+    v[i] = (low ? 0u : v[i] & 0xffffu) | (high ? 0u : v[i] & 0xffff0000u);
+    any |= low || high;
   }
-  return bad;
+  return any;
 }
+// Two fp32 rounded to the 16-bit type, nearest even, the first in the low half.
 template <bool BF16>
-__device__ __forceinline__ uint32_t drop_unbounded(uint32_t v) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  if ((v & e) == e) v &= 0xffff0000u;
-  if ((v >> 16 & e) == e) v &= 0xffffu;
-  return v;
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
+  typedef T T2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), T2));
+}
+// The largest over the four lanes c, c + 16, c + 32, c + 48.
+__device__ __forceinline__ float column_max(float v) {
+  auto both = [](auto r) { return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])); };
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const uint32_t w = __builtin_bit_cast(uint32_t, both(__builtin_amdgcn_permlane16_swap(u, u, false, false)));
+  return both(__builtin_amdgcn_permlane32_swap(w, w, false, false));
+}
+// Four rows of 16 16-bit values each, from LDS: the 16 lanes of a group give the addresses of a row's quarters, four lanes a row, and lane c has column c.
+__device__ __forceinline__ u32x2 read_columns(const char* p) {
+  typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
 
+// A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.
+constexpr float kSlack = 6.f;
+
 template <int D, bool BF16, bool FP8, int NW, int GT>
-__global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
-  typedef Stage<D, FP8> S;
+__global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
+  typedef Stage<D> S;
   constexpr int kThreads = NW * 64, kRows = NW * GT * 16;
-  constexpr int kPieces = (S::kItems + kThreads - 1) / kThreads;  // of K, and of V, a thread brings
-  constexpr int kEpl = D >= 128 ? 8 : D / 16;    // V elements of a lane and token
-  constexpr int kSets = D >= 128 ? D / 128 : 1;  // ... in so many groups of 16 lanes' worth
   constexpr int kEsz = FP8 ? 1 : 2;
+  constexpr int kRowBytes = D * kEsz;                     // of a cache row
+  constexpr int kItems = kChunk * kRowBytes / 16;         // 16-byte pieces of a chunk's K, and of its V
+  constexpr int kPieces = (kItems + kThreads - 1) / kThreads;  // ... a thread brings
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   // of chunk n in place n % 3: new tokens whose values hold infinities or NaN, as bits.  A place is read while the next is written and the one
@@ -296,16 +313,12 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
   const int c = lane & 15, j = lane >> 4;
   const Share s = share_of(p, kRows, blockIdx.x, lane);
   if (s.seq < 0) return;
-  const int seq = __builtin_amdgcn_readfirstlane(s.seq), h = __builtin_amdgcn_readfirstlane(s.h);
-  const int ctx = __builtin_amdgcn_readfirstlane(s.ctx), count = __builtin_amdgcn_readfirstlane(s.count);
-  const int token0 = __builtin_amdgcn_readfirstlane(s.first);
-  const int parts = __builtin_amdgcn_readfirstlane(s.parts), part = __builtin_amdgcn_readfirstlane(s.part);
-  const int all = __builtin_amdgcn_readfirstlane(s.end);
+  const int seq = s.seq, h = s.h, ctx = s.w.ctx, count = s.w.count, token0 = s.w.first, parts = s.parts, part = s.part, all = s.w.end;
   // even parts of whole chunks
   const int chunks = (all + kChunk - 1) / kChunk;
   const int tok_first = (int)((int64_t)chunks * part / parts) * kChunk;
   const int tok_end = min((int)((int64_t)chunks * (part + 1) / parts) * kChunk, all);
-  const int row0 = (__builtin_amdgcn_readfirstlane(s.block) * NW + wave) * GT * 16;  // first row of this wavefront
+  const int row0 = (s.block * NW + wave) * GT * 16;  // first row of this wavefront
   const int rows = count * p.group;
   const bool active = row0 < rows;
   if (threadIdx.x == 0) {
@@ -314,8 +327,10 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
 
-  // Query fragments (B operand): column = row c of the tile; k-group j of step u holds elements (u*4+j)*8..+8, or beside e4m3 keys, of which 16 bytes are
-  // two steps, ((u/2)*4+j)*16 + (u%2)*8..+8.
+  // Query fragments (B operand): column = row c of the tile; k-group j of step u holds elements (u*4+j)*8..+8.  A negative scale changes their sign, so that
+  // the largest product is the largest score.
+  const uint32_t flip = p.scale_log2e < 0.f ? 0x80008000u : 0u;
+  const float scale = fabsf(p.scale_log2e);
   u32x4 qf[GT][D / 32];
   int node[GT];
 #pragma unroll
@@ -327,21 +342,21 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
     const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + ((size_t)(token0 + node[t]) * p.hq + h * p.group + g) * D;
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) {
-      const int el = FP8 ? ((u >> 1) * 4 + j) * 16 + (u & 1) * 8 : (u * 4 + j) * 8;
       const u32x4 z = {0u, 0u, 0u, 0u};
-      qf[t][u] = there ? *reinterpret_cast<const u32x4*>(q + el) : z;
+      qf[t][u] = there ? *reinterpret_cast<const u32x4*>(q + (u * 4 + j) * 8) ^ flip : z;
     }
   }
-  f32x4 acc[GT][kSets][kEpl];
-  float m_run[GT], l_run[GT];
+  // acc[t][i][r]: row c of tile t, channel 16 i + 4 j + r; sum[t]: its probabilities' sum, in every lane of the column
+  f32x4 acc[GT][D / 16], sum[GT];
+  float m_run[GT];
+  const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const u32x4 ones = {one, one, one, one};
 #pragma unroll
   for (int t = 0; t < GT; ++t) {
 #pragma unroll
-    for (int a = 0; a < kSets; ++a)
-#pragma unroll
-      for (int i = 0; i < kEpl; ++i) acc[t][a][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 16; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     m_run[t] = kMinMax;
-    l_run[t] = 0.f;
   }
 
   // Block-table window: lane i holds the physical block (and the scales) of logical block win_base + i.
@@ -349,7 +364,7 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
   int win_base = 0, win_blk = 0;
   float win_ks = 1.f, win_vs = 1.f;
   bool bad_entry = false;
-  auto load_window = [&](int first_block) {
+  auto load_window = [&](int first_block) __attribute__((always_inline)) {
     win_base = first_block;
     const bool used = (int64_t)(first_block + lane) * p.bs < tok_end;
     win_blk = used ? table[first_block + lane] : 0;
@@ -362,218 +377,222 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
       win_vs = used ? p.v_scale[(size_t)win_blk * p.hkv + h] : 1.f;
     }
   };
-  auto slot_of = [&](int tok) {  // window slot of a token's block (uniform)
-    const int lb = tok / p.bs;
-    if (lb < win_base || lb >= win_base + 64) load_window(lb);
-    return lb - win_base;
-  };
+  // The next 16 tokens to be asked for: logical block and place in it (a block is a multiple of 16 tokens).
+  int lb = tok_first / p.bs, off = tok_first % p.bs;
 
-  u32x4 kr[kPieces], vr[kPieces];  // a chunk on its way to LDS
-  float k_mul_next = p.scale_log2e, v_unit_next = 1.f;
-  auto request = [&](int tok) {
+  // two chunks on their way to LDS, and the scales of their keys and values
+  u32x4 kr[2][kPieces], vr[2][kPieces];
+  float k_muls[2] = {scale, scale}, v_units[2] = {1.f, 1.f};
+  auto request = [&](auto set, int tok) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value;
     if (tok >= tok_end) return;
-    int slot0 = slot_of(tok);
-    const int tok1 = min(tok + 16, tok_end - 1);
-    const int lb1 = tok1 / p.bs;
-    if (lb1 >= win_base + 64) {  // the chunk's halves in two windows
-      load_window(tok / p.bs);
-      slot0 = 0;
+    int lb1 = lb, off1 = off + 16;
+    if (off1 == p.bs) {
+      off1 = 0;
+      ++lb1;
     }
-    const int slot1 = lb1 - win_base;
-    const int blk0 = __builtin_amdgcn_readlane(win_blk, slot0), blk1 = __builtin_amdgcn_readlane(win_blk, slot1);
+    if (lb1 >= win_base + 64) load_window(lb);
+    const int slot = lb - win_base;
+    const int blk0 = __builtin_amdgcn_readlane(win_blk, slot), blk1 = __builtin_amdgcn_readlane(win_blk, lb1 - win_base);
     if constexpr (FP8) {  // a chunk lies in one block
-      k_mul_next = p.scale_log2e * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_ks), slot0));
-      v_unit_next = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_vs), slot0));
+      k_muls[SET] = scale * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_ks), slot));
+      v_units[SET] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_vs), slot));
     }
-    const size_t at0 = (((size_t)blk0 * p.hkv + h) * p.bs + tok % p.bs) * S::kRow;
-    const size_t at1 = (((size_t)blk1 * p.hkv + h) * p.bs + (tok + 16) % p.bs) * S::kRow;
+    const size_t at0 = (((size_t)blk0 * p.hkv + h) * p.bs + off) * kRowBytes;
+    const size_t at1 = (((size_t)blk1 * p.hkv + h) * p.bs + off1) * kRowBytes - 16 * kRowBytes;
+    lb = lb1;
+    off = off1 + 16;
+    if (off == p.bs) {
+      off = 0;
+      ++lb;
+    }
+    const char* kc = reinterpret_cast<const char*>(p.kc);
+    const char* vc = reinterpret_cast<const char*>(p.vc);
+    auto bring = [&](bool whole) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int item = threadIdx.x + i * kThreads;
-      const int row = item * 16 / S::kRow;
-      // rows from tok_end on are zeros: what lies there has no part in anything
-      const bool there = (S::kItems % kThreads == 0 || item < S::kItems) && tok + row < tok_end;
-      const size_t at = (row < 16 ? at0 : at1 - 16 * S::kRow) + (size_t)item * 16;
-      const u32x4 z = {0u, 0u, 0u, 0u};
-      kr[i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.kc) + at)) : z;
-      vr[i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(p.vc) + at)) : z;
-    }
+      for (int i = 0; i < kPieces; ++i) {
+        const int item = threadIdx.x + i * kThreads, row = item * 16 / kRowBytes;
+        // rows from tok_end on are zeros: what lies there has no part in anything
+        const bool there = (kItems % kThreads == 0 || item < kItems) && (whole || tok + row < tok_end);
+        const size_t at = (row < 16 ? at0 : at1) + (size_t)item * 16;
+        const u32x4 z = {0u, 0u, 0u, 0u};
+        kr[SET][i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at)) : z;
+        vr[SET][i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at)) : z;
+      }
+    };
+    if (tok + kChunk <= tok_end) bring(true);
+    else bring(false);
   };
-  auto park = [&](int stage, int odd_place, int tok) {
+  auto park = [&](auto set, int stage, int odd_place, int tok) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value;
     char* base = lds + stage * S::kBytes;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int item = threadIdx.x + i * kThreads;
-      if (S::kItems % kThreads != 0 && item >= S::kItems) continue;
-      const int row = item * 16 / S::kRow, col = item * 16 % S::kRow;
-      *reinterpret_cast<u32x4*>(base + row * S::kPitch + col) = kr[i];
-      *reinterpret_cast<u32x4*>(base + (kChunk + row) * S::kPitch + col) = vr[i];
+      if (kItems % kThreads != 0 && item >= kItems) continue;
+      const int row = item * 16 / kRowBytes, col = item * 16 % kRowBytes * (2 / kEsz);
+      char* k = base + row * S::kPitch + col;
+      char* v = k + kChunk * S::kPitch;
+      u32x4 v0 = vr[SET][i], v1 = {0u, 0u, 0u, 0u};
+      if constexpr (FP8) {  // widened once for all wavefronts; exact
+        v0 = fp8x8_widen<BF16>(vr[SET][i][0], vr[SET][i][1]);
+        v1 = fp8x8_widen<BF16>(vr[SET][i][2], vr[SET][i][3]);
+      }
       if (tok + kChunk > ctx) {
-        if (tok + row >= ctx && any_unbounded<BF16, FP8>(vr[i])) atomicOr(&odd_keys[odd_place], 1u << row);
+        if (tok + row >= ctx) {
+          bool odd = drop_unbounded<BF16>(v0);
+          if constexpr (FP8) odd |= drop_unbounded<BF16>(v1);
+          if (odd) atomicOr(&odd_keys[odd_place], 1u << row);
+        }
+      }
+      if constexpr (FP8) {
+        *reinterpret_cast<u32x4*>(k) = fp8x8_widen<BF16>(kr[SET][i][0], kr[SET][i][1]);
+        *reinterpret_cast<u32x4*>(k + 16) = fp8x8_widen<BF16>(kr[SET][i][2], kr[SET][i][3]);
+        *reinterpret_cast<u32x4*>(v + 16) = v1;
+      } else {
+        *reinterpret_cast<u32x4*>(k) = kr[SET][i];
+      }
+      *reinterpret_cast<u32x4*>(v) = v0;
+    }
+  };
+
+  float k_mul = scale, v_unit = 1.f;
+  // A chunk's products from stage base `kbase`.  MASKED: some of its keys may be new tokens, or lie behind the last one.
+  auto multiply = [&](const char* kbase, int tok, unsigned int odd, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const char* vbase = kbase + kChunk * S::kPitch;
+    // S^T: rows = keys, columns = query rows
+    f32x4 s0[GT], s1[GT];
+#pragma unroll
+    for (int t = 0; t < GT; ++t) s0[t] = s1[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) {
+      const u32x4 a0 = *reinterpret_cast<const u32x4*>(kbase + c * S::kPitch + (u * 4 + j) * 16);
+      const u32x4 a1 = *reinterpret_cast<const u32x4*>(kbase + (16 + c) * S::kPitch + (u * 4 + j) * 16);
+#pragma unroll
+      for (int t = 0; t < GT; ++t) {
+        s0[t] = mfma16<BF16>(a0, qf[t][u], s0[t]);
+        s1[t] = mfma16<BF16>(a1, qf[t][u], s1[t]);
+      }
+    }
+    // The values' fragments are asked for in front of the softmax (head_dim 256: the first half): lane (c, j) has channel 16 i + c of the tokens whose
+    // probabilities it will have.
+    const char* vlane = vbase + (j * 4 + (c >> 2)) * S::kPitch + (c & 3) * 8;
+    constexpr int kHeld = D <= 128 ? D / 16 : 8;
+    u32x4 vt[kHeld];
+    auto fetch_values = [&](int from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const u32x2 lo = read_columns(vlane + (from + i) * 32), hi = read_columns(vlane + 16 * S::kPitch + (from + i) * 32);
+        vt[i] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    fetch_values(0);
+    asm volatile("" ::: "memory");  // not put off behind it
+    // online softmax, a column of lanes a row
+    u32x4 pf[GT];
+    uint32_t bits[GT];
+    float sv[GT][8], mx[GT];
+    bool risen = false;
+#pragma unroll
+    for (int t = 0; t < GT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sv[t][e] = e < 4 ? s0[t][e] : s1[t][e - 4];
+      if constexpr (MASKED) {
+        // the 32 keys from tok on, as this row sees them
+        const uint32_t* words = p.mask + (size_t)(token0 + node[t]) * p.words;
+        const int j0 = tok - ctx;
+        if (j0 <= -kChunk) {
+          bits[t] = 0xffffffffu;
+        } else if (j0 < 0) {
+          bits[t] = (words[0] << -j0) | ((1u << -j0) - 1u);
+        } else {
+          const int w = j0 >> 5, sh = j0 & 31;
+          const uint32_t lo = w < p.words ? words[w] : 0u, hi = w + 1 < p.words ? words[w + 1] : 0u;
+          bits[t] = (uint32_t)(((uint64_t)hi << 32 | lo) >> sh);
+        }
+        if (tok + kChunk > all) bits[t] &= (1u << (all - tok)) - 1u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!(bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u)) sv[t][e] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(sv[t][0], sv[t][1]), fmaxf(sv[t][2], sv[t][3])), fmaxf(fmaxf(sv[t][4], sv[t][5]), fmaxf(sv[t][6], sv[t][7])));
+      mx[t] = column_max(top) * k_mul;
+      risen |= mx[t] > m_run[t] + kSlack;
+    }
+    if (__builtin_amdgcn_ballot_w64(risen) != 0) {
+#pragma unroll
+      for (int t = 0; t < GT; ++t) {
+        const float m_new = fmaxf(m_run[t], mx[t]);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_new);
+        m_run[t] = m_new;
+        sum[t] *= alpha;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc[t][i] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < GT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sv[t][e] = __builtin_amdgcn_exp2f(fmaf(sv[t][e], k_mul, -m_run[t]));
+        if constexpr (MASKED) sv[t][e] = bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u ? sv[t][e] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) pf[t][e >> 1] = round_pair<BF16>(sv[t][e], sv[t][e + 1]);
+      sum[t] = mfma16<BF16>(ones, pf[t], sum[t]);  // of the probabilities as rounded
+    }
+    // O^T += V^T P^T
+#pragma unroll
+    for (int i0 = 0; i0 < D / 16; i0 += kHeld) {
+      if (i0) fetch_values(i0);
+#pragma unroll
+      for (int n = 0; n < kHeld; ++n) {
+        const int i = i0 + n;
+#pragma unroll
+        for (int t = 0; t < GT; ++t) acc[t][i] = mfma16<BF16>(vt[n], pf[t], acc[t][i]);
+      }
+    }
+    if constexpr (MASKED) {
+      // Values of new tokens that are infinite or NaN are zeros in LDS, where they would meet the zero probabilities of rows that do not see them, and are
+      // added here, from the cache, for the rows that do.
+      for (unsigned int left = odd; left; left &= left - 1) {
+        const int key = __builtin_ctz(left), n = tok + key;
+        const int e_key = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16 + c;
+        int block = table[n / p.bs];
+        if ((unsigned)block >= (unsigned)p.pool_blocks) block = 0;
+        const size_t row = (((size_t)block * p.hkv + h) * p.bs + n % p.bs) * D;
+#pragma unroll
+        for (int t = 0; t < GT; ++t) {
+          const uint32_t pair = (uint32_t)(e_key < 4 ? (e_key < 2 ? __shfl((int)pf[t][0], from) : __shfl((int)pf[t][1], from))
+                                                     : (e_key < 6 ? __shfl((int)pf[t][2], from) : __shfl((int)pf[t][3], from)));
+          const float prob = (float)__builtin_bit_cast(T, (uint16_t)(e_key & 1 ? pair >> 16 : pair));
+          if (!(bits[t] >> key & 1u)) continue;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float v = elem<typename std::conditional<FP8, uint8_t, T>::type>(p.vc, row + i * 16 + j * 4 + r);
+              if (!(fabsf(v) <= 3.4e38f)) acc[t][i][r] = fmaf(prob, v, acc[t][i][r]);
+            }
+        }
       }
     }
   };
 
-  float k_mul = p.scale_log2e, v_unit = 1.f;
-  load_window(tok_first / p.bs);
-  request(tok_first);
-  if constexpr (FP8) {
-    k_mul = k_mul_next;
-    v_unit = v_unit_next;
-  }
+  using pto_hip::block8::IntConst;
+  load_window(lb);
+  request(IntConst<0>{}, tok_first);
+  request(IntConst<1>{}, tok_first + kChunk);
   lds_barrier();  // the flags are cleared
-  if (tok_first < tok_end) park(0, 0, tok_first);
-  request(tok_first + kChunk);
-  lds_barrier();
-  int stage = 0, odd_place = 0;
-  for (int tok = tok_first; tok < tok_end; tok += kChunk) {
-    const float k_next = k_mul_next, v_next = v_unit_next;
-    if (tok + kChunk < tok_end) {
-      park(stage ^ 1, odd_place == 2 ? 0 : odd_place + 1, tok + kChunk);
-      request(tok + 2 * kChunk);
-    }
-    const char* kbase = lds + stage * S::kBytes;
-    const char* vbase = kbase + kChunk * S::kPitch;
-    if (active) {
-      const bool masked = tok + kChunk > ctx;
-      const unsigned int odd = masked ? odd_keys[odd_place] : 0u;
-      // S^T: rows = keys, columns = query rows
-      f32x4 s0[GT], s1[GT];
-#pragma unroll
-      for (int t = 0; t < GT; ++t) s0[t] = s1[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < S::kRow / 64; ++u) {
-        const u32x4 a0 = *reinterpret_cast<const u32x4*>(kbase + c * S::kPitch + (u * 4 + j) * 16);
-        const u32x4 a1 = *reinterpret_cast<const u32x4*>(kbase + (16 + c) * S::kPitch + (u * 4 + j) * 16);
-        if constexpr (FP8) {
-          const u32x4 lo0 = fp8x8_widen<BF16>(a0[0], a0[1]), hi0 = fp8x8_widen<BF16>(a0[2], a0[3]);
-          const u32x4 lo1 = fp8x8_widen<BF16>(a1[0], a1[1]), hi1 = fp8x8_widen<BF16>(a1[2], a1[3]);
-#pragma unroll
-          for (int t = 0; t < GT; ++t) {
-            s0[t] = mfma16<BF16>(lo0, qf[t][2 * u], s0[t]);
-            s1[t] = mfma16<BF16>(lo1, qf[t][2 * u], s1[t]);
-            s0[t] = mfma16<BF16>(hi0, qf[t][2 * u + 1], s0[t]);
-            s1[t] = mfma16<BF16>(hi1, qf[t][2 * u + 1], s1[t]);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < GT; ++t) {
-            s0[t] = mfma16<BF16>(a0, qf[t][u], s0[t]);
-            s1[t] = mfma16<BF16>(a1, qf[t][u], s1[t]);
-          }
-        }
-      }
-      // online softmax, a column of lanes a row
-      u32x4 pf[GT];
-      uint32_t bits[GT];
-#pragma unroll
-      for (int t = 0; t < GT; ++t) {
-        float sv[8] = {s0[t][0], s0[t][1], s0[t][2], s0[t][3], s1[t][0], s1[t][1], s1[t][2], s1[t][3]};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] *= k_mul;
-        bits[t] = 0xffffffffu;
-        if (masked) {
-          // the 32 keys from tok on, as this row sees them
-          const uint32_t* words = p.mask + (size_t)(token0 + node[t]) * p.words;
-          const int j0 = tok - ctx;
-          if (j0 < 0) {
-            bits[t] = (words[0] << -j0) | ((1u << -j0) - 1u);
-          } else {
-            const int w = j0 >> 5, sh = j0 & 31;
-            const uint32_t lo = w < p.words ? words[w] : 0u, hi = w + 1 < p.words ? words[w + 1] : 0u;
-            bits[t] = (uint32_t)(((uint64_t)hi << 32 | lo) >> sh);
-          }
-          if (tok + kChunk > all) bits[t] &= (1u << (all - tok)) - 1u;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!(bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u)) sv[e] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__builtin_amdgcn_ballot_w64(mx > m_run[t]) != 0) {
-          const float m_new = fmaxf(m_run[t], mx);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_new);
-          m_run[t] = m_new;
-          l_run[t] *= alpha;
-#pragma unroll
-          for (int a = 0; a < kSets; ++a)
-#pragma unroll
-            for (int i = 0; i < kEpl; ++i) acc[t][a][i] *= alpha;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          float ra, rb;
-          pf[t][e >> 1] = round_pack<BF16>(__builtin_amdgcn_exp2f(sv[e] - m_run[t]), __builtin_amdgcn_exp2f(sv[e + 1] - m_run[t]), ra, rb);
-          sum += ra + rb;
-        }
-        l_run[t] += sum;
-      }
-      // O^T += V^T P^T: a lane's 8 tokens x kEpl elements, transposed in registers
-#pragma unroll
-      for (int a = 0; a < kSets; ++a) {
-        u32x4 vw[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const char* src = vbase + ((e >> 2) * 16 + j * 4 + (e & 3)) * S::kPitch + (a * 16 + c) * kEpl * kEsz;
-          if constexpr (FP8) {
-            if constexpr (kEpl == 8) {
-              const u32x2 w = *reinterpret_cast<const u32x2*>(src);
-              vw[e] = fp8x8_widen<BF16>(w[0], w[1]);
-            } else {
-              vw[e] = fp8x8_widen<BF16>(*reinterpret_cast<const uint32_t*>(src), 0u);
-            }
-          } else if constexpr (kEpl == 8) {
-            vw[e] = *reinterpret_cast<const u32x4*>(src);
-          } else {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(src);
-            vw[e] = u32x4{w[0], w[1], 0u, 0u};
-          }
-        }
-        if (odd) {
-          // Values of new tokens that are infinite or NaN are left out of the product, where they would meet the zero probabilities of rows that do not see
-          // them, and added for the rows that do.
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (!(odd >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u)) continue;
-#pragma unroll
-            for (int i = 0; i < kEpl / 2; ++i) vw[e][i] = drop_unbounded<BF16>(vw[e][i]);
-          }
-          for (unsigned int left = odd; left; left &= left - 1) {
-            const int key = __builtin_ctz(left);
-            const int e_key = (key >> 4) * 4 + (key & 3), from = ((key >> 2) & 3) * 16 + c;
-#pragma unroll
-            for (int t = 0; t < GT; ++t) {
-              const uint32_t pair = (uint32_t)(e_key < 4 ? (e_key < 2 ? __shfl((int)pf[t][0], from) : __shfl((int)pf[t][1], from))
-                                                         : (e_key < 6 ? __shfl((int)pf[t][2], from) : __shfl((int)pf[t][3], from)));
-              const uint16_t half = (uint16_t)(e_key & 1 ? pair >> 16 : pair);
-              const float prob = (float)__builtin_bit_cast(T, half);
-              if (!(bits[t] >> key & 1u)) continue;
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int i = 0; i < kEpl; ++i) {
-                  const int el = (a * 16 + j * 4 + r) * kEpl + i;
-                  float v;
-                  if constexpr (FP8) v = __builtin_amdgcn_cvt_f32_fp8((int)*reinterpret_cast<const uint8_t*>(vbase + key * S::kPitch + el), 0);
-                  else v = (float)reinterpret_cast<const T*>(vbase + key * S::kPitch)[el];
-                  if (!(fabsf(v) <= 3.4e38f)) acc[t][a][i][r] = fmaf(prob, v, acc[t][a][i][r]);
-                }
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kEpl; ++i) {
-          const uint32_t sel = (i & 1) ? 0x07060302u : 0x05040100u;
-          u32x4 vt;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) vt[kk] = __builtin_amdgcn_perm(vw[2 * kk + 1][i >> 1], vw[2 * kk][i >> 1], sel);
-#pragma unroll
-          for (int t = 0; t < GT; ++t) acc[t][a][i] = mfma16<BF16>(vt, pf[t], acc[t][a][i]);
-        }
-      }
-    }
+  int odd_place = 0;
+  // Chunk `tok`, whose rows lie in stage SET: the next one goes to the other stage, the one behind that is asked for.
+  auto step = [&](auto set, int tok, auto masked) __attribute__((always_inline)) {
+    constexpr int SET = decltype(set)::value;
+    if (tok + kChunk < tok_end) park(IntConst<SET ^ 1>{}, SET ^ 1, odd_place == 2 ? 0 : odd_place + 1, tok + kChunk);
+    const float v_next = v_units[SET ^ 1], k_next = k_muls[SET ^ 1];
+    request(IntConst<SET ^ 1>{}, tok + 3 * kChunk);
+    if (active) multiply(lds + SET * S::kBytes, tok, decltype(masked)::value ? odd_keys[odd_place] : 0u, masked);
     if constexpr (FP8) {
       // the next chunk may be another block's: the accumulators go on in its values' scale
       if (tok + kChunk < tok_end) {
@@ -582,9 +601,7 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
 #pragma unroll
           for (int t = 0; t < GT; ++t)
 #pragma unroll
-            for (int a = 0; a < kSets; ++a)
-#pragma unroll
-              for (int i = 0; i < kEpl; ++i) acc[t][a][i] *= ratio;
+            for (int i = 0; i < D / 16; ++i) acc[t][i] *= ratio;
           v_unit = v_next;
         }
         k_mul = k_next;
@@ -592,45 +609,47 @@ __global__ __launch_bounds__(NW * 64) void tree_kernel(Params p) {
     }
     if (threadIdx.x == 0) odd_keys[odd_place == 0 ? 2 : odd_place - 1] = 0;
     lds_barrier();
-    stage ^= 1;
     odd_place = odd_place == 2 ? 0 : odd_place + 1;
+  };
+  if (tok_first < tok_end) {
+    park(IntConst<0>{}, 0, 0, tok_first);
+    if constexpr (FP8) {
+      k_mul = k_muls[0];
+      v_unit = v_units[0];
+    }
+    request(IntConst<0>{}, tok_first + 2 * kChunk);
+    lds_barrier();
+    // chunks that lie in the cache as it was, two at a time, then the others
+    int tok = tok_first;
+    const int plain_end = min(tok_end, ctx);
+    for (; tok + 2 * kChunk <= plain_end; tok += 2 * kChunk) {
+      step(IntConst<0>{}, tok, std::false_type{});
+      step(IntConst<1>{}, tok + kChunk, std::false_type{});
+    }
+    for (; tok < tok_end; tok += 2 * kChunk) {
+      step(IntConst<0>{}, tok, std::true_type{});
+      if (tok + kChunk < tok_end) step(IntConst<1>{}, tok + kChunk, std::true_type{});
+    }
   }
   if (bad_entry) *p.error_flag = 1;
   if (!active) return;
 #pragma unroll
   for (int t = 0; t < GT; ++t) {
-    float l = l_run[t];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const float l = sum[t][0];
     const int r = row0 + t * 16 + c;
     if (r >= rows) continue;
     const int head = h * p.group + r % p.group;
     if (parts == 1) {
       const float mul = l > 0.f || l != l ? v_unit / l : 0.f;
-      T* out = reinterpret_cast<T*>(p.out) + ((size_t)(token0 + node[t]) * p.hq + head) * D;
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)(token0 + node[t]) * p.hq + head) * D + j * 4;
 #pragma unroll
-      for (int a = 0; a < kSets; ++a)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint32_t w[kEpl / 2];
-#pragma unroll
-          for (int i = 0; i < kEpl; i += 2)
-            w[i / 2] = (uint32_t)__builtin_bit_cast(uint16_t, (T)(acc[t][a][i][u] * mul)) |
-                       (uint32_t)__builtin_bit_cast(uint16_t, (T)(acc[t][a][i + 1][u] * mul)) << 16;
-          T* dst = out + (a * 16 + j * 4 + u) * kEpl;
-          if constexpr (kEpl == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{w[0], w[1], w[2], w[3]};
-          else *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
-        }
+      for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<u32x2*>(out + i * 16) =
+            u32x2{round_pair<BF16>(acc[t][i][0] * mul, acc[t][i][1] * mul), round_pair<BF16>(acc[t][i][2] * mul, acc[t][i][3] * mul)};
     } else {
-      const size_t slot = ((size_t)(s.slot + (int64_t)part * count + node[t])) * p.hq + head;
+      const size_t slot = (size_t)(s.slot + part * count + node[t]) * p.hq + head;
 #pragma unroll
-      for (int a = 0; a < kSets; ++a)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int i = 0; i < kEpl; i += 4)
-            *reinterpret_cast<f32x4*>(p.part_o + slot * D + (a * 16 + j * 4 + u) * kEpl + i) =
-                f32x4{acc[t][a][i][u] * v_unit, acc[t][a][i + 1][u] * v_unit, acc[t][a][i + 2][u] * v_unit, acc[t][a][i + 3][u] * v_unit};
+      for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(p.part_o + slot * D + i * 16 + j * 4) = acc[t][i] * v_unit;
       if (j == 0) {
         p.part_ml[slot * 2] = m_run[t];
         p.part_ml[slot * 2 + 1] = l;
@@ -648,19 +667,18 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int rows) {
   const int token = (int)(row / p.hq), head = (int)(row % p.hq);
   const Work first64 = work_of(p, lane, rows);
   const int keys = part_keys(p, rows, lane, first64);
-  int64_t slots = 0;
+  int slots = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
-    const int parts = parts_of(w, keys);
-    const int64_t held = parts > 1 ? (int64_t)parts * w.count : 0;
-    const int64_t slot_to = slots + wave_scan(held, lane);
+    const int parts = parts_of(w, keys), held = held_of(p, w, parts);
+    const int slot_to = pto_hip::wave_running_sum(held) + slots;
     const uint64_t own = __ballot(w.count > 0 && w.first <= token && token < w.first + w.count);
     if (own) {
       const int k = __builtin_ctzll(own);
-      const int np = __shfl(parts, k), count = __shfl(w.count, k);
-      const int64_t slot = from_lane(slot_to - held, k);
-      if (np <= 1 || slot + (int64_t)np * count > p.slots) return;
-      const size_t first = ((size_t)slot + (token - __shfl(w.first, k))) * p.hq + head, step = (size_t)count * p.hq;
+      const int np = __builtin_amdgcn_readlane(parts, k), count = __builtin_amdgcn_readlane(w.count, k);
+      const int slot = __builtin_amdgcn_readlane(slot_to - held, k);
+      if (np <= 1 || slot < 0 || (int64_t)slot + (int64_t)np * count > p.slots) return;
+      const size_t first = ((size_t)slot + (token - __builtin_amdgcn_readlane(w.first, k))) * p.hq + head, step = (size_t)count * p.hq;
       float m = kMinMax, l = 0.f, o[D / 64];
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
@@ -702,7 +720,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int rows) {
       for (int i = 0; i < D / 64; ++i) reinterpret_cast<T*>(p.out)[((size_t)token * p.hq + head) * D + i * 64 + lane] = (T)(o[i] * inv);
       return;
     }
-    slots = from_lane(slot_to, 63);
+    slots = min(__builtin_amdgcn_readlane(slot_to, 63), p.slots + 1);
   }
 }
 
@@ -710,20 +728,21 @@ template <int D, bool BF16, bool FP8, int NW, int GT>
 int launch_tiles(Params& p, hipStream_t st) {
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
   constexpr int kRows = NW * GT * 16;
-  constexpr int kLds = 2 * Stage<D, FP8>::kBytes;
-  static bool allowed = false;
-  if (!allowed && kLds > 64 * 1024) {
-    PTO_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&tree_kernel<D, BF16, FP8, NW, GT>), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-    allowed = true;
+  constexpr int kLds = 2 * Stage<D>::kBytes;
+  static int resident = 0;  // workgroups that a CU holds (calls take turns: PTO_DISPATCH_LOCK)
+  if (resident == 0) {
+    const void* kernel = reinterpret_cast<const void*>(&tree_kernel<D, BF16, FP8, NW, GT>);
+    if (kLds > 64 * 1024) PTO_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+    int n = 0;
+    PTO_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, NW * 64, kLds));
+    resident = std::max(1, n);
   }
-  // wavefronts of 256 registers: two to a SIMD; LDS may hold fewer workgroups
-  const int by_waves = std::max(1, 8 / NW), by_lds = std::max(1, (160 * 1024) / (kLds + 64));
-  p.target = pto_hip::ctx().num_cu * std::min(by_waves, by_lds);
+  p.target = pto_hip::ctx().num_cu * resident;
   p.least = std::max(64, kRows);
   const int64_t blocks = (int64_t)p.tokens * p.group / kRows + std::min(p.batch, p.tokens);
   const int64_t grid = p.target + blocks * p.hkv;
   const int64_t slots = ((int64_t)p.target * kRows + p.hq - 1) / p.hq + p.tokens + 1;
-  PTO_CHECK_ARG(grid < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
+  PTO_CHECK_ARG(grid < 1ll << 24 && slots < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
   const size_t o_bytes = (size_t)slots * p.hq * D * 4, ml_bytes = (size_t)slots * p.hq * 8;
   void* ws = nullptr;
   const int rc = pto_hip::workspace(o_bytes + ml_bytes, &ws);
@@ -739,11 +758,11 @@ int launch_tiles(Params& p, hipStream_t st) {
 template <int D, bool BF16, bool FP8>
 int launch_rows(Params& p, hipStream_t st) {
   const int64_t rows = (int64_t)std::min<int64_t>((p.tokens + p.batch - 1) / p.batch, 32 * p.words) * p.group;  // of a sequence, on average
-  if (rows <= 32) return launch_tiles<D, BF16, FP8, 2, 1>(p, st);
-  if (rows <= 64) return launch_tiles<D, BF16, FP8, 4, 1>(p, st);
-  if constexpr (D == 256) {  // two tiles' accumulators of a wavefront would leave no room for a second one on its SIMD
+  if constexpr (D == 256) {  // fewer wavefronts would bring so much each that their registers did not hold it
     return launch_tiles<D, BF16, FP8, 8, 1>(p, st);
   } else {
+    if (rows <= 32) return launch_tiles<D, BF16, FP8, 2, 1>(p, st);
+    if (rows <= 64) return launch_tiles<D, BF16, FP8, 4, 1>(p, st);
     if (rows <= 128) return launch_tiles<D, BF16, FP8, 4, 2>(p, st);
     return launch_tiles<D, BF16, FP8, 8, 2>(p, st);
   }
