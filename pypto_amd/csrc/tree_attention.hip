@@ -248,12 +248,12 @@ __device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int
   return s;
 }
 
-// LDS of a stage: K rows and V rows as 16-bit values, 16 bytes apart from each other beyond their length, so that 16 rows read at one column lie in
-// different banks.
+// LDS of a stage: K rows and V rows as 16-bit values, 32 bytes apart from each other beyond their length: eight rows read 16 bytes wide at one column lie in
+// different banks, and so do four rows read 32 bytes wide.
 template <int D>
 struct Stage {
   static constexpr int kRow = 2 * D;
-  static constexpr int kPitch = kRow + 16;
+  static constexpr int kPitch = kRow + 32;
   static constexpr int kBytes = 2 * kChunk * kPitch;
 };
 
@@ -294,7 +294,7 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 }
 
 // A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.
-constexpr float kSlack = 6.f;
+constexpr int kSlack = 6;
 
 template <int D, bool BF16, bool FP8, int NW, int GT>
 __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
@@ -489,15 +489,21 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
     };
     fetch_values(0);
     asm volatile("" ::: "memory");  // not put off behind it
-    // online softmax, a column of lanes a row
+    // Online softmax, a column of lanes a row.  The probabilities are taken against the maximum so far first: as long as none passes 2^kSlack - each lane looks at its
+    // own - there is no need to know the chunk's maximum, nor to bring sums and accumulators to it.
     u32x4 pf[GT];
     uint32_t bits[GT];
-    float sv[GT][8], mx[GT];
+    float pv[GT][8];
     bool risen = false;
+    auto probabilities = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pv[t][e] = __builtin_amdgcn_exp2f(fmaf(e < 4 ? s0[t][e] : s1[t][e - 4], k_mul, -m_run[t]));
+        if constexpr (MASKED) pv[t][e] = bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u ? pv[t][e] : 0.f;
+      }
+    };
 #pragma unroll
     for (int t = 0; t < GT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sv[t][e] = e < 4 ? s0[t][e] : s1[t][e - 4];
       if constexpr (MASKED) {
         // the 32 keys from tok on, as this row sees them
         const uint32_t* words = p.mask + (size_t)(token0 + node[t]) * p.words;
@@ -512,34 +518,35 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
           bits[t] = (uint32_t)(((uint64_t)hi << 32 | lo) >> sh);
         }
         if (tok + kChunk > all) bits[t] &= (1u << (all - tok)) - 1u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!(bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u)) sv[t][e] = -INFINITY;
       }
-      const float top = fmaxf(fmaxf(fmaxf(sv[t][0], sv[t][1]), fmaxf(sv[t][2], sv[t][3])), fmaxf(fmaxf(sv[t][4], sv[t][5]), fmaxf(sv[t][6], sv[t][7])));
-      mx[t] = column_max(top) * k_mul;
-      risen |= mx[t] > m_run[t] + kSlack;
+      probabilities(t);
+      risen |= fmaxf(fmaxf(fmaxf(pv[t][0], pv[t][1]), fmaxf(pv[t][2], pv[t][3])), fmaxf(fmaxf(pv[t][4], pv[t][5]), fmaxf(pv[t][6], pv[t][7]))) >
+               (float)(1 << kSlack);
     }
     if (__builtin_amdgcn_ballot_w64(risen) != 0) {
 #pragma unroll
       for (int t = 0; t < GT; ++t) {
-        const float m_new = fmaxf(m_run[t], mx[t]);
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = e < 4 ? s0[t][e] : s1[t][e - 4];
+          bool seen = true;
+          if constexpr (MASKED) seen = bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u;
+          top = fmaxf(top, seen ? x : -INFINITY);
+        }
+        const float m_new = fmaxf(m_run[t], column_max(top) * k_mul);
         const float alpha = __builtin_amdgcn_exp2f(m_run[t] - m_new);
         m_run[t] = m_new;
         sum[t] *= alpha;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[t][i] *= alpha;
+        probabilities(t);
       }
     }
 #pragma unroll
     for (int t = 0; t < GT; ++t) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        sv[t][e] = __builtin_amdgcn_exp2f(fmaf(sv[t][e], k_mul, -m_run[t]));
-        if constexpr (MASKED) sv[t][e] = bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u ? sv[t][e] : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) pf[t][e >> 1] = round_pair<BF16>(sv[t][e], sv[t][e + 1]);
+      for (int e = 0; e < 8; e += 2) pf[t][e >> 1] = round_pair<BF16>(pv[t][e], pv[t][e + 1]);
       sum[t] = mfma16<BF16>(ones, pf[t], sum[t]);  // of the probabilities as rounded
     }
     // O^T += V^T P^T

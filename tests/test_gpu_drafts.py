@@ -401,7 +401,9 @@ def test_tree_reports_lengths_and_blocks_that_do_not_fit(worker):
 
 
 def test_tree_of_one_token_is_paged_attention(worker):
-    """One new token per sequence that sees itself: what paged_attention gives for contexts one longer."""
+    """One new token per sequence that sees itself: what paged_attention gives for contexts one longer.  Both round every probability once, to half a step
+    of bfloat16 on either side of its value, and their row sums are of the rounded ones: each is off by at most 2^-8 of sum p |v| + |out|, besides this one's
+    rounding of the result."""
     lens = [(0, 1), (77, 1), (1000, 1), (2047, 1)]
     b = Batch(9, lens, 8, 128, 128, BF)
     q = _randn(b.g, 4 * 32, 128).to(BF)
@@ -412,7 +414,9 @@ def test_tree_of_one_token_is_paged_attention(worker):
     cfg = torch.tensor([4, 32, 8, 128, 128, width, int(np.float32(128 ** -0.5).view(np.uint32))], dtype=torch.int64)
     worker.run(runtime.paged_attention, q, b.key, b.value, b.blocks.flatten(), b.ctx + 1, want, cfg)
     worker.sync()
-    assert ((out.float() - want).abs() <= 2.0 ** -7 * (want.abs() + 0.1)).all()
+    exact, mass, reach = od.tree_attention(q, b.key, b.value, b.blocks, b.ctx, b.starts, mask, 32, 8, 128, 128, 128 ** -0.5)
+    off = 2 * (2.0 ** -8 + 2 * reach * 140 * 2.0 ** -24 + 2.0 ** -19) * (mass + exact.abs()) + 2.0 ** -8 * exact.abs()
+    assert ((out.double() - want.double()).abs().cpu().view(4, 32, 128) <= off).all()
 
 
 # ---- sample_tokens ---------------------------------------------------------------------------------------
