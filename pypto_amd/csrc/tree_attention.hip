@@ -375,7 +375,10 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
     if constexpr (FP8) {
       win_ks = used ? p.k_scale[(size_t)win_blk * p.hkv + h] : 1.f;
       win_vs = used ? p.v_scale[(size_t)win_blk * p.hkv + h] : 1.f;
+      asm volatile("" : "+v"(win_ks), "+v"(win_vs));
     }
+    // the wait for these loads belongs here, on a branch rarely taken: left to their first use it would become one for every load in flight, each chunk
+    asm volatile("" : "+v"(win_blk));
   };
   // The next 16 tokens to be asked for: logical block and place in it (a block is a multiple of 16 tokens).
   int lb = tok_first / p.bs, off = tok_first % p.bs;
@@ -383,14 +386,13 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   // two chunks on their way to LDS, and the scales of their keys and values
   u32x4 kr[2][kPieces], vr[2][kPieces];
   float k_muls[2] = {scale, scale}, v_units[2] = {1.f, 1.f};
+  // Every request is as many loads, with nothing to skip them, so that the number in flight at each wait is known to the compiler.  Where no tokens are left the
+  // window's blocks are block 0, whose rows lie in the cache as any block's.
   auto request = [&](auto set, int tok) __attribute__((always_inline)) {
     constexpr int SET = decltype(set)::value;
-    if (tok >= tok_end) return;
     int lb1 = lb, off1 = off + 16;
-    if (off1 == p.bs) {
-      off1 = 0;
-      ++lb1;
-    }
+    lb1 += off1 == p.bs;
+    off1 = off1 == p.bs ? 0 : off1;
     if (lb1 >= win_base + 64) load_window(lb);
     const int slot = lb - win_base;
     const int blk0 = __builtin_amdgcn_readlane(win_blk, slot), blk1 = __builtin_amdgcn_readlane(win_blk, lb1 - win_base);
@@ -400,28 +402,19 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
     }
     const size_t at0 = (((size_t)blk0 * p.hkv + h) * p.bs + off) * kRowBytes;
     const size_t at1 = (((size_t)blk1 * p.hkv + h) * p.bs + off1) * kRowBytes - 16 * kRowBytes;
-    lb = lb1;
     off = off1 + 16;
-    if (off == p.bs) {
-      off = 0;
-      ++lb;
-    }
+    lb = lb1 + (off == p.bs);
+    off = off == p.bs ? 0 : off;
     const char* kc = reinterpret_cast<const char*>(p.kc);
     const char* vc = reinterpret_cast<const char*>(p.vc);
-    auto bring = [&](bool whole) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int item = threadIdx.x + i * kThreads, row = item * 16 / kRowBytes;
-        // rows from tok_end on are zeros: what lies there has no part in anything
-        const bool there = (kItems % kThreads == 0 || item < kItems) && (whole || tok + row < tok_end);
-        const size_t at = (row < 16 ? at0 : at1) + (size_t)item * 16;
-        const u32x4 z = {0u, 0u, 0u, 0u};
-        kr[SET][i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at)) : z;
-        vr[SET][i] = there ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at)) : z;
-      }
-    };
-    if (tok + kChunk <= tok_end) bring(true);
-    else bring(false);
+    for (int i = 0; i < kPieces; ++i) {
+      int item = threadIdx.x + i * kThreads;
+      if constexpr (kItems % kThreads != 0) item = min(item, kItems - 1);
+      const size_t at = (item * 16 / kRowBytes < 16 ? at0 : at1) + (size_t)item * 16;
+      kr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at));
+      vr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at));
+    }
   };
   auto park = [&](auto set, int stage, int odd_place, int tok) __attribute__((always_inline)) {
     constexpr int SET = decltype(set)::value;
@@ -433,10 +426,14 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
       const int row = item * 16 / kRowBytes, col = item * 16 % kRowBytes * (2 / kEsz);
       char* k = base + row * S::kPitch + col;
       char* v = k + kChunk * S::kPitch;
-      u32x4 v0 = vr[SET][i], v1 = {0u, 0u, 0u, 0u};
+      // rows from tok_end on are zeros: what lies there has no part in anything
+      const bool there = tok + row < tok_end;
+      const u32x4 z = {0u, 0u, 0u, 0u};
+      const u32x4 kx = there ? kr[SET][i] : z, vx = there ? vr[SET][i] : z;
+      u32x4 v0 = vx, v1 = z;
       if constexpr (FP8) {  // widened once for all wavefronts; exact
-        v0 = fp8x8_widen<BF16>(vr[SET][i][0], vr[SET][i][1]);
-        v1 = fp8x8_widen<BF16>(vr[SET][i][2], vr[SET][i][3]);
+        v0 = fp8x8_widen<BF16>(vx[0], vx[1]);
+        v1 = fp8x8_widen<BF16>(vx[2], vx[3]);
       }
       if (tok + kChunk > ctx) {
         if (tok + row >= ctx) {
@@ -446,11 +443,11 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
         }
       }
       if constexpr (FP8) {
-        *reinterpret_cast<u32x4*>(k) = fp8x8_widen<BF16>(kr[SET][i][0], kr[SET][i][1]);
-        *reinterpret_cast<u32x4*>(k + 16) = fp8x8_widen<BF16>(kr[SET][i][2], kr[SET][i][3]);
+        *reinterpret_cast<u32x4*>(k) = fp8x8_widen<BF16>(kx[0], kx[1]);
+        *reinterpret_cast<u32x4*>(k + 16) = fp8x8_widen<BF16>(kx[2], kx[3]);
         *reinterpret_cast<u32x4*>(v + 16) = v1;
       } else {
-        *reinterpret_cast<u32x4*>(k) = kr[SET][i];
+        *reinterpret_cast<u32x4*>(k) = kx;
       }
       *reinterpret_cast<u32x4*>(v) = v0;
     }
@@ -596,7 +593,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   // Chunk `tok`, whose rows lie in stage SET: the next one goes to the other stage, the one behind that is asked for.
   auto step = [&](auto set, int tok, auto masked) __attribute__((always_inline)) {
     constexpr int SET = decltype(set)::value;
-    if (tok + kChunk < tok_end) park(IntConst<SET ^ 1>{}, SET ^ 1, odd_place == 2 ? 0 : odd_place + 1, tok + kChunk);
+    park(IntConst<SET ^ 1>{}, SET ^ 1, odd_place == 2 ? 0 : odd_place + 1, tok + kChunk);
     const float v_next = v_units[SET ^ 1], k_next = k_muls[SET ^ 1];
     request(IntConst<SET ^ 1>{}, tok + 3 * kChunk);
     if (active) multiply(lds + SET * S::kBytes, tok, decltype(masked)::value ? odd_keys[odd_place] : 0u, masked);
