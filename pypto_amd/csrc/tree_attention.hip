@@ -296,7 +296,7 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 // A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.
 constexpr int kSlack = 6;
 
-template <int D, bool BF16, bool FP8, int NW, int GT>
+template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
 __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   typedef Stage<D> S;
   constexpr int kThreads = NW * 64, kRows = NW * GT * 16;
@@ -306,9 +306,14 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   constexpr int kPieces = (kItems + kThreads - 1) / kThreads;  // ... a thread brings
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // of chunk n in place n % 3: new tokens whose values hold infinities or NaN, as bits.  A place is read while the next is written and the one
-  // behind it cleared.
-  __shared__ unsigned int odd_keys[3];
+  // Chunk n lies in stage n % kStages.  Between two barriers the wavefronts multiply AHEAD chunks and bring the AHEAD behind those, each at its own pace: held
+  // together at every chunk, the two of a SIMD would be at the same kind of work all along.
+  constexpr int kStages = 2 * AHEAD;
+  // Of chunk n in place n % kPlaces: new tokens whose values hold infinities or NaN, as bits.  A place is read between two barriers, cleared between the next two
+  // and written again behind those.
+  constexpr int kPlaces = 3 * AHEAD;
+  __shared__ unsigned int odd_keys[kPlaces];
+  __shared__ float2 chunk_scale[kStages];  // e4m3 caches: of the chunk's keys and values
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, j = lane >> 4;
   const Share s = share_of(p, kRows, blockIdx.x, lane);
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   const int rows = count * p.group;
   const bool active = row0 < rows;
   if (threadIdx.x == 0) {
-    odd_keys[0] = odd_keys[1] = odd_keys[2] = 0;
+    for (int i = 0; i < kPlaces; ++i) odd_keys[i] = 0;
     const int64_t raw = p.ctx_lens[seq];
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
@@ -419,6 +424,9 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   auto park = [&](auto set, int stage, int odd_place, int tok) __attribute__((always_inline)) {
     constexpr int SET = decltype(set)::value;
     char* base = lds + stage * S::kBytes;
+    if constexpr (FP8) {
+      if (threadIdx.x == 0) chunk_scale[stage] = float2{k_muls[SET], v_units[SET]};
+    }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int item = threadIdx.x + i * kThreads;
@@ -589,39 +597,46 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   request(IntConst<0>{}, tok_first);
   request(IntConst<1>{}, tok_first + kChunk);
   lds_barrier();  // the flags are cleared
-  int odd_place = 0;
-  // Chunk `tok`, whose rows lie in stage SET: the next one goes to the other stage, the one behind that is asked for.
-  auto step = [&](auto set, int tok, auto masked) __attribute__((always_inline)) {
-    constexpr int SET = decltype(set)::value;
-    park(IntConst<SET ^ 1>{}, SET ^ 1, odd_place == 2 ? 0 : odd_place + 1, tok + kChunk);
-    const float v_next = v_units[SET ^ 1], k_next = k_muls[SET ^ 1];
-    request(IntConst<SET ^ 1>{}, tok + 3 * kChunk);
-    if (active) multiply(lds + SET * S::kBytes, tok, decltype(masked)::value ? odd_keys[odd_place] : 0u, masked);
+  int stage = 0, place = 0, until_barrier = AHEAD;  // of the chunk to be multiplied
+  auto behind = [](int i, int by, int n) { return i + by >= n ? i + by - n : i + by; };
+  // Chunk number n = PARITY modulo 2, of the tokens from `tok` on.  The AHEAD-th behind it goes to its stage, the second behind that is asked for.
+  auto step = [&](auto parity, int tok, auto masked) __attribute__((always_inline)) {
+    constexpr int SET = (decltype(parity)::value + AHEAD) & 1;
+    park(IntConst<SET>{}, behind(stage, AHEAD, kStages), behind(place, AHEAD, kPlaces), tok + AHEAD * kChunk);
+    request(IntConst<SET>{}, tok + (AHEAD + 2) * kChunk);
     if constexpr (FP8) {
-      // the next chunk may be another block's: the accumulators go on in its values' scale
-      if (tok + kChunk < tok_end) {
-        if (v_next != v_unit) {
-          const float ratio = v_unit / v_next;
+      const float2 s = chunk_scale[stage];
+      k_mul = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s.x)));
+      const float v_now = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s.y)));
+      // the chunk may be another block's than the one in front: the accumulators go on in its values' scale
+      if (v_now != v_unit) {
+        const float ratio = tok == tok_first ? 1.f : v_unit / v_now;
 #pragma unroll
-          for (int t = 0; t < GT; ++t)
+        for (int t = 0; t < GT; ++t)
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) acc[t][i] *= ratio;
-          v_unit = v_next;
-        }
-        k_mul = k_next;
+          for (int i = 0; i < D / 16; ++i) acc[t][i] *= ratio;
+        v_unit = v_now;
       }
     }
-    if (threadIdx.x == 0) odd_keys[odd_place == 0 ? 2 : odd_place - 1] = 0;
-    lds_barrier();
-    odd_place = odd_place == 2 ? 0 : odd_place + 1;
+    if (active) multiply(lds + stage * S::kBytes, tok, decltype(masked)::value ? odd_keys[place] : 0u, masked);
+    if (threadIdx.x == 0) odd_keys[behind(place, kPlaces - AHEAD, kPlaces)] = 0;
+    if (--until_barrier == 0) {
+      lds_barrier();
+      until_barrier = AHEAD;
+    }
+    stage = behind(stage, 1, kStages);
+    place = behind(place, 1, kPlaces);
   };
   if (tok_first < tok_end) {
-    park(IntConst<0>{}, 0, 0, tok_first);
-    if constexpr (FP8) {
-      k_mul = k_muls[0];
-      v_unit = v_units[0];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i += 2) {
+      park(IntConst<0>{}, i, i, tok_first + i * kChunk);
+      request(IntConst<0>{}, tok_first + (i + 2) * kChunk);
+      if (i + 1 < AHEAD) {
+        park(IntConst<1>{}, i + 1, i + 1, tok_first + (i + 1) * kChunk);
+        request(IntConst<1>{}, tok_first + (i + 3) * kChunk);
+      }
     }
-    request(IntConst<0>{}, tok_first + 2 * kChunk);
     lds_barrier();
     // chunks that lie in the cache as it was, two at a time, then the others
     int tok = tok_first;
@@ -728,14 +743,14 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p, int rows) {
   }
 }
 
-template <int D, bool BF16, bool FP8, int NW, int GT>
+template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
 int launch_tiles(Params& p, hipStream_t st) {
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
   constexpr int kRows = NW * GT * 16;
-  constexpr int kLds = 2 * Stage<D>::kBytes;
+  constexpr int kLds = 2 * AHEAD * Stage<D>::kBytes;
   static int resident = 0;  // workgroups that a CU holds (calls take turns: PTO_DISPATCH_LOCK)
   if (resident == 0) {
-    const void* kernel = reinterpret_cast<const void*>(&tree_kernel<D, BF16, FP8, NW, GT>);
+    const void* kernel = reinterpret_cast<const void*>(&tree_kernel<D, BF16, FP8, NW, GT, AHEAD>);
     if (kLds > 64 * 1024) PTO_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
     int n = 0;
     PTO_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, NW * 64, kLds));
@@ -754,7 +769,7 @@ int launch_tiles(Params& p, hipStream_t st) {
   p.slots = (int)slots;
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + o_bytes);
-  hipLaunchKernelGGL((tree_kernel<D, BF16, FP8, NW, GT>), dim3((unsigned)grid), dim3(NW * 64), kLds, st, p);
+  hipLaunchKernelGGL((tree_kernel<D, BF16, FP8, NW, GT, AHEAD>), dim3((unsigned)grid), dim3(NW * 64), kLds, st, p);
   hipLaunchKernelGGL((tree_join_kernel<D, T>), dim3((unsigned)(((int64_t)p.tokens * p.hq + 3) / 4)), dim3(256), 0, st, p, kRows);
   return PTO_HIP_OK;
 }
@@ -763,12 +778,12 @@ template <int D, bool BF16, bool FP8>
 int launch_rows(Params& p, hipStream_t st) {
   const int64_t rows = (int64_t)std::min<int64_t>((p.tokens + p.batch - 1) / p.batch, 32 * p.words) * p.group;  // of a sequence, on average
   if constexpr (D == 256) {  // fewer wavefronts would bring so much each that their registers did not hold it
-    return launch_tiles<D, BF16, FP8, 8, 1>(p, st);
+    return launch_tiles<D, BF16, FP8, 8, 1, 2>(p, st);
   } else {
-    if (rows <= 32) return launch_tiles<D, BF16, FP8, 2, 1>(p, st);
-    if (rows <= 64) return launch_tiles<D, BF16, FP8, 4, 1>(p, st);
-    if (rows <= 128) return launch_tiles<D, BF16, FP8, 4, 2>(p, st);
-    return launch_tiles<D, BF16, FP8, 8, 2>(p, st);
+    if (rows <= 32) return launch_tiles<D, BF16, FP8, 2, 1, 1>(p, st);
+    if (rows <= 64) return launch_tiles<D, BF16, FP8, 4, 1, 1>(p, st);
+    if (rows <= 128) return launch_tiles<D, BF16, FP8, 4, 2, 2>(p, st);
+    return launch_tiles<D, BF16, FP8, 8, 2, 4>(p, st);
   }
 }
 template <int D>
