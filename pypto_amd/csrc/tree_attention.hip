@@ -41,8 +41,11 @@ struct Params {
   // matrix form
   float scale_log2e;
   int target;         // workgroups that the keys are cut for
-  int least;          // fewest keys of a part
+  float per_target;   // 1 / target
+  float least;        // fewest chunks of a part
   int slots;          // partial results that there is room for, in tokens
+  uint32_t block_bytes;  // of a cache's block, all KV heads
+  int4* joins;        // [B] of each sequence: parts, slot, first token, tokens
   float* part_o;      // [slots * Hq, D]
   float* part_ml;     // [slots * Hq, 2]: running maximum in units of log 2, sum
 };
@@ -149,57 +152,61 @@ typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
 
 constexpr int kChunk = 32;
 
+// a / b of numbers below 2^24 whose quotient is below 2^20 (a division of integers is some 40 instructions).
+__device__ __forceinline__ int quotient(int a, int b) {
+  const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));  // off by one at most
+  const int r = a - q * b;
+  return q + (r >= b) - (r < 0);
+}
+
 // A sequence of the plan, as one lane holds it.
 struct Work {
   int first, count;  // its tokens
   int ctx, end;      // keys in front of its new ones, and all
   int blocks;        // row blocks
 };
+__device__ __forceinline__ int chunks_of(const Work& w) { return (w.end + kChunk - 1) / kChunk; }
 __device__ __forceinline__ Work work_of(const Params& p, int b, int rows) {
-  Work w{};
-  if (b < p.batch) {
-    const int first = p.starts[b], next = p.starts[b + 1];
-    const int ctx = p.ctx_lens[b];
-    const bool sound = first >= 0 && next > first && next <= p.tokens;
-    const int64_t room = (int64_t)p.max_blocks * p.bs;
-    w.first = first;
-    w.count = sound ? next - first : 0;
-    w.ctx = (int)min(max((int64_t)ctx, (int64_t)0), room);
-    w.end = sound ? (int)min((int64_t)w.ctx + min(w.count, 32 * p.words), room) : 0;
-    w.blocks = sound ? (w.count * p.group + rows - 1) / rows : 0;
-  }
+  const int at = min(b, p.batch - 1);
+  const int first = p.starts[at], next = p.starts[at + 1], ctx = p.ctx_lens[at];
+  const bool sound = b < p.batch && first >= 0 && next > first && next <= p.tokens;
+  const int room = p.max_blocks * p.bs;  // below 2^29
+  Work w;
+  w.first = first;
+  w.count = sound ? next - first : 0;
+  w.ctx = min(max(ctx, 0), room);
+  w.end = sound ? min(w.ctx + min(w.count, 32 * p.words), room) : 0;
+  w.blocks = (int)(((uint32_t)w.count * (uint32_t)p.group + (uint32_t)rows - 1) / (uint32_t)rows);
   return w;
 }
-__device__ __forceinline__ int parts_of(const Work& w, int keys) { return w.blocks ? max(1, (w.end + keys - 1) / keys) : 0; }
-
-// Keys of a part (wave-uniform): total / target, or a few eighths more, the least with which the workgroups are no more than target; twice as many where none of
+__device__ __forceinline__ int parts_of(const Work& w, int part) { return w.blocks ? max(1, quotient(chunks_of(w) + part - 1, part)) : 0; }
+// Chunks of a part (wave-uniform): total / target, or a few eighths more, the least with which the workgroups are no more than target; twice as many where none of
 // these will do, as with short sequences.
-__device__ __forceinline__ int part_keys(const Params& p, int rows, int lane, const Work& first64) {
+__device__ __forceinline__ int part_chunks(const Params& p, int rows, int lane, const Work& first64) {
   using pto_hip::wave_total;
   float total = 0.f;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
-    total += wave_total((float)w.end * (float)w.blocks);
+    total += wave_total((float)chunks_of(w) * (float)w.blocks);
   }
-  total *= (float)p.hkv * 1.0001f / (float)p.target;  // not below the exact quotient: the room for partial results counts on it
+  total *= (float)p.hkv * 1.0001f * p.per_target;  // not below the exact quotient: the room for partial results counts on it
   constexpr int kTries = 8;
-  int keys[kTries];
-  float count[kTries];
+  float part[kTries], count[kTries];
 #pragma unroll
   for (int i = 0; i < kTries; ++i) {
-    const float even = fminf(total * (1.f + 0.125f * i), 1e9f);
-    keys[i] = max(((int)even + kChunk) & ~(kChunk - 1), p.least);
-    count[i] = 0;
+    part[i] = fmaxf(floorf(fminf(total * (1.f + 0.125f * i), 1e7f)) + 1.f, p.least);
+    count[i] = 0.f;
   }
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
+    const float chunks = (float)chunks_of(w), blocks = (float)w.blocks;
 #pragma unroll
-    for (int i = 0; i < kTries; ++i) count[i] += wave_total((float)parts_of(w, keys[i]) * (float)w.blocks);
+    for (int i = 0; i < kTries; ++i) count[i] += wave_total(fmaxf(ceilf(chunks * __builtin_amdgcn_rcpf(part[i])), 1.f) * blocks);
   }
-  int found = keys[kTries - 1];
+  float found = part[kTries - 1];
 #pragma unroll
-  for (int i = kTries - 2; i >= 0; --i) found = count[i] * (float)p.hkv <= (float)p.target ? keys[i] : found;
-  return found;
+  for (int i = kTries - 2; i >= 0; --i) found = count[i] * (float)p.hkv <= (float)p.target ? part[i] : found;
+  return (int)found;
 }
 
 struct Share {
@@ -209,7 +216,9 @@ struct Share {
   int slot;  // of the sequence's first token in its first part
 };
 // A sequence's partial results, in tokens: none where it has one part.  No more than there can be room for, so that sums over 64 of them stay in 32 bits.
-__device__ __forceinline__ int held_of(const Params& p, const Work& w, int parts) { return parts > 1 ? (int)min((int64_t)parts * w.count, (int64_t)p.slots + 1) : 0; }
+__device__ __forceinline__ int held_of(const Params& p, const Work& w, int parts) {
+  return parts > 1 ? (int)fminf((float)parts * (float)w.count, (float)(p.slots + 1)) : 0;
+}
 __device__ __forceinline__ Work work_in_lane(const Work& w, int k) {
   return Work{__builtin_amdgcn_readlane(w.first, k), __builtin_amdgcn_readlane(w.count, k), __builtin_amdgcn_readlane(w.ctx, k),
               __builtin_amdgcn_readlane(w.end, k), __builtin_amdgcn_readlane(w.blocks, k)};
@@ -218,13 +227,13 @@ __device__ __forceinline__ Work work_in_lane(const Work& w, int k) {
 // multiple of the KV heads apart, on one XCD where these are a multiple of eight.
 __device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int lane) {
   const Work first64 = work_of(p, lane, rows);
-  const int keys = part_keys(p, rows, lane, first64);
+  const int part = part_chunks(p, rows, lane, first64);
   int ids = 0, slots = 0;
   Share s{};
   s.seq = -1;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
-    const int parts = parts_of(w, keys);
+    const int parts = parts_of(w, part);
     const int mine = parts * w.blocks * p.hkv, held = held_of(p, w, parts);
     const int to = pto_hip::wave_running_sum(mine) + ids, slot_to = pto_hip::wave_running_sum(held) + slots;
     const uint64_t behind = __ballot(to > id);
@@ -234,11 +243,11 @@ __device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int
       s.w = work_in_lane(w, k);
       s.parts = __builtin_amdgcn_readlane(parts, k);
       s.slot = __builtin_amdgcn_readlane(slot_to - held, k);
-      int at = id - __builtin_amdgcn_readlane(to - mine, k);
-      s.h = at % p.hkv;
-      at /= p.hkv;
-      s.block = at % s.w.blocks;
-      s.part = at / s.w.blocks;
+      const int at = id - __builtin_amdgcn_readlane(to - mine, k);
+      const int per_head = quotient(at, p.hkv);
+      s.h = at - per_head * p.hkv;
+      s.part = quotient(per_head, s.w.blocks);
+      s.block = per_head - s.part * s.w.blocks;
       if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) s.seq = -1;  // only where the starts do not rise
       return s;
     }
@@ -320,14 +329,15 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   if (s.seq < 0) return;
   const int seq = s.seq, h = s.h, ctx = s.w.ctx, count = s.w.count, token0 = s.w.first, parts = s.parts, part = s.part, all = s.w.end;
   // even parts of whole chunks
-  const int chunks = (all + kChunk - 1) / kChunk;
-  const int tok_first = (int)((int64_t)chunks * part / parts) * kChunk;
-  const int tok_end = min((int)((int64_t)chunks * (part + 1) / parts) * kChunk, all);
+  const int chunks = chunks_of(s.w), each = quotient(chunks, parts), more = chunks - each * parts;
+  const int tok_first = (part * each + min(part, more)) * kChunk;
+  const int tok_end = min(tok_first + (each + (part < more)) * kChunk, all);
   const int row0 = (s.block * NW + wave) * GT * 16;  // first row of this wavefront
   const int rows = count * p.group;
   const bool active = row0 < rows;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPlaces; ++i) odd_keys[i] = 0;
+    if (part == 0 && s.block == 0 && h == 0) p.joins[seq] = int4{parts, s.slot, token0, count};
     const int64_t raw = p.ctx_lens[seq];
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
@@ -342,8 +352,8 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   for (int t = 0; t < GT; ++t) {
     const int r = row0 + t * 16 + c;
     const bool there = r < rows;
-    node[t] = there ? r / p.group : 0;
-    const int g = there ? r % p.group : 0;
+    node[t] = there ? quotient(r, p.group) : 0;
+    const int g = there ? r - node[t] * p.group : 0;
     const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + ((size_t)(token0 + node[t]) * p.hq + h * p.group + g) * D;
 #pragma unroll
     for (int u = 0; u < D / 32; ++u) {
@@ -388,6 +398,8 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   // The next 16 tokens to be asked for: logical block and place in it (a block is a multiple of 16 tokens).
   int lb = tok_first / p.bs, off = tok_first % p.bs;
 
+  const char* k_head = reinterpret_cast<const char*>(p.kc) + (size_t)h * p.bs * kRowBytes;
+  const char* v_head = reinterpret_cast<const char*>(p.vc) + (size_t)h * p.bs * kRowBytes;
   // two chunks on their way to LDS, and the scales of their keys and values
   u32x4 kr[2][kPieces], vr[2][kPieces];
   float k_muls[2] = {scale, scale}, v_units[2] = {1.f, 1.f};
@@ -395,30 +407,37 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
   // window's blocks are block 0, whose rows lie in the cache as any block's.
   auto request = [&](auto set, int tok) __attribute__((always_inline)) {
     constexpr int SET = decltype(set)::value;
+    // a chunk's halves lie in one block where blocks are a multiple of it, and a wavefront's piece in one half
     int lb1 = lb, off1 = off + 16;
     lb1 += off1 == p.bs;
     off1 = off1 == p.bs ? 0 : off1;
     if (lb1 >= win_base + 64) load_window(lb);
     const int slot = lb - win_base;
-    const int blk0 = __builtin_amdgcn_readlane(win_blk, slot), blk1 = __builtin_amdgcn_readlane(win_blk, lb1 - win_base);
+    const uint32_t blk0 = __builtin_amdgcn_readlane(win_blk, slot), blk1 = __builtin_amdgcn_readlane(win_blk, lb1 - win_base);
     if constexpr (FP8) {  // a chunk lies in one block
       k_muls[SET] = scale * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_ks), slot));
       v_units[SET] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_vs), slot));
     }
-    const size_t at0 = (((size_t)blk0 * p.hkv + h) * p.bs + off) * kRowBytes;
-    const size_t at1 = (((size_t)blk1 * p.hkv + h) * p.bs + off1) * kRowBytes - 16 * kRowBytes;
+    const uint64_t at0 = (uint64_t)blk0 * p.block_bytes + (uint32_t)(off * kRowBytes);
+    const uint64_t at1 = (uint64_t)blk1 * p.block_bytes + (uint32_t)(off1 * kRowBytes) - 16 * kRowBytes;
     off = off1 + 16;
     lb = lb1 + (off == p.bs);
     off = off == p.bs ? 0 : off;
-    const char* kc = reinterpret_cast<const char*>(p.kc);
-    const char* vc = reinterpret_cast<const char*>(p.vc);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      int item = threadIdx.x + i * kThreads;
-      if constexpr (kItems % kThreads != 0) item = min(item, kItems - 1);
-      const size_t at = (item * 16 / kRowBytes < 16 ? at0 : at1) + (size_t)item * 16;
-      kr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at));
-      vr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at));
+      if constexpr (kItems % kThreads == 0 && kThreads * 16 >= 16 * kRowBytes) {
+        // every piece of the workgroup's lies in one half, or the wavefront's in one
+        const bool second = (wave * 64 + i * kThreads) * 16 >= 16 * kRowBytes;
+        const uint64_t at = (second ? at1 : at0) + (uint32_t)(i * kThreads * 16);
+        kr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_head + at + threadIdx.x * 16));
+        vr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_head + at + threadIdx.x * 16));
+      } else {
+        int item = threadIdx.x + i * kThreads;
+        if constexpr (kItems % kThreads != 0) item = min(item, kItems - 1);
+        const uint64_t at = (item * 16 / kRowBytes < 16 ? at0 : at1) + (uint32_t)(item * 16);
+        kr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_head + at));
+        vr[SET][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v_head + at));
+      }
     }
   };
   auto park = [&](auto set, int stage, int odd_place, int tok) __attribute__((always_inline)) {
@@ -657,7 +676,7 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
     const float l = sum[t][0];
     const int r = row0 + t * 16 + c;
     if (r >= rows) continue;
-    const int head = h * p.group + r % p.group;
+    const int head = h * p.group + r - node[t] * p.group;
     if (parts == 1) {
       const float mul = l > 0.f || l != l ? v_unit / l : 0.f;
       T* out = reinterpret_cast<T*>(p.out) + ((size_t)(token0 + node[t]) * p.hq + head) * D + j * 4;
@@ -679,67 +698,64 @@ __global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
 
 // Joins a row's parts: one wavefront each, lane i the channels i, i + 64, ...
 template <int D, typename T>
-__global__ __launch_bounds__(256) void tree_join_kernel(Params p, int rows) {
+__global__ __launch_bounds__(256) void tree_join_kernel(Params p) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)p.tokens * p.hq) return;
-  const int token = (int)(row / p.hq), head = (int)(row % p.hq);
-  const Work first64 = work_of(p, lane, rows);
-  const int keys = part_keys(p, rows, lane, first64);
-  int slots = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
-    const int parts = parts_of(w, keys), held = held_of(p, w, parts);
-    const int slot_to = pto_hip::wave_running_sum(held) + slots;
-    const uint64_t own = __ballot(w.count > 0 && w.first <= token && token < w.first + w.count);
-    if (own) {
-      const int k = __builtin_ctzll(own);
-      const int np = __builtin_amdgcn_readlane(parts, k), count = __builtin_amdgcn_readlane(w.count, k);
-      const int slot = __builtin_amdgcn_readlane(slot_to - held, k);
-      if (np <= 1 || slot < 0 || (int64_t)slot + (int64_t)np * count > p.slots) return;
-      const size_t first = ((size_t)slot + (token - __builtin_amdgcn_readlane(w.first, k))) * p.hq + head, step = (size_t)count * p.hq;
-      float m = kMinMax, l = 0.f, o[D / 64];
+  const int token = p.t0 + blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (head >= p.hq) return;
+  const TokenSeq own = pto_hip::sequence_of(p.starts, p.batch, token, lane);
+  if (own.seq < 0) return;
+  const int4 join = p.joins[own.seq];  // by the kernel in front, for every sequence that has tokens
+  const int np = join.x, slot = join.y, count = join.w;
+  if (join.z != own.first || count != own.count || np <= 1 || slot < 0 || (int64_t)slot + (int64_t)np * count > p.slots) return;
+  const size_t first = ((size_t)slot + (token - own.first)) * p.hq + head, step = (size_t)count * p.hq;
+  float m = kMinMax, l = 0.f, o[D / 64];
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-      for (int q0 = 0; q0 < np; q0 += 64) {
-        const int q = min(q0 + lane, np - 1);
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + q * step) * 2);
-        const bool there = q0 + lane < np;
-        float most = there ? ml.x : kMinMax;
+  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
+  for (int q0 = 0; q0 < np; q0 += 64) {
+    const int q = min(q0 + lane, np - 1);
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + q * step) * 2);
+    const bool there = q0 + lane < np;
+    float most = there ? ml.x : kMinMax;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
-        const float m_new = fmaxf(m, most), keep = __builtin_amdgcn_exp2f(m - m_new);
-        m = m_new;
-        const float weight = there ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f;
-        l = l * keep;
-        float sum = there ? weight * ml.y : 0.f;
+    for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
+    const float m_new = fmaxf(m, most), keep = __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    const float weight = there ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f;
+    l = l * keep;
+    float sum = there ? weight * ml.y : 0.f;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-        l += sum;
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    l += sum;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) o[i] *= keep;
-        const int n = min(64, np - q0);
-        constexpr int kBatch = 8;
-        for (int u0 = 0; u0 < n; u0 += kBatch) {
-          float v[kBatch][D / 64];
+    for (int i = 0; i < D / 64; ++i) o[i] *= keep;
+    const int n = min(64, np - q0);
+    constexpr int kBatch = 8;
+    for (int u0 = 0; u0 < n; u0 += kBatch) {
+      float v[kBatch][D / 64];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u)
+      for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) v[u][i] = p.part_o[(first + min(q0 + u0 + u, np - 1) * step) * D + i * 64 + lane];
+        for (int i = 0; i < D / 64; ++i) v[u][i] = p.part_o[(first + min(q0 + u0 + u, np - 1) * step) * D + i * 64 + lane];
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const float wgt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), min(u0 + u, 63)));
+      for (int u = 0; u < kBatch; ++u) {
+        const float wgt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), min(u0 + u, 63)));
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) o[i] = u0 + u < n ? fmaf(wgt, v[u][i], o[i]) : o[i];
-          }
-        }
+        for (int i = 0; i < D / 64; ++i) o[i] = u0 + u < n ? fmaf(wgt, v[u][i], o[i]) : o[i];
       }
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i) reinterpret_cast<T*>(p.out)[((size_t)token * p.hq + head) * D + i * 64 + lane] = (T)(o[i] * inv);
-      return;
     }
-    slots = min(__builtin_amdgcn_readlane(slot_to, 63), p.slots + 1);
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) reinterpret_cast<T*>(p.out)[((size_t)token * p.hq + head) * D + i * 64 + lane] = (T)(o[i] * inv);
+}
+
+// f(tokens) for the tokens of each launch: a launch holds fewer than 2^32 threads.
+template <typename F>
+void in_launches(Params& p, int64_t threads_a_token, F f) {
+  const int64_t most = std::max<int64_t>(1, (1ll << 31) / threads_a_token);
+  for (int64_t t = 0; t < p.tokens; t += most) {
+    p.t0 = (int)t;
+    f((unsigned)std::min<int64_t>(most, p.tokens - t));
   }
 }
 
@@ -757,20 +773,24 @@ int launch_tiles(Params& p, hipStream_t st) {
     resident = std::max(1, n);
   }
   p.target = pto_hip::ctx().num_cu * resident;
-  p.least = std::max(64, kRows);
+  p.per_target = 1.f / (float)p.target;
+  p.least = (float)(std::max(64, kRows) / kChunk);
+  p.block_bytes = (uint32_t)((int64_t)p.hkv * p.bs * D * (FP8 ? 1 : 2));
   const int64_t blocks = (int64_t)p.tokens * p.group / kRows + std::min(p.batch, p.tokens);
   const int64_t grid = p.target + blocks * p.hkv;
   const int64_t slots = ((int64_t)p.target * kRows + p.hq - 1) / p.hq + p.tokens + 1;
-  PTO_CHECK_ARG(grid < 1ll << 24 && slots < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
+  PTO_CHECK_ARG(grid < 1ll << 22 && slots < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
   const size_t o_bytes = (size_t)slots * p.hq * D * 4, ml_bytes = (size_t)slots * p.hq * 8;
   void* ws = nullptr;
-  const int rc = pto_hip::workspace(o_bytes + ml_bytes, &ws);
+  const int rc = pto_hip::workspace(o_bytes + ml_bytes + 16 + (size_t)p.batch * sizeof(int4), &ws);
   if (rc) return rc;
   p.slots = (int)slots;
+  p.joins = reinterpret_cast<int4*>(reinterpret_cast<char*>(ws) + o_bytes + (ml_bytes + 15) / 16 * 16);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + o_bytes);
   hipLaunchKernelGGL((tree_kernel<D, BF16, FP8, NW, GT, AHEAD>), dim3((unsigned)grid), dim3(NW * 64), kLds, st, p);
-  hipLaunchKernelGGL((tree_join_kernel<D, T>), dim3((unsigned)(((int64_t)p.tokens * p.hq + 3) / 4)), dim3(256), 0, st, p, kRows);
+  const unsigned heads = (p.hq + 3) / 4;
+  in_launches(p, 256 * heads, [&](unsigned n) { hipLaunchKernelGGL((tree_join_kernel<D, T>), dim3(n, heads), dim3(256), 0, st, p); });
   return PTO_HIP_OK;
 }
 
@@ -794,11 +814,7 @@ int launch_matrix(Params& p, bool bf16, bool fp8, hipStream_t st) {
 
 template <typename T, typename E>
 void launch_any(Params& p, hipStream_t st) {
-  const int64_t most = std::max<int64_t>(1, (1ll << 31) / (64 * p.hq));  // a launch holds fewer than 2^32 threads
-  for (int64_t t = 0; t < p.tokens; t += most) {
-    p.t0 = (int)t;
-    hipLaunchKernelGGL((tree_any_kernel<T, E>), dim3((unsigned)std::min<int64_t>(most, p.tokens - t), p.hq), dim3(64), 0, st, p);
-  }
+  in_launches(p, 64 * p.hq, [&](unsigned n) { hipLaunchKernelGGL((tree_any_kernel<T, E>), dim3(n, p.hq), dim3(64), 0, st, p); });
 }
 
 }  // namespace
@@ -816,8 +832,8 @@ extern "C" int pto_hip_tree_attention(const PtoHipTreeAttentionArgs* args, void*
   PTO_CHECK_ARG(a.head_dim > 0 && a.block_size > 0 && a.max_num_blocks_per_req > 0 && a.pool_blocks > 0 && a.mask_words > 0,
                 "tree_attention: non-positive extent");
   PTO_CHECK_ARG(a.block_size < 1ll << 31 && a.max_num_blocks_per_req < 1ll << 31 && a.pool_blocks < 1ll << 31 && a.batch < 1ll << 30 &&
-                    a.block_size * a.max_num_blocks_per_req < 1ll << 30,
-                "tree_attention: extent beyond 2^31, or a table of 2^30 tokens and more");
+                    a.block_size * a.max_num_blocks_per_req < 1ll << 29,
+                "tree_attention: extent beyond 2^31, or a table of 2^29 tokens and more");
   PTO_CHECK_ARG(a.dtype == PTO_HIP_BF16 || a.dtype == PTO_HIP_FP16, "tree_attention: query dtype %s not in {BF16, FP16}", dtype_name(a.dtype));
   PTO_CHECK_ARG(a.kv_dtype == 0 || a.kv_dtype == a.dtype || fp8, "tree_attention: caches of %s under queries of %s", dtype_name(a.kv_dtype),
                 dtype_name(a.dtype));
@@ -873,7 +889,8 @@ extern "C" int pto_hip_tree_attention(const PtoHipTreeAttentionArgs* args, void*
   const DeviceScope scope(ctx().device);
   hipStream_t st = (hipStream_t)stream;
   p.scale_log2e = a.scale * 1.4426950408889634f;
-  if ((a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && a.block_size % (fp8 ? 32 : 16) == 0) {
+  if ((a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && a.block_size % (fp8 ? 32 : 16) == 0 &&
+      a.kv_head_num * a.block_size * a.head_dim * csz < 1ll << 31 && a.tokens * p.group < 1ll << 24) {
     const bool bf16 = a.dtype == PTO_HIP_BF16;
     const int rc = a.head_dim == 64 ? launch_matrix<64>(p, bf16, fp8, st) : a.head_dim == 128 ? launch_matrix<128>(p, bf16, fp8, st)
                                                                                               : launch_matrix<256>(p, bf16, fp8, st);
