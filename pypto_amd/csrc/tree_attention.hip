@@ -306,7 +306,7 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 constexpr int kSlack = 6;
 
 template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
-__global__ __launch_bounds__(NW * 64, 2) void tree_kernel(Params p) {
+__global__ __launch_bounds__(NW * 64, GT == 4 ? 1 : 2) void tree_kernel(Params p) {
   typedef Stage<D> S;
   constexpr int kThreads = NW * 64, kRows = NW * GT * 16;
   constexpr int kEsz = FP8 ? 1 : 2;
@@ -774,7 +774,7 @@ int launch_tiles(Params& p, hipStream_t st) {
   }
   p.target = pto_hip::ctx().num_cu * resident;
   p.per_target = 1.f / (float)p.target;
-  p.least = (float)(std::max(64, kRows) / kChunk);
+  p.least = (float)(std::max(256, kRows) / kChunk);
   p.block_bytes = (uint32_t)((int64_t)p.hkv * p.bs * D * (FP8 ? 1 : 2));
   const int64_t blocks = (int64_t)p.tokens * p.group / kRows + std::min(p.batch, p.tokens);
   const int64_t grid = p.target + blocks * p.hkv;
