@@ -305,8 +305,13 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 // A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.
 constexpr int kSlack = 6;
 
+// Whether a wavefront has registers for three others on its SIMD: with one tile of rows, over e4m3 caches, whose rows on their way are half as long (32 sequences of 4 to 8
+// drafts, 64 heads: 190 -> 179 us; with 16-bit caches registers spill).
+template <int D, bool FP8, int GT>
+constexpr bool lean() { return GT == 1 && FP8 && D <= 128; }
+
 template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
-__global__ __launch_bounds__(NW * 64, GT == 4 ? 1 : 2) void tree_kernel(Params p) {
+__global__ __launch_bounds__(NW * 64, lean<D, FP8, GT>() ? 4 : 2) void tree_kernel(Params p) {
   typedef Stage<D> S;
   constexpr int kThreads = NW * 64, kRows = NW * GT * 16;
   constexpr int kEsz = FP8 ? 1 : 2;
@@ -499,10 +504,10 @@ __global__ __launch_bounds__(NW * 64, GT == 4 ? 1 : 2) void tree_kernel(Params p
         s1[t] = mfma16<BF16>(a1, qf[t][u], s1[t]);
       }
     }
-    // The values' fragments are asked for in front of the softmax (head_dim 256: the first half): lane (c, j) has channel 16 i + c of the tokens whose
+    // The values' fragments are asked for in front of the softmax (as many as there are registers for): lane (c, j) has channel 16 i + c of the tokens whose
     // probabilities it will have.
     const char* vlane = vbase + (j * 4 + (c >> 2)) * S::kPitch + (c & 3) * 8;
-    constexpr int kHeld = D <= 128 ? D / 16 : 8;
+    constexpr int kHeld = lean<D, FP8, GT>() ? 4 : D <= 128 ? D / 16 : 8;
     u32x4 vt[kHeld];
     auto fetch_values = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
