@@ -311,7 +311,7 @@ template <int D, bool FP8, int GT>
 constexpr bool lean() { return GT == 1 && FP8 && D <= 128; }
 
 template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
-__global__ __launch_bounds__(NW * 64, lean<D, FP8, GT>() ? 4 : 2) void tree_kernel(Params p) {
+__global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_kernel(Params p) {
   typedef Stage<D> S;
   constexpr int kThreads = NW * 64, kRows = NW * GT * 16;
   constexpr int kEsz = FP8 ? 1 : 2;
