@@ -40,6 +40,7 @@ struct Params {
   int32_t* tokens;
   float* probs;
   int rows, vocab;
+  int row0;  // the launch's first row
 };
 
 // Unsigned integers in the order of the values; NaN is -inf.
@@ -76,6 +77,12 @@ struct Weights {
   double rate;    // 64 log2(e) / T
   const Powers* powers;
   __device__ __forceinline__ double steps(float v) const { return v == best ? 0.0 : ((double)best - (double)v) * rate; }
+  // A logit below it lies more than `limit` steps down: rounded towards smaller ones, so that one comparison in 32 bits leaves out what weighs nothing
+  __device__ __forceinline__ float cut(double limit) const {
+    const double v = (double)best - (limit + 1.0) / rate;
+    const float f = (float)v;
+    return f - fabsf(f) * 0x1p-23f;  // NaN (infinite logits, infinite temperatures): leaves nothing out
+  }
   // w 2^up, as a number; z in [0, 2^31)
   __device__ __forceinline__ double scaled(double z, int up) const {
     const int whole = (int)z;
@@ -302,7 +309,7 @@ struct Scratch {
   unsigned int* collected;     // [1] tokens of the border's intervals
   unsigned long long* tokens;  // [kCollected] their places
   unsigned long long* sums;    // [slices] weights surely kept
-  unsigned long long* front;   // [3] tokens and weights in front of the border's intervals, weights of all
+  unsigned long long* front;   // [5] tokens and weights in front of the border's intervals, weights of all; their first step and steps
   int slices, slice;           // elements of a slice, a multiple of kStep
 };
 
@@ -347,7 +354,7 @@ __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) 
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
   __shared__ unsigned long long waves[kSliceThreads / 64];
-  const int slice = blockIdx.x, r = blockIdx.y;
+  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   // a thread meets its elements by rising index: of equal ones the first stays
@@ -393,7 +400,7 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   __shared__ Powers powers;
   __shared__ unsigned long long weight[kIntervals];
   __shared__ unsigned int count[kIntervals];
-  const int slice = blockIdx.x, r = blockIdx.y;
+  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
   if (!(t > 0.f) || !f.any()) return;
@@ -408,7 +415,9 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const Weights w = weights_of(best, t, &powers);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  const float cut = w.cut(kSteps);
   in_steps<T, WIDE>(row, first, end, [&](float v, int) {
+    if (v < cut) return;
     const double z = w.steps(v);
     if (z < (double)kSteps) {
       const int at = (int)z >> 1;
@@ -513,7 +522,7 @@ template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratch s) {
   __shared__ Powers powers;
   __shared__ unsigned long long waves[kSliceThreads / 64];
-  const int slice = blockIdx.x, r = blockIdx.y;
+  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
   const float t = p.temperature[r];
   if (!(t > 0.f)) return;
   const Filters f = filters_of(p, r);
@@ -523,23 +532,30 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   BorderIntervals at{kIntervals, kIntervals, 0, 0, 0};
   if (f.any()) at = find_intervals(s, r, f);
   if (slice == 0 && threadIdx.x == 0) {
-    s.front[3 * (size_t)r] = at.tokens_front;
-    s.front[3 * (size_t)r + 1] = at.weight_front;
-    s.front[3 * (size_t)r + 2] = at.weight_all;
+    unsigned long long* front = s.front + 5 * (size_t)r;
+    front[0] = at.tokens_front;
+    front[1] = at.weight_front;
+    front[2] = at.weight_all;
+    front[3] = 2 * at.first;
+    front[4] = 2 * (at.last - at.first + 1);
   }
   __syncthreads();
   const Weights w = weights_of(best, t, &powers);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
-  const double z_first = 2.0 * at.first, z_behind = min(2.0 * (at.last + 1), (double)kSteps);
+  // of what is surely kept, min_p leaves out what is further down than this (a step more than it has to be)
+  const double z_least = 64.0 * (kUnit - log2((double)f.least)) + 1.0;
+  const double z_first = 2.0 * at.first, z_sure = min(z_first, z_least), z_behind = min(2.0 * (at.last + 1), (double)kSteps);
+  const float cut = w.cut(at.first < kIntervals ? z_behind : z_sure);
   const double least = (double)f.least;
   double own = 0.0;  // at most 64 elements': exact
   in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
+    if (v < cut) return;
     const double z = w.steps(v);
-    if (z < z_first) {
+    if (z < z_sure) {
       const double x = w.units(z);
       own += x >= least ? x : 0.0;
-    } else if (z < z_behind) {
+    } else if (z >= z_first && z < z_behind) {
       const unsigned int n = atomicAdd(&s.collected[r], 1u);
       if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v, i);
     }
@@ -554,18 +570,94 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   }
 }
 
+constexpr int kCells = 1024;  // of the border's intervals
 struct DrawShared {
   Powers powers;
-  unsigned long long tokens[kCollected];
   unsigned long long sums[kMaxVocab / kStep];
+  unsigned long long found[6];
+  unsigned long long waves[kWaves];
+  unsigned int gathered;
+  unsigned long long tokens[kCollected];  // of one cell, in order
   union {
     Shared row;
     struct {
-      unsigned long long waves[kWaves];
-      unsigned long long found[4];
-    } draw;
+      unsigned long long weight[kCells];
+      unsigned int count[kCells];
+    } cells;
   };
 };
+
+// Where the running sum of the collected tokens (by_weight: of their weights), in order and from what lies in front of them on, reaches `need`: the place of that token and
+// the sum of the weights up to it.  The cell that it lies in first, then the cell's tokens in order.  All threads take part; `need` is reached.
+struct Reached {
+  uint64_t place, weight;
+};
+template <typename Cell, typename Weight>
+__device__ Reached reach(DrawShared& sh, const unsigned long long* tokens, int n, bool by_weight, uint64_t tokens_front, uint64_t weight_front, uint64_t need,
+                         Cell cell, Weight weight) {
+  constexpr int kOwn = kCells / kThreads;
+  uint64_t n_own = 0, x_own = 0;
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    n_own += sh.cells.count[threadIdx.x * kOwn + u];
+    x_own += sh.cells.weight[threadIdx.x * kOwn + u];
+  }
+  unsigned long long all;
+  uint64_t n_front = tokens_front + sum_in_front<unsigned long long>(n_own, sh.waves, &all);
+  uint64_t x_front = weight_front + sum_in_front<unsigned long long>(x_own, sh.waves, &all);
+  if (threadIdx.x == 0) sh.gathered = 0;
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    const uint64_t c = sh.cells.count[threadIdx.x * kOwn + u], x = sh.cells.weight[threadIdx.x * kOwn + u];
+    const uint64_t front = by_weight ? x_front : n_front;
+    if (front < need && front + (by_weight ? x : c) >= need) {
+      sh.found[0] = threadIdx.x * kOwn + u;
+      sh.found[1] = n_front;
+      sh.found[2] = x_front;
+    }
+    n_front += c;
+    x_front += x;
+  }
+  __syncthreads();
+  const int here = (int)sh.found[0];
+  const uint64_t n_cell = sh.found[1], x_cell = sh.found[2];
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    if (cell(tokens[i]) == here) sh.tokens[atomicAdd(&sh.gathered, 1u)] = tokens[i];
+  __syncthreads();
+  const int m = (int)sh.gathered;
+  int size = 1;
+  while (size < m) size *= 2;
+  for (int i = m + threadIdx.x; i < size; i += kThreads) sh.tokens[i] = 0;  // the last places
+  __syncthreads();
+  for (int span = 2; span <= size; span *= 2)
+    for (int gap = span / 2; gap > 0; gap /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int a = 2 * i - (i & (gap - 1)), b = a + gap;
+        const uint64_t va = sh.tokens[a], vb = sh.tokens[b];
+        if ((va < vb) == ((a & span) == 0)) {
+          sh.tokens[a] = vb;
+          sh.tokens[b] = va;
+        }
+      }
+      __syncthreads();
+    }
+  // neighbouring tokens a thread
+  const int per = (m + kThreads - 1) / kThreads, first = threadIdx.x * per;
+  uint64_t own = 0;
+  for (int u = first; u < min(first + per, m); ++u) own += weight(sh.tokens[u]);
+  uint64_t x = x_cell + sum_in_front<unsigned long long>(own, sh.waves, &all);
+  for (int u = first; u < min(first + per, m); ++u) {
+    const uint64_t each = weight(sh.tokens[u]);
+    const bool reached = by_weight ? x < need && x + each >= need : n_cell + u + 1 == need;
+    x += each;
+    if (reached) {
+      sh.found[3] = sh.tokens[u];
+      sh.found[4] = x;
+    }
+  }
+  __syncthreads();
+  return Reached{sh.found[3], sh.found[4]};
+}
 
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
@@ -602,64 +694,35 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
       if (threadIdx.x % 64 == 0 && x) atomicAdd(&sh.sums[i0 / s.slice], (unsigned long long)x);  // a slice is a multiple of kThreads
     }
   } else if (n > 0) {
-    // in order, the last places filled up with nothing
-    int size = 1;
-    while (size < n) size *= 2;
-    for (int i = threadIdx.x; i < size; i += kThreads) sh.tokens[i] = i < n ? s.tokens[(size_t)r * kCollected + i] : 0;
+    const unsigned long long* tokens = s.tokens + (size_t)r * kCollected;
+    const unsigned long long* front = s.front + 5 * (size_t)r;
+    const double z_first = (double)front[3], per_step = (double)kCells / (double)front[4];
+    auto weight = [&](uint64_t token) { return w(value_of((uint32_t)(token >> 32))); };
+    auto cell = [&](uint64_t token) { return min((int)((w.steps(value_of((uint32_t)(token >> 32))) - z_first) * per_step), kCells - 1); };
+    for (int i = threadIdx.x; i < kCells; i += kThreads) {
+      sh.cells.weight[i] = 0;
+      sh.cells.count[i] = 0;
+    }
     __syncthreads();
-    for (int span = 2; span <= size; span *= 2)
-      for (int gap = span / 2; gap > 0; gap /= 2) {
-        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-          const int a = 2 * i - (i & (gap - 1)), b = a + gap;
-          const uint64_t va = sh.tokens[a], vb = sh.tokens[b];
-          if ((va < vb) == ((a & span) == 0)) {
-            sh.tokens[a] = vb;
-            sh.tokens[b] = va;
-          }
-        }
-        __syncthreads();
-      }
-    const uint64_t n_front = s.front[3 * (size_t)r], w_front = s.front[3 * (size_t)r + 1];
-    constexpr int kOwn = kCollected / kThreads;
-    uint64_t x[kOwn], own = 0;
-#pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int i = threadIdx.x * kOwn + u;
-      x[u] = i < n ? w(value_of((uint32_t)(sh.tokens[i] >> 32))) : 0;
-      own += x[u];
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int at = cell(tokens[i]);
+      atomicAdd(&sh.cells.count[at], 1u);
+      atomicAdd(&sh.cells.weight[at], (unsigned long long)weight(tokens[i]));
     }
-    unsigned long long all;
-    const uint64_t in_front = sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
-    const bool by_count = f.k > 0 && n_front + n >= (uint64_t)f.k;
-    int kept = by_count ? (int)(f.k - n_front) : n;  // of them
+    __syncthreads();
+    uint64_t sum = front[2];
+    if (f.k > 0 && front[0] + n >= (uint64_t)f.k) {
+      const Reached k = reach(sh, tokens, n, false, front[0], front[1], (uint64_t)f.k, cell, weight);
+      border = k.place;
+      sum = k.weight;
+    }
     if (f.by_sum) {
-      // what the first `kept` weigh, then how many of them reach the share
-      if (threadIdx.x == 0) sh.draw.found[0] = all;
-      __syncthreads();
-      uint64_t to = in_front;
-#pragma unroll
-      for (int u = 0; u < kOwn; ++u) {
-        to += x[u];
-        if (threadIdx.x * kOwn + u + 1 == kept) sh.draw.found[0] = to;
-      }
-      __syncthreads();
-      const uint64_t need = needed(f, by_count ? w_front + sh.draw.found[0] : s.front[3 * (size_t)r + 2]);
-      if (threadIdx.x == 0) sh.draw.found[1] = kept;
-      __syncthreads();
-      uint64_t a = w_front + in_front;
-#pragma unroll
-      for (int u = 0; u < kOwn; ++u) {
-        if (a < need && a + x[u] >= need) sh.draw.found[1] = threadIdx.x * kOwn + u + 1;
-        a += x[u];
-      }
-      __syncthreads();
-      kept = min(kept, (int)sh.draw.found[1]);
+      const Reached at = reach(sh, tokens, n, true, front[0], front[1], needed(f, sum), cell, weight);
+      border = at.place > border ? at.place : border;
     }
-    border = sh.tokens[kept - 1];
-#pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int i = threadIdx.x * kOwn + u;
-      if (i < kept && x[u] >= f.least) atomicAdd(&sh.sums[(int)~(uint32_t)sh.tokens[i] / s.slice], (unsigned long long)x[u]);
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint64_t x = tokens[i] >= border ? weight(tokens[i]) : 0;
+      if (x >= f.least) atomicAdd(&sh.sums[(int)~(uint32_t)tokens[i] / s.slice], (unsigned long long)x);
     }
   }
   __syncthreads();
@@ -686,17 +749,17 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       if (front <= target && front + x[i] > target) {
-        sh.draw.found[0] = threadIdx.x * kOwn + i;
-        sh.draw.found[1] = target;
-        sh.draw.found[2] = front;
-        sh.draw.found[3] = sum;
+        sh.found[0] = threadIdx.x * kOwn + i;
+        sh.found[1] = target;
+        sh.found[2] = front;
+        sh.found[3] = sum;
       }
       front += x[i];
     }
   }
   __syncthreads();
-  const int first = (int)sh.draw.found[0] * s.slice, end = min(p.vocab, first + s.slice);
-  const uint64_t target = sh.draw.found[1], sum = sh.draw.found[3];
+  const int first = (int)sh.found[0] * s.slice, end = min(p.vocab, first + s.slice);
+  const uint64_t target = sh.found[1], sum = sh.found[3];
   // the thread whose tokens hold it, neighbouring ones, and its wavefront looks for the token among them
   const int per = s.slice / kThreads, lane = threadIdx.x % 64;
   auto kept = [&](int i) -> uint64_t {
@@ -716,7 +779,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
     }
   }
   unsigned long long all;
-  const uint64_t front = sh.draw.found[2] + sum_in_front<unsigned long long>(own, sh.draw.waves, &all);
+  const uint64_t front = sh.found[2] + sum_in_front<unsigned long long>(own, sh.waves, &all);
   const uint64_t here = __ballot(front <= target && front + own > target);
   if (!here) return;
   const int from = __builtin_ctzll(here), i = first + ((int)(threadIdx.x & ~63u) + from) * per + lane;
@@ -734,12 +797,19 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   }
 }
 
+// Rows are read two or three times: a group's logits fit the last-level cache.
+constexpr int64_t kGroupBytes = 96 << 20;
 template <typename T, bool WIDE>
-void launch_slices(const Params& p, const Scratch& s, hipStream_t st) {
-  const dim3 grid(s.slices, p.rows), threads(kSliceThreads);
-  hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-  if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-  hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+void launch_slices(Params& p, const Scratch& s, hipStream_t st) {
+  const int64_t group = std::max<int64_t>(1, kGroupBytes / ((int64_t)p.vocab * (int64_t)sizeof(T)));
+  for (int64_t r = 0; r < p.rows; r += group) {
+    p.row0 = (int)r;
+    const dim3 grid(s.slices, (unsigned)std::min(group, p.rows - r)), threads(kSliceThreads);
+    hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+    if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+    hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  }
+  p.row0 = 0;
   hipLaunchKernelGGL((draw_kernel<T, WIDE>), dim3(p.rows), dim3(kThreads), 0, st, p, s);
 }
 
@@ -752,7 +822,7 @@ int launch(Params p, hipStream_t st) {
   Scratch s{};
   s.slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(kStep, (even + kStep - 1) / kStep * kStep));
   s.slices = (p.vocab + s.slice - 1) / s.slice;
-  const size_t per_row = 8 * (2 * (size_t)s.slices + kIntervals + kCollected + 3) + 4 * (kIntervals + 2);
+  const size_t per_row = 8 * (2 * (size_t)s.slices + kIntervals + kCollected + 5) + 4 * (kIntervals + 2);
   void* ws = nullptr;
   const int rc = pto_hip::workspace(per_row * at_once, &ws);
   if (rc) return rc;
@@ -761,7 +831,7 @@ int launch(Params p, hipStream_t st) {
   s.weight = s.sums + at_once * s.slices;
   s.tokens = s.weight + at_once * kIntervals;
   s.front = s.tokens + at_once * kCollected;
-  s.count = reinterpret_cast<unsigned int*>(s.front + 3 * at_once);
+  s.count = reinterpret_cast<unsigned int*>(s.front + 5 * at_once);
   s.collected = s.count + at_once * kIntervals;
   const bool wide = (uintptr_t)p.logits % 16 == 0 && (int64_t)p.vocab * sizeof(T) % 16 == 0;
   const Params whole = p;
@@ -808,7 +878,7 @@ extern "C" int pto_hip_sample_tokens(const void* logits, const float* temperatur
   }
   const DeviceScope scope(ctx().device);
   hipStream_t st = (hipStream_t)stream;
-  const Params p{logits, temperature, top_k, top_p, min_p, uniform, tokens, probs, (int)rows, (int)vocab};
+  const Params p{logits, temperature, top_k, top_p, min_p, uniform, tokens, probs, (int)rows, (int)vocab, 0};
   const int rc = logits_dtype == PTO_HIP_FP32 ? launch<float>(p, st) : logits_dtype == PTO_HIP_BF16 ? launch<__bf16>(p, st) : launch<_Float16>(p, st);
   if (rc) return rc;
   PTO_CHECK_HIP(hipGetLastError());
