@@ -40,7 +40,6 @@ struct Params {
   int32_t* tokens;
   float* probs;
   int rows, vocab;
-  int row0;  // the launch's first row
 };
 
 // Unsigned integers in the order of the values; NaN is -inf.
@@ -51,14 +50,14 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 __device__ __forceinline__ float value_of(uint32_t k) { return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 constexpr uint32_t kNone = 0x007fffffu;  // the key of -inf
 
-// 2^(-i / 64), kept in LDS by every workgroup: 64 places in 64 banks, two at most in one.
+// 2^(44 - i / 64), kept in LDS by every workgroup: 64 places in 64 banks, two at most in one.
 struct Powers {
   double of[64];
 };
 __device__ __forceinline__ void fill(Powers& t) {  // and a barrier
   if (threadIdx.x < 64) {
     const int i = threadIdx.x;
-    double v = i & 1 ? 0x1.fa7c1819e90d8p-1 : 1.0;  // 2^(-1 / 64)
+    double v = i & 1 ? 0x1.fa7c1819e90d8p+43 : (double)kOne;  // 2^(-1 / 64)
     v *= i & 2 ? 0x1.f50765b6e4540p-1 : 1.0;
     v *= i & 4 ? 0x1.ea4afa2a490dap-1 : 1.0;
     v *= i & 8 ? 0x1.d5818dcfba487p-1 : 1.0;
@@ -70,46 +69,53 @@ __device__ __forceinline__ void fill(Powers& t) {  // and a barrier
 constexpr int kSteps = 46 * 64;          // weights end behind 45 of the 64ths of a power of two
 constexpr int kIntervals = kSteps / 2;
 
-// What a logit of a row weighs.  With z = 64 log2(best's weight / its own): z's whole part is a place in the table and a power of two, the rest, below
-// 1 / 64 of one, six terms of the exponential's series (off by 3e-15 of it).
+// What a logit of a row weighs.  With z = 64 log2(best's weight / its own): the whole number next to z is a place in the table and a power of two, the rest, half of
+// a 64th at most, five terms of the exponential's series (off by 4e-14 of it, less than a unit).
 struct Weights {
   float best;     // the largest logit
   double rate;    // 64 log2(e) / T
   const Powers* powers;
+  float half_best, fast_rate;  // intervals are by a difference in 32 bits, halved so that it stays finite
   __device__ __forceinline__ double steps(float v) const { return v == best ? 0.0 : ((double)best - (double)v) * rate; }
-  // A logit below it lies more than `limit` steps down: rounded towards smaller ones, so that one comparison in 32 bits leaves out what weighs nothing
+  // of a finite best: nothing has to be asked.  (The minimum is for temperatures whose rate 32 bits do not hold.)
+  __device__ __forceinline__ double finite_steps(float v) const { return fmin(((double)best - (double)v) * rate, kSteps + 63.0); }
+  // The interval that a logit lies in, by a function that never falls with the distance from a finite best; kIntervals and more, or NaN: none, and no weight.  (Its 32-bit
+  // roundings are a few 2^-23 of it: what lies behind the last interval is more than 45 powers of two down.)
+  __device__ __forceinline__ float interval(float v) const { return fmaf(-0.5f, v, half_best) * fast_rate; }
+  // A logit below it lies more than `limit` intervals down: one comparison leaves out what weighs nothing
   __device__ __forceinline__ float cut(double limit) const {
-    const double v = (double)best - (limit + 1.0) / rate;
+    const double v = (double)best - 2.0 * (limit + 1.0) / (double)fast_rate;
     const float f = (float)v;
-    return f - fabsf(f) * 0x1p-23f;  // NaN (infinite logits, infinite temperatures): leaves nothing out
+    return f - fabsf(f) * 0x1p-23f;  // below it, whichever way it was rounded; of an infinite temperature -inf
   }
-  // w 2^up, as a number; z in [0, 2^31)
-  __device__ __forceinline__ double scaled(double z, int up) const {
-    const int whole = (int)z;
+  // The weight in units of 2^-44, not yet rounded; z in [0, kSteps + 64)
+  __device__ __forceinline__ double scaled(double z) const {
+    constexpr double magic = 6755399441055744.0;  // 1.5 2^52: what is added to it is rounded to a whole number, its lowest bits
+    const double t = z + magic;
+    const int whole = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
     constexpr double c = -0.69314718055994530942 / 64.0;
-    const double f = z - (double)whole;
-    double s = c * c * c * c * c / 120.0;
-    s = fma(s, f, c * c * c * c / 24.0);
-    s = fma(s, f, c * c * c / 6.0);
+    const double f = z - (t - magic);
+    double s = fma(c * c * c * c / 24.0, f, c * c * c / 6.0);
     s = fma(s, f, c * c / 2.0);
     s = fma(s, f, c);
     s = fma(s, f, 1.0);
-    return ldexp(s * powers->of[whole & 63], up - (whole >> 6));
+    const uint64_t power = __builtin_bit_cast(uint64_t, powers->of[whole & 63]) - ((uint64_t)(uint32_t)(whole >> 6) << 52);
+    return s * __builtin_bit_cast(double, power);
   }
-  // in units of 2^-44, rounded to the nearest, as a number: sums of up to 2^9 of them are exact; z in [0, kSteps)
+  // ... rounded to the nearest, as a number: sums of up to 2^9 of them are exact
   __device__ __forceinline__ double units(double z) const {
-    const double big = 4503599627370496.0;  // 2^52: what is added to it is rounded to a whole number
-    return (scaled(z, kUnit) + big) - big;
+    const double big = 4503599627370496.0;  // 2^52
+    return (scaled(z) + big) - big;
   }
   __device__ __forceinline__ uint64_t at(double z) const {
     const double big = 4503599627370496.0;
-    return __builtin_bit_cast(uint64_t, scaled(z, kUnit) + big) - __builtin_bit_cast(uint64_t, big);
+    return __builtin_bit_cast(uint64_t, scaled(z) + big) - __builtin_bit_cast(uint64_t, big);
   }
   __device__ __forceinline__ uint64_t operator()(float v) const {
     const double z = steps(v);
     return z < (double)kSteps ? at(z) : 0;  // NaN: nothing
   }
-  __device__ __forceinline__ double exact(float v) const { return scaled(fmin(steps(v), 64000.0), 0); }
+  __device__ __forceinline__ double exact(float v) const { return scaled(fmin(steps(v), 64000.0)) * (1.0 / (double)kOne); }
 };
 
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
@@ -298,7 +304,7 @@ __device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int 
 // ---- slices ----
 constexpr int kSliceThreads = kThreads;
 constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
-constexpr int kMaxSlice = 64 * kThreads;  // a wavefront has a lane for each of a thread's tokens
+constexpr int kMaxSlice = 16384;
 constexpr int kCollected = 4096;
 
 // What the kernels leave for each other, a row of each a row.
@@ -308,9 +314,10 @@ struct Scratch {
   unsigned int* count;         // [kIntervals]
   unsigned int* collected;     // [1] tokens of the border's intervals
   unsigned long long* tokens;  // [kCollected] their places
-  unsigned long long* sums;    // [slices] weights surely kept
-  unsigned long long* front;   // [5] tokens and weights in front of the border's intervals, weights of all; their first step and steps
+  unsigned long long* sums;    // [stretches] weights surely kept of each kStep elements
+  unsigned long long* front;   // [5] tokens and weights in front of the border's intervals, weights of all; the first of these and their number
   int slices, slice;           // elements of a slice, a multiple of kStep
+  int stretches;               // kStep elements each
 };
 
 // Eight elements from i on, -inf behind the end.
@@ -351,10 +358,20 @@ __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) 
   }
 }
 
+// ... of one step.
+template <typename T, bool WIDE, typename F>
+__device__ __forceinline__ void in_step(const T* row, int first, int end, F f) {
+  const int i = first + threadIdx.x * 8;
+  float a[8];
+  load8<T, WIDE>(row, i, end, a);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) f(a[u], i + u);
+}
+
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
   __shared__ unsigned long long waves[kSliceThreads / 64];
-  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
+  const int slice = blockIdx.x, r = blockIdx.y;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   // a thread meets its elements by rising index: of equal ones the first stays
@@ -392,7 +409,10 @@ __device__ __forceinline__ uint64_t best_of_row(const Scratch& s, int r) {
   return wave_max(best);
 }
 __device__ __forceinline__ Weights weights_of(uint64_t best, float temperature, const Powers* powers) {
-  return Weights{value_of((uint32_t)(best >> 32)), 64.0 * 1.4426950408889634074 / (double)temperature, powers};
+  const float v = value_of((uint32_t)(best >> 32));
+  const double rate = 64.0 * 1.4426950408889634074 / (double)temperature;
+  return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate, 1e38)};  // of half the distance and two steps an interval
+
 }
 
 template <typename T, bool WIDE>
@@ -400,37 +420,40 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   __shared__ Powers powers;
   __shared__ unsigned long long weight[kIntervals];
   __shared__ unsigned int count[kIntervals];
-  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
+  const int slice = blockIdx.x, r = blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
   if (!(t > 0.f) || !f.any()) return;
   const uint64_t best = best_of_row(s, r);
-  if ((uint32_t)(best >> 32) <= kNone) return;
+  const Weights w = weights_of(best, t, &powers);
+  if (!(fabsf(w.best) <= 3.4028234664e38f)) return;  // nothing to choose from, or infinite: the last kernel looks at the row
   fill(powers);
   for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads) {
     weight[i] = 0;
     count[i] = 0;
   }
   __syncthreads();
-  const Weights w = weights_of(best, t, &powers);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
-  const float cut = w.cut(kSteps);
-  in_steps<T, WIDE>(row, first, end, [&](float v, int) {
-    if (v < cut) return;
-    const double z = w.steps(v);
-    if (z < (double)kSteps) {
-      const int at = (int)z >> 1;
-      atomicAdd(&count[at], 1u);
-      if (f.by_sum) atomicAdd(&weight[at], (unsigned long long)w.at(z));
-    }
-  });
+  const bool by_count = f.k > 0;
+  auto each = [&](auto counts, auto weighs) {
+    in_steps<T, WIDE>(row, first, end, [&](float v, int) {
+      const float i = w.interval(v);
+      if (i < (float)kIntervals) {
+        if constexpr (decltype(counts)::value != 0) atomicAdd(&count[(int)i], 1u);
+        if constexpr (decltype(weighs)::value != 0) atomicAdd(&weight[(int)i], (unsigned long long)w.at(w.finite_steps(v)));
+      }
+    });
+  };
+  using pto_hip::block8::IntConst;
+  if (by_count && f.by_sum) each(IntConst<1>{}, IntConst<1>{});
+  else if (by_count) each(IntConst<1>{}, IntConst<0>{});
+  else each(IntConst<0>{}, IntConst<1>{});
   __syncthreads();
-  for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads)
-    if (count[i]) {
-      atomicAdd(&s.count[(size_t)r * kIntervals + i], count[i]);
-      if (f.by_sum) atomicAdd(&s.weight[(size_t)r * kIntervals + i], weight[i]);
-    }
+  for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads) {
+    if (by_count && count[i]) atomicAdd(&s.count[(size_t)r * kIntervals + i], count[i]);
+    if (f.by_sum && weight[i]) atomicAdd(&s.weight[(size_t)r * kIntervals + i], weight[i]);
+  }
 }
 
 // The intervals in which a row's border may lie: first and last, and what lies in front of the first.
@@ -447,7 +470,7 @@ __device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int 
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int at = threadIdx.x * kOwn + i;
-    n[i] = at < kIntervals ? s.count[(size_t)r * kIntervals + at] : 0;
+    n[i] = at < kIntervals && f.k ? s.count[(size_t)r * kIntervals + at] : 0;
     x[i] = at < kIntervals && f.by_sum ? s.weight[(size_t)r * kIntervals + at] : 0;
     n_own += n[i];
     x_own += x[i];
@@ -521,14 +544,21 @@ __device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int 
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratch s) {
   __shared__ Powers powers;
-  __shared__ unsigned long long waves[kSliceThreads / 64];
-  const int slice = blockIdx.x, r = p.row0 + blockIdx.y;
+  __shared__ unsigned long long sums[kMaxSlice / kStep];
+  const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
   if (!(t > 0.f)) return;
   const Filters f = filters_of(p, r);
   const uint64_t best = best_of_row(s, r);
   if ((uint32_t)(best >> 32) <= kNone) return;
+  const Weights w = weights_of(best, t, &powers);
+  const bool infinite = !(w.best <= 3.4028234664e38f);
+  if (infinite && f.any()) {
+    if (slice == 0 && threadIdx.x == 0) s.collected[r] = kCollected + 1;  // for the last kernel to look at the row
+    return;
+  }
   fill(powers);
+  if (threadIdx.x < kMaxSlice / kStep) sums[threadIdx.x] = 0;
   BorderIntervals at{kIntervals, kIntervals, 0, 0, 0};
   if (f.any()) at = find_intervals(s, r, f);
   if (slice == 0 && threadIdx.x == 0) {
@@ -536,38 +566,41 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     front[0] = at.tokens_front;
     front[1] = at.weight_front;
     front[2] = at.weight_all;
-    front[3] = 2 * at.first;
-    front[4] = 2 * (at.last - at.first + 1);
+    front[3] = at.first;
+    front[4] = at.last - at.first + 1;
   }
   __syncthreads();
-  const Weights w = weights_of(best, t, &powers);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
-  // of what is surely kept, min_p leaves out what is further down than this (a step more than it has to be)
-  const double z_least = 64.0 * (kUnit - log2((double)f.least)) + 1.0;
-  const double z_first = 2.0 * at.first, z_sure = min(z_first, z_least), z_behind = min(2.0 * (at.last + 1), (double)kSteps);
-  const float cut = w.cut(at.first < kIntervals ? z_behind : z_sure);
   const double least = (double)f.least;
-  double own = 0.0;  // at most 64 elements': exact
-  in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
+  // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
+  const float i_least = (float)(32.0 * (kUnit - log2(least)) + 1.0);
+  const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
+  const float cut = infinite ? w.best : w.cut(at.first < kIntervals ? i_behind : i_sure);
+  double own = 0.0;  // of a step or two: exact
+  auto take = [&](float v, int i) __attribute__((always_inline)) {
     if (v < cut) return;
-    const double z = w.steps(v);
-    if (z < z_sure) {
-      const double x = w.units(z);
+    const float at_i = w.interval(v);
+    if (at_i < i_sure) {
+      const double x = w.units(w.finite_steps(v));
       own += x >= least ? x : 0.0;
-    } else if (z >= z_first && z < z_behind) {
+    } else if (at_i >= i_first && at_i < i_behind) {
       const unsigned int n = atomicAdd(&s.collected[r], 1u);
       if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v, i);
     }
-  });
-  uint64_t sum = (uint64_t)own;
-  sum = wave_sum((unsigned long long)sum);
-  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kSliceThreads / 64; ++i) sum += waves[i];
-    s.sums[(size_t)r * s.slices + slice] = sum;
+  };
+  auto take_infinite = [&](float v, int) { own += v == w.best ? (double)kOne : 0.0; };
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    own = 0.0;
+    const int to = min(i0 + kStep, end);
+    if (infinite) in_step<T, WIDE>(row, i0, to, take_infinite);
+    else in_step<T, WIDE>(row, i0, to, take);
+    const uint64_t sum = wave_sum((unsigned long long)own);
+    if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sums[(i0 - first) / kStep], (unsigned long long)sum);
   }
+  __syncthreads();
+  const int stretch = first / kStep + threadIdx.x;
+  if (threadIdx.x < s.slice / kStep && stretch < s.stretches) s.sums[(size_t)r * s.stretches + stretch] = sums[threadIdx.x];
 }
 
 constexpr int kCells = 1024;  // of the border's intervals
@@ -677,28 +710,28 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   const Filters f = filters_of(p, r);
   fill(sh.powers);
   const Weights w = weights_of(best, t, &sh.powers);
-  for (int i = threadIdx.x; i < s.slices; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.slices + i];
+  for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
   const int n = f.any() ? (int)min(s.collected[r], (unsigned int)kCollected + 1) : 0;
   uint64_t border = (uint64_t)(kNone + 1) << 32;
   __syncthreads();
   if (n > kCollected) {
     border = border_of_row(sh.row, row, p.vocab, w, f);
-    // the slices' sums lack what the border's intervals keep
-    for (int i = threadIdx.x; i < s.slices; i += kThreads) sh.sums[i] = 0;
+    // the stretches' sums lack what the border's intervals keep
+    for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = 0;
     __syncthreads();
     for (int i0 = 0; i0 < p.vocab; i0 += kThreads) {
       const int i = i0 + threadIdx.x;
       const float v = i < p.vocab ? logit(row, i) : -INFINITY;
       uint64_t x = i < p.vocab && packed(v, i) >= border ? w(v) : 0;
       x = wave_sum((unsigned long long)(x >= f.least ? x : 0));
-      if (threadIdx.x % 64 == 0 && x) atomicAdd(&sh.sums[i0 / s.slice], (unsigned long long)x);  // a slice is a multiple of kThreads
+      if (threadIdx.x % 64 == 0 && x) atomicAdd(&sh.sums[i0 / kStep], (unsigned long long)x);  // a stretch is a multiple of kThreads
     }
   } else if (n > 0) {
     const unsigned long long* tokens = s.tokens + (size_t)r * kCollected;
     const unsigned long long* front = s.front + 5 * (size_t)r;
-    const double z_first = (double)front[3], per_step = (double)kCells / (double)front[4];
+    const float i_first = (float)front[3], per_interval = (float)kCells / (float)front[4];
     auto weight = [&](uint64_t token) { return w(value_of((uint32_t)(token >> 32))); };
-    auto cell = [&](uint64_t token) { return min((int)((w.steps(value_of((uint32_t)(token >> 32))) - z_first) * per_step), kCells - 1); };
+    auto cell = [&](uint64_t token) { return min((int)((w.interval(value_of((uint32_t)(token >> 32))) - i_first) * per_interval), kCells - 1); };
     for (int i = threadIdx.x; i < kCells; i += kThreads) {
       sh.cells.weight[i] = 0;
       sh.cells.count[i] = 0;
@@ -722,18 +755,18 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
     }
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const uint64_t x = tokens[i] >= border ? weight(tokens[i]) : 0;
-      if (x >= f.least) atomicAdd(&sh.sums[(int)~(uint32_t)tokens[i] / s.slice], (unsigned long long)x);
+      if (x >= f.least) atomicAdd(&sh.sums[(int)~(uint32_t)tokens[i] / kStep], (unsigned long long)x);
     }
   }
   __syncthreads();
-  // the slice in which the running sum passes its share
+  // the stretch in which the running sum passes its share
   if (threadIdx.x < 64) {
     constexpr int kOwn = kMaxVocab / kStep / 64;
     uint64_t x[kOwn], own = 0;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
       const int i = threadIdx.x * kOwn + u;
-      x[u] = i < s.slices ? sh.sums[i] : 0;
+      x[u] = i < s.stretches ? sh.sums[i] : 0;
       own += x[u];
     }
     uint64_t to = own;
@@ -758,58 +791,39 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
     }
   }
   __syncthreads();
-  const int first = (int)sh.found[0] * s.slice, end = min(p.vocab, first + s.slice);
+  const int first = (int)sh.found[0] * kStep, end = min(p.vocab, first + kStep);
   const uint64_t target = sh.found[1], sum = sh.found[3];
-  // the thread whose tokens hold it, neighbouring ones, and its wavefront looks for the token among them
-  const int per = s.slice / kThreads, lane = threadIdx.x % 64;
-  auto kept = [&](int i) -> uint64_t {
-    const float v = logit(row, i);
-    const uint64_t x = packed(v, i) >= border ? w(v) : 0;
-    return x >= f.least ? x : 0;
-  };
-  uint64_t own = 0;
-  for (int u = 0; u < per; u += 8) {
-    const int i = first + threadIdx.x * per + u;
-    float v[8];
-    load8<T, WIDE>(row, i, end, v);
+  // the thread whose eight tokens hold it, and the token among them
+  const int mine = first + threadIdx.x * 8;
+  float v[8];
+  load8<T, WIDE>(row, mine, end, v);
+  uint64_t x[8], own = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint64_t x = i + e < end && packed(v[e], i + e) >= border ? w(v[e]) : 0;
-      own += x >= f.least ? x : 0;
-    }
+  for (int e = 0; e < 8; ++e) {
+    x[e] = mine + e < end && packed(v[e], mine + e) >= border ? w(v[e]) : 0;
+    x[e] = x[e] >= f.least ? x[e] : 0;
+    own += x[e];
   }
   unsigned long long all;
-  const uint64_t front = sh.found[2] + sum_in_front<unsigned long long>(own, sh.waves, &all);
-  const uint64_t here = __ballot(front <= target && front + own > target);
-  if (!here) return;
-  const int from = __builtin_ctzll(here), i = first + ((int)(threadIdx.x & ~63u) + from) * per + lane;
-  const uint64_t x = lane < per && i < end ? kept(i) : 0;
-  uint64_t to = x;
+  uint64_t front = sh.found[2] + sum_in_front<unsigned long long>(own, sh.waves, &all);
+  if (front <= target && front + own > target) {
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_up((unsigned long long)to, off);
-    if (lane >= off) to += o;
-  }
-  to += __shfl((unsigned long long)front, from);
-  if (to - x <= target && to > target) {
-    p.tokens[r] = i;
-    if (p.probs) p.probs[r] = (float)(w.exact(logit(row, i)) / ((double)sum * (1.0 / (double)kOne)));
+    for (int e = 0; e < 8; ++e) {
+      if (front <= target && front + x[e] > target) {
+        p.tokens[r] = mine + e;
+        if (p.probs) p.probs[r] = (float)(w.exact(v[e]) / ((double)sum * (1.0 / (double)kOne)));
+      }
+      front += x[e];
+    }
   }
 }
 
-// Rows are read two or three times: a group's logits fit the last-level cache.
-constexpr int64_t kGroupBytes = 96 << 20;
 template <typename T, bool WIDE>
-void launch_slices(Params& p, const Scratch& s, hipStream_t st) {
-  const int64_t group = std::max<int64_t>(1, kGroupBytes / ((int64_t)p.vocab * (int64_t)sizeof(T)));
-  for (int64_t r = 0; r < p.rows; r += group) {
-    p.row0 = (int)r;
-    const dim3 grid(s.slices, (unsigned)std::min(group, p.rows - r)), threads(kSliceThreads);
-    hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-    if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-    hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
-  }
-  p.row0 = 0;
+void launch_slices(const Params& p, const Scratch& s, hipStream_t st) {
+  const dim3 grid(s.slices, p.rows), threads(kSliceThreads);
+  hipLaunchKernelGGL((best_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  if (p.top_k || p.top_p) hipLaunchKernelGGL((histogram_kernel<T, WIDE>), grid, threads, 0, st, p, s);
+  hipLaunchKernelGGL((collect_kernel<T, WIDE>), grid, threads, 0, st, p, s);
   hipLaunchKernelGGL((draw_kernel<T, WIDE>), dim3(p.rows), dim3(kThreads), 0, st, p, s);
 }
 
@@ -822,13 +836,14 @@ int launch(Params p, hipStream_t st) {
   Scratch s{};
   s.slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(kStep, (even + kStep - 1) / kStep * kStep));
   s.slices = (p.vocab + s.slice - 1) / s.slice;
-  const size_t per_row = 8 * (2 * (size_t)s.slices + kIntervals + kCollected + 5) + 4 * (kIntervals + 2);
+  s.stretches = (p.vocab + kStep - 1) / kStep;
+  const size_t per_row = 8 * ((size_t)s.slices + s.stretches + kIntervals + kCollected + 5) + 4 * (kIntervals + 2);
   void* ws = nullptr;
   const int rc = pto_hip::workspace(per_row * at_once, &ws);
   if (rc) return rc;
   s.best = reinterpret_cast<unsigned long long*>(ws);
   s.sums = s.best + at_once * s.slices;
-  s.weight = s.sums + at_once * s.slices;
+  s.weight = s.sums + at_once * s.stretches;
   s.tokens = s.weight + at_once * kIntervals;
   s.front = s.tokens + at_once * kCollected;
   s.count = reinterpret_cast<unsigned int*>(s.front + 5 * at_once);
@@ -878,7 +893,7 @@ extern "C" int pto_hip_sample_tokens(const void* logits, const float* temperatur
   }
   const DeviceScope scope(ctx().device);
   hipStream_t st = (hipStream_t)stream;
-  const Params p{logits, temperature, top_k, top_p, min_p, uniform, tokens, probs, (int)rows, (int)vocab, 0};
+  const Params p{logits, temperature, top_k, top_p, min_p, uniform, tokens, probs, (int)rows, (int)vocab};
   const int rc = logits_dtype == PTO_HIP_FP32 ? launch<float>(p, st) : logits_dtype == PTO_HIP_BF16 ? launch<__bf16>(p, st) : launch<_Float16>(p, st);
   if (rc) return rc;
   PTO_CHECK_HIP(hipGetLastError());
