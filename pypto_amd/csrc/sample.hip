@@ -306,6 +306,7 @@ constexpr int kSliceThreads = kThreads;
 constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
 constexpr int kMaxSlice = 16384;
 constexpr int kCollected = 4096;
+constexpr int kGathered = 1024;  // by a workgroup for itself, with one place asked for in the row's list
 
 // What the kernels leave for each other, a row of each a row.
 struct Scratch {
@@ -358,14 +359,28 @@ __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) 
   }
 }
 
-// ... of one step.
-template <typename T, bool WIDE, typename F>
-__device__ __forceinline__ void in_step(const T* row, int first, int end, F f) {
-  const int i = first + threadIdx.x * 8;
-  float a[8];
-  load8<T, WIDE>(row, i, end, a);
+// f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile.
+template <typename T, bool WIDE, typename F, typename Done>
+__device__ __forceinline__ void step_by_step(const T* row, int first, int end, F f, Done done) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  const auto load = [&](int i) __attribute__((always_inline)) {
+    T8 v;
+    if constexpr (WIDE) {
+      if (i + 8 <= end) return *reinterpret_cast<const T8*>(row + i);
+    }
 #pragma unroll
-  for (int u = 0; u < 8; ++u) f(a[u], i + u);
+    for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
+    return v;
+  };
+  T8 next = load(first + threadIdx.x * 8);
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    const T8 v = next;
+    if (i0 + kStep < end) next = load(i + kStep);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f((float)v[u], i + u);
+    done((i0 - first) / kStep);
+  }
 }
 
 template <typename T, bool WIDE>
@@ -545,6 +560,8 @@ template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratch s) {
   __shared__ Powers powers;
   __shared__ unsigned long long sums[kMaxSlice / kStep];
+  __shared__ unsigned long long tokens[kGathered];
+  __shared__ unsigned int gathered, place;
   const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
   if (!(t > 0.f)) return;
@@ -559,6 +576,7 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   }
   fill(powers);
   if (threadIdx.x < kMaxSlice / kStep) sums[threadIdx.x] = 0;
+  if (threadIdx.x == 0) gathered = 0;
   BorderIntervals at{kIntervals, kIntervals, 0, 0, 0};
   if (f.any()) at = find_intervals(s, r, f);
   if (slice == 0 && threadIdx.x == 0) {
@@ -576,31 +594,47 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
   const float i_least = (float)(32.0 * (kUnit - log2(least)) + 1.0);
   const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
-  const float cut = infinite ? w.best : w.cut(at.first < kIntervals ? i_behind : i_sure);
-  double own = 0.0;  // of a step or two: exact
+  const float cut = w.cut(i_behind);
+  double own = 0.0;  // of a step: exact
   auto take = [&](float v, int i) __attribute__((always_inline)) {
-    if (v < cut) return;
+    if (v < cut) return;  // most logits of a row with a border
     const float at_i = w.interval(v);
     if (at_i < i_sure) {
       const double x = w.units(w.finite_steps(v));
       own += x >= least ? x : 0.0;
     } else if (at_i >= i_first && at_i < i_behind) {
-      const unsigned int n = atomicAdd(&s.collected[r], 1u);
-      if (n < kCollected) s.tokens[(size_t)r * kCollected + n] = packed(v, i);
+      const unsigned int n = atomicAdd(&gathered, 1u);
+      if (n < kGathered) {
+        tokens[n] = packed(v, i);
+      } else {
+        const unsigned int m = atomicAdd(&s.collected[r], 1u);
+        if (m < kCollected) s.tokens[(size_t)r * kCollected + m] = packed(v, i);
+      }
     }
   };
+  // of a row without a border: nearly all of its logits weigh something, and nothing is branched around
+  auto take_all = [&](float v, int) __attribute__((always_inline)) {
+    const double x = w.units(w.finite_steps(v));
+    own += x >= least ? x : 0.0;
+  };
   auto take_infinite = [&](float v, int) { own += v == w.best ? (double)kOne : 0.0; };
-  for (int i0 = first; i0 < end; i0 += kStep) {
-    own = 0.0;
-    const int to = min(i0 + kStep, end);
-    if (infinite) in_step<T, WIDE>(row, i0, to, take_infinite);
-    else in_step<T, WIDE>(row, i0, to, take);
+  auto done = [&](int step) __attribute__((always_inline)) {
     const uint64_t sum = wave_sum((unsigned long long)own);
-    if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sums[(i0 - first) / kStep], (unsigned long long)sum);
-  }
+    if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sums[step], (unsigned long long)sum);
+    own = 0.0;
+  };
+  if (infinite) step_by_step<T, WIDE>(row, first, end, take_infinite, done);
+  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, take_all, done);
+  else step_by_step<T, WIDE>(row, first, end, take, done);
   __syncthreads();
   const int stretch = first / kStep + threadIdx.x;
   if (threadIdx.x < s.slice / kStep && stretch < s.stretches) s.sums[(size_t)r * s.stretches + stretch] = sums[threadIdx.x];
+  const unsigned int n = min(gathered, (unsigned int)kGathered);
+  if (n == 0) return;
+  if (threadIdx.x == 0) place = atomicAdd(&s.collected[r], n);
+  __syncthreads();
+  for (unsigned int i = threadIdx.x; i < n; i += kSliceThreads)
+    if (place + i < kCollected) s.tokens[(size_t)r * kCollected + place + i] = tokens[i];
 }
 
 constexpr int kCells = 1024;  // of the border's intervals
