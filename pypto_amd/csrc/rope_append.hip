@@ -21,6 +21,7 @@ using pto_hip::TokenSeq;
 constexpr int kThreads = 256;
 constexpr int64_t kMaxTokens = 1 << 20;
 constexpr float kE4m3Max = 448.f;
+constexpr int kManyGroups = 16;
 
 struct Params {
   const void* qkv;  // [T, (Hq + 2 Hkv) D]
@@ -90,10 +91,25 @@ __device__ __forceinline__ void load_f8(const float* p, float (&x)[8]) {  // any
   for (int i = 0; i < 8; ++i) x[i] = p[i];
 }
 
+// The cosines and sines of a lane's eight elements.
+struct Angles {
+  float c[8], s[8];
+};
+__device__ __forceinline__ Angles load_angles(const Params& p, int pos, int e0) {
+  Angles a{};
+  if (e0 < 2 * p.rope_half) {
+    // a table of one angle a pair is read at the pair's number, the reference's tables at the element's own
+    const size_t at = (size_t)pos * p.rope_w + (p.rope_w == p.d || e0 < p.rope_half ? e0 : e0 - p.rope_half);
+    load_f8(p.cos + at, a.c);
+    load_f8(p.sin + at, a.s);
+  }
+  return a;
+}
+
 // Norm and rotation of one head's row by the LANES lanes that hold it, eight elements each (lanes past the row hold none): y = what
 // becomes of the lane's own.  All lanes of the group take part.
 template <typename In, int LANES>
-__device__ __forceinline__ void turn_row(const Params& p, const Raw8<In>& raw, const float* gamma, int pos, bool turn, int e0, float (&y)[8]) {
+__device__ __forceinline__ void turn_row(const Params& p, const Raw8<In>& raw, const float* gamma, const Angles& angles, bool turn, int e0, float (&y)[8]) {
   widen8(raw, y);
   if (!turn) return;  // a value's row
   const bool inside = e0 < p.d;
@@ -126,13 +142,8 @@ __device__ __forceinline__ void turn_row(const Params& p, const Raw8<In>& raw, c
     }
   }
   if (inside && turned) {
-    // a table of one angle a pair is read at the pair's number, the reference's tables at the element's own
-    const size_t at = (size_t)pos * p.rope_w + (p.rope_w == p.d ? e0 : low ? e0 : e0 - half);
-    float c[8], s[8];
-    load_f8(p.cos + at, c);
-    load_f8(p.sin + at, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = low ? y[i] * c[i] - x[i] * s[i] : y[i] * c[i] + x[i] * s[i];
+    for (int i = 0; i < 8; ++i) y[i] = low ? y[i] * angles.c[i] - x[i] * angles.s[i] : y[i] * angles.c[i] + x[i] * angles.s[i];
   }
 }
 
@@ -149,17 +160,19 @@ __device__ __forceinline__ bool cache_place(const Params& p, int seq, int number
   return ok;
 }
 
-// A workgroup for kThreads / LANES heads of one token, LANES lanes a head.  Q_ONLY: the queries alone (beside an e4m3 cache).
-template <typename In, typename T, int LANES, bool Q_ONLY>
+// A workgroup for GROUPS times kThreads / LANES heads of one token, LANES lanes a head.  Q_ONLY: the queries alone (beside an e4m3 cache).
+template <typename In, typename T, int LANES, bool Q_ONLY, int GROUPS>
 __global__ __launch_bounds__(kThreads) void append_kernel(Params p) {
+  constexpr int kHeads = kThreads / LANES;
   const int t = p.t0 + blockIdx.x, lane = threadIdx.x % 64;
-  const int head = blockIdx.y * (kThreads / LANES) + threadIdx.x / LANES;
+  const int head0 = blockIdx.y * (GROUPS * kHeads) + threadIdx.x / LANES;
   const int heads = Q_ONLY ? p.hq : p.hq + 2 * p.hkv;
   const int e0 = threadIdx.x % LANES * 8;
-  const bool inside = e0 < p.d && head < heads;
   const int width = p.hq + 2 * p.hkv;
-  Raw8<In> raw{};
-  if (inside) raw = load8(reinterpret_cast<const In*>(p.qkv) + ((size_t)t * width + head) * p.d + e0);
+  Raw8<In> raw[GROUPS] = {};
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g)
+    if (e0 < p.d && head0 + g * kHeads < heads) raw[g] = load8(reinterpret_cast<const In*>(p.qkv) + ((size_t)t * width + head0 + g * kHeads) * p.d + e0);
   const int pos = p.positions[t];
   const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, t, lane);
   if (s.seq < 0) return;  // nobody's token
@@ -167,20 +180,25 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Params p) {
     if (threadIdx.x == 0) *p.error_flag = 1;
     return;
   }
+  const Angles angles = load_angles(p, pos, e0);
   int block = 0, place = 0;
   if (!cache_place(p, s.seq, t - s.first, &block, &place)) return;
-  const bool is_q = head < p.hq, is_k = !is_q && head < p.hq + p.hkv;
-  float y[8];
-  turn_row<In, LANES>(p, raw, is_q ? p.gamma_q : p.gamma_k, pos, is_q || is_k, e0, y);
-  if (!inside) return;
-  T* dst;
-  if (is_q) {
-    dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.hq + head) * p.d;
-  } else {
-    const int h = head - p.hq - (is_k ? 0 : p.hkv);
-    dst = reinterpret_cast<T*>(is_k ? p.key_cache : p.value_cache) + (((size_t)block * p.hkv + h) * p.bs + place) * p.d;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int head = head0 + g * kHeads;
+    const bool is_q = head < p.hq, is_k = !is_q && head < p.hq + p.hkv;
+    float y[8];
+    turn_row<In, LANES>(p, raw[g], is_q ? p.gamma_q : p.gamma_k, angles, is_q || is_k, e0, y);
+    if (e0 >= p.d || head >= heads) continue;
+    T* dst;
+    if (is_q) {
+      dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.hq + head) * p.d;
+    } else {
+      const int h = head - p.hq - (is_k ? 0 : p.hkv);
+      dst = reinterpret_cast<T*>(is_k ? p.key_cache : p.value_cache) + (((size_t)block * p.hkv + h) * p.bs + place) * p.d;
+    }
+    store8(dst + e0, y);
   }
-  store8(dst + e0, y);
 }
 
 // Any even head_dim and any tables: one wavefront a head, pair by pair.
@@ -269,7 +287,7 @@ __global__ __launch_bounds__(kThreads) void append_fp8_kernel(Params p) {
     const int pos = p.positions[token];
     const bool ok = r < rows && pos >= 0 && pos < p.max_pos;
     if (r < rows && !ok) *p.error_flag = 1;
-    turn_row<In, LANES>(p, raw, p.gamma_k, ok ? pos : 0, is_k, e0, y);
+    turn_row<In, LANES>(p, raw, p.gamma_k, is_k ? load_angles(p, ok ? pos : 0, e0) : Angles{}, is_k, e0, y);
     return ok;
   };
   constexpr int kGroups = kThreads / LANES;
@@ -354,10 +372,16 @@ void launch(Params& p, bool fp8, bool wide, hipStream_t st) {
   with_lanes(p.d, [&](auto lanes) {
     constexpr int L = decltype(lanes)::value, kHeads = kThreads / L;
     const int groups = ((fp8 ? p.hq : heads) + kHeads - 1) / kHeads;
-    in_launches(p, (int64_t)kThreads * groups, [&](unsigned n) {
-      if (fp8) hipLaunchKernelGGL((append_kernel<In, T, L, true>), dim3(n, groups), dim3(kThreads), 0, st, p);
-      else hipLaunchKernelGGL((append_kernel<In, T, L, false>), dim3(n, groups), dim3(kThreads), 0, st, p);
-    });
+    auto rows = [&](auto per, auto q_only) {
+      constexpr int G = decltype(per)::value;
+      const unsigned y = (groups + G - 1) / G;
+      in_launches(p, (int64_t)kThreads * y, [&](unsigned n) {
+        hipLaunchKernelGGL((append_kernel<In, T, L, decltype(q_only)::value != 0, G>), dim3(n, y), dim3(kThreads), 0, st, p);
+      });
+    };
+    auto of = [&](auto per) { fp8 ? rows(per, Lanes<1>{}) : rows(per, Lanes<0>{}); };
+    if ((int64_t)p.tokens * groups >= kManyGroups * pto_hip::ctx().num_cu) of(Lanes<4>{});
+    else of(Lanes<1>{});
     if (fp8)
       in_launches(p, (int64_t)kThreads * 2 * p.hkv,
                   [&](unsigned n) { hipLaunchKernelGGL((append_fp8_kernel<In, L>), dim3(n, 2 * p.hkv), dim3(kThreads), 0, st, p); });
