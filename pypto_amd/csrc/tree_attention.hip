@@ -485,7 +485,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     }
   };
 
-  float k_mul = scale, v_unit = 1.f;
+  float k_mul = scale, v_unit = 1.f, v_top = 0.f;
   // A chunk's products from stage base `kbase`.  MASKED: some of its keys may be new tokens, or lie behind the last one.
   auto multiply = [&](const char* kbase, int tok, unsigned int odd, auto masked) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked)::value;
@@ -631,8 +631,12 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     if constexpr (FP8) {
       const float2 s = chunk_scale[stage];
       k_mul = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s.x)));
-      const float v_now = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s.y)));
-      // the chunk may be another block's than the one in front: the accumulators go on in its values' scale
+      float v_now = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, s.y)));
+      // The chunk may be another block's than the one in front: the accumulators go on in its values' scale.  One below 2^-60 of the largest counts as that (its values are
+      // off by 2^-51 of that scale at most), and 0 as the smallest number at least, so that they stay finite.
+      v_top = fmaxf(v_top, v_now);
+      const float v_least = fmaxf(v_top * 0x1p-60f, 0x1p-149f);
+      v_now = v_now < v_least ? v_least : v_now;
       if (v_now != v_unit) {
         const float ratio = tok == tok_first ? 1.f : v_unit / v_now;
 #pragma unroll
@@ -769,13 +773,14 @@ int launch_tiles(Params& p, hipStream_t st) {
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
   constexpr int kRows = NW * GT * 16;
   constexpr int kLds = 2 * AHEAD * Stage<D>::kBytes;
-  static int resident = 0;  // workgroups that a CU holds (calls take turns: PTO_DISPATCH_LOCK)
-  if (resident == 0) {
+  static int resident = 0, asked = -1;  // workgroups that a CU holds, of the device that was asked (calls take turns: PTO_DISPATCH_LOCK)
+  if (asked != pto_hip::ctx().device) {
     const void* kernel = reinterpret_cast<const void*>(&tree_kernel<D, BF16, FP8, NW, GT, AHEAD>);
     if (kLds > 64 * 1024) PTO_CHECK_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
     int n = 0;
     PTO_CHECK_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, NW * 64, kLds));
     resident = std::max(1, n);
+    asked = pto_hip::ctx().device;
   }
   p.target = pto_hip::ctx().num_cu * resident;
   p.per_target = 1.f / (float)p.target;
