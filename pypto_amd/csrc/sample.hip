@@ -638,6 +638,7 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
 }
 
 constexpr int kCells = 1024;  // of the border's intervals
+constexpr int kCounted = 512;  // tokens of a cell
 struct DrawShared {
   Powers powers;
   unsigned long long sums[kMaxVocab / kStep];
@@ -692,22 +693,45 @@ __device__ Reached reach(DrawShared& sh, const unsigned long long* tokens, int n
     if (cell(tokens[i]) == here) sh.tokens[atomicAdd(&sh.gathered, 1u)] = tokens[i];
   __syncthreads();
   const int m = (int)sh.gathered;
-  int size = 1;
-  while (size < m) size *= 2;
-  for (int i = m + threadIdx.x; i < size; i += kThreads) sh.tokens[i] = 0;  // the last places
-  __syncthreads();
-  for (int span = 2; span <= size; span *= 2)
-    for (int gap = span / 2; gap > 0; gap /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-        const int a = 2 * i - (i & (gap - 1)), b = a + gap;
-        const uint64_t va = sh.tokens[a], vb = sh.tokens[b];
-        if ((va < vb) == ((a & span) == 0)) {
-          sh.tokens[a] = vb;
-          sh.tokens[b] = va;
-        }
-      }
-      __syncthreads();
+  // in order
+  if (m <= kCounted) {
+    // every token's place is the number of those in front of it: m / 2 reads of LDS for each of m / 256 tokens a thread, all on their way at once
+    constexpr int kMine = kCounted / kThreads;
+    uint64_t mine[kMine];
+    int at[kMine];
+#pragma unroll
+    for (int u = 0; u < kMine; ++u) {
+      mine[u] = threadIdx.x + u * kThreads < m ? sh.tokens[threadIdx.x + u * kThreads] : 0;
+      at[u] = 0;
     }
+    for (int i = 0; i < m; ++i) {
+      const uint64_t other = sh.tokens[i];
+#pragma unroll
+      for (int u = 0; u < kMine; ++u) at[u] += other > mine[u];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kMine; ++u)
+      if (threadIdx.x + u * kThreads < m) sh.tokens[at[u]] = mine[u];
+    __syncthreads();
+  } else {
+    int size = 1;
+    while (size < m) size *= 2;
+    for (int i = m + threadIdx.x; i < size; i += kThreads) sh.tokens[i] = 0;  // the last places
+    __syncthreads();
+    for (int span = 2; span <= size; span *= 2)
+      for (int gap = span / 2; gap > 0; gap /= 2) {
+        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+          const int a = 2 * i - (i & (gap - 1)), b = a + gap;
+          const uint64_t va = sh.tokens[a], vb = sh.tokens[b];
+          if ((va < vb) == ((a & span) == 0)) {
+            sh.tokens[a] = vb;
+            sh.tokens[b] = va;
+          }
+        }
+        __syncthreads();
+      }
+  }
   // neighbouring tokens a thread
   const int per = (m + kThreads - 1) / kThreads, first = threadIdx.x * per;
   uint64_t own = 0;
