@@ -5,6 +5,11 @@
 //
 // at positions[t]; token i of sequence b goes to cache row (block_table[b][n / bs] * Hkv + h) * bs + n % bs with n = context_lens[b] + i.
 // The form for one token per sequence is rope.hip's (examples/models/qwen3_jit/kernels/attention.py:39-102).
+//
+// Every row is read once and written once, eight elements a lane; a pair's other element comes from another lane.  Large batches are bound by memory: 12000 tokens of 40 + 16
+// fp16 heads of 128 take 69 us, 350 MB at 5.1 TB/s, what a large copy reaches.  Small ones are bound by their chain of loads - the token's sequence, its length, its block, and
+// the row's angles beside them -: one token of 32 + 16 heads 3.4 us, 408 tokens 6.2 us.  Over e4m3 caches a block's scale has to be known before its rows are coded: a workgroup takes
+// all new rows of a (block, head) and reads them twice (385 tokens of 64 + 16 heads 11 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

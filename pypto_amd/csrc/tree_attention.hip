@@ -4,6 +4,11 @@
 //   n < context_lens[b], and n = context_lens[b] + j for the new tokens j of its sequence whose bit is set in tree_mask[t]
 //
 // The form for one token per sequence is paged_attention.hip's (examples/models/04_paged_attention.py:62-227).
+//
+// With few rows a sequence the caches' bytes bound it, with many the products: 16 sequences of 512 to 4096 bf16 keys and 1 to 40 new tokens, 32 heads over 8: 55 us (158 MB;
+// 30 us at the 5.2 TB/s of a large copy), 32 sequences of 2000 to 16000 e4m3 keys and 4 to 8 tokens, 64 heads over 8: 155 us (596 MB, 115 us), 4 sequences of 20000 to 32000 fp16 keys and
+// 64 tokens, 64 heads: 275 us (218 GFLOP, 182 us at the 1.2 PFLOP/s of a large product), one sequence of 4096 keys and 16 tokens: 19 us (14 and the join's 5), a chain of the
+// plan, the first loads, some 8 chunks and the join.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -302,11 +307,12 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
 }
 
-// A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.
+// A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.  At 0, with every rise followed: 65 us for 55 over 16 sequences,
+// 317 us for 273 over four long ones.
 constexpr int kSlack = 6;
 
 // Whether a wavefront has registers for three others on its SIMD: with one tile of rows, over e4m3 caches, whose rows on their way are half as long (32 sequences of 4 to 8
-// drafts, 64 heads: 190 -> 179 us; with 16-bit caches registers spill).
+// drafts, 64 heads: 190 -> 179 us by the kernel; with 16-bit caches registers spill).
 template <int D, bool FP8, int GT>
 constexpr bool lean() { return GT == 1 && FP8 && D <= 128; }
 
@@ -784,6 +790,7 @@ int launch_tiles(Params& p, hipStream_t st) {
   }
   p.target = pto_hip::ctx().num_cu * resident;
   p.per_target = 1.f / (float)p.target;
+  // parts of 256 keys at least: one sequence of 4096 keys takes 18.6 us, by parts of 64 keys 24.7, of 512 21.7 (what one launch saves the join takes, and the other way round)
   p.least = (float)(std::max(256, kRows) / kChunk);
   p.block_bytes = (uint32_t)((int64_t)p.hkv * p.bs * D * (FP8 ? 1 : 2));
   const int64_t blocks = (int64_t)p.tokens * p.group / kRows + std::min(p.batch, p.tokens);
@@ -810,7 +817,9 @@ int launch_rows(Params& p, hipStream_t st) {
   if constexpr (D == 256) {  // fewer wavefronts would bring so much each that their registers did not hold it
     return launch_tiles<D, BF16, FP8, 8, 1, 2>(p, st);
   } else {
-    if (rows <= 32) return launch_tiles<D, BF16, FP8, 2, 1, 1>(p, st);
+    // A sequence's rows in one workgroup as long as they fit: its keys are read once.  16 sequences of 4096 keys, 8 KV heads of 128 in bf16 (e4m3), by four wavefronts of one tile of
+    // rows / four of two / eight of two: 64 rows 62 / 66 / 71 us (60 / 67 / 87), 128 rows 85 / 76 / 81 (85 / 75 / 100), 256 rows 137 / 128 / 119 (145 / 126 / 119); 8 rows 54 / 57 / 64, and 58 by two
+    // wavefronts.  More tiles also want more chunks between barriers: the wavefronts of a SIMD drift apart, one in its products while the other is in its softmax.
     if (rows <= 64) return launch_tiles<D, BF16, FP8, 4, 1, 1>(p, st);
     if (rows <= 128) return launch_tiles<D, BF16, FP8, 4, 2, 2>(p, st);
     return launch_tiles<D, BF16, FP8, 8, 2, 4>(p, st);
