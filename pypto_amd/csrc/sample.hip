@@ -366,24 +366,26 @@ __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) 
   }
 }
 
-// f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile.
-template <typename T, bool WIDE, typename F, typename Done>
-__device__ __forceinline__ void step_by_step(const T* row, int first, int end, F f, Done done) {
-  typedef T T8 __attribute__((ext_vector_type(8)));
-  const auto load = [&](int i) __attribute__((always_inline)) {
-    T8 v;
-    if constexpr (WIDE) {
-      if (i + 8 <= end) return *reinterpret_cast<const T8*>(row + i);
-    }
+// A thread's eight elements as they lie in memory; -inf behind the end.
+template <typename T>
+using Raw8 = T __attribute__((ext_vector_type(8)));
+template <typename T, bool WIDE>
+__device__ __forceinline__ Raw8<T> load_raw(const T* row, int i, int end) {
+  if constexpr (WIDE) {
+    if (i + 8 <= end) return *reinterpret_cast<const Raw8<T>*>(row + i);
+  }
+  Raw8<T> v;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
-    return v;
-  };
-  T8 next = load(first + threadIdx.x * 8);
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
+  return v;
+}
+// f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile; `next`: the first step's, asked for long before.
+template <typename T, bool WIDE, typename F, typename Done>
+__device__ __forceinline__ void step_by_step(const T* row, int first, int end, Raw8<T> next, F f, Done done) {
   for (int i0 = first; i0 < end; i0 += kStep) {
     const int i = i0 + threadIdx.x * 8;
-    const T8 v = next;
-    if (i0 + kStep < end) next = load(i + kStep);
+    const Raw8<T> v = next;
+    if (i0 + kStep < end) next = load_raw<T, WIDE>(row, i + kStep, end);
 #pragma unroll
     for (int u = 0; u < 8; ++u) f((float)v[u], i + u);
     done((i0 - first) / kStep);
@@ -445,8 +447,11 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const int slice = blockIdx.x, r = blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
-  if (!(t > 0.f) || !f.any()) return;
   const uint64_t best = best_of_row(s, r);
+  if (!(t > 0.f) || !f.any()) return;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
   const Weights w = weights_of(best, t, &powers);
   if (!(fabsf(w.best) <= 3.4028234664e38f)) return;  // nothing to choose from, or infinite: the last kernel looks at the row
   fill(powers);
@@ -455,17 +460,15 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
     count[i] = 0;
   }
   __syncthreads();
-  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
-  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const bool by_count = f.k > 0;
   auto each = [&](auto counts, auto weighs) {
-    in_steps<T, WIDE>(row, first, end, [&](float v, int) {
+    step_by_step<T, WIDE>(row, first, end, ahead, [&](float v, int) __attribute__((always_inline)) {
       const float i = w.interval(v);
       if (i < (float)kIntervals) {
         if constexpr (decltype(counts)::value != 0) atomicAdd(&count[(int)i], 1u);
         if constexpr (decltype(weighs)::value != 0) atomicAdd(&weight[(int)i], (unsigned long long)w.at(w.finite_steps(v)));
       }
-    });
+    }, [](int) {});
   };
   using pto_hip::block8::IntConst;
   if (by_count && f.by_sum) each(IntConst<1>{}, IntConst<1>{});
@@ -571,10 +574,12 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   __shared__ unsigned int gathered, place;
   const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
-  if (!(t > 0.f)) return;
   const Filters f = filters_of(p, r);
   const uint64_t best = best_of_row(s, r);
-  if ((uint32_t)(best >> 32) <= kNone) return;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
+  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
+  if (!(t > 0.f) || (uint32_t)(best >> 32) <= kNone) return;
   const Weights w = weights_of(best, t, &powers);
   const bool infinite = !(w.best <= 3.4028234664e38f);
   if (infinite && f.any()) {
@@ -595,11 +600,9 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     front[4] = at.last - at.first + 1;
   }
   __syncthreads();
-  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
-  const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const double least = (double)f.least;
   // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
-  const float i_least = (float)(32.0 * (kUnit - log2(least)) + 1.0);
+  const float i_least = 32.f * ((float)kUnit - __builtin_amdgcn_logf((float)least)) + 1.f;
   const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
   const float cut = w.cut(i_behind);
   double own = 0.0;  // of a step: exact
@@ -630,9 +633,9 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sums[step], (unsigned long long)sum);
     own = 0.0;
   };
-  if (infinite) step_by_step<T, WIDE>(row, first, end, take_infinite, done);
-  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, take_all, done);
-  else step_by_step<T, WIDE>(row, first, end, take, done);
+  if (infinite) step_by_step<T, WIDE>(row, first, end, ahead, take_infinite, done);
+  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, ahead, take_all, done);
+  else step_by_step<T, WIDE>(row, first, end, ahead, take, done);
   __syncthreads();
   const int stretch = first / kStep + threadIdx.x;
   if (threadIdx.x < s.slice / kStep && stretch < s.stretches) s.sums[(size_t)r * s.stretches + stretch] = sums[threadIdx.x];
@@ -763,9 +766,13 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   __shared__ DrawShared sh;
   const int r = blockIdx.x;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
-  const uint64_t best = best_of_row(s, r);
-  const uint32_t top = (uint32_t)(best >> 32);
+  // everything that others left, asked for at once
   const float t = p.temperature[r];
+  const Filters f = filters_of(p, r);
+  const unsigned int collected = s.collected[r];
+  const uint64_t best = best_of_row(s, r);
+  for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
+  const uint32_t top = (uint32_t)(best >> 32);
   if (top <= kNone || !(t > 0.f)) {  // nothing to choose from, or no choice
     if (threadIdx.x == 0) {
       p.tokens[r] = top <= kNone ? -1 : (int32_t)~(uint32_t)best;
@@ -773,11 +780,9 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
     }
     return;
   }
-  const Filters f = filters_of(p, r);
   fill(sh.powers);
   const Weights w = weights_of(best, t, &sh.powers);
-  for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
-  const int n = f.any() ? (int)min(s.collected[r], (unsigned int)kCollected + 1) : 0;
+  const int n = f.any() ? (int)min(collected, (unsigned int)kCollected + 1) : 0;
   uint64_t border = (uint64_t)(kNone + 1) << 32;
   __syncthreads();
   if (n > kCollected) {
