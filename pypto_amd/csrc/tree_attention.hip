@@ -50,7 +50,7 @@ struct Params {
   float least;        // fewest chunks of a part
   int slots;          // partial results that there is room for, in tokens
   uint32_t block_bytes;  // of a cache's block, all KV heads
-  int4* joins;        // [B] of each sequence: parts, slot, first token, tokens
+  int4* joins;        // [T] of each token: parts, slot of its first part, tokens of its sequence
   float* part_o;      // [slots * Hq, D]
   float* part_ml;     // [slots * Hq, 2]: running maximum in units of log 2, sum
 };
@@ -348,10 +348,12 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
   const bool active = row0 < rows;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPlaces; ++i) odd_keys[i] = 0;
-    if (part == 0 && s.block == 0 && h == 0) p.joins[seq] = int4{parts, s.slot, token0, count};
     const int64_t raw = p.ctx_lens[seq];
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
+
+  if (part == 0 && s.block == 0 && h == 0)
+    for (int i = threadIdx.x; i < count; i += kThreads) p.joins[token0 + i] = int4{parts, s.slot + i, count, 0};
 
   // Query fragments (B operand): column = row c of the tile; k-group j of step u holds elements (u*4+j)*8..+8.  A negative scale changes their sign, so that
   // the largest product is the largest score.
@@ -717,18 +719,26 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p) {
   const int lane = threadIdx.x & 63;
   const int token = p.t0 + blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (head >= p.hq) return;
-  const TokenSeq own = pto_hip::sequence_of(p.starts, p.batch, token, lane);
-  if (own.seq < 0) return;
-  const int4 join = p.joins[own.seq];  // by the kernel in front, for every sequence that has tokens
-  const int np = join.x, slot = join.y, count = join.w;
-  if (join.z != own.first || count != own.count || np <= 1 || slot < 0 || (int64_t)slot + (int64_t)np * count > p.slots) return;
-  const size_t first = ((size_t)slot + (token - own.first)) * p.hq + head, step = (size_t)count * p.hq;
+  const int from = p.starts[0], to = p.starts[p.batch];
+  const int4 join = p.joins[token];  // by the kernel in front, for every token that a sequence has
+  const int np = join.x, count = join.z;
+  if (token < from || token >= to || np <= 1) return;
+  if (join.y < 0 || count < 1 || (int64_t)join.y + (int64_t)(np - 1) * count >= p.slots) return;  // only where the starts do not rise
+  const size_t first = (size_t)join.y * p.hq + head, step = (size_t)count * p.hq;
+  const float2* part_ml = reinterpret_cast<const float2*>(p.part_ml) + first;
+  const float* part_o = p.part_o + first * D + lane;
+  constexpr int kBatch = 8;
+  float ahead[kBatch][D / 64];  // the first parts' values, on their way while their weights are made
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) ahead[u][i] = part_o[min(u, np - 1) * step * D + i * 64];
   float m = kMinMax, l = 0.f, o[D / 64];
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
   for (int q0 = 0; q0 < np; q0 += 64) {
     const int q = min(q0 + lane, np - 1);
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (first + q * step) * 2);
+    const float2 ml = part_ml[q * step];
     const bool there = q0 + lane < np;
     float most = there ? ml.x : kMinMax;
 #pragma unroll
@@ -744,13 +754,18 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) o[i] *= keep;
     const int n = min(64, np - q0);
-    constexpr int kBatch = 8;
     for (int u0 = 0; u0 < n; u0 += kBatch) {
       float v[kBatch][D / 64];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) v[u][i] = p.part_o[(first + min(q0 + u0 + u, np - 1) * step) * D + i * 64 + lane];
+        for (int i = 0; i < D / 64; ++i) v[u][i] = ahead[u][i];
+      if (q0 + u0 + kBatch < np) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) ahead[u][i] = part_o[min(q0 + u0 + kBatch + u, np - 1) * step * D + i * 64];
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const float wgt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), min(u0 + u, 63)));
@@ -799,7 +814,7 @@ int launch_tiles(Params& p, hipStream_t st) {
   PTO_CHECK_ARG(grid < 1ll << 22 && slots < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
   const size_t o_bytes = (size_t)slots * p.hq * D * 4, ml_bytes = (size_t)slots * p.hq * 8;
   void* ws = nullptr;
-  const int rc = pto_hip::workspace(o_bytes + ml_bytes + 16 + (size_t)p.batch * sizeof(int4), &ws);
+  const int rc = pto_hip::workspace(o_bytes + ml_bytes + 16 + (size_t)p.tokens * sizeof(int4), &ws);
   if (rc) return rc;
   p.slots = (int)slots;
   p.joins = reinterpret_cast<int4*>(reinterpret_cast<char*>(ws) + o_bytes + (ml_bytes + 15) / 16 * 16);
