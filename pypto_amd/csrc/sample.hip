@@ -74,6 +74,10 @@ __device__ __forceinline__ void fill(Powers& t) {  // and a barrier
 constexpr int kSteps = 46 * 64;          // weights end behind 45 of the 64ths of a power of two
 constexpr int kIntervals = kSteps / 2;
 
+constexpr double kBig = 4503599627370496.0;  // 2^52
+// The whole number that was added to kBig.
+__device__ __forceinline__ uint64_t whole(double sum) { return __builtin_bit_cast(uint64_t, sum) - __builtin_bit_cast(uint64_t, kBig); }
+
 // What a logit of a row weighs.  With z = 64 log2(best's weight / its own): the whole number next to z is a place in the table and a power of two, the rest, half of
 // a 64th at most, five terms of the exponential's series (off by 4e-14 of it, less than a unit).
 struct Weights {
@@ -93,29 +97,22 @@ struct Weights {
     const float f = (float)v;
     return f - fabsf(f) * 0x1p-23f;  // below it, whichever way it was rounded; of an infinite temperature -inf
   }
-  // The weight in units of 2^-44, not yet rounded; z in [0, kSteps + 64)
+  // The weight in units of 2^-44, not yet rounded; z in [0, kSteps + 64).  Its lowest bit is set, so that it never lies halfway between two whole numbers: a sum that starts at
+  // kBig, where doubles are whole, rounds each in the same way whatever it holds already.
   __device__ __forceinline__ double scaled(double z) const {
     constexpr double magic = 6755399441055744.0;  // 1.5 2^52: what is added to it is rounded to a whole number, its lowest bits
     const double t = z + magic;
-    const int whole = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
+    const int near = (int)(uint32_t)__builtin_bit_cast(uint64_t, t);
     constexpr double c = -0.69314718055994530942 / 64.0;
     const double f = z - (t - magic);
     double s = fma(c * c * c * c / 24.0, f, c * c * c / 6.0);
     s = fma(s, f, c * c / 2.0);
     s = fma(s, f, c);
     s = fma(s, f, 1.0);
-    const uint64_t power = __builtin_bit_cast(uint64_t, powers->of[whole & 63]) - ((uint64_t)(uint32_t)(whole >> 6) << 52);
-    return s * __builtin_bit_cast(double, power);
+    const uint64_t power = __builtin_bit_cast(uint64_t, powers->of[near & 63]) - ((uint64_t)(uint32_t)(near >> 6) << 52);
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, s * __builtin_bit_cast(double, power)) | 1);
   }
-  // ... rounded to the nearest, as a number: sums of up to 2^9 of them are exact
-  __device__ __forceinline__ double units(double z) const {
-    const double big = 4503599627370496.0;  // 2^52
-    return (scaled(z) + big) - big;
-  }
-  __device__ __forceinline__ uint64_t at(double z) const {
-    const double big = 4503599627370496.0;
-    return __builtin_bit_cast(uint64_t, scaled(z) + big) - __builtin_bit_cast(uint64_t, big);
-  }
+  __device__ __forceinline__ uint64_t at(double z) const { return whole(scaled(z) + kBig); }
   __device__ __forceinline__ uint64_t operator()(float v) const {
     const double z = steps(v);
     return z < (double)kSteps ? at(z) : 0;  // NaN: nothing
@@ -600,18 +597,18 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     front[4] = at.last - at.first + 1;
   }
   __syncthreads();
-  const double least = (double)f.least;
+  const double least = (double)f.least, more_than = least - 0.5;  // of a weight not yet rounded
   // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
   const float i_least = 32.f * ((float)kUnit - __builtin_amdgcn_logf((float)least)) + 1.f;
   const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
   const float cut = w.cut(i_behind);
-  double own = 0.0;  // of a step: exact
+  double own = kBig;  // and the weights of a step: exact
   auto take = [&](float v, int i) __attribute__((always_inline)) {
     if (v < cut) return;  // most logits of a row with a border
     const float at_i = w.interval(v);
     if (at_i < i_sure) {
-      const double x = w.units(w.finite_steps(v));
-      own += x >= least ? x : 0.0;
+      const double x = w.scaled(w.finite_steps(v));
+      own += x > more_than ? x : 0.0;
     } else if (at_i >= i_first && at_i < i_behind) {
       const unsigned int n = atomicAdd(&gathered, 1u);
       if (n < kGathered) {
@@ -623,18 +620,20 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     }
   };
   // of a row without a border: nearly all of its logits weigh something, and nothing is branched around
-  auto take_all = [&](float v, int) __attribute__((always_inline)) {
-    const double x = w.units(w.finite_steps(v));
-    own += x >= least ? x : 0.0;
+  auto take_all = [&](float v, int) __attribute__((always_inline)) { own += w.scaled(w.finite_steps(v)); };
+  auto take_heavy = [&](float v, int) __attribute__((always_inline)) {
+    const double x = w.scaled(w.finite_steps(v));
+    own += x > more_than ? x : 0.0;
   };
   auto take_infinite = [&](float v, int) { own += v == w.best ? (double)kOne : 0.0; };
   auto done = [&](int step) __attribute__((always_inline)) {
-    const uint64_t sum = wave_sum((unsigned long long)own);
+    const uint64_t sum = wave_sum((unsigned long long)whole(own));
     if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sums[step], (unsigned long long)sum);
-    own = 0.0;
+    own = kBig;
   };
   if (infinite) step_by_step<T, WIDE>(row, first, end, ahead, take_infinite, done);
-  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, ahead, take_all, done);
+  else if (at.first == kIntervals && f.least == 1) step_by_step<T, WIDE>(row, first, end, ahead, take_all, done);  // what is below a half adds nothing
+  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, ahead, take_heavy, done);
   else step_by_step<T, WIDE>(row, first, end, ahead, take, done);
   __syncthreads();
   const int stretch = first / kStep + threadIdx.x;
