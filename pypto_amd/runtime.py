@@ -99,17 +99,17 @@ route_experts_biased = HipProgram("route_experts", (IN, IN, OUT, OUT),
 experts_ffn_fp8_block = HipProgram("experts_ffn_fp8_block", (IN,) * 10 + (OUT,))
 
 # a step that verifies drafted tokens, several new ones per sequence: qkv, positions, token_starts, context_lens, rope_cos, rope_sin,
-# [gamma_q, gamma_k,] block_table, key_cache, value_cache, [k_scale, v_scale,] q_out
-rope_append_tokens = HipProgram("rope_append_tokens", (IN,) * 7 + (INOUT, INOUT, OUT),
+# [gamma_q, gamma_k,] block_table, key_cache, value_cache, [k_scale, v_scale,] q_out (INOUT: rows that belong to nobody stay as they were)
+rope_append_tokens = HipProgram("rope_append_tokens", (IN,) * 7 + (INOUT,) * 3,
                                 scalars=("num_heads", "kv_head_num", "head_dim", "block_size"))
-rope_append_tokens_normed = HipProgram("rope_append_tokens", (IN,) * 9 + (INOUT, INOUT, OUT),
+rope_append_tokens_normed = HipProgram("rope_append_tokens", (IN,) * 9 + (INOUT,) * 3,
                                        scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "eps"))
-rope_append_tokens_fp8 = HipProgram("rope_append_tokens_fp8", (IN,) * 7 + (INOUT,) * 4 + (OUT,),
+rope_append_tokens_fp8 = HipProgram("rope_append_tokens_fp8", (IN,) * 7 + (INOUT,) * 5,
                                     scalars=("num_heads", "kv_head_num", "head_dim", "block_size"))
-rope_append_tokens_fp8_normed = HipProgram("rope_append_tokens_fp8", (IN,) * 9 + (INOUT,) * 4 + (OUT,),
+rope_append_tokens_fp8_normed = HipProgram("rope_append_tokens_fp8", (IN,) * 9 + (INOUT,) * 5,
                                            scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "eps"))
 # query, key_cache, value_cache, block_table, context_lens, token_starts, tree_mask, out [, k_scale, v_scale]
-tree_attention = HipProgram("tree_attention", (IN,) * 7 + (OUT, IN, IN), optional=2,
+tree_attention = HipProgram("tree_attention", (IN,) * 7 + (INOUT, IN, IN), optional=2,
                             scalars=("num_heads", "kv_head_num", "head_dim", "block_size", "scale"))
 # logits, temperature, top_k, top_p, min_p, uniform, tokens, probs
 sample_tokens = HipProgram("sample_tokens", (IN,) * 6 + (OUT, OUT))

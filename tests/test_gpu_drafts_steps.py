@@ -378,3 +378,23 @@ def test_calls_on_host_tensors(worker):
     host = torch.zeros((20, 64), dtype=BF)
     worker.run(runtime.tree_attention, q.cpu(), b.key.cpu(), b.value.cpu(), b.blocks.cpu(), b.ctx.cpu(), b.starts.cpu(), mask.cpu(), host, 4, 2, 64, 16, 0.125)
     assert torch.equal(host, out.cpu())
+
+
+@pytest.mark.parametrize("cache", [BF, F8])
+def test_rows_of_nobody_stay_as_they_were_in_host_memory_too(worker, cache):
+    b = Batch(3, [(9, 3), (30, 2)], 2, 64, 32, cache, pad=4, first=2)
+    mask = _tree_masks(random.Random(2), b.lens, b.tokens, 2, "tree")
+    scales = [x.cpu() for x in b.scales()]
+    caches = [b.key.cpu(), b.value.cpu()]
+    table = torch.ones((40, 32))
+    q, out = (torch.full((b.tokens * 4, 64), 7.0, dtype=BF) for _ in range(2))
+    program = runtime.rope_append_tokens_fp8 if cache == F8 else runtime.rope_append_tokens
+    qkv = _randn(b.g, b.tokens, 8 * 64).to(BF).cpu()
+    worker.run(program, qkv, torch.arange(b.tokens, dtype=torch.int32), b.starts.cpu(), b.ctx.cpu(), table, table * 0, b.blocks.cpu(), *caches, *scales, q, 4, 2, 64, 32)
+    worker.run(runtime.tree_attention, q, *caches, b.blocks.cpu(), b.ctx.cpu(), b.starts.cpu(), mask.cpu(), out, *scales, 4, 2, 64, 32, 0.125)
+    nobody = torch.ones(b.tokens, dtype=torch.bool)
+    nobody[2:7] = False
+    for x in (q, out):
+        rows = x.view(b.tokens, -1).float()
+        assert (rows[nobody] == 7).all() and (rows[~nobody] != 7).any(1).all()
+    assert torch.equal(q.view(b.tokens, -1)[2:7], qkv[2:7, :256])  # turned by nothing
