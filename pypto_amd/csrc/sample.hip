@@ -169,12 +169,76 @@ struct Shared {
   unsigned long long found[4];
 };
 
+constexpr int kSliceThreads = kThreads;
+constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
+
+// Eight elements from i on, -inf behind the end.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8]) {
+  if constexpr (WIDE) {
+    if (i + 8 <= end) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(row + i)[0], b = reinterpret_cast<const float4*>(row + i)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        typedef T T8 __attribute__((ext_vector_type(8)));
+        const T8 a = *reinterpret_cast<const T8*>(row + i);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = (float)a[u];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : -INFINITY;
+}
+
+// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; -inf behind the end.
+template <typename T, bool WIDE, typename F>
+__device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
+  for (int i0 = first; i0 < end; i0 += 2 * kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    float a[8], b[8];
+    load8<T, WIDE>(row, i, end, a);
+    load8<T, WIDE>(row, i + kStep, end, b);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f(a[u], i + u);
+    if (i0 + kStep < end) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f(b[u], i + kStep + u);
+    }
+  }
+}
+
+// A thread's eight elements as they lie in memory; -inf behind the end.
 template <typename T>
-__device__ __forceinline__ float logit(const T* row, int i) { return (float)row[i]; }
+using Raw8 = T __attribute__((ext_vector_type(8)));
+template <typename T, bool WIDE>
+__device__ __forceinline__ Raw8<T> load_raw(const T* row, int i, int end) {
+  if constexpr (WIDE) {
+    if (i + 8 <= end) return *reinterpret_cast<const Raw8<T>*>(row + i);
+  }
+  Raw8<T> v;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
+  return v;
+}
+// f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile; `next`: the first step's, asked for long before.
+template <typename T, bool WIDE, typename F, typename Done>
+__device__ __forceinline__ void step_by_step(const T* row, int first, int end, Raw8<T> next, F f, Done done) {
+  for (int i0 = first; i0 < end; i0 += kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    const Raw8<T> v = next;
+    if (i0 + kStep < end) next = load_raw<T, WIDE>(row, i + kStep, end);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f((float)v[u], i + u);
+    done((i0 - first) / kStep);
+  }
+}
 
 // The border behind which the running sum, of tokens (by_weight: of weights) in the order, reaches `need`, from `in_front` on; it lies between the keys
 // lo and hi, or nowhere (false).  Eleven bits of the key a pass over the row.
-template <typename T>
+template <typename T, bool WIDE>
 __device__ bool find_border(Shared& sh, const T* row, int vocab, const Weights& w, bool by_weight, uint64_t need, uint32_t lo, uint32_t hi, Border* border,
                             uint64_t* weight_to_border) {
   uint64_t tokens_front = 0, weight_front = 0;
@@ -186,15 +250,14 @@ __device__ bool find_border(Shared& sh, const T* row, int vocab, const Weights& 
       sh.weight[b] = 0;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < vocab; i += kThreads) {
-      const float v = logit(row, i);
+    in_steps<T, WIDE>(row, 0, vocab, [&](float v, int) {
       const uint32_t key = ordered(v);
-      if (key < lo || key > hi) continue;
+      if (key < lo || key > hi) return;
       const int bin = (hi - key) >> shift;
       atomicAdd(&sh.count[bin], 1u);
       const uint64_t x = w(v);
       if (x) atomicAdd(&sh.weight[bin], (unsigned long long)x);
-    }
+    });
     __syncthreads();
     constexpr int kOwn = kBins / kThreads;
     uint64_t n_own = 0, x_own = 0;
@@ -264,23 +327,23 @@ __device__ __forceinline__ uint64_t needed(const Filters& f, uint64_t sum) { ret
 __device__ __forceinline__ uint64_t packed(float v, int i) { return (uint64_t)ordered(v) << 32 | (uint32_t)~i; }
 
 // The place of the last token that a row's filters keep, from the row alone (all threads of a workgroup of kThreads).
-template <typename T>
+template <typename T, bool WIDE>
 __device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, const Weights& w, const Filters& f) {
   const uint32_t top = ordered(w.best);
   Border border{kNone, 0};
   uint64_t total = 0;
   bool bounded = false;
-  if (f.k) bounded = find_border(sh, row, vocab, w, false, (uint64_t)f.k, kNone + 1, top, &border, &total);
+  if (f.k) bounded = find_border<T, WIDE>(sh, row, vocab, w, false, (uint64_t)f.k, kNone + 1, top, &border, &total);
   if (f.by_sum) {
     if (!bounded) {
-      for (int i = threadIdx.x; i < vocab; i += kThreads) total += w(logit(row, i));
+      in_steps<T, WIDE>(row, 0, vocab, [&](float v, int) { total += w(v); });
       unsigned long long all;
       sum_in_front<unsigned long long>(total, sh.waves, &all);
       total = all;
     }
     Border nearer;
     uint64_t unused;
-    if (find_border(sh, row, vocab, w, true, needed(f, total), bounded ? border.key : kNone + 1, top, &nearer, &unused)) {
+    if (find_border<T, WIDE>(sh, row, vocab, w, true, needed(f, total), bounded ? border.key : kNone + 1, top, &nearer, &unused)) {
       border = nearer;
       bounded = true;
     }
@@ -291,12 +354,21 @@ __device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int 
   __syncthreads();
   if (threadIdx.x == 0) sh.found[0] = 0;
   __syncthreads();
-  for (int i0 = 0; i0 < vocab && before < border.ties; i0 += kThreads) {
-    const int i = i0 + threadIdx.x;
-    const bool tie = i < vocab && ordered(logit(row, i)) == border.key;
+  for (int i0 = 0; i0 < vocab && before < border.ties; i0 += kStep) {
+    const int i = i0 + threadIdx.x * 8;
+    float v[8];
+    load8<T, WIDE>(row, i, vocab, v);
+    uint64_t own = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) own += i + u < vocab && ordered(v[u]) == border.key;
     unsigned long long all;
-    const uint64_t number = before + sum_in_front<unsigned long long>(tie, sh.waves, &all);
-    if (tie && number + 1 == border.ties) sh.found[0] = (uint32_t)~i;
+    uint64_t number = before + sum_in_front<unsigned long long>(own, sh.waves, &all);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool tie = i + u < vocab && ordered(v[u]) == border.key;
+      number += tie;
+      if (tie && number == border.ties) sh.found[0] = (uint32_t)~(i + u);
+    }
     before += all;
   }
   __syncthreads();
@@ -304,8 +376,6 @@ __device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int 
 }
 
 // ---- slices ----
-constexpr int kSliceThreads = kThreads;
-constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
 // Slices are for some four workgroups a CU, and at most this long: of 500 rows of 128000 the histogram takes 57 / 60 / 49 us and collecting 72 / 78 / 98 us by slices of
 // 16384 / 32768 / 65536.
 constexpr int kMaxSlice = 16384;
@@ -324,70 +394,6 @@ struct Scratch {
   int slices, slice;           // elements of a slice, a multiple of kStep
   int stretches;               // kStep elements each
 };
-
-// Eight elements from i on, -inf behind the end.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8]) {
-  if constexpr (WIDE) {
-    if (i + 8 <= end) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(row + i)[0], b = reinterpret_cast<const float4*>(row + i)[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        typedef T T8 __attribute__((ext_vector_type(8)));
-        const T8 a = *reinterpret_cast<const T8*>(row + i);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = (float)a[u];
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : -INFINITY;
-}
-
-// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; -inf behind the end.
-template <typename T, bool WIDE, typename F>
-__device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
-  for (int i0 = first; i0 < end; i0 += 2 * kStep) {
-    const int i = i0 + threadIdx.x * 8;
-    float a[8], b[8];
-    load8<T, WIDE>(row, i, end, a);
-    load8<T, WIDE>(row, i + kStep, end, b);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) f(a[u], i + u);
-    if (i0 + kStep < end) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) f(b[u], i + kStep + u);
-    }
-  }
-}
-
-// A thread's eight elements as they lie in memory; -inf behind the end.
-template <typename T>
-using Raw8 = T __attribute__((ext_vector_type(8)));
-template <typename T, bool WIDE>
-__device__ __forceinline__ Raw8<T> load_raw(const T* row, int i, int end) {
-  if constexpr (WIDE) {
-    if (i + 8 <= end) return *reinterpret_cast<const Raw8<T>*>(row + i);
-  }
-  Raw8<T> v;
-#pragma unroll
-  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
-  return v;
-}
-// f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile; `next`: the first step's, asked for long before.
-template <typename T, bool WIDE, typename F, typename Done>
-__device__ __forceinline__ void step_by_step(const T* row, int first, int end, Raw8<T> next, F f, Done done) {
-  for (int i0 = first; i0 < end; i0 += kStep) {
-    const int i = i0 + threadIdx.x * 8;
-    const Raw8<T> v = next;
-    if (i0 + kStep < end) next = load_raw<T, WIDE>(row, i + kStep, end);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) f((float)v[u], i + u);
-    done((i0 - first) / kStep);
-  }
-}
 
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
@@ -785,17 +791,19 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   uint64_t border = (uint64_t)(kNone + 1) << 32;
   __syncthreads();
   if (n > kCollected) {
-    border = border_of_row(sh.row, row, p.vocab, w, f);
+    border = border_of_row<T, WIDE>(sh.row, row, p.vocab, w, f);
     // the stretches' sums lack what the border's intervals keep
     for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < p.vocab; i0 += kThreads) {
-      const int i = i0 + threadIdx.x;
-      const float v = i < p.vocab ? logit(row, i) : -INFINITY;
-      uint64_t x = i < p.vocab && packed(v, i) >= border ? w(v) : 0;
-      x = wave_sum((unsigned long long)(x >= f.least ? x : 0));
-      if (threadIdx.x % 64 == 0 && x) atomicAdd(&sh.sums[i0 / kStep], (unsigned long long)x);  // a stretch is a multiple of kThreads
-    }
+    uint64_t own = 0;
+    step_by_step<T, WIDE>(row, 0, p.vocab, load_raw<T, WIDE>(row, threadIdx.x * 8, p.vocab), [&](float v, int i) {
+      const uint64_t x = i < p.vocab && packed(v, i) >= border ? w(v) : 0;
+      own += x >= f.least ? x : 0;
+    }, [&](int step) {
+      const uint64_t sum = wave_sum((unsigned long long)own);
+      if (threadIdx.x % 64 == 0 && sum) atomicAdd(&sh.sums[step], (unsigned long long)sum);
+      own = 0;
+    });
   } else if (n > 0) {
     const unsigned long long* tokens = s.tokens + (size_t)r * kCollected;
     const unsigned long long* front = s.front + 5 * (size_t)r;
