@@ -124,7 +124,8 @@ def tree_attention(query, key, value, table, ctx_lens, starts, mask, hq, hkv, d,
 
 
 def sample(logits, temperature, top_k, top_p, min_p, uniform) -> tuple[int, float]:
-    """Token and probability of one row; None or neutral values leave a filter out."""
+    """Token and probability of one row; None or neutral values leave a filter out.  Weights are 64-bit values, their running sums have 64 bits of mantissa: of ten thousand
+    weights that differ by 1e-13, sums in 64-bit values are off by more than the differences make."""
     l = np.asarray(logits, dtype=np.float64).copy()
     l[np.isnan(l)] = -np.inf
     best = l.max()
@@ -140,13 +141,13 @@ def sample(logits, temperature, top_k, top_p, min_p, uniform) -> tuple[int, floa
     if top_k is not None and top_k > 0:
         order = order[:top_k]
     if top_p is not None and top_p < 1:
-        sums = np.cumsum(w[order])
+        sums = np.cumsum(w[order].astype(np.longdouble))
         need = max(float(top_p), 0.0) * sums[-1]
         order = order[:int(np.sum(sums < need)) + 1]
     if min_p is not None and min_p > 0:
         order = order[w[order] >= min(float(min_p), 1.0)]
     order = np.sort(order)
-    sums = np.cumsum(w[order])
+    sums = np.cumsum(w[order].astype(np.longdouble))
     u = min(max(float(uniform), 2.0 ** -25), 1 - 2.0 ** -24)
     at = int(np.sum(sums <= u * sums[-1]))
     return int(order[at]), float(w[order[at]] / sums[-1])

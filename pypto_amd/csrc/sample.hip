@@ -9,7 +9,7 @@
 // the work is split, and next to a border or the random number the decision is that of the definition in 64 bits up to 2^-45 a token.
 //
 // Four kernels, the first three over slices of the rows so that few rows fill the chip too: the largest logit; of rows with top_k or top_p, how many
-// tokens or how much weight lie in each of 1472 intervals of 2^(1/32) below it; for each 2048 tokens the sum of what they surely keep, and the tokens of the border's
+// tokens or how much weight lie in each of 1472 intervals of 2^(1/32) below it (finer ones where its logits lie closer together); for each 2048 tokens the sum of what they surely keep, and the tokens of the border's
 // interval; and, a workgroup a row, the border among those (by 1024 cells of the interval, then in order), the 2048 tokens in which the random number falls and the token
 // among them.  Where more tokens share the border's interval than are collected (thousands of nearly equal logits), the last kernel looks for the border in the
 // row itself, eleven bits of the key a pass.
@@ -85,6 +85,7 @@ struct Weights {
   double rate;    // 64 log2(e) / T
   const Powers* powers;
   float half_best, fast_rate;  // intervals are by a difference in 32 bits, halved so that it stays finite
+  float finer;                 // intervals of an interval of 2^(1/32): 1, or more where the row's logits lie closer together than all of those
   __device__ __forceinline__ double steps(float v) const { return v == best ? 0.0 : ((double)best - (double)v) * rate; }
   // of a finite best: nothing has to be asked.  (The minimum is for temperatures whose rate 32 bits do not hold.)
   __device__ __forceinline__ double finite_steps(float v) const { return fmin(((double)best - (double)v) * rate, kSteps + 63.0); }
@@ -126,6 +127,11 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     const uint64_t o = __shfl_xor((unsigned long long)v, off);
     v = o > v ? o : v;
   }
+  return v;
+}
+__device__ __forceinline__ float wave_min(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fminf(v, __shfl_xor(v, off));
   return v;
 }
 template <typename V>
@@ -172,7 +178,7 @@ struct Shared {
 constexpr int kSliceThreads = kThreads;
 constexpr int kStep = 8 * kSliceThreads;  // elements of a workgroup's step
 
-// Eight elements from i on, -inf behind the end.
+// Eight elements from i on, NaN behind the end: as a logit it is none.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8]) {
   if constexpr (WIDE) {
@@ -190,10 +196,10 @@ __device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8
     }
   }
 #pragma unroll
-  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : -INFINITY;
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : __builtin_nanf("");
 }
 
-// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; -inf behind the end.
+// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; NaN behind the end.
 template <typename T, bool WIDE, typename F>
 __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
   for (int i0 = first; i0 < end; i0 += 2 * kStep) {
@@ -210,7 +216,7 @@ __device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) 
   }
 }
 
-// A thread's eight elements as they lie in memory; -inf behind the end.
+// A thread's eight elements as they lie in memory; NaN behind the end.
 template <typename T>
 using Raw8 = T __attribute__((ext_vector_type(8)));
 template <typename T, bool WIDE>
@@ -220,7 +226,7 @@ __device__ __forceinline__ Raw8<T> load_raw(const T* row, int i, int end) {
   }
   Raw8<T> v;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)-INFINITY;
+  for (int u = 0; u < 8; ++u) v[u] = i + u < end ? row[i + u] : (T)__builtin_nanf("");
   return v;
 }
 // f(logit, index) likewise and behind every step done(step), the next step's loads on their way meanwhile; `next`: the first step's, asked for long before.
@@ -328,12 +334,12 @@ __device__ __forceinline__ uint64_t packed(float v, int i) { return (uint64_t)or
 
 // The place of the last token that a row's filters keep, from the row alone (all threads of a workgroup of kThreads).
 template <typename T, bool WIDE>
-__device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, const Weights& w, const Filters& f) {
-  const uint32_t top = ordered(w.best);
+__device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int vocab, float low, const Weights& w, const Filters& f) {
+  const uint32_t top = ordered(w.best), bottom = max(ordered(low), kNone + 1);
   Border border{kNone, 0};
   uint64_t total = 0;
   bool bounded = false;
-  if (f.k) bounded = find_border<T, WIDE>(sh, row, vocab, w, false, (uint64_t)f.k, kNone + 1, top, &border, &total);
+  if (f.k) bounded = find_border<T, WIDE>(sh, row, vocab, w, false, (uint64_t)f.k, bottom, top, &border, &total);
   if (f.by_sum) {
     if (!bounded) {
       in_steps<T, WIDE>(row, 0, vocab, [&](float v, int) { total += w(v); });
@@ -343,7 +349,7 @@ __device__ __forceinline__ uint64_t border_of_row(Shared& sh, const T* row, int 
     }
     Border nearer;
     uint64_t unused;
-    if (find_border<T, WIDE>(sh, row, vocab, w, true, needed(f, total), bounded ? border.key : kNone + 1, top, &nearer, &unused)) {
+    if (find_border<T, WIDE>(sh, row, vocab, w, true, needed(f, total), bounded ? border.key : bottom, top, &nearer, &unused)) {
       border = nearer;
       bounded = true;
     }
@@ -385,6 +391,7 @@ constexpr int kGathered = 1024;  // by a workgroup for itself, with one place as
 // What the kernels leave for each other, a row of each a row.
 struct Scratch {
   unsigned long long* best;    // [slices] places of the slices' largest logits
+  float* low;                  // [slices] and their smallest
   unsigned long long* weight;  // [kIntervals]
   unsigned int* count;         // [kIntervals]
   unsigned int* collected;     // [1] tokens of the border's intervals
@@ -398,16 +405,18 @@ struct Scratch {
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
   __shared__ unsigned long long waves[kSliceThreads / 64];
+  __shared__ float lows[kSliceThreads / 64];
   const int slice = blockIdx.x, r = blockIdx.y;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   // a thread meets its elements by rising index: of equal ones the first stays
-  float most = -INFINITY;
+  float most = -INFINITY, low = INFINITY;
   int where = first;
   in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
     const bool more = v > most;
     most = more ? v : most;
     where = more ? i : where;
+    low = fminf(low, v);  // NaN: the other
   });
   uint64_t best = packed(most, where);
   // the histogram of the next kernel starts from nothing
@@ -418,28 +427,46 @@ __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s
   }
   if (slice == 0 && threadIdx.x == 0) s.collected[r] = 0;
   best = wave_max(best);
-  if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64] = best;
+  low = wave_min(low);
+  if (threadIdx.x % 64 == 0) {
+    waves[threadIdx.x / 64] = best;
+    lows[threadIdx.x / 64] = low;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kSliceThreads / 64; ++w) best = waves[w] > best ? waves[w] : best;
+    for (int w = 1; w < kSliceThreads / 64; ++w) {
+      best = waves[w] > best ? waves[w] : best;
+      low = fminf(low, lows[w]);
+    }
     s.best[(size_t)r * s.slices + slice] = best;
+    s.low[(size_t)r * s.slices + slice] = low;
   }
 }
 
-// The place of a row's largest logit, by every wavefront for itself.
-__device__ __forceinline__ uint64_t best_of_row(const Scratch& s, int r) {
-  uint64_t best = 0;
+// The place of a row's largest logit and the smallest, by every wavefront for itself.
+struct Span {
+  uint64_t best;
+  float low;
+};
+__device__ __forceinline__ Span span_of_row(const Scratch& s, int r) {
+  Span span{0, INFINITY};
   for (int i = threadIdx.x % 64; i < s.slices; i += 64) {
     const uint64_t b = s.best[(size_t)r * s.slices + i];
-    best = b > best ? b : best;
+    const float l = s.low[(size_t)r * s.slices + i];
+    span.best = b > span.best ? b : span.best;
+    span.low = fminf(span.low, l);
   }
-  return wave_max(best);
+  return Span{wave_max(span.best), wave_min(span.low)};
 }
-__device__ __forceinline__ Weights weights_of(uint64_t best, float temperature, const Powers* powers) {
-  const float v = value_of((uint32_t)(best >> 32));
+__device__ __forceinline__ Weights weights_of(const Span& span, float temperature, const Powers* powers) {
+  const float v = value_of((uint32_t)(span.best >> 32));
   const double rate = 64.0 * 1.4426950408889634074 / (double)temperature;
-  return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate, 1e38)};  // of half the distance and two steps an interval
-
+  // Half the distance and two steps an interval.  At a high temperature, or of an even distribution, that is few intervals for the whole row, and thousands of tokens in the
+  // border's: then there are as many intervals between its logits as there is room for (64 rows of 151936 at a temperature of 30: 61 us, by the row's own passes 657).
+  // Rows that are flat but for masked logits, -inf or far down, have one.
+  const double whole = ((double)v - (double)span.low) * rate * 0.5;
+  const double finer = fmin(fmax((kIntervals - 1) / whole, 1.0), 1e6);  // of no distance: NaN or infinity, 1e6 or 1
+  return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate * finer, 1e38), (float)finer};
 }
 
 template <typename T, bool WIDE>
@@ -450,12 +477,12 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const int slice = blockIdx.x, r = blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
-  const uint64_t best = best_of_row(s, r);
+  const Span span = span_of_row(s, r);
   if (!(t > 0.f) || !f.any()) return;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
-  const Weights w = weights_of(best, t, &powers);
+  const Weights w = weights_of(span, t, &powers);
   if (!(fabsf(w.best) <= 3.4028234664e38f)) return;  // nothing to choose from, or infinite: the last kernel looks at the row
   fill(powers);
   for (int i = threadIdx.x; i < kIntervals; i += kSliceThreads) {
@@ -578,12 +605,12 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
-  const uint64_t best = best_of_row(s, r);
+  const Span span = span_of_row(s, r);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
-  if (!(t > 0.f) || (uint32_t)(best >> 32) <= kNone) return;
-  const Weights w = weights_of(best, t, &powers);
+  if (!(t > 0.f) || (uint32_t)(span.best >> 32) <= kNone) return;
+  const Weights w = weights_of(span, t, &powers);
   const bool infinite = !(w.best <= 3.4028234664e38f);
   if (infinite && f.any()) {
     if (slice == 0 && threadIdx.x == 0) s.collected[r] = kCollected + 1;  // for the last kernel to look at the row
@@ -605,7 +632,7 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   __syncthreads();
   const double least = (double)f.least, more_than = least - 0.5;  // of a weight not yet rounded
   // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
-  const float i_least = 32.f * ((float)kUnit - __builtin_amdgcn_logf((float)least)) + 1.f;
+  const float i_least = (32.f * ((float)kUnit - __builtin_amdgcn_logf((float)least)) + 1.f) * w.finer;
   const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
   const float cut = w.cut(i_behind);
   double own = kBig;  // and the weights of a step: exact
@@ -775,23 +802,23 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
   const unsigned int collected = s.collected[r];
-  const uint64_t best = best_of_row(s, r);
+  const Span span = span_of_row(s, r);
   for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
-  const uint32_t top = (uint32_t)(best >> 32);
+  const uint32_t top = (uint32_t)(span.best >> 32);
   if (top <= kNone || !(t > 0.f)) {  // nothing to choose from, or no choice
     if (threadIdx.x == 0) {
-      p.tokens[r] = top <= kNone ? -1 : (int32_t)~(uint32_t)best;
+      p.tokens[r] = top <= kNone ? -1 : (int32_t)~(uint32_t)span.best;
       if (p.probs) p.probs[r] = top <= kNone ? 0.f : 1.f;
     }
     return;
   }
   fill(sh.powers);
-  const Weights w = weights_of(best, t, &sh.powers);
+  const Weights w = weights_of(span, t, &sh.powers);
   const int n = f.any() ? (int)min(collected, (unsigned int)kCollected + 1) : 0;
   uint64_t border = (uint64_t)(kNone + 1) << 32;
   __syncthreads();
   if (n > kCollected) {
-    border = border_of_row<T, WIDE>(sh.row, row, p.vocab, w, f);
+    border = border_of_row<T, WIDE>(sh.row, row, p.vocab, span.low, w, f);
     // the stretches' sums lack what the border's intervals keep
     for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = 0;
     __syncthreads();
@@ -915,7 +942,7 @@ int launch(Params p, hipStream_t st) {
   s.slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(kStep, (even + kStep - 1) / kStep * kStep));
   s.slices = (p.vocab + s.slice - 1) / s.slice;
   s.stretches = (p.vocab + kStep - 1) / kStep;
-  const size_t per_row = 8 * ((size_t)s.slices + s.stretches + kIntervals + kCollected + 5) + 4 * (kIntervals + 2);
+  const size_t per_row = 8 * ((size_t)s.slices + s.stretches + kIntervals + kCollected + 5) + 4 * (kIntervals + 2 + (size_t)s.slices);
   void* ws = nullptr;
   const int rc = pto_hip::workspace(per_row * at_once, &ws);
   if (rc) return rc;
@@ -926,6 +953,7 @@ int launch(Params p, hipStream_t st) {
   s.front = s.tokens + at_once * kCollected;
   s.count = reinterpret_cast<unsigned int*>(s.front + 5 * at_once);
   s.collected = s.count + at_once * kIntervals;
+  s.low = reinterpret_cast<float*>(s.collected + at_once);
   const bool wide = (uintptr_t)p.logits % 16 == 0 && (int64_t)p.vocab * sizeof(T) % 16 == 0;
   const Params whole = p;
   for (int64_t r = 0; r < rows; r += at_once) {

@@ -74,6 +74,24 @@ def test_sample_of_many_rows_and_of_the_longest(worker, rows, vocab, dtype):
         assert probs[r] == pytest.approx(prob, rel=2.0 ** -22, abs=1e-30)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_sample_of_rows_that_are_nearly_flat(worker, dtype):
+    """High temperatures and logits close together: the whole row within a few powers of two, or within one of them."""
+    g = _gen(13)
+    vocab = 60000
+    logits = (_randn(g, 16, vocab) * torch.tensor([2.0, 0.1, 1e-4, 0.0], device="cuda").repeat_interleave(4)[:, None]).to(dtype)
+    logits[3] += 1000
+    logits[7, 100:200] = -float("inf")
+    logits[9, 5] = float("nan")
+    t = torch.tensor([1.0, 30.0, 1e4, 1e9] * 4)
+    for k, p, m in ((0, 0.9, 0.0), (30000, 1.0, 0.0), (20000, 0.5, 0.0), (0, 0.99, 0.97), (59999, 1.0, 0.5)):
+        tokens, probs, given = _sample(worker, logits, t, k, p, m, torch.rand(16, device="cuda", generator=g))
+        for r, row in enumerate(logits.double().cpu().numpy()):
+            token, prob = od.sample(row, *(x[r] for x in given))
+            assert tokens[r] == token
+            assert probs[r] == pytest.approx(prob, rel=2.0 ** -22, abs=1e-30)
+
+
 def test_sample_of_tiny_temperatures_and_logits(worker):
     """Differences and temperatures near the smallest numbers: 64 log2(e) / T is more than 32 bits hold."""
     g = _gen(3)
