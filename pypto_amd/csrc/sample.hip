@@ -14,9 +14,9 @@
 // among them.  Where more tokens share the border's interval than are collected (thousands of nearly equal logits), the last kernel looks for the border in the
 // row itself, eleven bits of the key a pass.
 //
-// A row is read two or three times and its weights are computed in 64 bits.  One row of 151936 bf16 logits with top_p: 24 to 28 us, of which the four kernels' chains of
-// dependent loads and barriers 3.5 + 6 + 7 + 10; 64 rows of 151936 fp32 ones with mixed filters: 43 to 48 us (8 + 10 + 18 + 12); 320 rows of 32000 fp16 ones without: 30 us, collecting 16
-// of them, bound by the exponentials; 500 rows of 128000 fp32 ones, mixed: 185 to 189 us, the first read at 5.1 TB/s, the histogram of half of the rows bound by LDS atomics
+// A row is read two or three times and its weights are computed in 64 bits.  One row of 151936 bf16 logits with top_p: 24 to 29 us, of which the four kernels' chains of
+// dependent loads and barriers 3.5 + 6 + 7 + 10; 64 rows of 151936 fp32 ones with mixed filters: 43 to 48 us (8 + 10 + 18 + 12); 320 rows of 32000 fp16 ones without: 30 to 32 us, collecting 16
+// of them, bound by the exponentials; 500 rows of 128000 fp32 ones, mixed: 185 to 190 us, the first read at 5.1 TB/s, the histogram of half of the rows bound by LDS atomics
 // (57 to 60 us; a second copy of it in LDS, for half of the conflicts, takes 66, as fewer workgroups fit), the collecting read 70 us, the vector units 85 % busy.
 #include <hip/hip_runtime.h>
 
