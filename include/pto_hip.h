@@ -506,7 +506,7 @@ PTO_HIP_API int pto_hip_rope_kv_cache_update_fp8(const float* qkv, const int32_t
  * FP8E4M3FN caches have one scale per (block, KV head).  All new rows of a block are taken together: where the first of them is the block's first row,
  * scale = max |new rows| / 448 (1 for zeros); otherwise the scale only grows to that, and where it does the block's rows in front are coded
  * again.  Infinite and NaN elements are left out of the maximum; infinite ones give codes of 448.  head_dim a multiple of 8 and R of 16, at most 512 (PTO_HIP_ERR_UNSUPPORTED otherwise).
- * A block that a call appends to belongs to one sequence.  At most 2^20 tokens. */
+ * A block that a call appends to belongs to one sequence, at one place of its table.  At most 2^20 tokens. */
 typedef struct PtoHipRopeAppendArgs {
   const void* qkv;              /* [T, (Hq + 2 Hkv) D]: q heads, k heads, v heads */
   const int32_t* positions;     /* [T] rows of the rope tables */
