@@ -14,8 +14,8 @@
 // among them.  Where more tokens share the border's interval than are collected (thousands of nearly equal logits), the last kernel looks for the border in the
 // row itself, eleven bits of the key a pass.
 //
-// A row is read two or three times and its weights are computed in 64 bits.  One row of 151936 bf16 logits with top_p: 24 to 29 us, of which the four kernels' chains of
-// dependent loads and barriers 3.5 + 6 + 7 + 10; 64 rows of 151936 fp32 ones with mixed filters: 43 to 48 us (8 + 10 + 18 + 12); 320 rows of 32000 fp16 ones without: 30 to 32 us, collecting 16
+// A row is read two or three times and its weights are computed in 64 bits.  One row of 151936 bf16 logits with top_p: 24 to 31 us, of which the four kernels' chains of
+// dependent loads and barriers 3.5 + 7 + 7 + 11; 64 rows of 151936 fp32 ones with mixed filters: 46 to 48 us (9 + 11 + 18 + 11); 320 rows of 32000 fp16 ones without: 31 us, collecting 16
 // of them, bound by the exponentials; 500 rows of 128000 fp32 ones, mixed: 185 to 190 us, the first read at 5.1 TB/s, the histogram of half of the rows bound by LDS atomics
 // (57 to 60 us; a second copy of it in LDS, for half of the conflicts, takes 66, as fewer workgroups fit), the collecting read 70 us, the vector units 85 % busy.
 #include <hip/hip_runtime.h>
@@ -445,12 +445,12 @@ __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s
   }
 }
 
-// The place of a row's largest logit and the smallest, by every wavefront for itself.
+// The place of a row's largest logit and, where it has filters, the smallest, by every wavefront for itself.
 struct Span {
   uint64_t best;
   float low;
 };
-__device__ __forceinline__ Span span_of_row(const Scratch& s, int r) {
+__device__ __forceinline__ Span span_of_row(const Scratch& s, int r, bool filtered) {
   Span span{0, INFINITY};
   for (int i = threadIdx.x % 64; i < s.slices; i += 64) {
     const uint64_t b = s.best[(size_t)r * s.slices + i];
@@ -458,7 +458,7 @@ __device__ __forceinline__ Span span_of_row(const Scratch& s, int r) {
     span.best = b > span.best ? b : span.best;
     span.low = fminf(span.low, l);
   }
-  return Span{wave_max(span.best), wave_min(span.low)};
+  return Span{wave_max(span.best), filtered ? wave_min(span.low) : -INFINITY};
 }
 __device__ __forceinline__ Weights weights_of(const Span& span, float temperature, const Powers* powers) {
   const float v = value_of((uint32_t)(span.best >> 32));
@@ -466,9 +466,9 @@ __device__ __forceinline__ Weights weights_of(const Span& span, float temperatur
   // Half the distance and two steps an interval.  At a high temperature, or of an even distribution, that is few intervals for the whole row, and thousands of tokens in the
   // border's: then there are as many intervals between its logits as there is room for (64 rows of 151936 at a temperature of 30: 61 us, by the row's own passes 657).
   // Rows that are flat but for masked logits, -inf or far down, have one.
-  const double whole = ((double)v - (double)span.low) * rate * 0.5;
-  const double finer = fmin(fmax((kIntervals - 1) / whole, 1.0), 1e6);  // of no distance: NaN or infinity, 1e6 or 1
-  return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate * finer, 1e38), (float)finer};
+  const float whole = (float)(((double)v - (double)span.low) * rate * 0.5);
+  const float finer = fminf(fmaxf((kIntervals - 2) * __builtin_amdgcn_rcpf(whole), 1.f), 1e6f);  // of no distance 1e6, of an infinite or undefined one 1
+  return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate * finer, 1e38), finer};
 }
 
 template <typename T, bool WIDE>
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const int slice = blockIdx.x, r = blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
-  const Span span = span_of_row(s, r);
+  const Span span = span_of_row(s, r, f.any());
   if (!(t > 0.f) || !f.any()) return;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
-  const Span span = span_of_row(s, r);
+  const Span span = span_of_row(s, r, f.any());
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
@@ -804,7 +804,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
   const unsigned int collected = s.collected[r];
-  const Span span = span_of_row(s, r);
+  const Span span = span_of_row(s, r, f.any());
   for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
   const uint32_t top = (uint32_t)(span.best >> 32);
   if (top <= kNone || !(t > 0.f)) {  // nothing to choose from, or no choice
