@@ -493,7 +493,8 @@ PTO_HIP_API int pto_hip_rope_kv_cache_update_fp8(const float* qkv, const int32_t
 
 /* ---- a step that verifies drafted tokens: several new tokens per sequence (none has a counterpart in the reference) ----
  * Sequence b's new tokens are rows token_starts[b] .. token_starts[b+1] - 1 of the ragged batch (rising, token_starts[B] <= T; rows outside of
- * [token_starts[0], token_starts[B]) belong to nobody and what they would write is left as it was).  Its i-th new token lies at index
+ * [token_starts[0], token_starts[B]) belong to nobody and what they would write is left as it was; a start below 0 counts as 0, one past T as T, and
+ * both are reported by the next pto_hip_sync).  Its i-th new token lies at index
  * context_lens[b] + i of its cache, found through block_table; context_lens counts the tokens in front of the new ones.  The calls read these tensors
  * on the device: a captured call serves any lengths that fit its T, B and table. */
 

@@ -167,6 +167,11 @@ __device__ __forceinline__ bool cache_place(const Params& p, int seq, int number
   return ok;
 }
 
+// By the first workgroup of the launch with the queries' heads.
+__device__ __forceinline__ void report_starts(const Params& p, int part) {
+  if (p.t0 + blockIdx.x == 0 && part == 0 && threadIdx.x == 0 && pto_hip::pass_the_rows(p.starts, p.batch, p.tokens)) *p.error_flag = 1;
+}
+
 // A workgroup for GROUPS times kThreads / LANES heads of one token, LANES lanes a head, number `part` of the token.  Q_ONLY: the queries alone (beside an e4m3 cache).
 template <typename In, typename T, int LANES, bool Q_ONLY, int GROUPS>
 __device__ __forceinline__ void append_heads(const Params& p, int part) {
@@ -181,7 +186,8 @@ __device__ __forceinline__ void append_heads(const Params& p, int part) {
   for (int g = 0; g < GROUPS; ++g)
     if (e0 < p.d && head0 + g * kHeads < heads) raw[g] = load8(reinterpret_cast<const In*>(p.qkv) + ((size_t)t * width + head0 + g * kHeads) * p.d + e0);
   const int pos = p.positions[t];
-  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, t, lane);
+  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, p.tokens, t, lane);
+  report_starts(p, part);
   if (s.seq < 0) return;  // nobody's token
   if (pos < 0 || pos >= p.max_pos) {
     if (threadIdx.x == 0) *p.error_flag = 1;
@@ -218,7 +224,8 @@ template <typename In, typename T>
 __global__ __launch_bounds__(64) void append_any_kernel(Params p) {
   const int t = p.t0 + blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
   const int pos = p.positions[t];
-  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, t, lane);
+  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, p.tokens, t, lane);
+  report_starts(p, head);
   if (s.seq < 0) return;
   if (pos < 0 || pos >= p.max_pos) {
     if (lane == 0) *p.error_flag = 1;
@@ -279,7 +286,7 @@ __device__ __forceinline__ void append_codes(const Params& p, int kv_head) {
   const int t = p.t0 + blockIdx.x, lane = threadIdx.x % 64;
   const bool is_k = kv_head < p.hkv;
   const int h = is_k ? kv_head : kv_head - p.hkv;
-  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, t, lane);
+  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, p.tokens, t, lane);
   if (s.seq < 0) return;
   int block = 0, place = 0;
   {
@@ -288,7 +295,7 @@ __device__ __forceinline__ void append_codes(const Params& p, int kv_head) {
     if (n >= 0 && t > s.first && n % p.bs != 0) return;
   }
   if (!cache_place(p, s.seq, t - s.first, &block, &place)) return;
-  const int rows = min(min(s.count - (t - s.first), p.tokens - t), p.bs - place);
+  const int rows = min(s.count - (t - s.first), p.bs - place);
   const int head = p.hq + (is_k ? 0 : p.hkv) + h, width = p.hq + 2 * p.hkv;
   const int group = threadIdx.x / LANES, e0 = threadIdx.x % LANES * 8;
   const bool inside = e0 < p.d;

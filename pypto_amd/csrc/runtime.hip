@@ -1310,10 +1310,10 @@ int pto_hip_sync(void* stream) {
     if (flags[3]) return fail(PTO_HIP_ERR_INVALID_VALUE, "experts_ffn_fp8_block: an expert id names an expert that there is not");
     if (flags[4])
       return fail(PTO_HIP_ERR_INVALID_VALUE,
-                  "rope_append_tokens: a position lies outside the rope tables, or a token's index outside the block table or the cache");
+                  "rope_append_tokens: a position lies outside the rope tables, a token's index outside the block table or the cache, or a start outside the batch's rows");
     if (flags[5])
       return fail(PTO_HIP_ERR_INVALID_VALUE,
-                  "tree_attention: a sequence has more tokens than its mask has bits or its block table room, or a block outside the cache");
+                  "tree_attention: a sequence has more tokens than its mask has bits or its block table room, a block outside the cache or a start outside the batch's rows");
     return fail(PTO_HIP_ERR_INVALID_VALUE,
                 "paged_attention: a block_table entry a sequence uses addresses a block outside the cache");
   }

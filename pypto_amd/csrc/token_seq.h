@@ -31,9 +31,14 @@ struct TokenSeq {
   int count;  // and how many it has
 };
 
+// A start as every kernel takes it: one in front of the batch's rows or behind them counts as their end on that side, so that a sequence which passes them has the tokens that there are.
+__device__ __forceinline__ int within(int start, int tokens) { return min(max(start, 0), tokens); }
+// Whether there are such starts (they rise): to be reported, by one thread of a launch.
+__device__ __forceinline__ bool pass_the_rows(const int32_t* starts, int batch, int tokens) { return starts[0] < 0 || starts[batch] > tokens; }
+
 // The last sequence that starts at `token` or in front of it, looked for by a whole wavefront: 64 starts a step, so that 64 sequences take one
-// trip to memory and 4096 two.  starts[0 .. batch]; whatever they hold, no other element is read and the answer lies in the batch.
-__device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch, int token, int lane) {
+// trip to memory and 4096 two.  starts[0 .. batch], of a batch of `tokens` rows; whatever they hold, no other element is read and the answer lies in the batch.
+__device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch, int tokens, int token, int lane) {
   int lo = 0, n = batch;
   while (n > 64) {
     const int step = (n + 63) / 64;
@@ -44,7 +49,7 @@ __device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch
     n = min(step, n - k * step);
   }
   const int at = min(lo + lane, batch);
-  const int start = starts[at], next = starts[min(at + 1, batch)];
+  const int start = within(starts[at], tokens), next = within(starts[min(at + 1, batch)], tokens);
   const int k = max((int)__popcll(__ballot(lane < n && start <= token)) - 1, 0);
   const int first = __shfl(start, k), end = __shfl(next, k);
   return TokenSeq{first <= token && token < end ? lo + k : -1, first, end - first};

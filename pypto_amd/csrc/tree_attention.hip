@@ -81,7 +81,8 @@ __global__ __launch_bounds__(64) void tree_any_kernel(Params p) {
   __shared__ float qs[kMaxD];
   const int t = p.t0 + blockIdx.x, hq = blockIdx.y, h = hq / p.group, lane = threadIdx.x;
   const int d = p.d, bs = p.bs;
-  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, t, lane);
+  const TokenSeq s = pto_hip::sequence_of(p.starts, p.batch, p.tokens, t, lane);
+  if (t == 0 && hq == 0 && lane == 0 && pto_hip::pass_the_rows(p.starts, p.batch, p.tokens)) *p.error_flag = 1;
   if (s.seq < 0) return;
   const size_t row = (size_t)t * p.hq + hq;
   for (int i = lane; i < d; i += 64) qs[i] = (float)reinterpret_cast<const T*>(p.q)[row * d + i] * p.scale;
@@ -173,8 +174,8 @@ struct Work {
 __device__ __forceinline__ int chunks_of(const Work& w) { return (w.end + kChunk - 1) / kChunk; }
 __device__ __forceinline__ Work work_of(const Params& p, int b, int rows) {
   const int at = min(b, p.batch - 1);
-  const int first = p.starts[at], next = p.starts[at + 1], ctx = p.ctx_lens[at];
-  const bool sound = b < p.batch && first >= 0 && next > first && next <= p.tokens;
+  const int first = pto_hip::within(p.starts[at], p.tokens), next = pto_hip::within(p.starts[at + 1], p.tokens), ctx = p.ctx_lens[at];
+  const bool sound = b < p.batch && next > first;
   const int room = p.max_blocks * p.bs;  // below 2^29
   Work w;
   w.first = first;
@@ -217,7 +218,7 @@ __device__ __forceinline__ int part_chunks(const Params& p, int rows, int lane, 
 struct Share {
   int seq;  // -1: nothing to do
   Work w;
-  int parts, part, block, h;
+  int parts, part, block, h;  // no parts: no room for their results
   int slot;  // of the sequence's first token in its first part
 };
 // A sequence's partial results, in tokens: none where it has one part.  No more than there can be room for, so that sums over 64 of them stay in 32 bits.
@@ -253,7 +254,7 @@ __device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int
       s.h = at - per_head * p.hkv;
       s.part = quotient(per_head, s.w.blocks);
       s.block = per_head - s.part * s.w.blocks;
-      if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) s.seq = -1;  // only where the starts do not rise
+      if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) s.parts = 0;  // only where the starts do not rise
       return s;
     }
     ids = __builtin_amdgcn_readlane(to, 63);
@@ -337,8 +338,12 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, j = lane >> 4;
   const Share s = share_of(p, kRows, blockIdx.x, lane);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && pto_hip::pass_the_rows(p.starts, p.batch, p.tokens)) *p.error_flag = 1;
   if (s.seq < 0) return;
   const int seq = s.seq, h = s.h, ctx = s.w.ctx, count = s.w.count, token0 = s.w.first, parts = s.parts, part = s.part, all = s.w.end;
+  if (part == 0 && s.block == 0 && h == 0)
+    for (int i = threadIdx.x; i < count; i += kThreads) p.joins[token0 + i] = int4{parts, s.slot + i, count, 0};
+  if (parts == 0) return;
   // even parts of whole chunks
   const int chunks = chunks_of(s.w), each = quotient(chunks, parts), more = chunks - each * parts;
   const int tok_first = (part * each + min(part, more)) * kChunk;
@@ -351,9 +356,6 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     const int64_t raw = p.ctx_lens[seq];
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
-
-  if (part == 0 && s.block == 0 && h == 0)
-    for (int i = threadIdx.x; i < count; i += kThreads) p.joins[token0 + i] = int4{parts, s.slot + i, count, 0};
 
   // Query fragments (B operand): column = row c of the tile; k-group j of step u holds elements (u*4+j)*8..+8.  A negative scale changes their sign, so that
   // the largest product is the largest score.
