@@ -633,8 +633,8 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   }
   __syncthreads();
   const double least = (double)f.least, more_than = least - 0.5;  // of a weight not yet rounded
-  // of what is surely kept, min_p leaves out what is further down than this (an interval more than it has to be)
-  const float i_least = (32.f * ((float)kUnit - __builtin_amdgcn_logf((float)least)) + 1.f) * w.finer;
+  // of what is surely kept, min_p - or the rounding to whole units - leaves out what is further down than this (an interval more than it has to be)
+  const float i_least = (32.f * ((float)kUnit - __builtin_amdgcn_logf((float)more_than)) + 1.f) * w.finer;
   const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
   const float cut = w.cut(i_behind);
   double own = kBig;  // and the weights of a step: exact

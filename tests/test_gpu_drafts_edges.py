@@ -47,3 +47,24 @@ def test_append_of_sequences_that_pass_the_batch_has_the_tokens_that_are_there(w
             worker.sync()
         worker.sync()
         _check_append(b, got, want, out)
+
+
+@pytest.mark.parametrize("step", [1, 2])
+def test_sample_counts_weights_of_one_unit(worker, step):
+    """Weights are whole numbers of 2^-44 of the largest, rounded: one of 0.93 units counts as one, also where the border of top_k lies behind it.  The smallest random number asks for
+    a running sum of more than 2^19 units: the first token has a thousand fewer, 1500 tokens of one unit follow (a step apart), the largest logit comes last."""
+    vocab, best, ln2 = 20000, 19000, float(np.log(2.0))
+    logits = torch.full((1, vocab), -45.5 * ln2)  # a third of a unit: nothing
+    logits[0, 0] = float(np.log(2.0 ** 19 - 1000)) - 44 * ln2
+    small = torch.arange(1, 1 + 1500 * step, step)
+    logits[0, small] = -44.1 * ln2
+    logits[0, 5000:5010] = -44.8 * ln2  # the border's, more than half a unit
+    logits[0, best] = 0.0
+    units = np.exp(logits[0].double().numpy()) * 2.0 ** 44
+    assert abs(units[0] - round(units[0])) < 0.49 and (units[small] > 0.6).all() and (units[small] < 1.4).all()
+    need = 2 ** 19 - round(units[0]) + 1  # so many of them pass 2^19
+    assert 900 < need < 1100
+    tokens, probs, _ = _sample(worker, logits.cuda(), 1.0, 2 + 1500 + 5, 1.0, 0.0, 0.0)
+    assert tokens == [int(small[need - 1])]
+    total = 2 ** 44 + round(units[0]) + 1500 + 5
+    assert probs[0] == pytest.approx(units[small[0]] / total, rel=2.0 ** -22)
