@@ -158,7 +158,7 @@ typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2;
 
 constexpr int kChunk = 32;
 
-// a / b of numbers below 2^24 whose quotient is below 2^20 (a division of integers is some 40 instructions).
+// a / b of numbers below 2^26 whose quotient is below 2^20 (a division of integers is some 40 instructions).
 __device__ __forceinline__ int quotient(int a, int b) {
   const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));  // off by one at most
   const int r = a - q * b;
@@ -195,12 +195,12 @@ __device__ __forceinline__ int part_chunks(const Params& p, int rows, int lane, 
     const Work w = b0 == 0 ? first64 : work_of(p, b0 + lane, rows);
     total += wave_total((float)chunks_of(w) * (float)w.blocks);
   }
-  total *= (float)p.hkv * 1.0001f * p.per_target;  // not below the exact quotient: the room for partial results counts on it
+  total *= (float)p.hkv * 1.0001f * p.per_target;  // not below the exact quotient: the grid and the room for partial results count on it
   constexpr int kTries = 8;
   float part[kTries], count[kTries];
 #pragma unroll
   for (int i = 0; i < kTries; ++i) {
-    part[i] = fmaxf(floorf(fminf(total * (1.f + 0.125f * i), 1e7f)) + 1.f, p.least);
+    part[i] = fmaxf(floorf(fminf(total * (1.f + 0.125f * i), 0x1p25f)) + 1.f, p.least);  // 2^25 chunks: of no sequence more than one part
     count[i] = 0.f;
   }
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
@@ -812,8 +812,10 @@ int launch_tiles(Params& p, hipStream_t st) {
   p.block_bytes = (uint32_t)((int64_t)p.hkv * p.bs * D * (FP8 ? 1 : 2));
   const int64_t blocks = (int64_t)p.tokens * p.group / kRows + std::min(p.batch, p.tokens);
   const int64_t grid = p.target + blocks * p.hkv;
-  const int64_t slots = ((int64_t)p.target * kRows + p.hq - 1) / p.hq + p.tokens + 1;
-  PTO_CHECK_ARG(grid < 1ll << 22 && slots < 1ll << 24 && slots * p.hq * D < 1ll << 33, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
+  // Partial results, in tokens of all heads.  parts * blocks * hkv, over the sequences, is at most target + blocks * hkv: target * rows and the tokens themselves.  And with P chunks
+  // a part a sequence that is cut has over P of them, so that its parts are fewer than 2 chunks / P: no more than 2 target row blocks, however many tokens.
+  const int64_t slots = std::min<int64_t>(((int64_t)p.target * kRows + p.hq - 1) / p.hq + p.tokens, (2ll * p.target * kRows + p.hq - 1) / p.hq) + 1;
+  PTO_CHECK_ARG(grid < 1ll << 22, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
   const size_t o_bytes = (size_t)slots * p.hq * D * 4, ml_bytes = (size_t)slots * p.hq * 8;
   void* ws = nullptr;
   const int rc = pto_hip::workspace(o_bytes + ml_bytes + 16 + (size_t)p.tokens * sizeof(int4), &ws);

@@ -68,3 +68,35 @@ def test_sample_counts_weights_of_one_unit(worker, step):
     assert tokens == [int(small[need - 1])]
     total = 2 ** 44 + round(units[0]) + 1500 + 5
     assert probs[0] == pytest.approx(units[small[0]] / total, rel=2.0 ** -22)
+
+
+def test_tree_keeps_scratch_for_what_is_cut(worker):
+    """Partial results are of sequences whose keys are cut: 2^15 tokens of 64 heads of 128 in long prompts, 1.07 GB of them in 32 bits, take no such scratch."""
+    n, seqs, hq, d, bs = 512, 64, 64, 128, 128
+    tokens = n * seqs
+    pool = seqs * (n // bs)
+    g = _gen(1)
+    key, value = (_randn(g, pool * 8 * bs, d).to(BF) for _ in range(2))
+    table = torch.arange(pool, dtype=torch.int32, device="cuda").view(seqs, -1)
+    starts = torch.arange(0, tokens + 1, n, dtype=torch.int32, device="cuda")
+    ctx = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    chain = [(1 << (i + 1)) - 1 for i in range(n)]
+    words = [[m >> 32 * w & 0xFFFFFFFF for w in range(n // 32)] for m in chain]
+    mask = torch.tensor([[w - (1 << 32) if w >> 31 else w for w in r] for r in words], dtype=torch.int64).to(torch.int32).cuda().repeat(seqs, 1)
+    q = torch.randn((tokens * hq, d), dtype=BF, device="cuda", generator=g)
+    out = torch.empty_like(q)
+    worker.sync()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    worker.run(runtime.tree_attention, q, key, value, table, ctx, starts, mask, out, hq, 8, d, bs, d ** -0.5)
+    worker.sync()
+    assert before - torch.cuda.mem_get_info()[0] < 600 << 20
+    # of three sequences' first, middle and last rows what the oracle says
+    for s in (0, 31, 63):
+        for i in (0, 255, 511):
+            t = s * n + i
+            want, mass, reach = od.tree_attention(q.view(tokens, -1)[t].view(hq, d), key, value, table[s:s + 1], _ints([i]), _ints([0, 1]), _ints([[1]]), hq, 8, d, bs,
+                                                  d ** -0.5)
+            got = out.view(tokens, hq, d)[t].double().cpu()
+            off = HALF_STEP[BF] + 2 * reach * (d + 12) * 2.0 ** -24 + 2.0 ** -19
+            assert ((got - want[0]).abs() <= (off * (mass + want.abs()) + HALF_STEP[BF] * want.abs())[0]).all()
