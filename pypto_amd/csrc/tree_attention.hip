@@ -791,6 +791,13 @@ void in_launches(Params& p, int64_t threads_a_token, F f) {
   }
 }
 
+// Every workgroup makes the plan of all sequences, which grows with the square of their number: one token each, 64 heads over 8 of 64 channels, contexts of 8 to 15 (250 to 500) keys: 1024
+// sequences 272 (383) us by the matrix form and 87 (1618) by the plain one, 4096 3.4 (3.9) and 0.3 (6.2) ms, 16384 52 (54) and 1.5 (24) ms, 65536 824 (831) and 6.1 (96) ms.  The host does not know the
+// contexts; from the most on that this form takes it is behind with those of a few thousand too.
+constexpr int kMaxSequences = 1 << 15;
+constexpr int64_t kMaxGrid = 1 << 22;
+constexpr int kOtherForm = -1;  // no status: what this form does not take
+
 template <int D, bool BF16, bool FP8, int NW, int GT, int AHEAD>
 int launch_tiles(Params& p, hipStream_t st) {
   typedef typename std::conditional<BF16, __bf16, _Float16>::type T;
@@ -815,7 +822,7 @@ int launch_tiles(Params& p, hipStream_t st) {
   // Partial results, in tokens of all heads.  parts * blocks * hkv, over the sequences, is at most target + blocks * hkv: target * rows and the tokens themselves.  And with P chunks
   // a part a sequence that is cut has over P of them, so that its parts are fewer than 2 chunks / P: no more than 2 target row blocks, however many tokens.
   const int64_t slots = std::min<int64_t>(((int64_t)p.target * kRows + p.hq - 1) / p.hq + p.tokens, (2ll * p.target * kRows + p.hq - 1) / p.hq) + 1;
-  PTO_CHECK_ARG(grid < 1ll << 22, "tree_attention: %d tokens of %d heads are more than one call takes", p.tokens, p.hq);
+  if (grid >= kMaxGrid) return kOtherForm;
   const size_t o_bytes = (size_t)slots * p.hq * D * 4, ml_bytes = (size_t)slots * p.hq * 8;
   void* ws = nullptr;
   const int rc = pto_hip::workspace(o_bytes + ml_bytes + 16 + (size_t)p.tokens * sizeof(int4), &ws);
@@ -928,13 +935,15 @@ extern "C" int pto_hip_tree_attention(const PtoHipTreeAttentionArgs* args, void*
   hipStream_t st = (hipStream_t)stream;
   p.scale_log2e = a.scale * 1.4426950408889634f;
   if ((a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && a.block_size % (fp8 ? 32 : 16) == 0 &&
-      a.kv_head_num * a.block_size * a.head_dim * csz < 1ll << 31 && a.tokens * p.group < 1ll << 24) {
+      a.kv_head_num * a.block_size * a.head_dim * csz < 1ll << 31 && a.tokens * p.group < 1ll << 24 && a.batch <= kMaxSequences) {
     const bool bf16 = a.dtype == PTO_HIP_BF16;
     const int rc = a.head_dim == 64 ? launch_matrix<64>(p, bf16, fp8, st) : a.head_dim == 128 ? launch_matrix<128>(p, bf16, fp8, st)
                                                                                               : launch_matrix<256>(p, bf16, fp8, st);
-    if (rc) return rc;
-    PTO_CHECK_HIP(hipGetLastError());
-    return PTO_HIP_OK;
+    if (rc != kOtherForm) {
+      if (rc) return rc;
+      PTO_CHECK_HIP(hipGetLastError());
+      return PTO_HIP_OK;
+    }
   }
   if (a.dtype == PTO_HIP_BF16) fp8 ? launch_any<__bf16, uint8_t>(p, st) : launch_any<__bf16, __bf16>(p, st);
   else fp8 ? launch_any<_Float16, uint8_t>(p, st) : launch_any<_Float16, _Float16>(p, st);
