@@ -75,6 +75,9 @@ __device__ __forceinline__ KeyRange key_range(const Params& p, const TokenSeq& s
   return KeyRange{(int)from, (int)to, ctx < 0 || ctx + s.count > room || s.count > 32 * p.words};
 }
 
+// A score below it weighs nothing, by either form: where the running maximum, of the matrix form in units of log 2, starts.
+constexpr float kLeastScore = pto_hip::attn::kMinMax * 0.69314718f;
+
 // Any shape: one wavefront for each query head of a token.  64 keys at a time, a lane each for the scores, a lane per channel for the values.
 template <typename T, typename E>
 __global__ __launch_bounds__(64) void tree_any_kernel(Params p) {
@@ -90,7 +93,7 @@ __global__ __launch_bounds__(64) void tree_any_kernel(Params p) {
   const KeyRange keys = key_range(p, s);
   bool bad = keys.bad;
   float o[kMaxD / 64] = {0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
+  float m = kLeastScore, l = 0.f;
   for (int n0 = 0; n0 < keys.end; n0 += 64) {
     const int n = n0 + lane, j = n - keys.ctx;
     const bool sees = n < keys.end && (j < 0 || (p.mask[(size_t)t * p.words + j / 32] >> (j % 32) & 1));
@@ -114,10 +117,10 @@ __global__ __launch_bounds__(64) void tree_any_kernel(Params p) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off));
     const float m_new = fmaxf(m, most);
-    if (m_new == -INFINITY && __ballot(sees) == 0) continue;  // nobody of these is seen
-    const float keep = m == m_new ? 1.f : expf(m - m_new);
+    if (__ballot(sees) == 0) continue;  // nobody of these is seen
+    const float keep = expf(m - m_new);
     m = m_new;
-    const float prob = sees ? (score == m ? 1.f : expf(score - m)) : 0.f;
+    const float prob = sees ? expf(score - m) : 0.f;
     float sum = prob;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);

@@ -125,3 +125,42 @@ def test_tree_of_very_many_sequences(worker, batch):
     want, mass, reach = od.tree_attention(q.view(batch, -1)[at].reshape(-1, d), key, value, table[at], ctx[at], torch.arange(len(at) + 1), mask[at], hkv, hkv, d, bs, d ** -0.5)
     off = HALF_STEP[BF] + 2 * reach * (d + 12) * 2.0 ** -24 + 2.0 ** -19
     assert ((got[at].double().cpu() - want).abs() <= off * (mass + want.abs()) + HALF_STEP[BF] * want.abs()).all()
+
+
+@pytest.mark.parametrize("d", [80])
+def test_tree_scores_that_are_no_ordinary_numbers(worker, d):
+    """By either form: a score below -6.9e29 weighs nothing, among others or alone; infinite ones are NaN, as their softmax is; one of -1e29 counts."""
+    b = Batch(d, [(64, 4), (3, 2), (5, 1), (2, 1), (33, 1)], 2, d, 32, BF)
+    hq = 4
+    key = b.key.view(b.pool, 2, 32, d)
+
+    def put(seq, n, v):
+        key[b.table[seq][n // 32], :, n % 32] = v
+
+    big = 1.0e15
+    q = torch.full((b.tokens * hq, d), big, device="cuda").to(BF)
+    unit = float(torch.tensor(big).to(BF)) * d  # a key of v all over scores v * unit
+    for n in range(68):
+        put(0, n, -2.0e30 / unit)          # weighs nothing ...
+    put(0, 50, -1.0e29 / unit)             # ... this alone counts
+    for n in range(5):
+        put(1, n, -1.0e31 / unit)          # nothing that counts: zeros
+    for n in range(6):
+        put(2, n, -5.0e29 / unit)          # every one as much as the others
+    put(3, 0, float("inf"))
+    put(3, 1, 1.0 / unit)
+    for n in range(34):
+        put(4, n, -float("inf"))
+    put(4, 33, 1.0 / unit)                 # the token itself
+    mask = torch.full((b.tokens, 1), -1, dtype=torch.int32, device="cuda")
+    q, out = _attend(worker, b, hq, BF, mask, 1.0, q=q)
+    worker.sync()
+    got = out.view(b.tokens, 2, 2, d).double().cpu()
+    value = b.value.view(b.pool, 2, 32, d).double().cpu()
+    at = lambda seq, n: value[b.table[seq][n // 32], :, n % 32]
+    assert torch.equal(got[:4], at(0, 50)[None, :, None].expand(4, 2, 2, d))
+    assert (got[4:6] == 0).all()
+    rows = torch.stack([at(2, n) for n in range(6)])
+    assert ((got[6] - rows.mean(0)[:, None]).abs() <= 2.0 ** -7 * rows.abs().mean(0)[:, None]).all()
+    assert got[7].isnan().all()
+    assert torch.equal(got[8], at(4, 33)[:, None].expand(2, 2, d))
