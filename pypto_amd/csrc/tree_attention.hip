@@ -221,7 +221,7 @@ __device__ __forceinline__ int part_chunks(const Params& p, int rows, int lane, 
 struct Share {
   int seq;  // -1: nothing to do
   Work w;
-  int parts, part, block, h;  // no parts: no room for their results
+  int parts, part, block, h;
   int slot;  // of the sequence's first token in its first part
 };
 // A sequence's partial results, in tokens: none where it has one part.  No more than there can be room for, so that sums over 64 of them stay in 32 bits.
@@ -257,7 +257,10 @@ __device__ __forceinline__ Share share_of(const Params& p, int rows, int id, int
       s.h = at - per_head * p.hkv;
       s.part = quotient(per_head, s.w.blocks);
       s.block = per_head - s.part * s.w.blocks;
-      if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) s.parts = 0;  // only where the starts do not rise
+      if (s.parts > 1 && (s.slot < 0 || (int64_t)s.slot + (int64_t)s.parts * s.w.count > p.slots)) {  // only where the starts do not rise
+        s.seq = -1;
+        for (int i = lane; i < s.w.count; i += 64) p.joins[s.w.first + i] = int4{0, 0, 0, 0};
+      }
       return s;
     }
     ids = __builtin_amdgcn_readlane(to, 63);
@@ -344,9 +347,6 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
   if (blockIdx.x == 0 && threadIdx.x == 0 && pto_hip::pass_the_rows(p.starts, p.batch, p.tokens)) *p.error_flag = 1;
   if (s.seq < 0) return;
   const int seq = s.seq, h = s.h, ctx = s.w.ctx, count = s.w.count, token0 = s.w.first, parts = s.parts, part = s.part, all = s.w.end;
-  if (part == 0 && s.block == 0 && h == 0)
-    for (int i = threadIdx.x; i < count; i += kThreads) p.joins[token0 + i] = int4{parts, s.slot + i, count, 0};
-  if (parts == 0) return;
   // even parts of whole chunks
   const int chunks = chunks_of(s.w), each = quotient(chunks, parts), more = chunks - each * parts;
   const int tok_first = (part * each + min(part, more)) * kChunk;
@@ -359,6 +359,9 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     const int64_t raw = p.ctx_lens[seq];
     if (raw < 0 || raw + count > (int64_t)p.max_blocks * p.bs || count > 32 * p.words) *p.error_flag = 1;
   }
+
+  if (part == 0 && s.block == 0 && h == 0)
+    for (int i = threadIdx.x; i < count; i += kThreads) p.joins[token0 + i] = int4{parts, s.slot + i, count, 0};
 
   // Query fragments (B operand): column = row c of the tile; k-group j of step u holds elements (u*4+j)*8..+8.  A negative scale changes their sign, so that
   // the largest product is the largest score.
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
   const char* v_head = reinterpret_cast<const char*>(p.vc) + (size_t)h * p.bs * kRowBytes;
   // two chunks on their way to LDS, and the scales of their keys and values
   u32x4 kr[2][kPieces], vr[2][kPieces];
-  float k_muls[2] = {scale, scale}, v_units[2] = {1.f, 1.f};
+  float k_units[2] = {1.f, 1.f}, v_units[2] = {1.f, 1.f};
   // Every request is as many loads, with nothing to skip them, so that the number in flight at each wait is known to the compiler.  Where no tokens are left the
   // window's blocks are block 0, whose rows lie in the cache as any block's.
   auto request = [&](auto set, int tok) __attribute__((always_inline)) {
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     const int slot = lb - win_base;
     const uint32_t blk0 = __builtin_amdgcn_readlane(win_blk, slot), blk1 = __builtin_amdgcn_readlane(win_blk, lb1 - win_base);
     if constexpr (FP8) {  // a chunk lies in one block
-      k_muls[SET] = scale * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_ks), slot));
+      k_units[SET] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_ks), slot));
       v_units[SET] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, win_vs), slot));
     }
     const uint64_t at0 = (uint64_t)blk0 * p.block_bytes + (uint32_t)(off * kRowBytes);
@@ -462,7 +465,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     constexpr int SET = decltype(set)::value;
     char* base = lds + stage * S::kBytes;
     if constexpr (FP8) {
-      if (threadIdx.x == 0) chunk_scale[stage] = float2{k_muls[SET], v_units[SET]};
+      if (threadIdx.x == 0) chunk_scale[stage] = float2{scale * k_units[SET], v_units[SET]};
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
