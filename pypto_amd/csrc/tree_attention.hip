@@ -540,10 +540,14 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     uint32_t bits[GT];
     float pv[GT][8];
     bool risen = false;
-    auto probabilities = [&](int t) __attribute__((always_inline)) {
+    // Against a maximum of this chunk's own the product is rounded first, as the maximum was: none passes 1, where scores are so large that what a product is rounded by is more than an
+    // exponential holds (from 2^30 on).
+    auto probabilities = [&](int t, auto own) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        pv[t][e] = __builtin_amdgcn_exp2f(fmaf(e < 4 ? s0[t][e] : s1[t][e - 4], k_mul, -m_run[t]));
+#pragma clang fp contract(off)
+        const float s = e < 4 ? s0[t][e] : s1[t][e - 4];
+        pv[t][e] = __builtin_amdgcn_exp2f(decltype(own)::value ? s * k_mul - m_run[t] : fmaf(s, k_mul, -m_run[t]));
         if constexpr (MASKED) pv[t][e] = bits[t] >> ((e >> 2) * 16 + j * 4 + (e & 3)) & 1u ? pv[t][e] : 0.f;
       }
     };
@@ -564,7 +568,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
         }
         if (tok + kChunk > all) bits[t] &= (1u << (all - tok)) - 1u;
       }
-      probabilities(t);
+      probabilities(t, std::false_type{});
       risen |= fmaxf(fmaxf(fmaxf(pv[t][0], pv[t][1]), fmaxf(pv[t][2], pv[t][3])), fmaxf(fmaxf(pv[t][4], pv[t][5]), fmaxf(pv[t][6], pv[t][7]))) >
                (float)(1 << kSlack);
     }
@@ -585,7 +589,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
         sum[t] *= alpha;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[t][i] *= alpha;
-        probabilities(t);
+        probabilities(t, std::true_type{});
       }
     }
 #pragma unroll

@@ -127,7 +127,7 @@ def test_tree_of_very_many_sequences(worker, batch):
     assert ((got[at].double().cpu() - want).abs() <= off * (mass + want.abs()) + HALF_STEP[BF] * want.abs()).all()
 
 
-@pytest.mark.parametrize("d", [80])
+@pytest.mark.parametrize("d", [64, 128, 256, 80])
 def test_tree_scores_that_are_no_ordinary_numbers(worker, d):
     """By either form: a score below -6.9e29 weighs nothing, among others or alone; infinite ones are NaN, as their softmax is; one of -1e29 counts."""
     b = Batch(d, [(64, 4), (3, 2), (5, 1), (2, 1), (33, 1)], 2, d, 32, BF)
