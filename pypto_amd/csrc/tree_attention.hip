@@ -317,6 +317,7 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 // A row's maximum may fall behind by so much (in powers of two) before sums and accumulators are brought up to it.  At 0, with every rise followed: 65 us for 55 over 16 sequences,
 // 317 us for 273 over four long ones.
 constexpr int kSlack = 6;
+constexpr int kLarge = 12;
 
 // Whether a wavefront has registers for three others on its SIMD: with one tile of rows, over e4m3 caches, whose rows on their way are half as long (32 sequences of 4 to 8
 // drafts, 64 heads: 190 -> 179 us by the kernel; with 16-bit caches registers spill).
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     float pv[GT][8];
     bool risen = false;
     // Against a maximum of this chunk's own the product is rounded first, as the maximum was: none passes 1, where scores are so large that what a product is rounded by is more than an
-    // exponential holds (from 2^30 on).
+    // exponential holds (from 2^30 on).  Rows whose maximum passes 2^kLarge always take this way, so that equal scores weigh the same; below, the difference is 2^-13 at most.
     auto probabilities = [&](int t, auto own) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -569,6 +570,7 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
         if (tok + kChunk > all) bits[t] &= (1u << (all - tok)) - 1u;
       }
       probabilities(t, std::false_type{});
+      risen |= fabsf(m_run[t]) > (float)(1 << kLarge);
       risen |= fmaxf(fmaxf(fmaxf(pv[t][0], pv[t][1]), fmaxf(pv[t][2], pv[t][3])), fmaxf(fmaxf(pv[t][4], pv[t][5]), fmaxf(pv[t][6], pv[t][7]))) >
                (float)(1 << kSlack);
     }

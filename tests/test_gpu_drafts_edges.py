@@ -164,3 +164,27 @@ def test_tree_scores_that_are_no_ordinary_numbers(worker, d):
     assert ((got[6] - rows.mean(0)[:, None]).abs() <= 2.0 ** -7 * rows.abs().mean(0)[:, None]).all()
     assert got[7].isnan().all()
     assert torch.equal(got[8], at(4, 33)[:, None].expand(2, 2, d))
+
+
+@pytest.mark.parametrize("d,cache", [(64, BF), (128, FP), (256, BF), (128, F8), (80, FP)])
+def test_tree_equal_scores_weigh_the_same_however_large(worker, d, cache):
+    """A thousand equal keys: the mean of their values, by scores of 10 to 10^10 that the scale rounds."""
+    b = Batch(d, [(1000, 24)], 2, d, 32, cache)
+    b.key.copy_((torch.sign(_randn(b.g, d)) * (256 if cache == F8 else 40000)).to(cache)[None].expand_as(b.key).clone())
+    if cache == F8:
+        b.k_scale.fill_(150.0)
+    sign = torch.sign(b.key[0].float())
+    dtype = BF if cache == F8 else cache
+    size = torch.logspace(-6.5, 3.0, 24, device="cuda")  # of the scores too, times 40000 d
+    size[1::2] *= -1
+    q = (size[:, None, None] * sign).expand(24, 4, d).reshape(-1, d).to(dtype)
+    mask = torch.full((24, 1), -1, dtype=torch.int32, device="cuda")
+    scale = 1.1
+    q, out = _attend(worker, b, 4, dtype, mask, scale, q=q)
+    worker.sync()
+    value = b.value.view(b.pool, 2, 32, d).double().cpu() * (b.v_scale.double().cpu()[:, :, None, None] if cache == F8 else 1)
+    rows = torch.stack([value[b.table[0][n // 32], :, n % 32] for n in range(1024)])
+    want, mass = rows.mean(0)[None, :, None], rows.abs().mean(0)[None, :, None]
+    got = out.view(24, 2, 2, d).double().cpu()
+    # weights of 1 to 2^-13 either way, sums in 32 bits, a rounding
+    assert ((got - want).abs() <= (2.0 ** -12 + 2.0 ** -13) * mass + HALF_STEP[dtype] * want.abs()).all()
