@@ -539,11 +539,12 @@ PTO_HIP_API int pto_hip_rope_append_tokens(const PtoHipRopeAppendArgs* args, voi
  * mask_words is reported by the next pto_hip_sync, its tokens from there on seen by nobody.  A row that sees nothing gives zeros; what a row does not
  * see has no part in it, infinities and NaN among it.  Scores, their sums and out are kept in fp32; probabilities are rounded to the query's type in front
  * of their product with the values, and summed as rounded (a plain kernel's stay in fp32); out is rounded once.  FP8E4M3FN scales are not negative; within
- * a sequence a value scale below 2^-60 of another's counts as that.  A table entry outside the cache reads block 0
- * and is reported by the next pto_hip_sync.  A score below -6.9e29 weighs nothing; one of +inf makes its row NaN.  Uses the library's scratch: like
- * all calls that do, calls are ordered on one stream, or synchronised, and a size is called once eagerly before it is captured.  head_dim 64, 128 and 256 with blocks of a multiple of 16 tokens (32 for FP8E4M3FN caches)
- * and up to 2^15 sequences run on matrix instructions, as long as a block (all KV heads) is below 2 GiB, T Hq / Hkv below 2^24 and T Hq / 64 + B Hkv
- * below 2^22 - 2^11; any other head_dim up to 256, block_size and batch on a plain kernel (beyond: PTO_HIP_ERR_UNSUPPORTED).  At most 2^20 tokens, mask_words 32. */
+ * a sequence a value scale below 2^-60 of another's counts as that, and an infinite or NaN one leaves nothing finite in the rows that see a token of its
+ * block.  A table entry outside the cache reads block 0 and is reported by the next pto_hip_sync.  A score below -6.9e29 weighs nothing; one of +inf
+ * makes its row NaN.  Uses the library's scratch: like all calls that do, calls are ordered on one stream, or synchronised, and a size is called once
+ * eagerly before it is captured.  head_dim 64, 128 and 256 with blocks of a multiple of 16 tokens (32 for FP8E4M3FN caches) and up to 2^15 sequences
+ * run on matrix instructions, as long as a block (all KV heads) is below 2 GiB, T Hq / Hkv below 2^24 and T Hq / 64 + B Hkv below 2^22 - 2^11; any
+ * other head_dim up to 256, block_size and batch on a plain kernel (beyond: PTO_HIP_ERR_UNSUPPORTED).  At most 2^20 tokens, mask_words 32. */
 typedef struct PtoHipTreeAttentionArgs {
   const void* query;            /* [T * Hq, D] dtype */
   const void* key_cache;        /* [pool_blocks * Hkv * block_size, D] */

@@ -466,7 +466,11 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
     constexpr int SET = decltype(set)::value;
     char* base = lds + stage * S::kBytes;
     if constexpr (FP8) {
-      if (threadIdx.x == 0) chunk_scale[stage] = float2{scale * k_units[SET], v_units[SET]};
+      if (threadIdx.x == 0) {
+        // of an infinite or NaN value scale: rows that see one of the keys are NaN by their scores, the others have no part in it
+        const bool bounded = fabsf(v_units[SET]) <= 3.4028234664e38f;
+        chunk_scale[stage] = float2{bounded ? scale * k_units[SET] : __builtin_nanf(""), bounded ? v_units[SET] : 0.f};
+      }
     }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {

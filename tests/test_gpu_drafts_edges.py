@@ -188,3 +188,48 @@ def test_tree_equal_scores_weigh_the_same_however_large(worker, d, cache):
     got = out.view(24, 2, 2, d).double().cpu()
     # weights of 1 to 2^-13 either way, sums in 32 bits, a rounding
     assert ((got - want).abs() <= (2.0 ** -12 + 2.0 ** -13) * mass + HALF_STEP[dtype] * want.abs()).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 80])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_tree_rows_are_not_reached_by_scales_of_blocks_that_they_do_not_see(worker, d, which):
+    """A block of drafts whose scale is infinite or NaN, between others: what sees none of its tokens is as ever, what does is nothing finite."""
+    for bad in (float("inf"), float("nan")):
+        b = Batch(d, [(32, 100), (70, 20)], 2, d, 32, F8)
+        inside = range(32, 64)  # drafts of the middle block
+        mask = _tree_masks(random.Random(d), b.lens, b.tokens, 0, "any")
+        mask[::2, 1] = 0  # half of the rows see nothing of it
+        q = _randn(b.g, b.tokens * 4, d).to(BF)
+        scales = getattr(b, which).clone()
+        getattr(b, which)[b.table[0][2]] = bad
+        _, out = _attend(worker, b, 4, BF, mask, d ** -0.5, q=q)
+        worker.sync()
+        setattr(b, which, scales)
+        want, mass, reach = od.tree_attention(q, b.key, b.value, b.blocks, b.ctx, b.starts, mask, 4, 2, d, 32, d ** -0.5, b.k_scale, b.v_scale)
+        got = out.view(b.tokens, 4, d).double().cpu()
+        sees = mask[:, 1].cpu() != 0
+        sees[100:] = False
+        assert sees.sum() > 40 and (~sees[:100]).sum() == 50 and len(inside) == 32
+        off = HALF_STEP[BF] + 2 * reach * (d + 12) * 2.0 ** -24 + 2.0 ** -19
+        assert ((got - want).abs() <= off * (mass + want.abs()) + HALF_STEP[BF] * want.abs())[~sees].all()
+        if which == "v_scale" or bad != bad:
+            assert not got[sees].isfinite().any()
+
+
+def test_tree_a_bad_scale_in_front_of_a_tiny_one(worker):
+    """Rows that do not see the first block, whose value scale is NaN, over one of the smallest numbers."""
+    b = Batch(3, [(0, 40)], 2, 128, 32, F8)
+    mask = torch.zeros((40, 2), dtype=torch.int32, device="cuda")
+    mask[:, 1] = 0xFF
+    mask[::3, 0] = 1
+    q = _randn(b.g, 40 * 4, 128).to(BF)
+    for tiny in (1e-40, 2.0 ** -149, 0.0, 1.0, 1e30):
+        b.v_scale[b.table[0][0]], b.v_scale[b.table[0][1]] = 0.5, tiny
+        want, mass, _ = od.tree_attention(q, b.key, b.value, b.blocks, b.ctx, b.starts, mask, 4, 2, 128, 32, 0.1, b.k_scale, b.v_scale)
+        b.v_scale[b.table[0][0]] = float("nan")
+        _, out = _attend(worker, b, 4, BF, mask, 0.1, q=q)
+        worker.sync()
+        got = out.view(40, 4, 128).double().cpu()
+        sees = torch.arange(40) % 3 == 0
+        assert ((got - want).abs() <= 2.0 ** -6 * mass + 2.0 ** -134 + 448 * 2.0 ** -149)[~sees].all()
+        assert not got[sees].isfinite().any()
