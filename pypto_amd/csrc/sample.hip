@@ -201,21 +201,34 @@ __device__ __forceinline__ void load8(const T* row, int i, int end, float (&v)[8
   for (int u = 0; u < 8; ++u) v[u] = i + u < end ? (float)row[i + u] : __builtin_nanf("");
 }
 
-// f(logit, index) for a thread's elements of [first, end), two steps' worth on their way at once; NaN behind the end.
+// Two steps' worth of a thread's elements, on their way at once; NaN behind the end.
+struct Two {
+  float a[8], b[8];
+};
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_two(const T* row, int i0, int end, Two& v) {
+  load8<T, WIDE>(row, i0 + threadIdx.x * 8, end, v.a);
+  load8<T, WIDE>(row, i0 + threadIdx.x * 8 + kStep, end, v.b);
+}
+// f(eight logits, index of the first) for a thread's elements of [first, end); v: the first of them, asked for before.
 template <typename T, bool WIDE, typename F>
-__device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
+__device__ __forceinline__ void in_eights(const T* row, int first, int end, Two& v, F f) {
   for (int i0 = first; i0 < end; i0 += 2 * kStep) {
     const int i = i0 + threadIdx.x * 8;
-    float a[8], b[8];
-    load8<T, WIDE>(row, i, end, a);
-    load8<T, WIDE>(row, i + kStep, end, b);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) f(a[u], i + u);
-    if (i0 + kStep < end) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) f(b[u], i + kStep + u);
-    }
+    f(v.a, i);
+    if (i0 + kStep < end) f(v.b, i + kStep);
+    if (i0 + 2 * kStep < end) load_two<T, WIDE>(row, i0 + 2 * kStep, end, v);
   }
+}
+// f(logit, index) likewise.
+template <typename T, bool WIDE, typename F>
+__device__ __forceinline__ void in_steps(const T* row, int first, int end, F f) {
+  Two v;
+  if (first < end) load_two<T, WIDE>(row, first, end, v);
+  in_eights<T, WIDE>(row, first, end, v, [&](const float (&v)[8], int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f(v[u], i + u);
+  });
 }
 
 // A thread's eight elements as they lie in memory; NaN behind the end.
@@ -393,7 +406,7 @@ constexpr int kGathered = 1024;  // by a workgroup for itself, with one place as
 // What the kernels leave for each other, a row of each a row.
 struct Scratch {
   unsigned long long* best;    // [slices] places of the slices' largest logits
-  float* low;                  // [slices] and their smallest
+  float* low;                  // [slices] and the smallest beside them (Beside)
   unsigned long long* weight;  // [kIntervals]
   unsigned int* count;         // [kIntervals]
   unsigned int* collected;     // [1] tokens of the border's intervals
@@ -404,6 +417,17 @@ struct Scratch {
   int stretches;               // kStep elements each
 };
 
+// The smallest of a row's logits that weigh anything, or less: what lies 46 powers of two below the largest - masked logits, whatever they are masked by - has no part in how
+// close together a row's logits lie.  Of a part of the row the largest is known before the row's: its smallest is not below the bound of its own largest, and moves up with that.
+struct Beside {
+  float span;  // 46 powers of two: 31.9 temperatures, somewhat more
+  __device__ __forceinline__ explicit Beside(float temperature) : span(32.5f * temperature) {}
+  // logits that are not above it weigh nothing beside `most`
+  __device__ __forceinline__ float bound(float most) const { return most - span - fabsf(most) * 0x1p-22f; }
+  // a part's smallest beside a larger logit than the part's; of a part that weighs nothing none
+  __device__ __forceinline__ float moved(float low, float part_most, float bound) const { return part_most > bound ? fmaxf(low, bound) : INFINITY; }
+};
+
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s) {
   __shared__ unsigned long long waves[kSliceThreads / 64];
@@ -411,15 +435,32 @@ __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s
   const int slice = blockIdx.x, r = blockIdx.y;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
+  Two ahead;
+  load_two<T, WIDE>(row, first, end, ahead);
+  const Beside beside(p.temperature[r]);
   // a thread meets its elements by rising index: of equal ones the first stays
   float most = -INFINITY, low = INFINITY;
   int where = first;
-  in_steps<T, WIDE>(row, first, end, [&](float v, int i) {
-    const bool more = v > most;
-    most = more ? v : most;
-    where = more ? i : where;
-    low = fminf(low, v);  // NaN: the other
-  });
+  auto more_of = [&](const float (&v)[8], int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const bool more = v[u] > most;
+      most = more ? v[u] : most;
+      where = more ? i + u : where;
+    }
+  };
+  if (filters_of(p, r).any()) {
+    in_eights<T, WIDE>(row, first, end, ahead, [&](const float (&v)[8], int i) __attribute__((always_inline)) {
+      const float before = most;
+      more_of(v, i);
+      const float bound = beside.bound(most);
+      low = beside.moved(low, before, bound);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) low = fminf(low, v[u] > bound ? v[u] : INFINITY);
+    });
+  } else {
+    in_eights<T, WIDE>(row, first, end, ahead, more_of);
+  }
   uint64_t best = packed(most, where);
   // the histogram of the next kernel starts from nothing
   const int per = (kIntervals + s.slices - 1) / s.slices;
@@ -429,43 +470,67 @@ __global__ __launch_bounds__(kSliceThreads) void best_kernel(Params p, Scratch s
   }
   if (slice == 0 && threadIdx.x == 0) s.collected[r] = 0;
   best = wave_max(best);
-  low = wave_min(low);
+  low = wave_min(beside.moved(low, most, beside.bound(value_of((uint32_t)(best >> 32)))));
   if (threadIdx.x % 64 == 0) {
     waves[threadIdx.x / 64] = best;
     lows[threadIdx.x / 64] = low;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kSliceThreads / 64; ++w) {
-      best = waves[w] > best ? waves[w] : best;
-      low = fminf(low, lows[w]);
-    }
+    for (int w = 1; w < kSliceThreads / 64; ++w) best = waves[w] > best ? waves[w] : best;
+    const float bound = beside.bound(value_of((uint32_t)(best >> 32)));
+    low = INFINITY;
+    for (int w = 0; w < kSliceThreads / 64; ++w) low = fminf(low, beside.moved(lows[w], value_of((uint32_t)(waves[w] >> 32)), bound));
     s.best[(size_t)r * s.slices + slice] = best;
     s.low[(size_t)r * s.slices + slice] = low;
   }
 }
 
-// The place of a row's largest logit and, where it has filters, the smallest, by every wavefront for itself.
+// The place of a row's largest logit and, where it has filters, the smallest beside it, by every wavefront for itself.
 struct Span {
   uint64_t best;
   float low;
 };
-__device__ __forceinline__ Span span_of_row(const Scratch& s, int r, bool filtered) {
-  Span span{0, INFINITY};
-  for (int i = threadIdx.x % 64; i < s.slices; i += 64) {
-    const uint64_t b = s.best[(size_t)r * s.slices + i];
-    const float l = s.low[(size_t)r * s.slices + i];
-    span.best = b > span.best ? b : span.best;
-    span.low = fminf(span.low, l);
+__device__ __forceinline__ Span span_of_row(const Scratch& s, int r, bool filtered, float temperature) {
+  const int lane = threadIdx.x % 64;
+  const unsigned long long* bests = s.best + (size_t)r * s.slices;
+  const float* lows = s.low + (size_t)r * s.slices;
+  constexpr int kOwn = kMaxVocab / kStep / 64;
+  uint64_t own[kOwn];
+  float own_low[kOwn];
+  auto ask = [&](int u) __attribute__((always_inline)) {  // behind the last slice the last again
+    const int i = min(lane + 64 * u, s.slices - 1);
+    own[u] = bests[i];
+    own_low[u] = lows[i];
+  };
+  const bool many = s.slices > 64;
+  ask(0);
+  if (many) {
+#pragma unroll
+    for (int u = 1; u < kOwn; ++u) ask(u);
   }
-  return Span{wave_max(span.best), filtered ? wave_min(span.low) : -INFINITY};
+  uint64_t best = own[0];
+  if (many) {
+#pragma unroll
+    for (int u = 1; u < kOwn; ++u) best = max(best, own[u]);
+  }
+  best = wave_max(best);
+  if (!filtered) return Span{best, -INFINITY};
+  const Beside beside(temperature);
+  const float bound = beside.bound(value_of((uint32_t)(best >> 32)));
+  float low = beside.moved(own_low[0], value_of((uint32_t)(own[0] >> 32)), bound);
+  if (many) {
+#pragma unroll
+    for (int u = 1; u < kOwn; ++u) low = fminf(low, beside.moved(own_low[u], value_of((uint32_t)(own[u] >> 32)), bound));
+  }
+  return Span{best, wave_min(low)};
 }
 __device__ __forceinline__ Weights weights_of(const Span& span, float temperature, const Powers* powers) {
   const float v = value_of((uint32_t)(span.best >> 32));
   const double rate = 64.0 * 1.4426950408889634074 / (double)temperature;
   // Half the distance and two steps an interval.  At a high temperature, or of an even distribution, that is few intervals for the whole row, and thousands of tokens in the
-  // border's: then there are as many intervals between its logits as there is room for (64 rows of 151936 at a temperature of 30: 61 us, by the row's own passes 657).
-  // Rows that are flat but for masked logits, -inf or far down, have one.
+  // border's: then there are as many intervals between its logits as there is room for (64 rows of 151936 at a temperature of 30: 61 us, by the row's own passes 657; the same
+  // with masked logits among them).
   const float whole = (float)(((double)v - (double)span.low) * rate * 0.5);
   const float finer = fminf(fmaxf((kIntervals - 2) * __builtin_amdgcn_rcpf(whole), 1.f), 1e6f);  // of no distance 1e6, of an infinite or undefined one 1
   return Weights{v, rate, powers, 0.5f * v, (float)fmin(rate * finer, 1e38), finer};
@@ -479,7 +544,7 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   const int slice = blockIdx.x, r = blockIdx.y;
   const Filters f = filters_of(p, r);
   const float t = p.temperature[r];
-  const Span span = span_of_row(s, r, f.any());
+  const Span span = span_of_row(s, r, f.any(), t);
   if (!(t > 0.f) || !f.any()) return;
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
@@ -607,7 +672,7 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   const int slice = blockIdx.x, r = blockIdx.y;
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
-  const Span span = span_of_row(s, r, f.any());
+  const Span span = span_of_row(s, r, f.any(), t);
   const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.vocab;
   const int first = slice * s.slice, end = min(p.vocab, first + s.slice);
   const Raw8<T> ahead = load_raw<T, WIDE>(row, first + threadIdx.x * 8, end);
@@ -804,7 +869,7 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
   const float t = p.temperature[r];
   const Filters f = filters_of(p, r);
   const unsigned int collected = s.collected[r];
-  const Span span = span_of_row(s, r, f.any());
+  const Span span = span_of_row(s, r, f.any(), t);
   for (int i = threadIdx.x; i < s.stretches; i += kThreads) sh.sums[i] = s.sums[(size_t)r * s.stretches + i];
   const uint32_t top = (uint32_t)(span.best >> 32);
   if (top <= kNone || !(t > 0.f)) {  // nothing to choose from, or no choice
