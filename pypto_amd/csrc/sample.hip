@@ -403,6 +403,8 @@ constexpr int kMaxSlice = 16384;
 constexpr int kCollected = 4096;
 constexpr int kGathered = 1024;  // by a workgroup for itself, with one place asked for in the row's list
 
+constexpr int kFront = 9;
+
 // What the kernels leave for each other, a row of each a row.
 struct Scratch {
   unsigned long long* best;    // [slices] places of the slices' largest logits
@@ -412,7 +414,7 @@ struct Scratch {
   unsigned int* collected;     // [1] tokens of the border's intervals
   unsigned long long* tokens;  // [kCollected] their places
   unsigned long long* sums;    // [stretches] weights surely kept of each kStep elements
-  unsigned long long* front;   // [5] tokens and weights in front of the border's intervals, weights of all; the first of these and their number
+  unsigned long long* front;   // [kFront] of top_k's interval and of top_p's: the first, their number, tokens and weights in front; the weights of all
   int slices, slice;           // elements of a slice, a multiple of kStep
   int stretches;               // kStep elements each
 };
@@ -578,10 +580,16 @@ __global__ __launch_bounds__(kSliceThreads) void histogram_kernel(Params p, Scra
   }
 }
 
-// The intervals in which a row's border may lie: first and last, and what lies in front of the first.
-struct BorderIntervals {
+// Neighbouring intervals and what lies in front of them; kIntervals: none.
+struct Stretch {
   int first, last;
-  uint64_t tokens_front, weight_front, weight_all;
+  uint64_t tokens_front, weight_front;
+  __device__ __forceinline__ bool there() const { return first < kIntervals; }
+};
+// The intervals in which a row's borders may lie: top_k's, one, and top_p's, which are in front of it or end with it.  Thousands of tokens may lie between the two.
+struct BorderIntervals {
+  Stretch k, p;
+  uint64_t weight_all;
 };
 // Each thread holds the sums of its kIntervals / kSliceThreads intervals.
 __device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int r, const Filters& f) {
@@ -638,7 +646,7 @@ __device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int 
     __syncthreads();
   }
   const int k_at = (int)found[0];
-  BorderIntervals out{k_at, k_at, k_at < kIntervals ? found[3] : 0, k_at < kIntervals ? found[1] : 0, all};
+  BorderIntervals out{{k_at, k_at, k_at < kIntervals ? found[3] : 0, k_at < kIntervals ? found[1] : 0}, {kIntervals, kIntervals, 0, 0}, all};
   if (f.by_sum) {
     // the weights of what top_k keeps lie between those in front of its interval and those up to its end
     const uint64_t lo = needed(f, k_at < kIntervals ? found[1] : all), hi = needed(f, k_at < kIntervals ? found[2] : all);
@@ -655,10 +663,7 @@ __device__ __forceinline__ BorderIntervals find_intervals(const Scratch& s, int 
       b += x[i];
     }
     __syncthreads();
-    out.first = (int)found[4];
-    out.tokens_front = found[5];
-    out.weight_front = found[6];
-    out.last = k_at < kIntervals ? k_at : (int)found[7];
+    out.p = Stretch{(int)found[4], (int)found[7], found[5], found[6]};
   }
   return out;
 }
@@ -686,30 +691,39 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
   fill(powers);
   if (threadIdx.x < kMaxSlice / kStep) sums[threadIdx.x] = 0;
   if (threadIdx.x == 0) gathered = 0;
-  BorderIntervals at{kIntervals, kIntervals, 0, 0, 0};
+  BorderIntervals at{{kIntervals, kIntervals, 0, 0}, {kIntervals, kIntervals, 0, 0}, 0};
   if (f.any()) at = find_intervals(s, r, f);
   if (slice == 0 && threadIdx.x == 0) {
-    unsigned long long* front = s.front + 5 * (size_t)r;
-    front[0] = at.tokens_front;
-    front[1] = at.weight_front;
-    front[2] = at.weight_all;
-    front[3] = at.first;
-    front[4] = at.last - at.first + 1;
+    unsigned long long* front = s.front + kFront * (size_t)r;
+    auto leave = [&](unsigned long long* to, const Stretch& x) {
+      to[0] = x.first;
+      to[1] = x.last - x.first + 1;
+      to[2] = x.tokens_front;
+      to[3] = x.weight_front;
+    };
+    leave(front, at.k);
+    leave(front + 4, at.p);
+    front[8] = at.weight_all;
   }
   __syncthreads();
   const double least = (double)f.least, more_than = least - 0.5;  // of a weight not yet rounded
   // of what is surely kept, min_p - or the rounding to whole units - leaves out what is further down than this (an interval more than it has to be)
   const float i_least = (32.f * ((float)kUnit - __builtin_amdgcn_logf((float)more_than)) + 1.f) * w.finer;
-  const float i_first = (float)at.first, i_sure = fminf(i_first, i_least), i_behind = fminf((float)(at.last + 1), (float)kIntervals);
+  using pto_hip::block8::IntConst;
+  // collected is what lies in the borders' intervals: from i_first to i_last and from i_again to i_behind
+  const bool both = at.k.there() && at.p.there() && at.p.last < at.k.first;
+  const float i_first = (float)min(at.k.first, at.p.first), i_sure = fminf(i_first, i_least);
+  const float i_behind = fminf((float)(at.k.there() ? at.k.last + 1 : at.p.last + 1), (float)kIntervals);
+  const float i_last = both ? (float)(at.p.last + 1) : i_behind, i_again = both ? (float)at.k.first : i_behind;
   const float cut = w.cut(i_behind);
   double own = kBig;  // and the weights of a step: exact
-  auto take = [&](float v, int i) __attribute__((always_inline)) {
+  auto take = [&](float v, int i, auto apart) __attribute__((always_inline)) {
     if (v < cut) return;  // most logits of a row with a border
     const float at_i = w.interval(v);
     if (at_i < i_sure) {
       const double x = w.scaled(w.finite_steps(v));
       own += x > more_than ? x : 0.0;
-    } else if (at_i >= i_first && at_i < i_behind) {
+    } else if (at_i >= i_first && at_i < i_behind && (decltype(apart)::value == 0 || at_i < i_last || at_i >= i_again)) {
       const unsigned int n = atomicAdd(&gathered, 1u);
       if (n < kGathered) {
         tokens[n] = packed(v, i);
@@ -732,9 +746,10 @@ __global__ __launch_bounds__(kSliceThreads) void collect_kernel(Params p, Scratc
     own = kBig;
   };
   if (infinite) step_by_step<T, WIDE>(row, first, end, ahead, take_infinite, done);
-  else if (at.first == kIntervals && f.least == 1) step_by_step<T, WIDE>(row, first, end, ahead, take_all, done);  // what is below a half adds nothing
-  else if (at.first == kIntervals) step_by_step<T, WIDE>(row, first, end, ahead, take_heavy, done);
-  else step_by_step<T, WIDE>(row, first, end, ahead, take, done);
+  else if (i_first == (float)kIntervals && f.least == 1) step_by_step<T, WIDE>(row, first, end, ahead, take_all, done);  // what is below a half adds nothing
+  else if (i_first == (float)kIntervals) step_by_step<T, WIDE>(row, first, end, ahead, take_heavy, done);
+  else if (both) step_by_step<T, WIDE>(row, first, end, ahead, [&](float v, int i) __attribute__((always_inline)) { take(v, i, IntConst<1>{}); }, done);
+  else step_by_step<T, WIDE>(row, first, end, ahead, [&](float v, int i) __attribute__((always_inline)) { take(v, i, IntConst<0>{}); }, done);
   __syncthreads();
   const int stretch = first / kStep + threadIdx.x;
   if (threadIdx.x < s.slice / kStep && stretch < s.stretches) s.sums[(size_t)r * s.stretches + stretch] = sums[threadIdx.x];
@@ -766,15 +781,38 @@ struct DrawShared {
   };
 };
 
-// Where the running sum of the collected tokens (by_weight: of their weights), in order and from what lies in front of them on, reaches `need`: the place of that token and
-// the sum of the weights up to it.  The cell that it lies in first, then the cell's tokens in order.  All threads take part; `need` is reached.
+// Where the running sum of the collected tokens of a border's intervals (by_weight: of their weights), in order and from what lies in front of them on, reaches `need`: the place of
+// that token and the sum of the weights up to it.  The cell that it lies in first, then the cell's tokens in order.  All threads take part; `need` is reached.
 struct Reached {
   uint64_t place, weight;
 };
-template <typename Cell, typename Weight>
-__device__ Reached reach(DrawShared& sh, const unsigned long long* tokens, int n, bool by_weight, uint64_t tokens_front, uint64_t weight_front, uint64_t need,
-                         Cell cell, Weight weight) {
+// The intervals that they are looked for in, as the kernel in front left them: first and number.
+struct Within {
+  float first, behind, cells_each;
+  uint64_t tokens_front, weight_front;
+  __device__ __forceinline__ explicit Within(const unsigned long long* at)
+      : first((float)at[0]), behind((float)(at[0] + at[1])), cells_each((float)kCells / (float)at[1]), tokens_front(at[2]), weight_front(at[3]) {}
+  // the cell of a token by its interval; -1: one in front of them or behind
+  __device__ __forceinline__ int cell(float interval) const {
+    return interval >= first && interval < behind ? min((int)((interval - first) * cells_each), kCells - 1) : -1;
+  }
+};
+template <typename Interval, typename Weight>
+__device__ Reached reach(DrawShared& sh, const unsigned long long* tokens, int n, bool by_weight, const Within& within, uint64_t need, Interval interval, Weight weight) {
   constexpr int kOwn = kCells / kThreads;
+  const uint64_t tokens_front = within.tokens_front, weight_front = within.weight_front;
+  for (int i = threadIdx.x; i < kCells; i += kThreads) {
+    sh.cells.weight[i] = 0;
+    sh.cells.count[i] = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const int at = within.cell(interval(tokens[i]));
+    if (at < 0) continue;
+    atomicAdd(&sh.cells.count[at], 1u);
+    atomicAdd(&sh.cells.weight[at], (unsigned long long)weight(tokens[i]));
+  }
+  __syncthreads();
   uint64_t n_own = 0, x_own = 0;
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
@@ -801,7 +839,7 @@ __device__ Reached reach(DrawShared& sh, const unsigned long long* tokens, int n
   const int here = (int)sh.found[0];
   const uint64_t n_cell = sh.found[1], x_cell = sh.found[2];
   for (int i = threadIdx.x; i < n; i += kThreads)
-    if (cell(tokens[i]) == here) sh.tokens[atomicAdd(&sh.gathered, 1u)] = tokens[i];
+    if (within.cell(interval(tokens[i])) == here) sh.tokens[atomicAdd(&sh.gathered, 1u)] = tokens[i];
   __syncthreads();
   const int m = (int)sh.gathered;
   // in order
@@ -900,29 +938,17 @@ __global__ __launch_bounds__(kThreads) void draw_kernel(Params p, Scratch s) {
     });
   } else if (n > 0) {
     const unsigned long long* tokens = s.tokens + (size_t)r * kCollected;
-    const unsigned long long* front = s.front + 5 * (size_t)r;
-    const float i_first = (float)front[3], per_interval = (float)kCells / (float)front[4];
+    const unsigned long long* front = s.front + kFront * (size_t)r;
     auto weight = [&](uint64_t token) { return w(value_of((uint32_t)(token >> 32))); };
-    auto cell = [&](uint64_t token) { return min((int)((w.interval(value_of((uint32_t)(token >> 32))) - i_first) * per_interval), kCells - 1); };
-    for (int i = threadIdx.x; i < kCells; i += kThreads) {
-      sh.cells.weight[i] = 0;
-      sh.cells.count[i] = 0;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int at = cell(tokens[i]);
-      atomicAdd(&sh.cells.count[at], 1u);
-      atomicAdd(&sh.cells.weight[at], (unsigned long long)weight(tokens[i]));
-    }
-    __syncthreads();
-    uint64_t sum = front[2];
-    if (f.k > 0 && front[0] + n >= (uint64_t)f.k) {
-      const Reached k = reach(sh, tokens, n, false, front[0], front[1], (uint64_t)f.k, cell, weight);
+    auto interval = [&](uint64_t token) { return w.interval(value_of((uint32_t)(token >> 32))); };
+    uint64_t sum = front[8];
+    if (front[0] < kIntervals) {
+      const Reached k = reach(sh, tokens, n, false, Within(front), (uint64_t)f.k, interval, weight);
       border = k.place;
       sum = k.weight;
     }
     if (f.by_sum) {
-      const Reached at = reach(sh, tokens, n, true, front[0], front[1], needed(f, sum), cell, weight);
+      const Reached at = reach(sh, tokens, n, true, Within(front + 4), needed(f, sum), interval, weight);
       border = at.place > border ? at.place : border;
     }
     for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -1009,7 +1035,7 @@ int launch(Params p, hipStream_t st) {
   s.slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(kStep, (even + kStep - 1) / kStep * kStep));
   s.slices = (p.vocab + s.slice - 1) / s.slice;
   s.stretches = (p.vocab + kStep - 1) / kStep;
-  const size_t per_row = 8 * ((size_t)s.slices + s.stretches + kIntervals + kCollected + 5) + 4 * (kIntervals + 2 + (size_t)s.slices);
+  const size_t per_row = 8 * ((size_t)s.slices + s.stretches + kIntervals + kCollected + kFront) + 4 * (kIntervals + 2 + (size_t)s.slices);
   void* ws = nullptr;
   const int rc = pto_hip::workspace(per_row * at_once, &ws);
   if (rc) return rc;
@@ -1018,7 +1044,7 @@ int launch(Params p, hipStream_t st) {
   s.weight = s.sums + at_once * s.stretches;
   s.tokens = s.weight + at_once * kIntervals;
   s.front = s.tokens + at_once * kCollected;
-  s.count = reinterpret_cast<unsigned int*>(s.front + 5 * at_once);
+  s.count = reinterpret_cast<unsigned int*>(s.front + kFront * at_once);
   s.collected = s.count + at_once * kIntervals;
   s.low = reinterpret_cast<float*>(s.collected + at_once);
   const bool wide = (uintptr_t)p.logits % 16 == 0 && (int64_t)p.vocab * sizeof(T) % 16 == 0;

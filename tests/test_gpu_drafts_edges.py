@@ -268,3 +268,17 @@ def test_sample_of_masked_rows_is_like_that_of_others(worker, dtype, masked):
         args = (30.0, torch.tensor([0, 60000] * 3), torch.tensor([0.9, 0.5, 1.0] * 2), 0.0, torch.rand(6, device="cuda", generator=g))
         _check_sample(worker, rows[:6].contiguous(), *args)
         assert _fastest(worker, rows, 30.0, 0, 0.9, 0.0, 0.4) < 3 * plain
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_sample_by_a_large_top_k_and_top_p(worker, dtype):
+    """Far apart, the two borders' intervals are collected by themselves and nothing of what lies between: 64 rows of 151936 ordinary logits, of which top_k leaves thousands."""
+    g = _gen(12)
+    logits = (2 * _randn(g, 64, 151936)).to(dtype)
+    logits[:, 17:57] += 6
+    alone = _fastest(worker, logits, 1.0, 0, 0.9, 0.0, 0.4)
+    for k in (5000, 20000, 50000):
+        ks = torch.tensor([k, k + 1, k - 7, k] * 2)
+        _check_sample(worker, logits[:8].contiguous(), 1.0, ks, torch.tensor([0.9, 0.5, 0.99, 0.999, 0.9999, 0.95, 0.0, 0.3]), torch.tensor([0.0] * 7 + [1e-4]),
+                      torch.rand(8, device="cuda", generator=g))
+        assert _fastest(worker, logits, 1.0, k, 0.9, 0.0, 0.4) < 3 * alone
