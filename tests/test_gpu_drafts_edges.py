@@ -282,3 +282,17 @@ def test_sample_by_a_large_top_k_and_top_p(worker, dtype):
         _check_sample(worker, logits[:8].contiguous(), 1.0, ks, torch.tensor([0.9, 0.5, 0.99, 0.999, 0.9999, 0.95, 0.0, 0.3]), torch.tensor([0.0] * 7 + [1e-4]),
                       torch.rand(8, device="cuda", generator=g))
         assert _fastest(worker, logits, 1.0, k, 0.9, 0.0, 0.4) < 3 * alone
+
+
+@pytest.mark.parametrize("d,cache", [(64, BF), (128, F8), (256, FP), (80, BF), (96, F8)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_tree_of_negative_scales_and_of_none(worker, d, cache, scale):
+    """Signs of the queries turned, and every key of the same weight; rows that see nothing of a chunk among them."""
+    lens = [(0, 7), (5, 0), (31, 1), (33, 40), (600, 3), (0, 70)]
+    for kind in ("tree", "any", "none"):
+        b = Batch(d, lens, 2, d, 32, cache, pad=1, first=1)
+        dtype = FP if cache == F8 else cache
+        mask = _tree_masks(random.Random(d), lens, b.tokens, 1, kind)
+        q, out = _attend(worker, b, 8, dtype, mask, scale)
+        worker.sync()
+        _check_tree(b, 8, dtype, mask, scale, q, out)
