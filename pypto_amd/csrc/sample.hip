@@ -9,14 +9,14 @@
 // the work is split, and next to a border or the random number the decision is that of the definition up to half a unit a token.
 //
 // Four kernels, the first three over slices of the rows so that few rows fill the chip too: the largest logit; of rows with top_k or top_p, how many
-// tokens or how much weight lie in each of 1472 intervals of 2^(1/32) below it (finer ones where its logits lie closer together); for each 2048 tokens the sum of what they surely keep, and the tokens of the border's
-// interval; and, a workgroup a row, the border among those (by 1024 cells of the interval, then in order), the 2048 tokens in which the random number falls and the token
-// among them.  Where more tokens share the border's interval than are collected (thousands of nearly equal logits), the last kernel looks for the border in the
-// row itself, eleven bits of the key a pass.
+// tokens or how much weight lie in each of 1472 intervals of 2^(1/32) below it (finer ones where its logits lie closer together, masked ones left out); for each 2048 tokens the sum of what they
+// surely keep, and the tokens of the borders' intervals, top_k's and top_p's; and, a workgroup a row, the border among those (by 1024 cells of the intervals, then in order), the 2048 tokens in
+// which the random number falls and the token among them.  Where more tokens share a border's interval than are collected (thousands of equal or nearly equal logits), the last kernel looks for
+// the border in the row itself, eleven bits of the key a pass: 0.7 ms for a row of 151936 in one launch, 0.8 to 1.3 ms for 64 of them.
 //
 // A row is read two or three times and its weights are computed in 64 bits.  One row of 151936 bf16 logits with top_p: 24 to 31 us, of which the four kernels' chains of
-// dependent loads and barriers 3.5 + 7 + 7 + 11; 64 rows of 151936 fp32 ones with mixed filters: 46 to 48 us (9 + 11 + 18 + 11); 320 rows of 32000 fp16 ones without: 31 us, collecting 16
-// of them, bound by the exponentials; 500 rows of 128000 fp32 ones, mixed: 185 to 190 us, the first read at 5.1 TB/s, the histogram of half of the rows bound by LDS atomics
+// dependent loads and barriers 4 + 7 + 7 + 11; 64 rows of 151936 fp32 ones with mixed filters: 47 to 49 us (9 + 11 + 18 + 11), with top_k 20000 and top_p in every row 69; 320 rows of 32000 fp16 ones without: 31 us, collecting 16
+// of them, bound by the exponentials; 500 rows of 128000 fp32 ones, mixed: 187 to 190 us, the first read at 5.1 TB/s, the histogram of half of the rows bound by LDS atomics
 // (57 to 60 us; a second copy of it in LDS, for half of the conflicts, takes 66, as fewer workgroups fit), the collecting read 70 us, the vector units 85 % busy.
 #include <hip/hip_runtime.h>
 

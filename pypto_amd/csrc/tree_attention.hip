@@ -6,8 +6,8 @@
 // The form for one token per sequence is paged_attention.hip's (examples/models/04_paged_attention.py:62-227).
 //
 // With few rows a sequence the caches' bytes bound it, with many the products: 16 sequences of 512 to 4096 bf16 keys and 1 to 40 new tokens, 32 heads over 8: 54 us (158 MB;
-// 30 us at the 5.2 TB/s of a large copy), 32 sequences of 2000 to 16000 e4m3 keys and 4 to 8 tokens, 64 heads over 8: 154 to 158 us (596 MB, 115 us), 4 sequences of 20000 to 32000 fp16 keys and
-// 64 tokens, 64 heads: 265 to 271 us (218 GFLOP, 182 us at the 1.2 PFLOP/s of a large product), one sequence of 4096 keys and 16 tokens: 18 us (14 and the join's 4), a chain of the
+// 30 us at the 5.2 TB/s of a large copy), 32 sequences of 2000 to 16000 e4m3 keys and 4 to 8 tokens, 64 heads over 8: 149 to 152 us (596 MB, 115 us), 4 sequences of 20000 to 32000 fp16 keys and
+// 64 tokens, 64 heads: 261 to 274 us (218 GFLOP, 182 us at the 1.2 PFLOP/s of a large product), one sequence of 4096 keys and 16 tokens: 18 us (14 and the join's 4), a chain of the
 // plan, the first loads, some 8 chunks and the join.
 #include <hip/hip_runtime.h>
 
@@ -319,8 +319,9 @@ __device__ __forceinline__ u32x2 read_columns(const char* p) {
 constexpr int kSlack = 6;
 constexpr int kLarge = 12;
 
-// Whether a wavefront has registers for three others on its SIMD: with one tile of rows, over e4m3 caches, whose rows on their way are half as long (32 sequences of 4 to 8
-// drafts, 64 heads: 190 -> 179 us by the kernel; with 16-bit caches registers spill).
+// Whether a wavefront shares its SIMD with three others: with one tile of rows, over e4m3 caches, whose rows on their way are half as long (32 sequences of 4 to 8 drafts, 64 heads:
+// 190 -> 179 us by the kernel).  128 registers hold all that the loop over cached keys needs (with 128 channels 20 values lie in scratch, of the chunks with new tokens and of the end); one
+// reload in that loop waits for every row on its way (157 -> 180 us).  16-bit caches need 178.
 template <int D, bool FP8, int GT>
 constexpr bool lean() { return GT == 1 && FP8 && D <= 128; }
 
@@ -601,6 +602,8 @@ __global__ __launch_bounds__(NW * 64, (lean<D, FP8, GT>() ? 4 : 2)) void tree_ke
 #pragma unroll
     for (int t = 0; t < GT; ++t) {
 #pragma unroll
+      // 16 bits are what the matrix instruction takes: half a step of each probability, which in the mean over the keys leaves the result 1.4 times as far from the exact one as its own
+      // rounding does (2.3e-3 and 1.7e-3 of its size in bfloat16).  A second product of what the rounding leaves would double the instructions of this half.
       for (int e = 0; e < 8; e += 2) pf[t][e >> 1] = round_pair<BF16>(pv[t][e], pv[t][e + 1]);
       sum[t] = mfma16<BF16>(ones, pf[t], sum[t]);  // of the probabilities as rounded
     }
@@ -856,7 +859,7 @@ int launch_tiles(Params& p, hipStream_t st) {
 template <int D, bool BF16, bool FP8>
 int launch_rows(Params& p, hipStream_t st) {
   const int64_t rows = (int64_t)std::min<int64_t>((p.tokens + p.batch - 1) / p.batch, 32 * p.words) * p.group;  // of a sequence, on average
-  if constexpr (D == 256) {  // fewer wavefronts would bring so much each that their registers did not hold it
+  if constexpr (D == 256) {  // four wavefronts would bring twice as much each: 13 to 46 registers of 16-bit caches' form lie in scratch then
     return launch_tiles<D, BF16, FP8, 8, 1, 2>(p, st);
   } else {
     // A sequence's rows in one workgroup as long as they fit: its keys are read once.  16 sequences of 4096 keys, 8 KV heads of 128 in bf16 (e4m3), by four wavefronts of one tile of
