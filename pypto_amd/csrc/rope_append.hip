@@ -21,6 +21,7 @@
 
 namespace {
 
+using pto_hip::in_launches;
 using pto_hip::TokenSeq;
 
 constexpr int kThreads = 256;
@@ -376,16 +377,6 @@ void with_lanes(int d, F f) {
   else if (d <= 128) f(Lanes<16>{});
   else if (d <= 256) f(Lanes<32>{});
   else f(Lanes<64>{});
-}
-
-// f(tokens) for the tokens of each launch: a launch holds fewer than 2^32 threads.
-template <typename F>
-void in_launches(Params& p, int64_t threads_a_token, F f) {
-  const int64_t most = std::max<int64_t>(1, (1ll << 31) / threads_a_token);
-  for (int64_t t = 0; t < p.tokens; t += most) {
-    p.t0 = (int)t;
-    f((unsigned)std::min<int64_t>(most, p.tokens - t));
-  }
 }
 
 template <typename In, typename T>

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 namespace pto_hip {
@@ -53,6 +54,16 @@ __device__ __forceinline__ TokenSeq sequence_of(const int32_t* starts, int batch
   const int k = max((int)__popcll(__ballot(lane < n && start <= token)) - 1, 0);
   const int first = __shfl(start, k), end = __shfl(next, k);
   return TokenSeq{first <= token && token < end ? lo + k : -1, first, end - first};
+}
+
+// f(tokens) for the tokens of each launch of a call with parameters p: a launch holds fewer than 2^32 threads.
+template <typename P, typename F>
+void in_launches(P& p, int64_t threads_a_token, F f) {
+  const int64_t most = std::max<int64_t>(1, (1ll << 31) / threads_a_token);
+  for (int64_t t = 0; t < p.tokens; t += most) {
+    p.t0 = (int)t;
+    f((unsigned)std::min<int64_t>(most, p.tokens - t));
+  }
 }
 
 // Sums over a wavefront without a trip through LDS: along rows of 16 lanes, then from row to row; lane 63 has all.

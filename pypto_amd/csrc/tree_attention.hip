@@ -22,6 +22,7 @@
 
 namespace {
 
+using pto_hip::in_launches;
 using pto_hip::TokenSeq;
 
 constexpr int64_t kMaxTokens = 1 << 20;
@@ -798,16 +799,6 @@ __global__ __launch_bounds__(256) void tree_join_kernel(Params p) {
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) reinterpret_cast<T*>(p.out)[((size_t)token * p.hq + head) * D + i * 64 + lane] = (T)(o[i] * inv);
-}
-
-// f(tokens) for the tokens of each launch: a launch holds fewer than 2^32 threads.
-template <typename F>
-void in_launches(Params& p, int64_t threads_a_token, F f) {
-  const int64_t most = std::max<int64_t>(1, (1ll << 31) / threads_a_token);
-  for (int64_t t = 0; t < p.tokens; t += most) {
-    p.t0 = (int)t;
-    f((unsigned)std::min<int64_t>(most, p.tokens - t));
-  }
 }
 
 // Every workgroup makes the plan of all sequences, which grows with the square of their number: one token each, 64 heads over 8 of 64 channels, contexts of 8 to 15 (250 to 500) keys: 1024
