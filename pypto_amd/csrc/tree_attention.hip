@@ -6,7 +6,7 @@
 // The form for one token per sequence is paged_attention.hip's (examples/models/04_paged_attention.py:62-227).
 //
 // With few rows a sequence the caches' bytes bound it, with many the products: 16 sequences of 512 to 4096 bf16 keys and 1 to 40 new tokens, 32 heads over 8: 54 us (158 MB;
-// 30 us at the 5.2 TB/s of a large copy), 32 sequences of 2000 to 16000 e4m3 keys and 4 to 8 tokens, 64 heads over 8: 149 to 152 us (596 MB, 115 us), 4 sequences of 20000 to 32000 fp16 keys and
+// 30 us at the 5.2 TB/s of a large copy), 32 sequences of 2000 to 16000 e4m3 keys and 4 to 8 tokens, 64 heads over 8: 146 to 152 us (596 MB, 115 us), 4 sequences of 20000 to 32000 fp16 keys and
 // 64 tokens, 64 heads: 261 to 274 us (218 GFLOP, 182 us at the 1.2 PFLOP/s of a large product), one sequence of 4096 keys and 16 tokens: 18 us (14 and the join's 4), a chain of the
 // plan, the first loads, some 8 chunks and the join.
 #include <hip/hip_runtime.h>

@@ -102,10 +102,10 @@ def test_tree_keeps_scratch_for_what_is_cut(worker):
             assert ((got - want[0]).abs() <= (off * (mass + want.abs()) + HALF_STEP[BF] * want.abs())[0]).all()
 
 
-@pytest.mark.parametrize("batch", [1 << 12, (1 << 15) + 1, 1 << 19])
-def test_tree_of_very_many_sequences(worker, batch):
+@pytest.mark.parametrize("batch,hkv", [(1 << 12, 8), ((1 << 15) + 1, 8), (1 << 19, 8), (1 << 15, 256)])
+def test_tree_of_very_many_sequences(worker, batch, hkv):
     """Single tokens without a context that see themselves alone: their values."""
-    hkv, d, bs, pool = 8, 64, 16, 64
+    d, bs, pool = 64, 16, 64
     g = _gen(batch)
     key, value = (_randn(g, pool * hkv * bs, d).to(BF) for _ in range(2))
     table = torch.randint(0, pool, (batch, 1), device="cuda", generator=g, dtype=torch.int32)
@@ -121,7 +121,7 @@ def test_tree_of_very_many_sequences(worker, batch):
     got = out.view(batch, hkv, d)
     half = batch // 2
     assert torch.equal(got[:half], rows[table[:half, 0].long(), :, 0])
-    at = list(range(half, batch, max(1, half // 50))) + [batch - 1]
+    at = list(range(half, batch, max(1, half * hkv // 400))) + [batch - 1]
     want, mass, reach = od.tree_attention(q.view(batch, -1)[at].reshape(-1, d), key, value, table[at], ctx[at], torch.arange(len(at) + 1), mask[at], hkv, hkv, d, bs, d ** -0.5)
     off = HALF_STEP[BF] + 2 * reach * (d + 12) * 2.0 ** -24 + 2.0 ** -19
     assert ((got[at].double().cpu() - want).abs() <= off * (mass + want.abs()) + HALF_STEP[BF] * want.abs()).all()
